@@ -138,10 +138,7 @@ def prepare(case, seed):
         targets[:masked_of(case)] = -1
         st["targets"] = targets
         if case["op"] == "gradient":
-            # what the forward call gave, and the gradient of the user's objective
-            s = logits.double() / case["temperature"]
-            st["lse"] = torch.logsumexp(s, dim=1).float()
-            st["entropy"] = (st["lse"].double() - (torch.exp(s - st["lse"].double()[:, None]) * s).sum(1)).float() if case["entropy"] else None
+            # the gradient of the user's objective
             st["dlogp"] = torch.randn(N, device="cuda", generator=g) / N
             st["dentropy"] = 0.1 * torch.randn(N, device="cuda", generator=g) / N if case["entropy"] else None
         return st
@@ -198,10 +195,9 @@ def run_own(state):
     op = case["op"]
     if op == "logprobs":
         r = fb.token_logprobs(state["logits"], state["targets"], temperature=case["temperature"], entropy=case["entropy"])
-        return (r.logp, r.lse, r.entropy) if case["entropy"] else (r.logp, r.lse)
+        return (r.logp, r.entropy) if case["entropy"] else r.logp
     if op == "gradient":
-        return fb.token_logprobs_gradient(state["logits"], state["targets"], state["lse"], state["dlogp"], entropy=state["entropy"],
-                                          dentropy=state["dentropy"], temperature=case["temperature"])
+        return fb.token_logprobs_gradient(state["logits"], state["targets"], state["dlogp"], dentropy=state["dentropy"], temperature=case["temperature"])
     if op == "policy":
         r = fb.policy_loss(state["logits"], state["targets"], state["old"], state["advantages"], ref_logp=state["ref"], weights=state["weights"],
                            clip_low=CLIP[0], clip_high=CLIP[1], kl_coef=case["kl"], temperature=case["temperature"], reduction=case["reduction"],
@@ -232,17 +228,18 @@ def run_plain(state):
     if op == "logprobs":
         s, lse, logp, has = softmax_parts(state["logits"], state["targets"], case["temperature"])
         if not case["entropy"]:
-            return logp, torch.where(has, lse, 0.0)
+            return logp
         ls = s - lse[:, None]
-        return logp, torch.where(has, lse, 0.0), torch.where(has, -(torch.exp(ls) * ls).sum(1), 0.0)
+        return logp, torch.where(has, -(torch.exp(ls) * ls).sum(1), 0.0)
     targets = state["targets"]
     if op == "gradient":
-        ls = state["logits"].float() * (1.0 / case["temperature"]) - state["lse"][:, None]
+        s, lse, _, _ = softmax_parts(state["logits"], targets, case["temperature"])
+        ls = s - lse[:, None]
         p = torch.exp(ls)
         d = -p * state["dlogp"][:, None]
         d.scatter_add_(1, targets.clamp(min=0).long()[:, None], state["dlogp"][:, None])
         if case["entropy"]:
-            d -= state["dentropy"][:, None] * p * (ls + state["entropy"][:, None])
+            d -= state["dentropy"][:, None] * p * (ls - (p * ls).sum(1)[:, None])
         return torch.where((targets >= 0)[:, None], d * (1.0 / case["temperature"]), 0.0).to(state["logits"].dtype)
     s, lse, logp, has = softmax_parts(state["logits"], targets, case["temperature"])
     A = state["advantages"]
@@ -307,18 +304,16 @@ def exact(case, seed):
     has = targets >= 0
     index = targets.clamp(min=0).long()
     logp = torch.zeros(N, device="cuda", dtype=torch.float64)
-    lse, entropy = torch.zeros_like(logp), torch.zeros_like(logp)
+    entropy = torch.zeros_like(logp)
     step = max(1, (1 << 26) // V)
     for i in range(0, N, step):
         rows = slice(i, min(N, i + step))
         ls = torch.log_softmax(logits[rows].double() / case["temperature"], dim=1)
-        lse[rows] = torch.logsumexp(logits[rows].double() / case["temperature"], dim=1)
         logp[rows] = ls[torch.arange(ls.shape[0], device="cuda"), index[rows]]
         entropy[rows] = -(ls.exp() * ls).sum(1)
     zero = torch.zeros_like(logp)
     if op == "logprobs":
-        out = (torch.where(has, logp, zero), torch.where(has, lse, zero))
-        return out + (torch.where(has, entropy, zero),) if case["entropy"] else out
+        return (torch.where(has, logp, zero), torch.where(has, entropy, zero)) if case["entropy"] else torch.where(has, logp, zero)
 
     def gradient(dlogp, dentropy=None):
         """Through log p(target) and the entropy to the logits."""
@@ -396,8 +391,8 @@ def work(case):
     N, V, size = rows_of(case), case["V"], 4 if case["dtype"] == "float32" else 2
     live = N - masked_of(case)
     if case["op"] == "logprobs":      # a scale, an exponential, a sum
-        return {"bytes": live * V * size + 4 * N * (4 if case["entropy"] else 3), "flops": (5 if case["entropy"] else 3) * live * V}
+        return {"bytes": live * V * size + 4 * N * (3 if case["entropy"] else 2), "flops": (5 if case["entropy"] else 3) * live * V}
     if case["op"] == "gradient":
-        return {"bytes": (live + N) * V * size + 4 * N * (5 if case["entropy"] else 3), "flops": (7 if case["entropy"] else 4) * live * V}
+        return {"bytes": (live + N) * V * size + 4 * N * (3 if case["entropy"] else 2), "flops": (9 if case["entropy"] else 6) * live * V}
     rows = 4 * N * (5 + (1 if case["kl"] else 0) + (1 if case["reduction"] == "sum" else 0))
     return {"bytes": (live + (N if case["gradient"] else 0)) * V * size + rows, "flops": (7 if case["gradient"] else 3) * live * V}
