@@ -62,6 +62,15 @@ class DecoderTensorC(C.Structure):
     _fields_ = [("name", C.c_char * 48), ("offset", C.c_int64), ("rows", C.c_int64), ("cols", C.c_int64)]
 
 
+class PolicyConfigC(C.Structure):
+    _fields_ = [("temperature", C.c_float), ("clip_low", C.c_float), ("clip_high", C.c_float), ("kl_coef", C.c_float), ("reduction", C.c_int32)]
+
+
+class PreferenceConfigC(C.Structure):
+    _fields_ = [("kind", C.c_int32), ("beta", C.c_float), ("margin", C.c_float), ("label_smoothing", C.c_float), ("length_normalised", C.c_int32),
+                ("reduction", C.c_int32)]
+
+
 class FemtoError(RuntimeError):
     def __init__(self, code, msg):
         super().__init__(f"libfemto error {code}: {msg}")
@@ -140,6 +149,10 @@ SIGNATURES = {
     "femto_rmsnorm_bwd": (I32, [I32, P, P, P, P, I32, I32, P]),
     "femto_embed_gather": (I32, [I32, P, P, P, I32, I32, I32, P]),
     "femto_muon_direction": (I32, [I32, P, P, P, P, I32, I32, I32, F, F, F, C.POINTER(F), I32, P]),
+    "femto_token_logprobs": (I32, [I32, P, I64, P, I32, I32, F, P, P, P]),
+    "femto_token_logprobs_gradient": (I32, [I32, P, I64, P, I64, P, I32, I32, F, P, P, P]),
+    "femto_policy_loss": (I32, [I32, P, I64, P, I32, I32, P, P, P, P, C.POINTER(PolicyConfigC), P, I64, P, P, P, P, P, P]),
+    "femto_preference_loss": (I32, [P, P, P, I32, P, I32, C.POINTER(PreferenceConfigC), P, P, P, P, P]),
     "femto_status_word": (I32, [P, C.POINTER(I32)]),
     "femto_sync": (I32, [P, P]),
     "femto_launch_count": (I64, [P]),

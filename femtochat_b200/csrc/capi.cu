@@ -79,6 +79,7 @@ static int standalone_finish(int rc, unsigned int* status, cudaStream_t s) {
   return 0;
 }
 unsigned int static_entry_status_word();   // attention_static.cu: status of the allocation-free entry point
+unsigned int objectives_status_word();     // objectives.cu
 
 static int require_device() {
   int n = 0;
@@ -573,7 +574,7 @@ int32_t femto_status_word(femto_handle* h, int32_t* out) {
       CUDA_TRY(cudaMemcpy(&v, g_sa_status[dev], sizeof(v), cudaMemcpyDeviceToHost));
       if (v) CUDA_TRY(cudaMemset(g_sa_status[dev], 0, sizeof(v)));   // read and clear
     }
-    *out = (int32_t)(v | static_entry_status_word());
+    *out = (int32_t)(v | static_entry_status_word() | objectives_status_word());
     return 0;
   }
   CUDA_TRY(cudaMemcpy(&v, h->status, sizeof(v), cudaMemcpyDeviceToHost));

@@ -42,6 +42,7 @@ extern long long g_femto_launches;  // host counter of kernel launches issued by
 #define ST_BAD_TOKEN 1u      // token / target / position out of range (clamped, flagged)
 #define ST_WAIT_TIMEOUT 2u   // a bounded mbarrier wait ran out
 #define ST_NONFINITE 4u
+#define ST_BAD_RANGE 8u      // a run of rows that leaves the array or ends before it starts (taken as empty, flagged)
 
 // ---- dtype helpers ----------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ float to_f(T v);

@@ -1,0 +1,416 @@
+// Objectives on a model's own answers: log-probabilities of chosen tokens with their entropy and the gradient of both, the clipped policy
+// loss with a KL term on logits, the paired preference loss on log-probabilities.  Every call is asynchronous, keeps no scratch of its own
+// (what is carried from one kernel to the next lies in the caller's outputs) and sums in a fixed order.
+#include <math.h>
+
+#include <algorithm>
+
+#include "objectives.cuh"
+
+namespace {
+// Bit 1: a target outside the vocabulary (its row counts as one without a target); bit 8: offsets that do not ascend inside the rows (the
+// answer counts as empty).  Part of the library image, so that no call allocates; femto_status_word(NULL, ..) reads and clears it.
+__device__ unsigned int g_objectives_status = 0;
+
+// The row's target, or -1 where it has none.
+__device__ __forceinline__ int checked_target(const int* tgt0, long long row, int V) {
+  int t = tgt0[row];
+  if (t >= V) { if (threadIdx.x == 0) atomicOr(&g_objectives_status, ST_BAD_TOKEN); t = -1; }
+  return t < 0 ? -1 : t;
+}
+
+// Statistics of one row by the whole block, the same in every thread.
+template <typename T, bool ENTROPY> __device__ RowStats row_stats(const T* z, int V, float c) {
+  __shared__ RowStats part[8];
+  RowStats s;
+  for (int v = threadIdx.x; v < V; v += 256) {
+    const float x = to_f<T>(z[v]);
+    if (x > s.m) rebase<ENTROPY>(s, x, c);
+    const float u = (x - finite_or_zero(s.m)) * c, e = exp2_fast(u);
+    s.l += e;
+    if (ENTROPY) s.a = fmaf(e, fmaxf(u, LEAST_U), s.a);
+  }
+  for (int o = 16; o > 0; o >>= 1) {
+    RowStats y;
+    y.m = __shfl_xor_sync(0xffffffffu, s.m, o);
+    y.l = __shfl_xor_sync(0xffffffffu, s.l, o);
+    y.a = __shfl_xor_sync(0xffffffffu, s.a, o);
+    s = merged<ENTROPY>(s, y, c);
+  }
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+  __syncthreads();
+  s = part[0];
+  for (int i = 1; i < 8; i++) s = merged<ENTROPY>(s, part[i], c);
+  return s;
+}
+
+template <typename T, bool ENTROPY>
+__global__ void __launch_bounds__(256) k_token_logprobs(const T* __restrict__ logits, long long ldl, const int* __restrict__ tgt0, int V, float c,
+                                                        float* __restrict__ logp, float* __restrict__ ent) {
+  pdl_trigger();
+  const long long row = blockIdx.x;
+  const int t = checked_target(tgt0, row, V);
+  if (t < 0) {
+    if (threadIdx.x == 0) {
+      logp[row] = 0.f;
+      if (ENTROPY) ent[row] = 0.f;
+    }
+    return;
+  }
+  const T* z = logits + row * ldl;
+  const RowStats s = row_stats<T, ENTROPY>(z, V, c);
+  if (threadIdx.x == 0) {
+    logp[row] = log_prob(s, to_f<T>(z[t]), c);
+    if (ENTROPY) ent[row] = entropy(s);
+  }
+}
+
+// dz_j = (1/tau) (dlp (1[j = t] - p_j) - dH p_j (log p_j + H)), in place where dlogits is logits.
+template <typename T, bool ENTROPY>
+__global__ void __launch_bounds__(256) k_token_logprobs_gradient(T* dlogits, long long ldd, const T* logits, long long ldl, const int* __restrict__ tgt0,
+                                                                 int V, float c, float inv_t, const float* __restrict__ dlogp,
+                                                                 const float* __restrict__ dent) {
+  pdl_trigger();
+  const long long row = blockIdx.x;
+  const int t = checked_target(tgt0, row, V);
+  const T* z = logits + row * ldl;
+  T* d = dlogits + row * ldd;
+  RowStats s;
+  if (t >= 0) s = row_stats<T, ENTROPY>(z, V, c);
+  if (s.l == 0.f) {      // no target, or no distribution
+    for (int v = threadIdx.x; v < V; v += 256) d[v] = from_f<T>(0.f);
+    return;
+  }
+  const float g = dlogp[row] * inv_t, inv_l = 1.f / s.l;
+  // log p + H = ln2 (u - a / l)
+  const float h = ENTROPY ? dent[row] * inv_t * (float)LN2 : 0.f, mean_u = ENTROPY ? s.a / s.l : 0.f;
+  for (int v = threadIdx.x; v < V; v += 256) {
+    const float u = (to_f<T>(z[v]) - s.m) * c, p = exp2_fast(u) * inv_l;
+    const float k = ENTROPY ? fmaf(h, fmaxf(u, LEAST_U) - mean_u, g) : g;
+    d[v] = from_f<T>((v == t ? g : 0.f) - k * p);
+  }
+}
+
+struct PolicyRows {
+  const int* tgt0;
+  const float *old, *ref, *adv, *w;
+  float *token_losses, *logp;
+  const int* n_valid;      // mean: the slopes are divided by it
+  PolicyTerm term;
+};
+__device__ __forceinline__ float policy_scale(const int* n_valid) { return n_valid ? 1.f / (float)n_valid[0] : 1.f; }
+
+template <typename T, bool GRADIENT>
+__global__ void __launch_bounds__(256) k_policy_rows(const T* logits, long long ldl, T* dlogits, long long ldd, int V, float c, float inv_t,
+                                                     const PolicyRows p) {
+  pdl_trigger();
+  __shared__ float slope_s;
+  const long long row = blockIdx.x;
+  const int t = checked_target(p.tgt0, row, V);
+  const T* z = logits + row * ldl;
+  T* d = dlogits + row * ldd;
+  if (t < 0) {
+    if (threadIdx.x == 0) p.token_losses[row] = p.logp[row] = 0.f;
+    if (GRADIENT) for (int v = threadIdx.x; v < V; v += 256) d[v] = from_f<T>(0.f);
+    return;
+  }
+  const RowStats s = row_stats<T, false>(z, V, c);
+  if (threadIdx.x == 0) {
+    const float lp = log_prob(s, to_f<T>(z[t]), c);
+    float loss, slope;
+    policy_token(p.term, lp, p.old[row], p.adv[row], p.term.kl != 0.f ? p.ref[row] : 0.f, p.w ? p.w[row] : 1.f, &loss, &slope);
+    p.token_losses[row] = loss;
+    p.logp[row] = lp;
+    slope_s = slope * policy_scale(p.n_valid) * inv_t;
+  }
+  if (!GRADIENT) return;
+  __syncthreads();
+  const float g = slope_s, inv_l = 1.f / s.l;
+  for (int v = threadIdx.x; v < V; v += 256) {
+    const float pj = exp2_fast((to_f<T>(z[v]) - s.m) * c) * inv_l;
+    d[v] = from_f<T>(s.l == 0.f ? 0.f : g * ((v == t ? 1.f : 0.f) - pj));
+  }
+}
+
+// One value for the whole block of 1024 threads: fixed tree.
+template <typename S> __device__ S block_total(S v) {
+  __shared__ S red[32];
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = red[threadIdx.x & 31];
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+__global__ void __launch_bounds__(1024) k_count_targets(const int* __restrict__ tgt0, int N, int V, int* __restrict__ out) {
+  pdl_trigger();
+  int n = 0;
+  for (long long i = threadIdx.x; i < N; i += 1024) n += tgt0[i] >= 0 && tgt0[i] < V;
+  n = block_total(n);
+  if (threadIdx.x == 0) *out = n;
+}
+
+// Sum (or mean over the rows with a target) of the token losses, and how many tokens the clipping held.
+__global__ void __launch_bounds__(1024) k_policy_sum(const PolicyRows p, int N, int V, int mean, float* __restrict__ loss_out, int* __restrict__ n_valid_out,
+                                                     int* __restrict__ n_clipped_out) {
+  pdl_trigger();
+  float sum = 0.f;
+  int n = 0, clipped = 0;
+  for (long long i = threadIdx.x; i < N; i += 1024) {
+    const int t = p.tgt0[i];
+    if (t < 0 || t >= V) continue;
+    n++;
+    sum += p.token_losses[i];
+    if (n_clipped_out && policy_clipped(p.term, policy_ratio(p.logp[i], p.old[i]), p.adv[i])) clipped++;
+  }
+  sum = block_total(sum);
+  n = block_total(n);
+  clipped = block_total(clipped);
+  if (threadIdx.x == 0) {
+    *loss_out = mean && n > 0 ? sum / (float)n : sum;
+    *n_valid_out = n;
+    if (n_clipped_out) *n_clipped_out = clipped;
+  }
+}
+
+// ---- paired preference loss ---------------------------------------------------------------------------------------------------------------
+struct Preference {
+  const float *logp, *ref;
+  const int *tgt0, *offsets;
+  int N, P, kind, normalised;
+  float beta, margin, smoothing, scale;      // scale: of the slopes (1 / P for the mean)
+  float *pair_losses, *ratios, *dlogp;
+};
+
+// The rows of one answer; offsets that leave the rows or descend make it empty.
+__device__ __forceinline__ int2 answer_rows(const Preference& p, int answer) {
+  const int a = p.offsets[answer], b = p.offsets[answer + 1];
+  if (a >= 0 && a <= b && b <= p.N) return make_int2(a, b);
+  if (threadIdx.x == 0) atomicOr(&g_objectives_status, ST_BAD_RANGE);
+  return make_int2(0, 0);
+}
+
+// One block per pair.  Sums of log ratios of two long answers nearly cancel: they are held in 64 bits.
+__global__ void __launch_bounds__(1024) k_preference_pairs(const Preference p) {
+  pdl_trigger();
+  __shared__ float slope_s[2];
+  const int pair = blockIdx.x;
+  int2 rows[2];
+  double rho[2];
+  int count[2];
+  for (int side = 0; side < 2; side++) {
+    rows[side] = answer_rows(p, 2 * pair + side);
+    double sum = 0.0;
+    int n = 0;
+    for (int i = rows[side].x + threadIdx.x; i < rows[side].y; i += 1024) {
+      if (p.tgt0 && p.tgt0[i] < 0) continue;
+      n++;
+      sum += (double)(p.ref ? p.logp[i] - p.ref[i] : p.logp[i]);
+    }
+    rho[side] = block_total(sum);
+    count[side] = block_total(n);
+  }
+  if (threadIdx.x == 0) {
+    double per[2];
+    for (int side = 0; side < 2; side++) {
+      per[side] = p.normalised ? 1.0 / max(count[side], 1) : 1.0;
+      rho[side] *= per[side];
+      p.ratios[2 * pair + side] = (float)rho[side];
+    }
+    const double delta = rho[0] - rho[1], beta = p.beta;
+    double loss, slope;      // slope: by delta
+    if (p.kind == FEMTO_PREFERENCE_SIGMOID) {
+      // -(1 - e) log sigma(h) - e log sigma(-h), with log(1 + e^-|h|) once
+      const double h = beta * delta - (double)p.margin, e = p.smoothing, q = exp(-fabs(h)), s = log1p(q);
+      loss = s + (1.0 - e) * fmax(-h, 0.0) + e * fmax(h, 0.0);
+      slope = beta * ((h >= 0.0 ? 1.0 / (1.0 + q) : q / (1.0 + q)) - (1.0 - e));
+    } else {
+      const double u = delta - 0.5 / beta;
+      loss = u * u;
+      slope = 2.0 * u;
+    }
+    p.pair_losses[pair] = (float)loss;
+    slope *= (double)p.scale;
+    slope_s[0] = (float)(slope * per[0]);
+    slope_s[1] = (float)(-slope * per[1]);
+  }
+  if (!p.dlogp) return;
+  __syncthreads();
+  for (int side = 0; side < 2; side++)
+    for (int i = rows[side].x + threadIdx.x; i < rows[side].y; i += 1024) p.dlogp[i] = p.tgt0 && p.tgt0[i] < 0 ? 0.f : slope_s[side];
+}
+
+// Sum or mean over the pairs, and zeros as the gradient of rows that belong to no answer.
+__global__ void __launch_bounds__(1024) k_preference_sum(const Preference p, int mean, float* __restrict__ loss_out) {
+  pdl_trigger();
+  if (blockIdx.x == 0) {
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < p.P; i += 1024) sum += (double)p.pair_losses[i];
+    sum = block_total(sum);
+    if (threadIdx.x == 0) *loss_out = (float)(mean && p.P > 0 ? sum / p.P : sum);
+  }
+  if (!p.dlogp) return;
+  const int first = p.P > 0 ? min(max(p.offsets[0], 0), p.N) : p.N, last = p.P > 0 ? min(max(p.offsets[2 * p.P], 0), p.N) : p.N;
+  const long long step = (long long)gridDim.x * 1024;
+  for (long long i = blockIdx.x * 1024ll + threadIdx.x; i < first; i += step) p.dlogp[i] = 0.f;
+  for (long long i = last + blockIdx.x * 1024ll + threadIdx.x; i < p.N; i += step) p.dlogp[i] = 0.f;
+}
+}  // namespace
+
+// Status word of these entry points on the current device; reading clears it.
+unsigned int objectives_status_word() {
+  unsigned int w = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&w, g_objectives_status, sizeof(w)) != cudaSuccess) return 0;
+  if (w) cudaMemcpyToSymbol(g_objectives_status, &zero, sizeof(zero));
+  return w;
+}
+
+// ---- checks of arguments ------------------------------------------------------------------------------------------------------------------
+namespace {
+int check_dtype(int dtype) {
+  return dtype == FEMTO_F32 || dtype == FEMTO_BF16 ? 0 : femto_fail(FEMTO_ERR_ARG, "dtype must be FEMTO_F32 or FEMTO_BF16");
+}
+int check_rows(int dtype, const void* logits, long long ldl, const int* tgt0, int N, int V) {
+  FEMTO_TRY(check_dtype(dtype));
+  if (N < 0 || V <= 0) return femto_fail(FEMTO_ERR_SHAPE, "N = %d rows of V = %d logits", N, V);
+  if (ldl < V) return femto_fail(FEMTO_ERR_SHAPE, "ldl = %lld is less than V = %d", ldl, V);
+  if (N > 0 && (!logits || !tgt0)) return femto_fail(FEMTO_ERR_ARG, "NULL argument");
+  const uintptr_t size = dtype == FEMTO_BF16 ? 2 : 4;
+  if (reinterpret_cast<uintptr_t>(logits) % size) return femto_fail(FEMTO_ERR_ALIGN, "logits are not aligned to their type");
+  return 0;
+}
+// The gradient lies apart from the logits, or in their place.
+int check_gradient(int dtype, const void* dlogits, long long ldd, const void* logits, long long ldl, int N, int V) {
+  if (ldd < V) return femto_fail(FEMTO_ERR_SHAPE, "ldd = %lld is less than V = %d", ldd, V);
+  const uintptr_t size = dtype == FEMTO_BF16 ? 2 : 4, a = reinterpret_cast<uintptr_t>(dlogits), b = reinterpret_cast<uintptr_t>(logits);
+  if (a % size) return femto_fail(FEMTO_ERR_ALIGN, "dlogits are not aligned to their type");
+  if (N == 0 || (a == b && ldd == ldl)) return 0;
+  const uintptr_t a_end = a + size * ((uintptr_t)(N - 1) * ldd + V), b_end = b + size * ((uintptr_t)(N - 1) * ldl + V);
+  if (a < b_end && b < a_end) return femto_fail(FEMTO_ERR_ARG, "dlogits overlap the logits: give the same rows and pitch, or memory of their own");
+  return 0;
+}
+int check_temperature(float t) {
+  return t > 0.f && isfinite(t) ? 0 : femto_fail(FEMTO_ERR_ARG, "temperature must be positive and finite");
+}
+float log2e_over(float temperature) { return (float)(1.4426950408889634074 / (double)temperature); }
+
+template <typename T>
+int token_logprobs(const void* logits, long long ldl, const int* tgt0, int N, int V, float temperature, float* logp, float* ent, cudaStream_t s) {
+  const float c = log2e_over(temperature);
+  if (ent) k_token_logprobs<T, true><<<N, 256, 0, s>>>((const T*)logits, ldl, tgt0, V, c, logp, ent);
+  else k_token_logprobs<T, false><<<N, 256, 0, s>>>((const T*)logits, ldl, tgt0, V, c, logp, ent);
+  KERNEL_CHECK();
+  return 0;
+}
+template <typename T>
+int token_logprobs_gradient(void* dlogits, long long ldd, const void* logits, long long ldl, const int* tgt0, int N, int V, float temperature, const float* dlogp,
+                            const float* dent, cudaStream_t s) {
+  const float c = log2e_over(temperature), inv = 1.f / temperature;
+  if (dent) k_token_logprobs_gradient<T, true><<<N, 256, 0, s>>>((T*)dlogits, ldd, (const T*)logits, ldl, tgt0, V, c, inv, dlogp, dent);
+  else k_token_logprobs_gradient<T, false><<<N, 256, 0, s>>>((T*)dlogits, ldd, (const T*)logits, ldl, tgt0, V, c, inv, dlogp, dent);
+  KERNEL_CHECK();
+  return 0;
+}
+template <typename T>
+int policy_rows(const void* logits, long long ldl, void* dlogits, long long ldd, int N, int V, float temperature, const PolicyRows& p, cudaStream_t s) {
+  const float c = log2e_over(temperature), inv = 1.f / temperature;
+  if (dlogits) k_policy_rows<T, true><<<N, 256, 0, s>>>((const T*)logits, ldl, (T*)dlogits, ldd, V, c, inv, p);
+  else k_policy_rows<T, false><<<N, 256, 0, s>>>((const T*)logits, ldl, nullptr, 0, V, c, inv, p);
+  KERNEL_CHECK();
+  return 0;
+}
+}  // namespace
+
+extern "C" int32_t femto_token_logprobs(int32_t dtype, const void* logits, int64_t ldl, const int32_t* targets0, int32_t N, int32_t V, float temperature,
+                                        float* logp, float* entropy_out, void* stream) {
+  FEMTO_TRY(check_rows(dtype, logits, ldl, targets0, N, V));
+  FEMTO_TRY(check_temperature(temperature));
+  if (N == 0) return 0;
+  if (!logp) return femto_fail(FEMTO_ERR_ARG, "NULL argument");
+  cudaStream_t s = (cudaStream_t)stream;
+  return dtype == FEMTO_BF16 ? token_logprobs<bf16>(logits, ldl, targets0, N, V, temperature, logp, entropy_out, s)
+                             : token_logprobs<float>(logits, ldl, targets0, N, V, temperature, logp, entropy_out, s);
+}
+
+extern "C" int32_t femto_token_logprobs_gradient(int32_t dtype, void* dlogits, int64_t ldd, const void* logits, int64_t ldl, const int32_t* targets0, int32_t N,
+                                                 int32_t V, float temperature, const float* dlogp, const float* dentropy, void* stream) {
+  FEMTO_TRY(check_rows(dtype, logits, ldl, targets0, N, V));
+  FEMTO_TRY(check_temperature(temperature));
+  FEMTO_TRY(check_gradient(dtype, dlogits, ldd, logits, ldl, N, V));
+  if (N == 0) return 0;
+  if (!dlogits || !dlogp) return femto_fail(FEMTO_ERR_ARG, "NULL argument");
+  cudaStream_t s = (cudaStream_t)stream;
+  return dtype == FEMTO_BF16
+             ? token_logprobs_gradient<bf16>(dlogits, ldd, logits, ldl, targets0, N, V, temperature, dlogp, dentropy, s)
+             : token_logprobs_gradient<float>(dlogits, ldd, logits, ldl, targets0, N, V, temperature, dlogp, dentropy, s);
+}
+
+int check_policy(const femto_policy_config* c, const float* ref_logp) {
+  if (!c) return femto_fail(FEMTO_ERR_ARG, "NULL configuration");
+  FEMTO_TRY(check_temperature(c->temperature));
+  if (!(c->clip_low >= 0.f && c->clip_low <= 1.f) || !(c->clip_high >= 0.f))
+    return femto_fail(FEMTO_ERR_ARG, "clip_low must lie in 0..1 and clip_high be 0 or more");
+  if (!(c->kl_coef >= 0.f) || !isfinite(c->kl_coef)) return femto_fail(FEMTO_ERR_ARG, "kl_coef must be 0 or more, and finite");
+  if (c->kl_coef > 0.f && !ref_logp) return femto_fail(FEMTO_ERR_ARG, "kl_coef needs ref_logp");
+  if (c->reduction != FEMTO_REDUCTION_SUM && c->reduction != FEMTO_REDUCTION_MEAN)
+    return femto_fail(FEMTO_ERR_ARG, "reduction must be FEMTO_REDUCTION_SUM or FEMTO_REDUCTION_MEAN");
+  return 0;
+}
+
+extern "C" int32_t femto_policy_loss(int32_t dtype, const void* logits, int64_t ldl, const int32_t* targets0, int32_t N, int32_t V, const float* old_logp,
+                                     const float* advantages, const float* ref_logp, const float* weights, const femto_policy_config* h_cfg, void* dlogits,
+                                     int64_t ldd, float* token_losses, float* logp, float* loss_out, int32_t* n_valid_out, int32_t* n_clipped_out,
+                                     void* stream) {
+  FEMTO_TRY(check_rows(dtype, logits, ldl, targets0, N, V));
+  FEMTO_TRY(check_policy(h_cfg, N > 0 ? ref_logp : h_cfg ? &h_cfg->kl_coef : nullptr));
+  if (dlogits) FEMTO_TRY(check_gradient(dtype, dlogits, ldd, logits, ldl, N, V));
+  if (!loss_out || !n_valid_out || (N > 0 && (!old_logp || !advantages || !token_losses || !logp))) return femto_fail(FEMTO_ERR_ARG, "NULL argument");
+  cudaStream_t s = (cudaStream_t)stream;
+  const bool mean = h_cfg->reduction == FEMTO_REDUCTION_MEAN;
+  PolicyRows p = {targets0, old_logp, ref_logp, advantages, weights, token_losses, logp, mean ? n_valid_out : nullptr,
+                  {1.f - h_cfg->clip_low, 1.f + h_cfg->clip_high, h_cfg->kl_coef}};
+  if (N > 0) {
+    if (mean && dlogits) { k_count_targets<<<1, 1024, 0, s>>>(targets0, N, V, n_valid_out); KERNEL_CHECK(); }
+    else p.n_valid = nullptr;
+    FEMTO_TRY(dtype == FEMTO_BF16 ? policy_rows<bf16>(logits, ldl, dlogits, ldd, N, V, h_cfg->temperature, p, s)
+                                  : policy_rows<float>(logits, ldl, dlogits, ldd, N, V, h_cfg->temperature, p, s));
+  }
+  k_policy_sum<<<1, 1024, 0, s>>>(p, N, V, mean, loss_out, n_valid_out, n_clipped_out);
+  KERNEL_CHECK();
+  return 0;
+}
+
+int check_preference(const femto_preference_config* c) {
+  if (!c) return femto_fail(FEMTO_ERR_ARG, "NULL configuration");
+  if (c->kind != FEMTO_PREFERENCE_SIGMOID && c->kind != FEMTO_PREFERENCE_SQUARED)
+    return femto_fail(FEMTO_ERR_ARG, "kind must be FEMTO_PREFERENCE_SIGMOID or FEMTO_PREFERENCE_SQUARED");
+  if (!(c->beta > 0.f) || !isfinite(c->beta)) return femto_fail(FEMTO_ERR_ARG, "beta must be positive and finite");
+  if (!isfinite(c->margin) || !(c->label_smoothing >= 0.f && c->label_smoothing <= 1.f))
+    return femto_fail(FEMTO_ERR_ARG, "the margin must be finite and label_smoothing lie in 0..1");
+  if (c->kind == FEMTO_PREFERENCE_SQUARED && (c->margin != 0.f || c->label_smoothing != 0.f))
+    return femto_fail(FEMTO_ERR_ARG, "the squared loss has no margin and no label smoothing");
+  if (c->reduction != FEMTO_REDUCTION_SUM && c->reduction != FEMTO_REDUCTION_MEAN)
+    return femto_fail(FEMTO_ERR_ARG, "reduction must be FEMTO_REDUCTION_SUM or FEMTO_REDUCTION_MEAN");
+  return 0;
+}
+
+extern "C" int32_t femto_preference_loss(const float* logp, const float* ref_logp, const int32_t* targets0, int32_t N, const int32_t* offsets, int32_t P,
+                                         const femto_preference_config* h_cfg, float* loss_out, float* pair_losses, float* ratios, float* dlogp,
+                                         void* stream) {
+  FEMTO_TRY(check_preference(h_cfg));
+  if (N < 0 || P < 0 || P > (1 << 29)) return femto_fail(FEMTO_ERR_SHAPE, "P = %d pairs of answers in N = %d rows", P, N);
+  if (!loss_out || (N > 0 && !logp) || (P > 0 && (!offsets || !pair_losses || !ratios))) return femto_fail(FEMTO_ERR_ARG, "NULL argument");
+  cudaStream_t s = (cudaStream_t)stream;
+  const bool mean = h_cfg->reduction == FEMTO_REDUCTION_MEAN;
+  const Preference p = {logp, ref_logp, targets0, offsets, N, P, h_cfg->kind, h_cfg->length_normalised != 0, h_cfg->beta, h_cfg->margin,
+                        h_cfg->label_smoothing, mean && P > 0 ? 1.f / (float)P : 1.f, pair_losses, ratios, dlogp};
+  if (P > 0) {
+    k_preference_pairs<<<P, 1024, 0, s>>>(p);
+    KERNEL_CHECK();
+  }
+  k_preference_sum<<<dlogp ? std::min(cdiv(N, 4096) + 1, 148) : 1, 1024, 0, s>>>(p, mean, loss_out);
+  KERNEL_CHECK();
+  return 0;
+}

@@ -1,0 +1,83 @@
+// Arithmetic that the objectives on a model's own answers share: the softmax statistics of a row of logits, the clipped policy term of a
+// token, the paired preference term (objectives.cu), also used behind the lm_head tail of a training step (xent.cu).
+#pragma once
+#include "common.cuh"
+
+// Softmax statistics of a row.  With c = log2(e) / temperature, m = max(z) and u_j = c (z_j - m) <= 0:
+//   l = sum 2^u_j,  a = sum 2^u_j u_j,  log p_j = ln2 u_j - ln l,  H = ln l - ln2 a / l.
+// The difference comes before the product: logits of the type's lowest value stay finite, and a large common offset costs nothing.
+struct RowStats {
+  float m = -INFINITY, l = 0.f, a = 0.f;
+};
+
+#ifdef __CUDACC__
+constexpr double LN2 = 0.69314718055994530942;
+constexpr float LEAST_U = -200.f;      // 2^u is 0 there, and u stays finite beside it
+
+__device__ __forceinline__ float exp2_fast(float x) {   // relative error 2^-22, 0 for -inf
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// What a maximum of -inf (nothing seen, or a row without any logit above -inf) is taken as: -inf - 0 gives 2^-inf = 0, where -inf + inf is NaN.
+__device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
+
+// Moves statistics to a maximum that is no lower: with d = c (m_old - m_new) every 2^u scales by 2^d and every u moves by d.
+template <bool ENTROPY> __device__ __forceinline__ void rebase(RowStats& s, float m, float c) {
+  if (s.l != 0.f) {
+    const float d = fmaxf((s.m - m) * c, LEAST_U), f = exp2_fast(d);
+    if (ENTROPY) s.a = f * fmaf(s.l, d, s.a);
+    s.l *= f;
+  }
+  s.m = m;
+}
+template <bool ENTROPY> __device__ __forceinline__ RowStats merged(RowStats x, RowStats y, float c) {
+  const float m = fmaxf(x.m, y.m);
+  rebase<ENTROPY>(x, m, c);
+  rebase<ENTROPY>(y, m, c);
+  x.l += y.l;
+  if (ENTROPY) x.a += y.a;
+  return x;
+}
+// l = 2^k f with f in [0.7, 1.4]: log l is k ln2 (in 64 bits) + log f, a small number.  log(l) in one piece has an error of 5e-7 at
+// l = 65536, and so has every log-probability then.
+__device__ __forceinline__ double log_sum(float l) {
+  if (!(l > 0.f && l < INFINITY)) return (double)logf(l);
+  int k;
+  float f = frexpf(l, &k);
+  if (f < 0.70710678f) { f *= 2.f; k--; }
+  return LN2 * k + (double)logf(f);
+}
+// log p of a logit z; a row without any logit above -inf (l = 0) has no distribution: -inf.
+__device__ __forceinline__ float log_prob(const RowStats& s, float z, float c) {
+  if (s.l == 0.f) return -INFINITY;
+  return (float)(LN2 * c * ((double)z - (double)s.m) - log_sum(s.l));
+}
+__device__ __forceinline__ float entropy(const RowStats& s) {
+  return s.l == 0.f ? 0.f : (float)(log_sum(s.l) - LN2 * (double)s.a / (double)s.l);
+}
+
+// ---- clipped policy term of one token ---------------------------------------------------------------------------------------------------
+// loss = w (-min(r A, clamp(r, lo, hi) A) + beta (e^g - g - 1)),  r = e^(lp - old),  g = ref - lp, and its derivative by lp.  The minimum is
+// the bounded product, which does not depend on lp, where A > 0 and r > hi or A < 0 and r < lo.  A weight of 0 counts nothing, whatever
+// the other numbers are.
+struct PolicyTerm {
+  float lo, hi, kl;
+};
+__device__ __forceinline__ bool policy_clipped(const PolicyTerm& t, float r, float A) { return (A > 0.f && r > t.hi) || (A < 0.f && r < t.lo); }
+__device__ __forceinline__ float policy_ratio(float lp, float old) { return expf(lp - old); }
+__device__ __forceinline__ void policy_token(const PolicyTerm& t, float lp, float old, float A, float ref, float w, float* loss, float* slope) {
+  if (w == 0.f) { *loss = *slope = 0.f; return; }
+  const float r = policy_ratio(lp, old);
+  const float gain = A == 0.f ? 0.f : r * A;      // r may be inf
+  const bool clipped = policy_clipped(t, r, A);
+  float l = clipped ? -(A > 0.f ? t.hi : t.lo) * A : -gain, d = clipped ? 0.f : -gain;
+  if (t.kl != 0.f) {
+    const float g = ref - lp, e = expm1f(g);
+    l += t.kl * (e - g);
+    d -= t.kl * e;
+  }
+  *loss = w * l;
+  *slope = w * d;
+}
+#endif

@@ -1,0 +1,207 @@
+"""Objectives on a model's own answers (femto_token_logprobs*, femto_policy_loss, femto_preference_loss): what a host calls after
+pretraining, when answers have rewards or come in pairs.  No counterpart in the reference.  Every call is asynchronous on the current
+stream and returns device tensors; nothing is read back, so a call may be captured into a graph.
+
+Logits are [..., V] with unit stride along V and one pitch between rows, as `GPT.logits` and `decode_step` give them, or cut from a wider
+buffer; float32 or bfloat16.  Targets are 0-based here (`targets0`; the model's own ids may start at 1), negative where a row counts for
+nothing.  Arrays of one number per token have the logits' leading shape and are float32."""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from typing import NamedTuple, Optional
+
+from . import _lib
+
+PREFERENCES = {"sigmoid": 0, "squared": 1}
+
+
+class TokenLogprobs(NamedTuple):
+    logp: object
+    entropy: Optional[object]
+
+
+class PolicyLoss(NamedTuple):
+    loss: object            # [1]
+    n_valid: object         # [1] int32, tokens with a target
+    n_clipped: object       # [1] int32, those that the clipping held
+    token_losses: object
+    logp: object
+    dlogits: Optional[object]
+
+
+class PreferenceLoss(NamedTuple):
+    loss: object            # [1]
+    pair_losses: object     # [P]
+    ratios: object          # [2 P]: rho of the chosen and the rejected answer in turn
+    dlogp: Optional[object]
+
+
+def _on_device(name, t, dtype, shape, device):
+    """A contiguous array of `shape` on `device`, or an error that names it."""
+    if t is None:
+        return None
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the logits on {device}")
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _rows(name, t):
+    """(rows, V, pitch) of [..., V] logits whose rows lie one pitch apart."""
+    import torch
+    if t.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"{name} must be float32 or bfloat16, not {t.dtype}")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be on a CUDA device")
+    if t.dim() < 1 or t.shape[-1] == 0:
+        raise ValueError(f"{name} must be [..., V]")
+    V, n = t.shape[-1], t.numel() // t.shape[-1]
+    if n == 0:
+        return 0, V, V
+    if n >= 1 << 31 or V >= 1 << 31:
+        raise ValueError(f"{name}: {n} rows of {V}")
+    if V > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name} must have unit stride along the vocabulary")
+    pitch, reach = None, 1
+    for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if size == 1:
+            continue
+        if pitch is None:
+            pitch = stride
+        elif stride != pitch * reach:
+            raise ValueError(f"the rows of {name} must lie one pitch apart")
+        reach *= size
+    if pitch is None:
+        pitch = V
+    if pitch < V:
+        raise ValueError(f"the rows of {name} overlap")
+    return n, V, pitch
+
+
+def _code(t):
+    import torch
+    return _lib.BF16 if t.dtype == torch.bfloat16 else _lib.F32
+
+
+def _gradient_of(logits, out):
+    """The tensor that takes the gradient, and its pitch."""
+    import torch
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
+        raise ValueError("out must have the logits' shape, type and device")
+    return out, _rows("out", out)[2]
+
+
+class _Device:
+    """Makes the tensors' device the current one where it is not."""
+
+    def __init__(self, device):
+        import torch
+        self.other = torch.cuda.device(device) if device.index != torch.cuda.current_device() else None
+
+    def __enter__(self):
+        if self.other is not None:
+            self.other.__enter__()
+
+    def __exit__(self, *exc):
+        if self.other is not None:
+            self.other.__exit__(*exc)
+
+
+def token_logprobs(logits, targets0, temperature: float = 1.0, entropy: bool = False) -> TokenLogprobs:
+    """Log-probabilities of the targets under softmax(logits / temperature), and the entropy where asked for."""
+    import torch
+    n, V, pitch = _rows("logits", logits)
+    shape = logits.shape[:-1]
+    targets0 = _on_device("targets0", targets0, torch.int32, shape, logits.device)
+    logp = torch.empty(shape, dtype=torch.float32, device=logits.device)
+    ent = torch.empty(shape, dtype=torch.float32, device=logits.device) if entropy else None
+    with _Device(logits.device):
+        _lib.check(_lib.lib().femto_token_logprobs(_code(logits), _lib.ptr(logits), pitch, _lib.ptr(targets0), n, V, temperature, _lib.ptr(logp),
+                                                   _lib.ptr(ent), _lib.stream_ptr()))
+    return TokenLogprobs(logp, ent)
+
+
+def token_logprobs_gradient(logits, targets0, dlogp, dentropy=None, temperature: float = 1.0, out=None):
+    """d objective / d logits from d objective / d logp (and / d entropy).  `out` may be the logits themselves."""
+    import torch
+    n, V, pitch = _rows("logits", logits)
+    shape, f32 = logits.shape[:-1], torch.float32
+    targets0 = _on_device("targets0", targets0, torch.int32, shape, logits.device)
+    dlogp, dentropy = _on_device("dlogp", dlogp, f32, shape, logits.device), _on_device("dentropy", dentropy, f32, shape, logits.device)
+    out, out_pitch = _gradient_of(logits, out)
+    with _Device(logits.device):
+        _lib.check(_lib.lib().femto_token_logprobs_gradient(_code(logits), _lib.ptr(out), out_pitch, _lib.ptr(logits), pitch, _lib.ptr(targets0), n, V,
+                                                            temperature, _lib.ptr(dlogp), _lib.ptr(dentropy), _lib.stream_ptr()))
+    return out
+
+
+def _policy_config(clip_low, clip_high, kl_coef, temperature, reduction):
+    if reduction not in _lib.REDUCTION:
+        raise ValueError(f"reduction must be 'sum' or 'mean', not {reduction!r}")
+    return _lib.PolicyConfigC(temperature, clip_low, math.inf if clip_high is None else clip_high, kl_coef, _lib.REDUCTION[reduction])
+
+
+def policy_loss(logits, targets0, old_logp, advantages, ref_logp=None, weights=None, clip_low: float = 0.2, clip_high: Optional[float] = 0.2,
+                kl_coef: float = 0.0, temperature: float = 1.0, reduction: str = "sum", gradient: bool = True, out=None) -> PolicyLoss:
+    """Clipped policy loss with a KL term, and its gradient by the logits in the same pass:
+    weight (-min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (e^g - g - 1)) per token, r = exp(logp - old_logp) and
+    g = ref_logp - logp.  clip_high=None bounds the ratio below only.  `out` may be the logits themselves."""
+    import torch
+    n, V, pitch = _rows("logits", logits)
+    shape, f32, device = logits.shape[:-1], torch.float32, logits.device
+    targets0 = _on_device("targets0", targets0, torch.int32, shape, device)
+    old_logp, advantages, ref_logp, weights = (_on_device(name, t, f32, shape, device) for name, t in
+                                               (("old_logp", old_logp), ("advantages", advantages), ("ref_logp", ref_logp), ("weights", weights)))
+    cfg = _policy_config(clip_low, clip_high, kl_coef, temperature, reduction)
+    d, d_pitch = _gradient_of(logits, out) if gradient else (None, V)
+    token_losses, logp = torch.empty((2,) + shape, dtype=f32, device=device)
+    loss = torch.empty(1, dtype=f32, device=device)
+    n_valid, n_clipped = torch.empty(2, 1, dtype=torch.int32, device=device)
+    with _Device(device):
+        _lib.check(_lib.lib().femto_policy_loss(
+            _code(logits), _lib.ptr(logits), pitch, _lib.ptr(targets0), n, V, _lib.ptr(old_logp), _lib.ptr(advantages), _lib.ptr(ref_logp),
+            _lib.ptr(weights), C.byref(cfg), _lib.ptr(d), d_pitch, _lib.ptr(token_losses), _lib.ptr(logp), _lib.ptr(loss), _lib.ptr(n_valid),
+            _lib.ptr(n_clipped), _lib.stream_ptr()))
+    return PolicyLoss(loss, n_valid, n_clipped, token_losses, logp, d)
+
+
+def _preference_config(kind, beta, margin, label_smoothing, length_normalised, reduction):
+    if kind not in PREFERENCES:
+        raise ValueError(f"kind must be 'sigmoid' or 'squared', not {kind!r}")
+    if reduction not in _lib.REDUCTION:
+        raise ValueError(f"reduction must be 'sum' or 'mean', not {reduction!r}")
+    return _lib.PreferenceConfigC(PREFERENCES[kind], beta, margin, label_smoothing, 1 if length_normalised else 0, _lib.REDUCTION[reduction])
+
+
+def preference_loss(logp, offsets, targets0=None, ref_logp=None, kind: str = "sigmoid", beta: float = 0.1, margin: float = 0.0,
+                    label_smoothing: float = 0.0, length_normalised: bool = False, reduction: str = "mean", gradient: bool = True) -> PreferenceLoss:
+    """Preference loss of pairs of answers from their tokens' log-probabilities (any shape, taken in order): answer k is the rows
+    offsets[k] .. offsets[k + 1] - 1 (int32 [2 P + 1], ascending), chosen and rejected in turn; tokens with a negative target do not count.
+    `dlogp` is what `token_logprobs_gradient` takes."""
+    import torch
+    if not logp.is_cuda:
+        raise ValueError("logp must be on a CUDA device")
+    f32, device, shape = torch.float32, logp.device, logp.shape
+    logp, ref_logp = _on_device("logp", logp, f32, shape, device), _on_device("ref_logp", ref_logp, f32, shape, device)
+    targets0 = _on_device("targets0", targets0, torch.int32, shape, device)
+    if offsets.dim() != 1 or offsets.shape[0] % 2 != 1:
+        raise ValueError(f"offsets must be [2 P + 1], not {tuple(offsets.shape)}")
+    offsets = _on_device("offsets", offsets, torch.int32, offsets.shape, device)
+    n, P = logp.numel(), offsets.shape[0] // 2
+    if n >= 1 << 31:
+        raise ValueError(f"{n} tokens")
+    cfg = _preference_config(kind, beta, margin, label_smoothing, length_normalised, reduction)
+    loss = torch.empty(1, dtype=f32, device=device)
+    pair_losses, ratios = torch.empty(P, dtype=f32, device=device), torch.empty(2 * P, dtype=f32, device=device)
+    dlogp = torch.empty(shape, dtype=f32, device=device) if gradient else None
+    with _Device(device):
+        _lib.check(_lib.lib().femto_preference_loss(
+            _lib.ptr(logp), _lib.ptr(ref_logp), _lib.ptr(targets0), n, _lib.ptr(offsets), P, C.byref(cfg), _lib.ptr(loss), _lib.ptr(pair_losses),
+            _lib.ptr(ratios), _lib.ptr(dlogp), _lib.stream_ptr()))
+    return PreferenceLoss(loss, pair_losses, ratios, dlogp)

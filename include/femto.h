@@ -441,6 +441,59 @@ int32_t femto_muon_direction(int32_t dtype, float* X_out, const float* G, float*
                              int32_t k, int32_t rows, int32_t cols, float mu, float beta2, float n_tokens,
                              const float* h_coeffs, int32_t steps, void* stream);
 
+/* ---- objectives on a model's own answers ------------------------------------------------------ */
+/* What comes after pretraining; no counterpart in the reference.  These calls are asynchronous on `stream`, allocate nothing and keep
+ * nothing: they may be captured, and calls on different streams do not meet.  Logits are [N][V] rows of `dtype`, ldl >= V elements apart and
+ * aligned to their type only.  targets0: 0-based, or negative where a row counts for nothing: neither its logits nor its entries in other
+ * arrays are then read, and its results are 0.  A target of V or more counts as none and raises bit 1 of the word that
+ * femto_status_word(NULL, ..) reads.  Logits of -inf are tokens that cannot be chosen; a row with nothing else has no distribution: its
+ * log-probability is -inf, its entropy and its gradient are 0.  NaN or +inf in a counted row give NaN there.  N = 0 is allowed. */
+/* Log-probabilities log p(target) of softmax(logits / temperature): logp [N]; entropy [N] (may be NULL). */
+int32_t femto_token_logprobs(int32_t dtype, const void* logits, int64_t ldl, const int32_t* targets0, int32_t N, int32_t V,
+                             float temperature, float* logp, float* entropy, void* stream);
+/* The way back: dlogits [N][V] = dlogp d logp / d logits + dentropy d entropy / d logits (dentropy may be NULL), the rows ldd elements apart.
+ * Overwrites; dlogits may be the logits themselves (same pitch), and may not overlap them otherwise. */
+int32_t femto_token_logprobs_gradient(int32_t dtype, void* dlogits, int64_t ldd, const void* logits, int64_t ldl,
+                                      const int32_t* targets0, int32_t N, int32_t V, float temperature, const float* dlogp,
+                                      const float* dentropy, void* stream);
+
+typedef struct femto_policy_config {
+  float temperature; /* > 0: at which the answers were sampled */
+  float clip_low, clip_high; /* the ratio r counts up to the range 1 - clip_low .. 1 + clip_high (infinity: no bound above) */
+  float kl_coef;     /* beta >= 0 */
+  int32_t reduction; /* FEMTO_REDUCTION_SUM, or _MEAN over the rows with a target */
+} femto_policy_config;
+/* Clipped policy loss with a KL term.  Of a row with a target, with lp = log p(target) and r = exp(lp - old_logp):
+ *   token_loss = weight (-min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A) + beta (e^(ref_logp - lp) - (ref_logp - lp) - 1))
+ * advantages A [N]; ref_logp [N] (may be NULL when beta is 0); weights [N] (NULL = 1; where a weight is 0 loss and gradient are 0).
+ * Outputs: token_losses [N], logp [N], the reduced loss, n_valid = rows with a target, n_clipped (may be NULL) = those whose minimum is
+ * the bounded product, which has no gradient.  dlogits (NULL: loss only) is overwritten with the gradient of the reduced loss, its rows ldd
+ * elements apart; it may be the logits themselves (same pitch), and may not overlap them otherwise. */
+int32_t femto_policy_loss(int32_t dtype, const void* logits, int64_t ldl, const int32_t* targets0, int32_t N, int32_t V,
+                          const float* old_logp, const float* advantages, const float* ref_logp, const float* weights,
+                          const femto_policy_config* h_cfg, void* dlogits, int64_t ldd, float* token_losses, float* logp,
+                          float* loss_out, int32_t* n_valid_out, int32_t* n_clipped_out, void* stream);
+
+#define FEMTO_PREFERENCE_SIGMOID 0
+#define FEMTO_PREFERENCE_SQUARED 1
+typedef struct femto_preference_config {
+  int32_t kind;
+  float beta;            /* > 0 */
+  float margin, label_smoothing; /* sigmoid only */
+  int32_t length_normalised; /* rho is divided by the number of the answer's counted rows */
+  int32_t reduction;     /* FEMTO_REDUCTION_SUM or _MEAN over the pairs */
+} femto_preference_config;
+/* Preference loss of P pairs of answers.  Answer k is the rows offsets[k] .. offsets[k + 1] - 1 (int32 [2 P + 1], device, ascending), 2 p
+ * the chosen and 2 p + 1 the rejected one of pair p; rho_k = sum over its rows of logp - ref_logp (ref_logp may be NULL = 0), without the
+ * rows whose target is negative (targets0 may be NULL: all count).  With D = rho_2p - rho_2p+1 and h = beta D - margin:
+ *   sigmoid: -(1 - label_smoothing) log sigma(h) - label_smoothing log sigma(-h)        squared: (D - 1 / (2 beta))^2
+ * Outputs: the reduced loss, pair_losses [P], ratios [2 P] = rho, dlogp [N] (may be NULL) = the gradient of the reduced loss, 0 in rows that
+ * count for nothing or belong to no answer.  Offsets that leave 0 .. N or descend make an answer empty and raise bit 8 of the word that
+ * femto_status_word(NULL, ..) reads; dlogp is then not complete. */
+int32_t femto_preference_loss(const float* logp, const float* ref_logp, const int32_t* targets0, int32_t N, const int32_t* offsets,
+                              int32_t P, const femto_preference_config* h_cfg, float* loss_out, float* pair_losses, float* ratios,
+                              float* dlogp, void* stream);
+
 /* ---- status --------------------------------------------------------------------------------- */
 /* Device status word (0 = ok): bounded waits that ran out (bit 2), out-of-range token ids (bit 1), ...
  * h == NULL reads AND CLEARS the word of the stand-alone kernel-level entry points on the current device (after a

@@ -1,0 +1,468 @@
+"""Objectives on a model's own answers against their definitions in 64 bits.
+
+Tolerances.  A log-probability is ln2 u - log l with l a sum of V exponentials.  Relative errors of l: 2^-22 of an exponential, 2^-24 ln2 |u|
+of its argument (|u| < 64 wherever 2^u counts), and at most one rounding per addition; a chain of additions is no longer than V / 256 + 48 in any
+form of the kernels.  The scale log2(e) / temperature is rounded once, which moves a log-probability by at most 2^-24 of its distance from the
+row's mean of log p, |lp| + H; the result is rounded to fp32.  So an error of `slack(V)` + 2^-23 (|lp| + H + 1), slack(V) = 2^-22 + 2^-24 (V / 256 + 96).
+A probability has the relative error of l, twice (its own exponential, and 1 / l)."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+import femtochat_b200 as fb
+from femtochat_b200 import _lib
+
+pytestmark = pytest.mark.gpu
+LO, HI = 0.2, 0.28
+
+
+def slack(V):
+    return 2.0 ** -22 + 2.0 ** -24 * (V / 256 + 96)
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def status():
+    out = C.c_int32(0)
+    _lib.check(_lib.lib().femto_status_word(None, C.byref(out)))
+    return out.value
+
+
+def make(N, V, dtype, pitch=0, offset=0, seed=0, spread=3.0, masked=0.0, temperature=1.0):
+    """Logits in a buffer of their own pitch that starts `offset` elements in, targets drawn from the softmax, some rows without."""
+    g = torch.Generator(device="cuda").manual_seed(1009 * seed + 31 * N + V)
+    buf = torch.full((offset + N * (V + pitch) + 64,), 7.0, device="cuda", dtype=dtype)
+    z = buf[offset:offset + N * (V + pitch)].view(N, V + pitch)[:, :V]
+    z.copy_(spread * torch.randn(N, V, device="cuda", generator=g))
+    t = torch.multinomial(torch.softmax(z.float() / temperature, 1), 1, generator=g)[:, 0].int() if V <= 1 << 20 else torch.zeros(N, device="cuda", dtype=torch.int32)
+    if masked:
+        t[torch.rand(N, device="cuda", generator=g) < masked] = -1
+    return z, t
+
+
+def reference(z, t, temperature=1.0):
+    """(logp, entropy, log p of every token) in 64 bits; 0 in rows without a target."""
+    s = z.double() / temperature
+    lse = torch.logsumexp(s, 1)
+    ls = torch.where(lse[:, None] == -math.inf, -math.inf, s - lse[:, None])
+    h = -torch.where(ls == -math.inf, 0.0, ls.exp() * ls).sum(1)
+    has = t >= 0
+    lp = ls.gather(1, t.clamp(min=0).long()[:, None])[:, 0]
+    return torch.where(has, lp, 0.0), torch.where(has, h, 0.0), ls
+
+
+def near(got, want, tol, what):
+    got, want = got.double(), want.double()
+    assert got.shape == want.shape, what
+    same = (got == want) | (got.isnan() & want.isnan())
+    bad = ~same & ~((got - want).abs() <= tol)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()}, largest {float((got - want).abs().nan_to_num(1e300).max()):.3e}"
+
+
+# a row that fits a thread, a warp, a block; odd; past every size that one block, or eight together, hold of it
+SHAPES = [(1, 1), (3, 2), (5, 7), (2, 33), (7, 255), (4, 1000), (9, 4099), (150, 4096), (600, 300), (3, 50021), (2, 65536), (1, 131073), (2, 300007)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,V", SHAPES)
+@pytest.mark.parametrize("pitch,offset,temperature", [(0, 0, 1.0), (3, 1, 0.75)])
+def test_token_logprobs(dtype, N, V, pitch, offset, temperature):
+    z, t = make(N, V, dtype, pitch, offset, masked=0.3 if N > 3 else 0.0)
+    lp, h, _ = reference(z, t, temperature)
+    for entropy in (False, True):
+        r = fb.token_logprobs(z, t, temperature=temperature, entropy=entropy)
+        near(r.logp, lp, slack(V) + 2.0 ** -23 * (lp.abs() + h + 1), "logp")
+        if entropy:     # the mean of -log p: as far off as a log-probability, and p as above
+            near(r.entropy, h, 3 * slack(V) * (h + 1), "entropy")
+    again = fb.token_logprobs(z, t, temperature=temperature, entropy=True)
+    assert torch.equal(r.logp, again.logp) and torch.equal(r.entropy, again.entropy)
+    assert status() == 0
+
+
+def check_gradient(d, z, coef, t, ls, V, dtype, inv_t, extra=0.0, what="dlogits"):
+    """d = inv_t coef (onehot - p), within the roundings of p, of the coefficient and of the result."""
+    p = ls.exp()
+    onehot = torch.nn.functional.one_hot(t.clamp(min=0).long(), V).double() * (t >= 0)[:, None]
+    want = inv_t * coef[:, None] * (onehot - p)
+    tol = half_step(dtype) * 1.01 * want.abs() + inv_t * coef.abs()[:, None] * (p + onehot) * (2 * slack(V) + 2.0 ** -21) + extra + 1e-38
+    near(d, want, tol, what)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,V", SHAPES)
+@pytest.mark.parametrize("pitch,offset,temperature", [(0, 0, 1.0), (5, 3, 1.25)])
+def test_token_logprobs_gradient(dtype, N, V, pitch, offset, temperature):
+    z, t = make(N, V, dtype, pitch, offset, seed=1, masked=0.3 if N > 3 else 0.0)
+    g = torch.Generator(device="cuda").manual_seed(N + V)
+    dlogp, dent = torch.randn(2, N, device="cuda", generator=g)
+    _, h, ls = reference(z, t, temperature)
+    has, inv = (t >= 0), 1.0 / temperature
+    d = fb.token_logprobs_gradient(z, t, dlogp, temperature=temperature)
+    check_gradient(d, z, torch.where(has, dlogp.double(), 0.0), t, ls, V, dtype, inv)
+    # with the entropy: - dH p (log p + H)
+    d2 = fb.token_logprobs_gradient(z, t, dlogp, dentropy=dent, temperature=temperature)
+    p = ls.exp()
+    onehot = torch.nn.functional.one_hot(t.clamp(min=0).long(), V).double()
+    k = dlogp.double()[:, None] + dent.double()[:, None] * (ls + h[:, None])
+    want = torch.where(has[:, None], inv * (dlogp.double()[:, None] * onehot - k * p), 0.0)
+    size = dlogp.double().abs()[:, None] * (onehot + p) + dent.double().abs()[:, None] * p * (ls.abs() + h[:, None] + 2)
+    near(d2, want, half_step(dtype) * 1.01 * want.abs() + inv * size * (4 * slack(V) + 2.0 ** -20) + 1e-38, "with the entropy")
+    assert status() == 0
+
+
+def tokens_of(N, lp, seed, ref=True):
+    """Old log-probabilities away from where the clipping begins, advantages of both signs and 0, a reference, weights (one of them 0)."""
+    g = torch.Generator(device="cuda").manual_seed(7 * seed + N)
+    old = lp - 0.25 * torch.randn(N, device="cuda", generator=g, dtype=torch.float64)
+    for edge in (1 - LO, 1 + HI):
+        old = torch.where(((lp - old).exp() / edge - 1).abs() < 1e-3, old + 0.01, old)
+    A = torch.randn(N, device="cuda", generator=g)
+    w = torch.rand(N, device="cuda", generator=g)
+    if N > 2:
+        A[1], w[2] = 0.0, 0.0
+    return old.float(), A, (lp + 0.4 * torch.randn(N, device="cuda", generator=g, dtype=torch.float64)).float(), w
+
+
+def policy_reference(lp, has, old, A, ref, w, kl):
+    """Token losses and their slopes by lp, where the minimum is the bounded product; and how far an error of lp moves them."""
+    r = (lp - old.double()).exp()
+    A, w = A.double(), (w.double() if w is not None else torch.ones_like(lp))
+    bounded = r.clamp(1 - LO, 1 + HI) * A
+    clipped = has & (bounded < r * A)
+    loss, slope = -torch.minimum(r * A, bounded), torch.where(clipped, 0.0, -r * A)
+    size = r * A.abs() + A.abs()
+    if kl:
+        gap = ref.double() - lp
+        loss = loss + kl * (torch.expm1(gap) - gap)
+        slope = slope - kl * torch.expm1(gap)
+        size = size + kl * (gap.exp() + gap.abs() + 1)
+    zero = torch.zeros_like(lp)
+    return torch.where(has, w * loss, zero), torch.where(has, w * slope, zero), clipped, torch.where(has, w * size, zero)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,V", SHAPES)
+@pytest.mark.parametrize("pitch,offset,temperature,kl,reduction", [(0, 0, 1.0, 0.0, "sum"), (8, 0, 0.8125, 0.125, "mean"), (1, 5, 1.0, 0.0625, "sum")])
+def test_policy_loss(dtype, N, V, pitch, offset, temperature, kl, reduction):
+    z, t = make(N, V, dtype, pitch, offset, seed=2, masked=0.4 if N > 3 else 0.0, temperature=temperature)
+    lp, h, ls = reference(z, t, temperature)
+    old, A, ref, w = tokens_of(N, lp, V)
+    w = w if offset else None
+    has = t >= 0
+    loss, slope, clipped, size = policy_reference(lp, has, old, A, ref, w, kl)
+    n = int(has.sum())
+    scale = 1.0 / max(n, 1) if reduction == "mean" else 1.0
+    dlp = slack(V) + 2.0 ** -23 * (lp.abs() + h + 1)
+    term = size * (2 * dlp + 2.0 ** -21)      # ratio and e^gap: the error of lp, of exp and of the products
+    kwargs = dict(ref_logp=ref if kl else None, weights=w, clip_low=LO, clip_high=HI, kl_coef=kl, temperature=temperature, reduction=reduction)
+    r = fb.policy_loss(z, t, old, A, **kwargs)
+    near(r.logp, lp, dlp, "logp")
+    near(r.token_losses, loss, term, "token losses")
+    near(r.loss, (scale * loss.sum()).reshape(1), scale * (term.sum() + loss.abs().sum() * 2.0 ** -24 * (N / 1024 + 16)), "loss")
+    assert int(r.n_valid) == n and int(r.n_clipped) == int(clipped.sum())
+    p = ls.exp()
+    onehot = torch.nn.functional.one_hot(t.clamp(min=0).long(), V).double()
+    check_gradient(r.dlogits, z, scale * slope, t, ls, V, dtype, 1 / temperature, scale / temperature * term[:, None] * (p + onehot))
+    # the loss alone is the same, and so is the gradient in the logits' place
+    only = fb.policy_loss(z, t, old, A, gradient=False, **kwargs)
+    near(only.loss, r.loss, scale * (2 * term.sum() + loss.abs().sum() * 2.0 ** -23 * (N / 1024 + 16)), "loss alone")
+    assert only.dlogits is None and torch.equal(only.n_clipped, r.n_clipped)
+    keep = z.clone()
+    inplace = fb.policy_loss(z, t, old, A, out=z, **kwargs)
+    assert inplace.dlogits is z and torch.equal(z, r.dlogits) and torch.equal(inplace.loss, r.loss)
+    z.copy_(keep)
+    assert status() == 0
+
+
+@pytest.mark.parametrize("V", [37, 5000, 70001])
+def test_rows_around_the_gradient_stay(V):
+    """What lies between and behind the rows of a padded gradient is not written; rows start anywhere."""
+    N, pad = 5, 11
+    for dtype in (torch.float32, torch.bfloat16):
+        for offset in (0, 1, 4):
+            z, t = make(N, V, dtype)
+            buf = torch.full((offset + N * (V + pad) + 40,), 5.0, device="cuda", dtype=dtype)
+            out = buf[offset:offset + N * (V + pad)].view(N, V + pad)[:, :V]
+            old = torch.zeros(N, device="cuda")
+            r = fb.policy_loss(z, t, old, torch.ones_like(old), clip_high=None, out=out)
+            d = fb.policy_loss(z, t, old, torch.ones_like(old), clip_high=None).dlogits
+            assert torch.equal(out, d)
+            out.fill_(5.0)
+            assert bool((buf == 5.0).all())
+            fb.token_logprobs_gradient(z, t, old + 1, out=out)
+            assert torch.equal(out, fb.token_logprobs_gradient(z, t, old + 1))
+            out.fill_(5.0)
+            assert bool((buf == 5.0).all())
+            assert r.dlogits is out
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [9, 3001, 66000])
+def test_masked_rows_and_masked_tokens(dtype, V):
+    """Rows without a target may hold anything; logits of -inf are tokens that cannot be chosen; a row of them has no distribution."""
+    N = 6
+    z, t = make(N, V, dtype, seed=3)
+    g = torch.Generator(device="cuda").manual_seed(V)
+    hidden = torch.rand(N, V, device="cuda", generator=g) < 0.6
+    hidden.scatter_(1, t.long()[:, None], False)
+    z.masked_fill_(hidden, -math.inf)
+    t[0], z[0] = -1, math.nan
+    z[1] = -math.inf
+    z[2] = torch.finfo(dtype).min        # the lowest value, everywhere: a uniform distribution
+    z[3, :] = -math.inf
+    z[3, int(t[3])] = 1.0                # one token left: it is certain
+    t[4] = -5
+    numbers = torch.tensor([math.nan, 0.5, -0.5, 1.0, math.inf, 0.25], device="cuda")
+    r = fb.token_logprobs(z, t, entropy=True)
+    lp, h, ls = reference(z, t)
+    lp[2], h[2] = -math.log(V), math.log(V)
+    near(r.logp, lp, slack(V) + 2.0 ** -23 * (lp.abs() + h + 1), "logp")
+    near(r.entropy, h, 3 * slack(V) * (h + 1), "entropy")
+    assert float(r.logp[1]) == -math.inf and float(r.logp[3]) == 0.0 and float(r.entropy[3]) == 0.0
+    d = fb.token_logprobs_gradient(z, t, numbers, dentropy=numbers)
+    assert not d.isnan().any()
+    for row in (0, 1, 4):
+        assert bool((d[row] == 0).all())
+    assert bool((d[hidden & (t >= 0)[:, None] & (torch.arange(N, device="cuda") != 2)[:, None]] == 0).all())
+    finite = torch.tensor([math.nan, 0.0, 0.0, 0.0, math.nan, -2.0], device="cuda")
+    q = fb.policy_loss(z, t, finite, numbers, ref_logp=torch.where(t < 0, math.nan, -3.0), weights=torch.where(t < 0, math.nan, 1.0))
+    for row in (0, 1, 4):
+        assert bool((q.dlogits[row] == 0).all()) and float(q.token_losses[row]) == 0
+    assert not q.dlogits.isnan().any() and math.isfinite(float(q.loss)) and int(q.n_valid) == 4
+    assert status() == 0
+
+
+def test_not_a_number_stays_in_its_row():
+    for V in (50, 40000):
+        z, t = make(4, V, torch.float32, seed=4)
+        z[1, 3], z[2, 4] = math.nan, math.inf
+        r = fb.token_logprobs(z, t, entropy=True)
+        assert r.logp[1:3].isnan().all() and r.entropy[1:3].isnan().all() and not r.logp[[0, 3]].isnan().any()
+        q = fb.policy_loss(z, t, torch.zeros(4, device="cuda"), torch.ones(4, device="cuda"), clip_high=None)
+        assert q.dlogits[1:3].isnan().all() and not q.dlogits[[0, 3]].isnan().any()
+
+
+def test_no_rows_and_rows_without_targets():
+    empty = torch.empty(0, 5, device="cuda")
+    i32, f32 = torch.empty(0, device="cuda", dtype=torch.int32), torch.empty(0, device="cuda")
+    assert fb.token_logprobs(empty, i32, entropy=True).logp.shape == (0,)
+    assert fb.token_logprobs_gradient(empty, i32, f32).shape == (0, 5)
+    for reduction in ("sum", "mean"):
+        r = fb.policy_loss(empty, i32, f32, f32, reduction=reduction)
+        assert float(r.loss) == 0 and int(r.n_valid) == 0 and int(r.n_clipped) == 0
+        z = torch.randn(3, 4000, device="cuda")
+        r = fb.policy_loss(z, torch.full((3,), -1, device="cuda", dtype=torch.int32), torch.zeros(3, device="cuda"), torch.ones(3, device="cuda"), reduction=reduction)
+        assert float(r.loss) == 0 and int(r.n_valid) == 0 and bool((r.dlogits == 0).all())
+
+
+def test_target_outside_the_vocabulary():
+    z, t = make(4, 1000, torch.bfloat16)
+    want = fb.token_logprobs(z, t).logp
+    bad = t.clone()
+    bad[2] = 1000
+    r = fb.token_logprobs(z, bad)
+    assert status() == 1 and status() == 0
+    assert float(r.logp[2]) == 0 and torch.equal(r.logp[[0, 1, 3]], want[[0, 1, 3]])
+    q = fb.policy_loss(z, bad, torch.zeros(4, device="cuda"), torch.ones(4, device="cuda"), reduction="mean")
+    assert status() == 1 and int(q.n_valid) == 3 and bool((q.dlogits[2] == 0).all())
+    fb.token_logprobs_gradient(z, bad, torch.ones(4, device="cuda"))
+    assert status() == 1
+
+
+def test_rows_past_32_bits():
+    """Row offsets beyond 2^32 bytes and 2^31 elements."""
+    pitch, V = (1 << 30) + 16, 5000
+    buf = torch.empty(2 * pitch + V, device="cuda", dtype=torch.bfloat16)
+    z = torch.as_strided(buf, (3, V), (pitch, 1))
+    small, t = make(3, V, torch.bfloat16, seed=5)
+    z.copy_(small)
+    assert torch.equal(fb.token_logprobs(z, t).logp, fb.token_logprobs(small, t).logp)
+    old, A = torch.full((3,), -5.0, device="cuda"), torch.ones(3, device="cuda")
+    want = fb.policy_loss(small, t, old, A).dlogits
+    assert torch.equal(fb.policy_loss(z, t, old, A, out=z).dlogits, want)
+
+
+def test_streams_and_graphs():
+    """Two calls at once on two streams, and a captured call replayed on other inputs while another graph of the same call lives."""
+    z, t = make(64, 9000, torch.bfloat16, seed=6)
+    y, u = make(64, 9000, torch.bfloat16, seed=7)
+    old, A = torch.full((64,), -4.0, device="cuda"), torch.linspace(-1, 1, 64, device="cuda")
+    want, other = (fb.policy_loss(a, b, old, A, reduction="mean") for a, b in ((z, t), (y, u)))
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        with torch.cuda.stream(s1):
+            a = fb.policy_loss(z, t, old, A, reduction="mean")
+        with torch.cuda.stream(s2):
+            b = fb.policy_loss(y, u, old, A, reduction="mean")
+        torch.cuda.synchronize()
+        for got, ref in ((a, want), (b, other)):
+            assert all(torch.equal(x, y) for x, y in zip(got, ref))
+    x, v, runs = z.clone(), t.clone(), torch.arange(0, 65, 16, device="cuda", dtype=torch.int32)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            p = fb.policy_loss(x, v, old, A, reduction="mean")
+            lp = fb.token_logprobs(x, v, entropy=True)
+            d = fb.token_logprobs_gradient(x, v, old, dentropy=A)
+            q = fb.preference_loss(lp.logp, runs, targets0=v, beta=0.375)
+        graphs.append((g, p, lp, d, q))
+    x.copy_(y), v.copy_(u)
+    for g, p, lp, d, q in graphs:
+        g.replay()
+    torch.cuda.synchronize()
+    fresh = fb.token_logprobs(y, u, entropy=True)
+    for g, p, lp, d, q in graphs:
+        assert all(torch.equal(a, b) for a, b in zip(p, other))
+        assert torch.equal(lp.entropy, fresh.entropy)
+        assert all(torch.equal(a, b) for a, b in zip(q, fb.preference_loss(fresh.logp, runs, targets0=u, beta=0.375)))
+        assert torch.equal(d, fb.token_logprobs_gradient(y, u, old, dentropy=A))
+
+
+def test_gradient_against_differences():
+    """The gradient of the reduced loss against central differences of the definition in 64 bits."""
+    N, V, kl = 4, 11, 0.125
+    z, t = make(N, V, torch.float32, seed=8)
+    lp, _, _ = reference(z, t, 0.875)
+    old, A, ref, w = tokens_of(N, lp, 3)
+    r = fb.policy_loss(z, t, old, A, ref_logp=ref, weights=w, clip_low=LO, clip_high=HI, kl_coef=kl, temperature=0.875)
+
+    def f(x):
+        return policy_reference(reference(x, t, 0.875)[0], t >= 0, old, A, ref, w, kl)[0].sum()
+
+    step = 1e-5
+    for i in range(N):
+        for j in range(V):
+            e = torch.zeros(N, V, device="cuda", dtype=torch.float64)
+            e[i, j] = step
+            slope = float((f(z.double() + e) - f(z.double() - e)) / (2 * step))
+            # differences: step^2 times a third derivative of a few, and roundings 2^-52 / step
+            assert abs(float(r.dlogits[i, j]) - slope) < 1e-5 * (1 + abs(slope))
+
+
+# ---- pairs ----------------------------------------------------------------------------------------------------------------------------------
+def pairs(P, longest, seed, ref=True, masked=0.0, before=0, behind=0):
+    g = torch.Generator().manual_seed(1000 * seed + 17 * P + longest)
+    n = torch.randint(0, longest + 1, (2 * P,), generator=g)
+    offsets = (before + torch.cat([torch.zeros(1, dtype=torch.int64), torch.cumsum(n, 0)])).int()
+    N = int(offsets[-1]) + behind
+    logp = -torch.empty(N).exponential_(0.7, generator=g)
+    t = torch.randint(0, 9, (N,), generator=g, dtype=torch.int32)
+    if masked:
+        t[torch.rand(N, generator=g) < masked] = -1
+    return logp.cuda(), (logp + 0.2 * torch.randn(N, generator=g)).cuda() if ref else None, t.cuda(), offsets.cuda()
+
+
+def preference_reference(logp, ref, t, offsets, kind, beta, margin, smoothing, normalised, reduction):
+    gap = logp.double() - (ref.double() if ref is not None else 0.0)
+    P = offsets.shape[0] // 2
+    o = offsets.tolist()
+    rho, size, per, d = [], [], [], torch.zeros_like(gap)
+    for k in range(2 * P):
+        rows = slice(o[k], o[k + 1])
+        m = (t[rows] >= 0).double() if t is not None else torch.ones_like(gap[rows])
+        c = max(float(m.sum()), 1.0) if normalised else 1.0
+        x = torch.where(m > 0, gap[rows], 0.0)
+        rho.append(x.sum() / c), size.append(x.abs().sum() / c), per.append(m / c)
+    rho = torch.stack(rho) if rho else torch.zeros(0, device="cuda", dtype=torch.float64)
+    D = (rho[0::2] - rho[1::2]).requires_grad_()
+    if kind == "sigmoid":
+        h = beta * D - margin
+        losses = -(1 - smoothing) * torch.nn.functional.logsigmoid(h) - smoothing * torch.nn.functional.logsigmoid(-h)
+    else:
+        losses = (D - 0.5 / beta) ** 2
+    loss = losses.sum() / (P if reduction == "mean" and P else 1)
+    slope = torch.autograd.grad(loss, D)[0] if P else D
+    for k in range(2 * P):
+        d[o[k]:o[k + 1]] = per[k] * slope[k // 2] * (1 if k % 2 == 0 else -1)
+    return loss.detach().reshape(1), losses.detach(), rho, d, (torch.stack(size) if P else rho)
+
+
+@pytest.mark.parametrize("P,longest", [(0, 4), (1, 1), (1, 24), (3, 200), (2, 5000), (1, 70000), (300, 40), (1500, 3)])
+@pytest.mark.parametrize("kind,ref,masked,normalised,reduction", [("sigmoid", True, 0.0, False, "mean"), ("sigmoid", False, 0.4, True, "sum"),
+                                                                  ("squared", True, 0.3, False, "mean")])
+def test_preference_loss(P, longest, kind, ref, masked, normalised, reduction):
+    logp, ref_logp, t, offsets = pairs(P, longest, 1, ref, masked, before=3, behind=9001)
+    beta = 1.5 if normalised else 0.125
+    margin, smoothing = (0.25, 0.125) if kind == "sigmoid" else (0.0, 0.0)
+    targets = t if masked else None
+    loss, losses, rho, d, size = preference_reference(logp, ref_logp, targets, offsets, kind, beta, margin, smoothing, normalised, reduction)
+    r = fb.preference_loss(logp, offsets, targets0=targets, ref_logp=ref_logp, kind=kind, beta=beta, margin=margin, label_smoothing=smoothing,
+                           length_normalised=normalised, reduction=reduction)
+    # each difference is rounded to fp32, everything else is in 64 bits until it is stored
+    drho = 2.0 ** -24 * size * 1.01
+    near(r.ratios, rho, drho + 2.0 ** -24 * rho.abs(), "ratios")
+    dD = drho[0::2] + drho[1::2]
+    slope = beta if kind == "sigmoid" else 2 * (rho[0::2] - rho[1::2]).abs() + 1 / beta
+    dl = slope * dD + dD ** 2 + 2.0 ** -23 * (losses.abs() + beta + abs(margin))
+    near(r.pair_losses, losses, dl, "pair losses")
+    near(r.loss, loss, (dl.sum() + 2.0 ** -24 * losses.sum()) / (P if reduction == "mean" and P else 1) + 1e-30, "loss")
+    curve = beta * beta / 4 if kind == "sigmoid" else 2.0
+    worst = float((curve * dD).max()) if P else 0.0
+    near(r.dlogp, d, 2.0 ** -22 * d.abs() + (worst + 2.0 ** -24 * beta) * (1.0 / P if reduction == "mean" and P else 1.0), "dlogp")
+    assert bool((r.dlogp[:3] == 0).all()) and bool((r.dlogp[logp.shape[0] - 9001:] == 0).all())
+    only = fb.preference_loss(logp, offsets, targets0=targets, ref_logp=ref_logp, kind=kind, beta=beta, margin=margin, label_smoothing=smoothing,
+                              length_normalised=normalised, reduction=reduction, gradient=False)
+    assert only.dlogp is None and torch.equal(only.loss, r.loss) and torch.equal(only.ratios, r.ratios)
+    assert status() == 0
+
+
+def test_preference_extremes():
+    """Answers that are far apart: the loss is linear there, not infinite; masked tokens may hold anything."""
+    logp = torch.tensor([-1e4, -1.0, math.nan, -2.0], device="cuda")
+    t = torch.tensor([3, 3, -1, 3], device="cuda", dtype=torch.int32)
+    offsets = torch.tensor([0, 1, 4], device="cuda", dtype=torch.int32)
+    r = fb.preference_loss(logp, offsets, targets0=t, beta=1.0)
+    assert float(r.loss) == pytest.approx(9997.0, rel=1e-6) and r.dlogp.tolist() == [-1.0, 1.0, 0.0, 1.0]
+    r = fb.preference_loss(logp, torch.tensor([1, 4, 4], device="cuda", dtype=torch.int32), targets0=t, beta=500.0)
+    assert float(r.loss) == pytest.approx(1500.0) and r.ratios.tolist() == [-3.0, 0.0]
+    r = fb.preference_loss(logp[1:2], torch.tensor([0, 0, 0], device="cuda", dtype=torch.int32), reduction="sum")
+    assert float(r.loss) == pytest.approx(math.log(2)) and r.dlogp.tolist() == [0.0]
+
+
+def test_bad_offsets_are_flagged():
+    logp = -torch.ones(10, device="cuda")
+    for bad in ([0, 4, 11], [0, 6, 5], [-1, 4, 6]):
+        r = fb.preference_loss(logp, torch.tensor(bad, device="cuda", dtype=torch.int32))
+        assert status() == 8 and math.isfinite(float(r.loss))
+    assert status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_preference_from_logits_to_logits(dtype):
+    """The three calls in a row, as a step makes them, against the gradient of the whole by differentiation in 64 bits."""
+    B, T, V = 6, 40, 3000
+    z, t = make(B * T, V, dtype, pitch=8, seed=9, masked=0.3)
+    offsets = (torch.arange(B + 1) * T).int().cuda()
+    ref = fb.token_logprobs(z + 0.1 * torch.randn_like(z), t).logp
+    s = fb.token_logprobs(z, t, temperature=0.875)
+    r = fb.preference_loss(s.logp, offsets, targets0=t, ref_logp=ref, beta=0.375)
+    d = fb.token_logprobs_gradient(z, t, r.dlogp, temperature=0.875)
+    x = z.double().requires_grad_()
+    ls = torch.log_softmax(x / 0.875, 1).gather(1, t.clamp(min=0).long()[:, None])[:, 0]
+    gap = torch.where(t >= 0, ls - ref.double(), 0.0).view(B, T).sum(1)
+    loss = -torch.nn.functional.logsigmoid(0.375 * (gap[0::2] - gap[1::2])).mean()
+    want, = torch.autograd.grad(loss, x)
+    p, onehot = torch.softmax(x.detach() / 0.875, 1), torch.nn.functional.one_hot(t.clamp(min=0).long(), V)
+    size = 0.125 / 0.875 * (p + onehot)      # |d loss / d lp| <= beta / pairs
+    dlp = T * 2 * (slack(V) + 2.0 ** -23 * 30)
+    assert abs(float(r.loss) - float(loss)) <= 0.375 * 2 * dlp + 1e-6
+    near(d, want, half_step(dtype) * 1.01 * want.abs() + size * (dlp + 4 * slack(V) + 2.0 ** -20), "dlogits")
+
+
+def test_tensors_as_the_model_gives_them():
+    """[B][T][V] logits of the model call, slices of a padded vocabulary, and arrays that are not contiguous."""
+    z, t = make(6, 500, torch.float32, pitch=12, seed=10)
+    z3, t3 = z.unflatten(0, (2, 3)), t.view(2, 3)
+    A = torch.tensor([1.0, -1.0], device="cuda")[:, None].expand(2, 3)
+    old = torch.full((3, 2), -6.0, device="cuda").t()
+    r = fb.policy_loss(z3, t3, old, A)
+    want = fb.policy_loss(z.contiguous(), t, old.flatten(), A.flatten())
+    assert r.dlogits.shape == z3.shape and torch.equal(r.dlogits.flatten(0, 1), want.dlogits) and torch.equal(r.loss, want.loss)
+    one = fb.token_logprobs(z[0], t[0])
+    assert one.logp.shape == () and torch.equal(one.logp, fb.token_logprobs(z, t).logp[0])

@@ -1,0 +1,107 @@
+"""What the objectives refuse, checked without a GPU: no call below reaches a launch."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+import femtochat_b200 as fb
+from femtochat_b200 import _lib
+
+BASE = 1 << 20      # stands for device memory that nobody reads
+
+
+def at(i):
+    return C.c_void_p(BASE * (i + 1))
+
+
+def rows(**change):
+    a = dict(dtype=1, logits=at(0), ldl=100, targets0=at(1), N=4, V=100)
+    a.update(change)
+    return a
+
+
+def logprobs(temperature=1.0, logp=at(2), **change):
+    a = rows(**change)
+    return _lib.lib().femto_token_logprobs(a["dtype"], a["logits"], a["ldl"], a["targets0"], a["N"], a["V"], temperature, logp, None, None)
+
+
+def gradient(dlogits=at(3), ldd=100, dlogp=at(4), dentropy=None, temperature=1.0, **change):
+    a = rows(**change)
+    return _lib.lib().femto_token_logprobs_gradient(a["dtype"], dlogits, ldd, a["logits"], a["ldl"], a["targets0"], a["N"], a["V"], temperature, dlogp, dentropy,
+                                                    None)
+
+
+def policy(old=at(2), adv=at(3), ref=None, token_losses=at(4), logp=at(5), loss=at(6), n_valid=at(7), dlogits=at(8), ldd=100, cfg=(1.0, 0.2, 0.2, 0.0, 0), **change):
+    a = rows(**change)
+    c = None if cfg is None else C.byref(_lib.PolicyConfigC(*cfg))
+    return _lib.lib().femto_policy_loss(a["dtype"], a["logits"], a["ldl"], a["targets0"], a["N"], a["V"], old, adv, ref, None, c, dlogits, ldd, token_losses, logp,
+                                        loss, n_valid, None, None)
+
+
+def preference(logp=at(0), N=10, offsets=at(1), P=2, cfg=(0, 0.1, 0.0, 0.0, 0, 1), loss=at(2), pair_losses=at(3), ratios=at(4)):
+    c = None if cfg is None else C.byref(_lib.PreferenceConfigC(*cfg))
+    return _lib.lib().femto_preference_loss(logp, None, None, N, offsets, P, c, loss, pair_losses, ratios, None, None)
+
+
+ARG, SHAPE, ALIGN = -1, -2, -3
+
+
+@pytest.mark.parametrize("call", [logprobs, gradient, policy])
+@pytest.mark.parametrize("change,code", [(dict(dtype=2), ARG), (dict(dtype=-1), ARG), (dict(logits=None), ARG), (dict(targets0=None), ARG), (dict(N=-1), SHAPE),
+                                         (dict(V=0), SHAPE), (dict(ldl=99), SHAPE), (dict(logits=C.c_void_p(BASE + 1)), ALIGN)])
+def test_rows_that_are_refused(call, change, code):
+    assert call(**change) == code
+    assert _lib.lib().femto_last_error(None)
+
+
+def test_log_probabilities_refuse():
+    for t in (0.0, -1.0, math.inf, math.nan):
+        assert logprobs(temperature=t) == ARG and gradient(temperature=t) == ARG
+    assert logprobs(logp=None) == ARG
+    assert gradient(dlogits=None) == ARG and gradient(dlogp=None) == ARG
+    assert gradient(ldd=99) == SHAPE
+    assert gradient(dlogits=C.c_void_p(3 * BASE + 1)) == ALIGN
+
+
+def test_a_gradient_in_place_has_the_same_rows():
+    for call in (gradient, policy):
+        assert call(dlogits=at(0), ldd=101) == ARG                          # the logits' place with another pitch
+        assert call(dlogits=C.c_void_p(BASE + 2)) == ARG                    # one element on
+        assert call(dlogits=C.c_void_p(BASE - 2 * 399)) == ARG              # its last element is the first logit
+
+
+def test_policy_refuses():
+    for name in ("old", "adv", "token_losses", "logp", "loss", "n_valid", "cfg"):
+        assert policy(**{name: None}) == ARG, name
+    for cfg in ((0.0, 0.2, 0.2, 0.0, 0), (1.0, -0.1, 0.2, 0.0, 0), (1.0, 1.1, 0.2, 0.0, 0), (1.0, 0.2, -0.2, 0.0, 0), (1.0, math.nan, 0.2, 0.0, 0),
+                (1.0, 0.2, math.nan, 0.0, 0), (1.0, 0.2, 0.2, -1.0, 0), (1.0, 0.2, 0.2, math.inf, 0), (1.0, 0.2, 0.2, 0.1, 0), (1.0, 0.2, 0.2, 0.0, 2)):
+        assert policy(cfg=cfg) == ARG, cfg
+
+
+def test_preference_refuses():
+    for name in ("logp", "offsets", "loss", "pair_losses", "ratios", "cfg"):
+        assert preference(**{name: None}) == ARG, name
+    assert preference(N=-1) == SHAPE and preference(P=-1) == SHAPE and preference(P=1 << 30) == SHAPE
+    for cfg in ((2, 0.1, 0, 0, 0, 1), (0, 0.0, 0, 0, 0, 1), (0, math.nan, 0, 0, 0, 1), (0, 0.1, math.inf, 0, 0, 1), (0, 0.1, 0, 1.5, 0, 1), (0, 0.1, 0, -0.1, 0, 1),
+                (1, 0.1, 0.5, 0, 0, 1), (1, 0.1, 0, 0.1, 0, 1), (0, 0.1, 0, 0, 0, 2)):
+        assert preference(cfg=cfg) == ARG, cfg
+
+
+def test_python_refuses_what_is_not_on_the_device():
+    z, t = torch.zeros(2, 5), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA"):
+        fb.token_logprobs(z, t)
+    with pytest.raises(ValueError, match="float32 or bfloat16"):
+        fb.token_logprobs(z.double(), t)
+    with pytest.raises(ValueError, match="CUDA"):
+        fb.preference_loss(torch.zeros(3), torch.tensor([0, 1, 3], dtype=torch.int32))
+
+
+def test_python_refuses_options():
+    from femtochat_b200 import objectives
+    with pytest.raises(ValueError, match="reduction"):
+        objectives._policy_config(0.2, 0.2, 0.0, 1.0, "none")
+    with pytest.raises(ValueError, match="kind"):
+        objectives._preference_config("hinge", 0.1, 0.0, 0.0, False, "mean")
+    assert objectives._policy_config(0.2, None, 0.0, 1.0, "sum").clip_high == math.inf
