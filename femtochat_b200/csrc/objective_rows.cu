@@ -1,0 +1,560 @@
+// Passes over rows of logits for the objectives on a model's own answers: softmax statistics, what they give for the row's token (its
+// log-probability, the entropy, the policy term), and the gradient by the logits, from one reading of the row.
+//
+// Two kernels.  k_rows holds a row in registers, of a few warps or (few rows) of a cluster of blocks; it takes narrow rows and few rows.
+// k_rows_ring brings wide rows through a ring in shared memory; it takes many wide rows.  Both give a warp's exponentials relative to a
+// maximum of its own, add the warps' (m, l, a) in a fixed order, and are bound by HBM: every logit is read once and its gradient written once.
+#include <algorithm>
+
+#include "objectives.cuh"
+#include "sm100_ptx.cuh"
+
+namespace {
+using namespace sm100;
+
+// Bit 1: a target outside the vocabulary (its row counts as one without a target); bit 2: a bounded wait ran out.  Part of the library
+// image, so that no call allocates; femto_status_word(NULL, ..) reads and clears it.
+__device__ unsigned int g_rows_status = 0;
+
+// The row's target, or -1 where it has none.
+__device__ __forceinline__ int checked_target(const RowsArgs& p, int t, bool flag) {
+  if (t >= p.V) { if (flag) atomicOr(&g_rows_status, ST_BAD_TOKEN); return -1; }
+  return t < 0 ? -1 : t;
+}
+
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) { uint64_t v; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b)); return v; }
+
+// A word that is there, or `none`.  One instruction each, volatile: with a branch around a plain load the compiler put every word's arithmetic
+// between its load and the next one's, and a thread waited for its words one after the other (8192 x 4096 in fp32: 44 -> 58 us).
+__device__ __forceinline__ uint4 load_word(const uint4* p, bool there, uint32_t none) {
+  uint4 q = make_uint4(none, none, none, none);
+  asm volatile("{\n.reg .pred there;\nsetp.ne.u32 there, %5, 0;\n@there ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n}"
+               : "+r"(q.x), "+r"(q.y), "+r"(q.z), "+r"(q.w) : "l"(p), "r"((uint32_t)there) : "memory");
+  return q;
+}
+
+// A 16-byte word of logits: its pairs in fp32, its largest element, and back.
+template <typename T> struct Word {
+  static constexpr int n = VecN<T>::n;
+  static constexpr uint32_t LEAST = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;      // -inf
+  static __device__ __forceinline__ uint64_t get(const uint4& q, int i) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    if constexpr (sizeof(T) == 4) return pack2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+    else return pack2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+  }
+  static __device__ __forceinline__ void put(uint4& q, int i, uint64_t v) {
+    float lo, hi;
+    unpack2(v, lo, hi);
+    uint32_t* w = reinterpret_cast<uint32_t*>(&q);
+    if constexpr (sizeof(T) == 4) { w[2 * i] = __float_as_uint(lo); w[2 * i + 1] = __float_as_uint(hi); }
+    else {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  static __device__ __forceinline__ float most(const uint4& q) {
+    if constexpr (sizeof(T) == 4)
+      return fmaxf(fmaxf(__uint_as_float(q.x), __uint_as_float(q.y)), fmaxf(__uint_as_float(q.z), __uint_as_float(q.w)));
+    else {
+      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&q);
+      const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+      return fmaxf(__low2float(m), __high2float(m));
+    }
+  }
+};
+
+// Where a row's 16-byte words lie.  The elements before the first and behind the last whole word belong to threads of the row's own.
+struct RowShape {
+  int head, nvec, tail;
+};
+template <typename T> __device__ __forceinline__ RowShape row_shape(const T* p, int V) {
+  RowShape r;
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+  r.head = min(V, (int)(((16u - (a & 15u)) & 15u) / sizeof(T)));
+  r.nvec = (V - r.head) / VecN<T>::n;
+  r.tail = V - r.head - r.nvec * VecN<T>::n;
+  return r;
+}
+// The element outside the words that thread i of the row takes, or -1.
+template <typename T> __device__ __forceinline__ int edge_of(const RowShape& r, int i) {
+  return i < r.head ? i : i >= 16 && i < 16 + r.tail ? r.head + r.nvec * VecN<T>::n + i - 16 : -1;
+}
+
+// Adds pairs of logits to a thread's sums, relative to an exponent.
+template <bool ENTROPY> struct Adder {
+  uint64_t c2, r2, l2 = 0, a2 = 0;
+  __device__ __forceinline__ void at(const Exponent& x) { c2 = pack2(x.c, x.c); r2 = pack2(-x.r, -x.r); l2 = a2 = 0; }
+  __device__ __forceinline__ void add(uint64_t z2) {
+    float u0, u1;
+    const uint64_t u2 = fma2(z2, c2, r2);
+    unpack2(u2, u0, u1);
+    const uint64_t e2 = pack2(exp2_fast(u0), exp2_fast(u1));
+    l2 = add2(l2, e2);
+    if (ENTROPY) a2 = fma2(e2, pack2(fmaxf(u0, LEAST_U), fmaxf(u1, LEAST_U)), a2);
+  }
+  // The sums so far join the statistics, which are rebased to m first; x is the exponent of m.
+  __device__ __forceinline__ void join(RowStats& s, const Exponent& x) {
+    float l0, l1, a0, a1;
+    unpack2(l2, l0, l1);
+    unpack2(a2, a0, a1);
+    const float f = exp2_fast(x.d), l = l0 + l1;
+    s.l = fmaf(f, l, s.l);
+    if (ENTROPY) s.a = fmaf(f, fmaf(l, x.d, a0 + a1), s.a);
+  }
+};
+
+// The statistics of `slots` warps (m, l, a in three runs of `pitch`), by every warp that calls it: fixed order, the same bits in all.
+template <bool ENTROPY> __device__ __forceinline__ RowStats merged_parts(const float* part, int pitch, int slots, float c) {
+  const int lane = threadIdx.x & 31;
+  RowStats r;
+  for (int i = lane; i < slots; i += 32) r.m = fmaxf(r.m, part[i]);
+  r.m = warp_max(r.m);
+  for (int i = lane; i < slots; i += 32) {
+    RowStats y;
+    y.m = part[i]; y.l = part[pitch + i]; y.a = ENTROPY ? part[2 * pitch + i] : 0.f;
+    rebase<ENTROPY>(y, r.m, c);
+    r.l += y.l;
+    if (ENTROPY) r.a += y.a;
+  }
+  r.l = warp_sum(r.l);
+  if (ENTROPY) r.a = warp_sum(r.a);
+  return r;
+}
+
+// What a row's token needs beside the statistics, asked for before the row is read.
+struct RowNumbers {
+  float z = 0.f, x[4] = {0.f, 0.f, 0.f, 1.f};
+};
+template <typename T, RowsMode MODE, bool ENTROPY> __device__ __forceinline__ RowNumbers row_numbers(const RowsArgs& p, long long row, const T* z, int t) {
+  RowNumbers r;
+  if (MODE != GRADIENT) r.z = to_f<T>(z[t]);
+  if (MODE == GRADIENT) { r.x[0] = p.dlogp[row]; if (ENTROPY) r.x[1] = p.dent[row]; }
+  if (MODE == POLICY) {
+    r.x[0] = p.old[row]; r.x[1] = p.adv[row];
+    if (p.term.kl != 0.f) r.x[2] = p.ref[row];
+    if (p.w) r.x[3] = p.w[row];
+  }
+  return r;
+}
+// The row's numbers go out (where `write`), and (g, h) of its gradient come back.
+template <RowsMode MODE, bool ENTROPY>
+__device__ __forceinline__ float2 row_result(const RowsArgs& p, long long row, const RowStats& s, const RowNumbers& k, float scale, bool write) {
+  if (MODE == LOGPROBS) {
+    if (write) {
+      p.logp[row] = log_prob(s, k.z, p.c);
+      if (ENTROPY) p.ent[row] = entropy(s);
+    }
+    return make_float2(0.f, 0.f);
+  }
+  if (MODE == GRADIENT) return make_float2(k.x[0] * p.inv_t, ENTROPY ? k.x[1] * p.inv_t * (float)LN2 : 0.f);
+  const float lp = log_prob(s, k.z, p.c);
+  float loss, slope;
+  policy_token(p.term, lp, k.x[0], k.x[1], k.x[2], k.x[3], &loss, &slope);
+  if (write) { p.token_losses[row] = loss; p.logp[row] = lp; }
+  return make_float2(slope * scale * p.inv_t, 0.f);
+}
+template <RowsMode MODE, bool ENTROPY> __device__ __forceinline__ void row_without_target(const RowsArgs& p, long long row) {
+  if (MODE == LOGPROBS) { p.logp[row] = 0.f; if (ENTROPY) p.ent[row] = 0.f; }
+  if (MODE == POLICY) p.logp[row] = p.token_losses[row] = 0.f;
+}
+
+// dz_j = g (1[j = t] - p_j) - h p_j (u_j - a / l), where log p + H = ln2 (u - a / l).  A row without a distribution has no gradient.
+template <typename T, bool ENTROPY> struct Slope {
+  static constexpr int n = VecN<T>::n;
+  uint64_t c2, r2, k2, h2;
+  float at_target;
+  int t;
+  __device__ __forceinline__ Slope(const RowStats& s, float2 gh, float c, int target) : t(target) {
+    const Exponent x = exponent_of(s.m, c);
+    const bool none = s.l == 0.f;
+    const float inv_l = exp2_fast(x.d) / s.l;
+    const float k = none ? 0.f : -(ENTROPY ? gh.x + gh.y * (x.d - s.a / s.l) : gh.x) * inv_l, h = none ? 0.f : -gh.y * inv_l;
+    c2 = pack2(x.c, x.c); r2 = pack2(-x.r, -x.r); k2 = pack2(k, k); h2 = pack2(h, h);
+    at_target = none ? 0.f : gh.x;
+  }
+  __device__ __forceinline__ uint64_t of(uint64_t z2) const {
+    float u0, u1;
+    unpack2(fma2(z2, c2, r2), u0, u1);
+    const uint64_t e2 = pack2(exp2_fast(u0), exp2_fast(u1));
+    return mul2(e2, ENTROPY ? fma2(h2, pack2(fmaxf(u0, LEAST_U), fmaxf(u1, LEAST_U)), k2) : k2);
+  }
+  // word v of the row, whose first element is j
+  __device__ __forceinline__ void store_word(T* d, int head, int v, const uint4& q, bool same) const {
+    const int j = head + v * n;
+    uint64_t y[n / 2];
+#pragma unroll
+    for (int i = 0; i < n / 2; i++) y[i] = of(Word<T>::get(q, i));
+    if ((unsigned)(t - j) < (unsigned)n)
+#pragma unroll
+      for (int i = 0; i < n / 2; i++) y[i] = add2(y[i], pack2(j + 2 * i == t ? at_target : 0.f, j + 2 * i + 1 == t ? at_target : 0.f));
+    if (same) {
+      uint4 o;
+#pragma unroll
+      for (int i = 0; i < n / 2; i++) Word<T>::put(o, i, y[i]);
+      reinterpret_cast<uint4*>(d + head)[v] = o;
+    } else {
+#pragma unroll
+      for (int i = 0; i < n / 2; i++) {
+        float lo, hi;
+        unpack2(y[i], lo, hi);
+        d[j + 2 * i] = from_f<T>(lo);
+        d[j + 2 * i + 1] = from_f<T>(hi);
+      }
+    }
+  }
+  __device__ __forceinline__ void store_edge(T* d, int at, float z) const {
+    float lo, hi;
+    unpack2(of(pack2(z, z)), lo, hi);
+    d[at] = from_f<T>(lo + (at == t ? at_target : 0.f));
+  }
+};
+// Words of the gradient may be stored whole where they lie as the logits' do.
+template <typename T> __device__ __forceinline__ bool same_phase(const T* z, const T* d) {
+  return ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0;
+}
+
+__device__ __forceinline__ uint32_t cluster_size() { uint32_t n; asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n)); return n; }
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void store_remote(const void* local, uint32_t rank, float v) {
+  uint32_t there;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(smem_u32(local)), "r"(rank));
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(v) : "memory");
+}
+__device__ __forceinline__ void group_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+
+// ---- rows in registers ------------------------------------------------------------------------------------------------------------------------
+// `W` warps share a row; a block has several such groups, which walk the rows in turn.  Clusters (few rows): one group a block, the cluster's
+// blocks share one row, and the statistics of all warps go to every block's shared memory.  A row takes at most C * W * 32 * NV words.
+constexpr int ROWS_WARPS = 8, MOST_CLUSTER = 8;
+
+template <typename T, RowsMode MODE, bool STORE, bool ENTROPY, int NV>
+__global__ void __launch_bounds__(32 * ROWS_WARPS) k_rows(const RowsArgs p, const int W) {
+  pdl_trigger();
+  __shared__ float part[2][3][MOST_CLUSTER * ROWS_WARPS];
+  __shared__ float2 slope_s[ROWS_WARPS];
+  const int C = (int)cluster_size(), rank = (int)cluster_rank();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = warp / W, groups = (blockDim.x >> 5) / W;
+  const int threads = W * 32, tid = threadIdx.x - group * threads, first_warp = group * W;
+  const bool one = warp == first_warp;      // of a group: it works the slopes out; of the first block: it writes the row's numbers
+  if (C > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");      // this block runs: its shared memory may be written
+  const float scale = MODE == POLICY && p.n_valid ? 1.f / (float)p.n_valid[0] : 1.f;
+  const long long step = (long long)(gridDim.x / C) * groups;
+  long long row = (long long)(blockIdx.x / C) * groups + group;
+  int t_next = row < p.N ? p.tgt0[row] : 0, turn = 0;
+  for (; row < p.N; row += step, turn ^= 1) {
+    const int t = checked_target(p, t_next, rank == 0 && tid == 0);
+    if (row + step < p.N) t_next = p.tgt0[row + step];
+    const T* z = reinterpret_cast<const T*>(p.logits) + row * p.ldl;
+    T* d = reinterpret_cast<T*>(p.dlogits) + row * p.ldd;
+    const RowShape r = row_shape<T>(STORE && t < 0 ? d : z, p.V);      // the logits', or, where they are not read, the gradient's
+    const int per = (r.nvec + C - 1) / C, first = min(r.nvec, rank * per), last = min(r.nvec, first + per);
+    const int at = rank == 0 ? edge_of<T>(r, tid) : -1;
+    if (t < 0) {
+      if (C > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+      if (rank == 0 && tid == 0) row_without_target<MODE, ENTROPY>(p, row);
+      if (STORE) {
+        for (int v = first + tid; v < last; v += threads) reinterpret_cast<uint4*>(d + r.head)[v] = make_uint4(0, 0, 0, 0);
+        if (at >= 0) d[at] = from_f<T>(0.f);
+      }
+      continue;
+    }
+    const uint4* words = reinterpret_cast<const uint4*>(z + r.head);
+    uint4 q[NV];
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+      const int v = first + k * threads + tid;
+      q[k] = load_word(words + v, v < last, Word<T>::LEAST);
+    }
+    RowNumbers numbers;
+    if (one) numbers = row_numbers<T, MODE, ENTROPY>(p, row, z, t);
+    const float edge = at >= 0 ? to_f<T>(z[at]) : -INFINITY;
+
+    RowStats s;
+    s.m = edge;
+#pragma unroll
+    for (int k = 0; k < NV; k++) s.m = fmaxf(s.m, Word<T>::most(q[k]));
+    s.m = warp_max(s.m);
+    {
+      const Exponent x = exponent_of(s.m, p.c);
+      Adder<ENTROPY> sum;
+      sum.at(x);
+      if (at >= 0) sum.add(pack2(edge, -INFINITY));
+#pragma unroll
+      for (int k = 0; k < NV; k++)
+#pragma unroll
+        for (int i = 0; i < VecN<T>::n / 2; i++) sum.add(Word<T>::get(q[k], i));
+      sum.join(s, x);
+    }
+    s.l = warp_sum(s.l);
+    if (ENTROPY) s.a = warp_sum(s.a);
+    if (W * C > 1) {
+      float* mine = part[turn][0];      // two buffers in turn: warps that are done with a row may be one row ahead of the one that adds it up
+      constexpr int pitch = MOST_CLUSTER * ROWS_WARPS;
+      if (C > 1) {
+        asm volatile("barrier.cluster.wait.acquire;" ::: "memory");      // all blocks run
+        const int slot = rank * W + warp;
+        if (lane < C) {
+          store_remote(mine + slot, lane, s.m); store_remote(mine + pitch + slot, lane, s.l);
+          if (ENTROPY) store_remote(mine + 2 * pitch + slot, lane, s.a);
+        }
+        asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+      } else {
+        if (lane == 0) { mine[warp] = s.m; mine[pitch + warp] = s.l; if (ENTROPY) mine[2 * pitch + warp] = s.a; }
+        group_barrier(1 + group, threads);
+        mine += first_warp;
+      }
+      if (STORE || one) s = merged_parts<ENTROPY>(mine, pitch, W * C, p.c);
+    }
+    float2 gh = make_float2(0.f, 0.f);
+    if (one) gh = row_result<MODE, ENTROPY>(p, row, s, numbers, scale, rank == 0 && lane == 0);
+    if (!STORE) continue;
+    if (W > 1) {
+      if (one && lane == 0) slope_s[group] = gh;
+      group_barrier(1 + group, threads);
+      gh = slope_s[group];
+    }
+    const Slope<T, ENTROPY> slope(s, gh, p.c, t);
+    const bool same = same_phase(z, d);
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+      const int v = first + k * threads + tid;
+      if (v < last) slope.store_word(d, r.head, v, q[k], same);
+    }
+    if (at >= 0) slope.store_edge(d, at, edge);
+  }
+}
+
+// ---- rows through a ring in shared memory -----------------------------------------------------------------------------------------------------
+// One block a multiprocessor: a warp brings the words of its rows in chunks (bulk copies, an mbarrier each), two groups of twelve warps take the
+// rows in turn, so that one's pass over a row goes on while the other works out its slopes or writes its gradient.  A row that the ring
+// holds (KEEP) is read once: its chunks are given back as its gradient is written.  A wider one is brought twice, the second time
+// behind the next row's first, from L2.
+constexpr int GROUP_WARPS = 12, GROUP_THREADS = 32 * GROUP_WARPS, CHUNK = 2 * GROUP_THREADS, SLOTS = 18;
+constexpr size_t RING_BYTES = (size_t)SLOTS * CHUNK * 16;
+
+__device__ __forceinline__ int next_slot(int slot) { return slot + 1 == SLOTS ? 0 : slot + 1; }
+
+template <typename T, RowsMode MODE, bool STORE, bool ENTROPY, bool KEEP>
+__global__ void __launch_bounds__(2 * GROUP_THREADS + 32) k_rows_ring(const RowsArgs p, const int chunks) {
+  pdl_trigger();
+  extern __shared__ __align__(128) uint4 ring[];
+  __shared__ uint64_t full[2][SLOTS], empty[SLOTS];
+  __shared__ float part[2][2][3][GROUP_WARPS];
+  __shared__ float2 slope_s[2];
+  __shared__ int abort_flag;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < SLOTS; i++) { mbar_init(&full[0][i], 1); mbar_init(&full[1][i], 1); mbar_init(&empty[i], GROUP_WARPS); }
+    abort_flag = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+  // Chunk numbers of a block's k-th row with a target.  Rows that are brought twice: 0, 1, 0 again, 2, 1 again, ..., the last again.
+  auto first_reading = [&](int k) { return KEEP || !STORE ? (long long)k * chunks : k == 0 ? 0ll : (long long)chunks * (2 * k - 1); };
+  auto second_reading = [&](int k, bool last) { return KEEP ? (long long)k * chunks : (long long)chunks * (2 * k + (last ? 1 : 2)); };
+
+  if (warp == 2 * GROUP_WARPS) {      // the warp that brings the rows
+    if (lane != 0) return;
+    int slot = 0, k = 0;
+    uint32_t round = 0, used[2] = {0, 0}, parity[2] = {0, 0};      // bits: slots that a group's barriers have been used for, and how often, modulo 2
+    bool alive = true;
+    auto bring = [&](long long row, int group) {
+      const T* z = reinterpret_cast<const T*>(p.logits) + row * p.ldl;
+      const RowShape r = row_shape<T>(z, p.V);
+      const uint4* words = reinterpret_cast<const uint4*>(z + r.head);
+      for (int c = 0; c < chunks; c++) {
+        if (round > 0) alive = mbar_wait(&empty[slot], (round - 1) & 1u, &abort_flag, &g_rows_status);
+        if (!alive) return;
+        const int n = min(CHUNK, r.nvec - c * CHUNK);
+        if (n > 0) {
+          mbar_expect_tx(&full[group][slot], (uint32_t)n * 16u);
+          bulk_load_1d(ring + (size_t)slot * CHUNK, words + (size_t)c * CHUNK, (uint32_t)n * 16u, &full[group][slot]);
+        } else mbar_arrive(&full[group][slot]);
+        used[group] |= 1u << slot;
+        parity[group] ^= 1u << slot;
+        slot = next_slot(slot);
+        if (slot == 0) round++;
+      }
+    };
+    long long before = -1;      // the row whose second reading is due
+    int t_next = blockIdx.x < p.N ? p.tgt0[blockIdx.x] : -1;
+    for (long long row = blockIdx.x; row < p.N && alive; row += gridDim.x) {
+      const int t = t_next;
+      if (row + gridDim.x < p.N) t_next = p.tgt0[row + gridDim.x];
+      if (t < 0 || t >= p.V) continue;
+      bring(row, k & 1);
+      if (STORE && !KEEP) {
+        if (before >= 0 && alive) bring(before, (k & 1) ^ 1);
+        before = row;
+      }
+      k++;
+    }
+    if (STORE && !KEEP && before >= 0 && alive) bring(before, (k & 1) ^ 1);
+    if (!alive)      // nothing may still be on its way to this block's memory when it ends
+      for (int i = 0; i < 2 * SLOTS; i++)
+        if (used[i / SLOTS] >> (i % SLOTS) & 1u)
+          for (uint32_t polls = 0; polls < WAIT_LIMIT && !mbar_try_wait(&full[i / SLOTS][i % SLOTS], (parity[i / SLOTS] >> (i % SLOTS) & 1u) ^ 1u); polls++) {}
+    return;
+  }
+
+  const int group = warp / GROUP_WARPS, tid = threadIdx.x - group * GROUP_THREADS, gwarp = warp - group * GROUP_WARPS;
+  const float scale = MODE == POLICY && p.n_valid ? 1.f / (float)p.n_valid[0] : 1.f;
+  bool alive = true;      // after a wait that ran out nothing is waited for any more; barriers of the group are
+  // How often the group has waited for each slot, modulo 2.  A group's barriers are its own: of a barrier for both, a group that waits while the
+  // other's row passes through the slot could not tell the phase it waits for from the one before the other's.
+  uint32_t parity = 0;
+  auto wait_full = [&](int slot) {
+    alive = alive && mbar_wait(&full[group][slot], parity >> slot & 1u, &abort_flag, &g_rows_status);
+    parity ^= 1u << slot;
+  };
+  int k = 0, turn = 0, nth = 0;
+  int t_next = blockIdx.x < p.N ? p.tgt0[blockIdx.x] : -1;
+  for (long long row = blockIdx.x; row < p.N; row += gridDim.x, nth++) {
+    const int t = checked_target(p, t_next, threadIdx.x == 0);
+    if (row + gridDim.x < p.N) t_next = p.tgt0[row + gridDim.x];
+    const T* z = reinterpret_cast<const T*>(p.logits) + row * p.ldl;
+    T* d = reinterpret_cast<T*>(p.dlogits) + row * p.ldd;
+    if (t < 0) {
+      if ((nth & 1) != group) continue;
+      if (tid == 0) row_without_target<MODE, ENTROPY>(p, row);
+      if (STORE) {
+        const RowShape r = row_shape<T>(d, p.V);
+        for (int v = tid; v < r.nvec; v += GROUP_THREADS) reinterpret_cast<uint4*>(d + r.head)[v] = make_uint4(0, 0, 0, 0);
+        const int at = edge_of<T>(r, tid);
+        if (at >= 0) d[at] = from_f<T>(0.f);
+      }
+      continue;
+    }
+    const int mine = k++;
+    if ((mine & 1) != group) continue;
+    const RowShape r = row_shape<T>(z, p.V);
+    const int at = edge_of<T>(r, tid);
+    RowNumbers numbers;
+    if (gwarp == 0) numbers = row_numbers<T, MODE, ENTROPY>(p, row, z, t);
+    const float edge = at >= 0 ? to_f<T>(z[at]) : -INFINITY;
+
+    RowStats s;
+    s.m = edge;
+    Exponent x = exponent_of(s.m, p.c);
+    Adder<ENTROPY> sum;
+    sum.at(x);
+    if (at >= 0) sum.add(pack2(edge, -INFINITY));
+    int slot = (int)(first_reading(mine) % SLOTS);
+    for (int c = 0; c < chunks; c++, slot = next_slot(slot)) {
+      wait_full(slot);
+      uint4 q[2];
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        q[h] = make_uint4(Word<T>::LEAST, Word<T>::LEAST, Word<T>::LEAST, Word<T>::LEAST);
+        if (c * CHUNK + h * GROUP_THREADS + tid < r.nvec) q[h] = ring[(size_t)slot * CHUNK + h * GROUP_THREADS + tid];
+      }
+      if (!(KEEP && STORE)) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[slot]);
+      }
+      const float m = fmaxf(Word<T>::most(q[0]), Word<T>::most(q[1]));
+      if (m > s.m) {      // a thread's own maximum grows a few times in a row
+        sum.join(s, x);
+        rebase<ENTROPY>(s, m, p.c);
+        x = exponent_of(m, p.c);
+        sum.at(x);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int i = 0; i < VecN<T>::n / 2; i++) sum.add(Word<T>::get(q[h], i));
+    }
+    sum.join(s, x);
+    rebase<ENTROPY>(s, warp_max(s.m), p.c);
+    s.l = warp_sum(s.l);
+    if (ENTROPY) s.a = warp_sum(s.a);
+    float* parts = part[group][turn][0];
+    turn ^= 1;
+    if (lane == 0) { parts[gwarp] = s.m; parts[GROUP_WARPS + gwarp] = s.l; if (ENTROPY) parts[2 * GROUP_WARPS + gwarp] = s.a; }
+    group_barrier(1 + group, GROUP_THREADS);
+    if (STORE || gwarp == 0) s = merged_parts<ENTROPY>(parts, GROUP_WARPS, GROUP_WARPS, p.c);
+    if (gwarp == 0) {
+      const float2 gh = row_result<MODE, ENTROPY>(p, row, s, numbers, scale, lane == 0);
+      if (STORE && lane == 0) slope_s[group] = gh;
+    }
+    if (!STORE) continue;
+    group_barrier(1 + group, GROUP_THREADS);
+    const Slope<T, ENTROPY> slope(s, slope_s[group], p.c, t);
+    const bool same = same_phase(z, d);
+    bool last = true;
+    if (!KEEP)
+      for (long long i = row + gridDim.x; last && i < p.N; i += gridDim.x) last = p.tgt0[i] < 0 || p.tgt0[i] >= p.V;
+    slot = (int)(second_reading(mine, last) % SLOTS);
+    for (int c = 0; c < chunks; c++, slot = next_slot(slot)) {
+      if (!KEEP) wait_full(slot);
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int v = c * CHUNK + h * GROUP_THREADS + tid;
+        if (v < r.nvec) slope.store_word(d, r.head, v, ring[(size_t)slot * CHUNK + h * GROUP_THREADS + tid], same);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[slot]);
+    }
+    if (at >= 0) slope.store_edge(d, at, edge);
+  }
+}
+
+// ---- launch -----------------------------------------------------------------------------------------------------------------------------------
+template <typename T, RowsMode MODE, bool STORE, bool ENTROPY> int launch(const RowsArgs& p, cudaStream_t s) {
+  const int words = std::max(1, p.V / VecN<T>::n), sms = device_sm_count();
+  constexpr int NV = 8;
+  const int most = ROWS_WARPS * 32 * NV;      // words that a block holds in registers
+  const int chunks = cdiv(words, CHUNK);
+  if ((words > most && p.N >= sms) || words > MOST_CLUSTER * most) {
+    const unsigned grid = (unsigned)std::min(p.N, sms);
+    const bool keep = !STORE || chunks <= SLOTS;
+    if (keep) {
+      FEMTO_TRY((allow_smem<k_rows_ring<T, MODE, STORE, ENTROPY, true>>(RING_BYTES)));
+      k_rows_ring<T, MODE, STORE, ENTROPY, true><<<grid, 2 * GROUP_THREADS + 32, RING_BYTES, s>>>(p, chunks);
+    } else {
+      FEMTO_TRY((allow_smem<k_rows_ring<T, MODE, STORE, ENTROPY, false>>(RING_BYTES)));
+      k_rows_ring<T, MODE, STORE, ENTROPY, false><<<grid, 2 * GROUP_THREADS + 32, RING_BYTES, s>>>(p, chunks);
+    }
+    KERNEL_CHECK();
+    return 0;
+  }
+  int C = 1;
+  while (words > C * most) C *= 2;
+  // few rows: more blocks for each, while a thread keeps a word or more
+  while (C < MOST_CLUSTER && (long long)p.N * C < sms && words > C * 32 * ROWS_WARPS) C *= 2;
+  int W = 1;
+  while (W < ROWS_WARPS && cdiv(words, C) > W * 32 * NV) W *= 2;
+  if (C > 1) W = ROWS_WARPS;
+  const int groups = ROWS_WARPS / W;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = C; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
+  cfg.gridDim = dim3(C > 1 ? (unsigned)(p.N * C) : (unsigned)std::min(cdiv(p.N, groups), sms * 4));
+  cfg.blockDim = dim3(32 * ROWS_WARPS); cfg.stream = s;
+  if (C > 1) { cfg.attrs = &at; cfg.numAttrs = 1; }
+  CUDA_TRY(cudaLaunchKernelEx(&cfg, k_rows<T, MODE, STORE, ENTROPY, NV>, p, W));
+  KERNEL_CHECK();
+  return 0;
+}
+template <RowsMode MODE, bool STORE, bool ENTROPY> int typed(int dtype, const RowsArgs& p, cudaStream_t s) {
+  return dtype == FEMTO_BF16 ? launch<bf16, MODE, STORE, ENTROPY>(p, s) : launch<float, MODE, STORE, ENTROPY>(p, s);
+}
+}  // namespace
+
+int objective_rows(int dtype, RowsMode mode, RowsArgs p, int N, cudaStream_t s) {
+  p.N = N;
+  switch (mode) {
+    case LOGPROBS: return p.ent ? typed<LOGPROBS, false, true>(dtype, p, s) : typed<LOGPROBS, false, false>(dtype, p, s);
+    case GRADIENT: return p.dent ? typed<GRADIENT, true, true>(dtype, p, s) : typed<GRADIENT, true, false>(dtype, p, s);
+    default: return p.dlogits ? typed<POLICY, true, false>(dtype, p, s) : typed<POLICY, false, false>(dtype, p, s);
+  }
+}
+
+// Status word of these kernels on the current device; reading clears it.
+unsigned int objective_rows_status_word() {
+  unsigned int w = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&w, g_rows_status, sizeof(w)) != cudaSuccess) return 0;
+  if (w) cudaMemcpyToSymbol(g_rows_status, &zero, sizeof(zero));
+  return w;
+}

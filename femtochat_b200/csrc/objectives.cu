@@ -8,129 +8,9 @@
 #include "objectives.cuh"
 
 namespace {
-// Bit 1: a target outside the vocabulary (its row counts as one without a target); bit 8: offsets that do not ascend inside the rows (the
-// answer counts as empty).  Part of the library image, so that no call allocates; femto_status_word(NULL, ..) reads and clears it.
+// Bit 8: offsets that do not ascend inside the rows (the answer counts as empty).  Part of the library image, so that no call allocates;
+// femto_status_word(NULL, ..) reads and clears it.
 __device__ unsigned int g_objectives_status = 0;
-
-// The row's target, or -1 where it has none.
-__device__ __forceinline__ int checked_target(const int* tgt0, long long row, int V) {
-  int t = tgt0[row];
-  if (t >= V) { if (threadIdx.x == 0) atomicOr(&g_objectives_status, ST_BAD_TOKEN); t = -1; }
-  return t < 0 ? -1 : t;
-}
-
-// Statistics of one row by the whole block, the same in every thread.
-template <typename T, bool ENTROPY> __device__ RowStats row_stats(const T* z, int V, float c) {
-  __shared__ RowStats part[8];
-  RowStats s;
-  for (int v = threadIdx.x; v < V; v += 256) {
-    const float x = to_f<T>(z[v]);
-    if (x > s.m) rebase<ENTROPY>(s, x, c);
-    const float u = (x - finite_or_zero(s.m)) * c, e = exp2_fast(u);
-    s.l += e;
-    if (ENTROPY) s.a = fmaf(e, fmaxf(u, LEAST_U), s.a);
-  }
-  for (int o = 16; o > 0; o >>= 1) {
-    RowStats y;
-    y.m = __shfl_xor_sync(0xffffffffu, s.m, o);
-    y.l = __shfl_xor_sync(0xffffffffu, s.l, o);
-    y.a = __shfl_xor_sync(0xffffffffu, s.a, o);
-    s = merged<ENTROPY>(s, y, c);
-  }
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
-  __syncthreads();
-  s = part[0];
-  for (int i = 1; i < 8; i++) s = merged<ENTROPY>(s, part[i], c);
-  return s;
-}
-
-template <typename T, bool ENTROPY>
-__global__ void __launch_bounds__(256) k_token_logprobs(const T* __restrict__ logits, long long ldl, const int* __restrict__ tgt0, int V, float c,
-                                                        float* __restrict__ logp, float* __restrict__ ent) {
-  pdl_trigger();
-  const long long row = blockIdx.x;
-  const int t = checked_target(tgt0, row, V);
-  if (t < 0) {
-    if (threadIdx.x == 0) {
-      logp[row] = 0.f;
-      if (ENTROPY) ent[row] = 0.f;
-    }
-    return;
-  }
-  const T* z = logits + row * ldl;
-  const RowStats s = row_stats<T, ENTROPY>(z, V, c);
-  if (threadIdx.x == 0) {
-    logp[row] = log_prob(s, to_f<T>(z[t]), c);
-    if (ENTROPY) ent[row] = entropy(s);
-  }
-}
-
-// dz_j = (1/tau) (dlp (1[j = t] - p_j) - dH p_j (log p_j + H)), in place where dlogits is logits.
-template <typename T, bool ENTROPY>
-__global__ void __launch_bounds__(256) k_token_logprobs_gradient(T* dlogits, long long ldd, const T* logits, long long ldl, const int* __restrict__ tgt0,
-                                                                 int V, float c, float inv_t, const float* __restrict__ dlogp,
-                                                                 const float* __restrict__ dent) {
-  pdl_trigger();
-  const long long row = blockIdx.x;
-  const int t = checked_target(tgt0, row, V);
-  const T* z = logits + row * ldl;
-  T* d = dlogits + row * ldd;
-  RowStats s;
-  if (t >= 0) s = row_stats<T, ENTROPY>(z, V, c);
-  if (s.l == 0.f) {      // no target, or no distribution
-    for (int v = threadIdx.x; v < V; v += 256) d[v] = from_f<T>(0.f);
-    return;
-  }
-  const float g = dlogp[row] * inv_t, inv_l = 1.f / s.l;
-  // log p + H = ln2 (u - a / l)
-  const float h = ENTROPY ? dent[row] * inv_t * (float)LN2 : 0.f, mean_u = ENTROPY ? s.a / s.l : 0.f;
-  for (int v = threadIdx.x; v < V; v += 256) {
-    const float u = (to_f<T>(z[v]) - s.m) * c, p = exp2_fast(u) * inv_l;
-    const float k = ENTROPY ? fmaf(h, fmaxf(u, LEAST_U) - mean_u, g) : g;
-    d[v] = from_f<T>((v == t ? g : 0.f) - k * p);
-  }
-}
-
-struct PolicyRows {
-  const int* tgt0;
-  const float *old, *ref, *adv, *w;
-  float *token_losses, *logp;
-  const int* n_valid;      // mean: the slopes are divided by it
-  PolicyTerm term;
-};
-__device__ __forceinline__ float policy_scale(const int* n_valid) { return n_valid ? 1.f / (float)n_valid[0] : 1.f; }
-
-template <typename T, bool GRADIENT>
-__global__ void __launch_bounds__(256) k_policy_rows(const T* logits, long long ldl, T* dlogits, long long ldd, int V, float c, float inv_t,
-                                                     const PolicyRows p) {
-  pdl_trigger();
-  __shared__ float slope_s;
-  const long long row = blockIdx.x;
-  const int t = checked_target(p.tgt0, row, V);
-  const T* z = logits + row * ldl;
-  T* d = dlogits + row * ldd;
-  if (t < 0) {
-    if (threadIdx.x == 0) p.token_losses[row] = p.logp[row] = 0.f;
-    if (GRADIENT) for (int v = threadIdx.x; v < V; v += 256) d[v] = from_f<T>(0.f);
-    return;
-  }
-  const RowStats s = row_stats<T, false>(z, V, c);
-  if (threadIdx.x == 0) {
-    const float lp = log_prob(s, to_f<T>(z[t]), c);
-    float loss, slope;
-    policy_token(p.term, lp, p.old[row], p.adv[row], p.term.kl != 0.f ? p.ref[row] : 0.f, p.w ? p.w[row] : 1.f, &loss, &slope);
-    p.token_losses[row] = loss;
-    p.logp[row] = lp;
-    slope_s = slope * policy_scale(p.n_valid) * inv_t;
-  }
-  if (!GRADIENT) return;
-  __syncthreads();
-  const float g = slope_s, inv_l = 1.f / s.l;
-  for (int v = threadIdx.x; v < V; v += 256) {
-    const float pj = exp2_fast((to_f<T>(z[v]) - s.m) * c) * inv_l;
-    d[v] = from_f<T>(s.l == 0.f ? 0.f : g * ((v == t ? 1.f : 0.f) - pj));
-  }
-}
 
 // One value for the whole block of 1024 threads: fixed tree.
 template <typename S> __device__ S block_total(S v) {
@@ -153,7 +33,7 @@ __global__ void __launch_bounds__(1024) k_count_targets(const int* __restrict__ 
 }
 
 // Sum (or mean over the rows with a target) of the token losses, and how many tokens the clipping held.
-__global__ void __launch_bounds__(1024) k_policy_sum(const PolicyRows p, int N, int V, int mean, float* __restrict__ loss_out, int* __restrict__ n_valid_out,
+__global__ void __launch_bounds__(1024) k_policy_sum(const RowsArgs p, int N, int V, int mean, float* __restrict__ loss_out, int* __restrict__ n_valid_out,
                                                      int* __restrict__ n_clipped_out) {
   pdl_trigger();
   float sum = 0.f;
@@ -264,7 +144,7 @@ unsigned int objectives_status_word() {
   unsigned int w = 0, zero = 0;
   if (cudaMemcpyFromSymbol(&w, g_objectives_status, sizeof(w)) != cudaSuccess) return 0;
   if (w) cudaMemcpyToSymbol(g_objectives_status, &zero, sizeof(zero));
-  return w;
+  return w | objective_rows_status_word();
 }
 
 // ---- checks of arguments ------------------------------------------------------------------------------------------------------------------
@@ -296,30 +176,11 @@ int check_temperature(float t) {
 }
 float log2e_over(float temperature) { return (float)(1.4426950408889634074 / (double)temperature); }
 
-template <typename T>
-int token_logprobs(const void* logits, long long ldl, const int* tgt0, int N, int V, float temperature, float* logp, float* ent, cudaStream_t s) {
-  const float c = log2e_over(temperature);
-  if (ent) k_token_logprobs<T, true><<<N, 256, 0, s>>>((const T*)logits, ldl, tgt0, V, c, logp, ent);
-  else k_token_logprobs<T, false><<<N, 256, 0, s>>>((const T*)logits, ldl, tgt0, V, c, logp, ent);
-  KERNEL_CHECK();
-  return 0;
-}
-template <typename T>
-int token_logprobs_gradient(void* dlogits, long long ldd, const void* logits, long long ldl, const int* tgt0, int N, int V, float temperature, const float* dlogp,
-                            const float* dent, cudaStream_t s) {
-  const float c = log2e_over(temperature), inv = 1.f / temperature;
-  if (dent) k_token_logprobs_gradient<T, true><<<N, 256, 0, s>>>((T*)dlogits, ldd, (const T*)logits, ldl, tgt0, V, c, inv, dlogp, dent);
-  else k_token_logprobs_gradient<T, false><<<N, 256, 0, s>>>((T*)dlogits, ldd, (const T*)logits, ldl, tgt0, V, c, inv, dlogp, dent);
-  KERNEL_CHECK();
-  return 0;
-}
-template <typename T>
-int policy_rows(const void* logits, long long ldl, void* dlogits, long long ldd, int N, int V, float temperature, const PolicyRows& p, cudaStream_t s) {
-  const float c = log2e_over(temperature), inv = 1.f / temperature;
-  if (dlogits) k_policy_rows<T, true><<<N, 256, 0, s>>>((const T*)logits, ldl, (T*)dlogits, ldd, V, c, inv, p);
-  else k_policy_rows<T, false><<<N, 256, 0, s>>>((const T*)logits, ldl, nullptr, 0, V, c, inv, p);
-  KERNEL_CHECK();
-  return 0;
+RowsArgs rows_args(const void* logits, long long ldl, const int* tgt0, int V, float temperature) {
+  RowsArgs p = {};
+  p.logits = logits; p.ldl = ldl; p.tgt0 = tgt0; p.V = V;
+  p.c = log2e_over(temperature); p.inv_t = 1.f / temperature;
+  return p;
 }
 }  // namespace
 
@@ -329,9 +190,9 @@ extern "C" int32_t femto_token_logprobs(int32_t dtype, const void* logits, int64
   FEMTO_TRY(check_temperature(temperature));
   if (N == 0) return 0;
   if (!logp) return femto_fail(FEMTO_ERR_ARG, "NULL argument");
-  cudaStream_t s = (cudaStream_t)stream;
-  return dtype == FEMTO_BF16 ? token_logprobs<bf16>(logits, ldl, targets0, N, V, temperature, logp, entropy_out, s)
-                             : token_logprobs<float>(logits, ldl, targets0, N, V, temperature, logp, entropy_out, s);
+  RowsArgs p = rows_args(logits, ldl, targets0, V, temperature);
+  p.logp = logp; p.ent = entropy_out;
+  return objective_rows(dtype, LOGPROBS, p, N, (cudaStream_t)stream);
 }
 
 extern "C" int32_t femto_token_logprobs_gradient(int32_t dtype, void* dlogits, int64_t ldd, const void* logits, int64_t ldl, const int32_t* targets0, int32_t N,
@@ -341,10 +202,9 @@ extern "C" int32_t femto_token_logprobs_gradient(int32_t dtype, void* dlogits, i
   FEMTO_TRY(check_gradient(dtype, dlogits, ldd, logits, ldl, N, V));
   if (N == 0) return 0;
   if (!dlogits || !dlogp) return femto_fail(FEMTO_ERR_ARG, "NULL argument");
-  cudaStream_t s = (cudaStream_t)stream;
-  return dtype == FEMTO_BF16
-             ? token_logprobs_gradient<bf16>(dlogits, ldd, logits, ldl, targets0, N, V, temperature, dlogp, dentropy, s)
-             : token_logprobs_gradient<float>(dlogits, ldd, logits, ldl, targets0, N, V, temperature, dlogp, dentropy, s);
+  RowsArgs p = rows_args(logits, ldl, targets0, V, temperature);
+  p.dlogits = dlogits; p.ldd = ldd; p.dlogp = dlogp; p.dent = dentropy;
+  return objective_rows(dtype, GRADIENT, p, N, (cudaStream_t)stream);
 }
 
 int check_policy(const femto_policy_config* c, const float* ref_logp) {
@@ -369,13 +229,17 @@ extern "C" int32_t femto_policy_loss(int32_t dtype, const void* logits, int64_t 
   if (!loss_out || !n_valid_out || (N > 0 && (!old_logp || !advantages || !token_losses || !logp))) return femto_fail(FEMTO_ERR_ARG, "NULL argument");
   cudaStream_t s = (cudaStream_t)stream;
   const bool mean = h_cfg->reduction == FEMTO_REDUCTION_MEAN;
-  PolicyRows p = {targets0, old_logp, ref_logp, advantages, weights, token_losses, logp, mean ? n_valid_out : nullptr,
-                  {1.f - h_cfg->clip_low, 1.f + h_cfg->clip_high, h_cfg->kl_coef}};
+  RowsArgs p = rows_args(logits, ldl, targets0, V, h_cfg->temperature);
+  p.dlogits = dlogits; p.ldd = ldd; p.logp = logp; p.token_losses = token_losses;
+  p.old = old_logp; p.ref = ref_logp; p.adv = advantages; p.w = weights;
+  p.term = {1.f - h_cfg->clip_low, 1.f + h_cfg->clip_high, h_cfg->kl_coef};
   if (N > 0) {
-    if (mean && dlogits) { k_count_targets<<<1, 1024, 0, s>>>(targets0, N, V, n_valid_out); KERNEL_CHECK(); }
-    else p.n_valid = nullptr;
-    FEMTO_TRY(dtype == FEMTO_BF16 ? policy_rows<bf16>(logits, ldl, dlogits, ldd, N, V, h_cfg->temperature, p, s)
-                                  : policy_rows<float>(logits, ldl, dlogits, ldd, N, V, h_cfg->temperature, p, s));
+    if (mean && dlogits) {
+      k_count_targets<<<1, 1024, 0, s>>>(targets0, N, V, n_valid_out);
+      KERNEL_CHECK();
+      p.n_valid = n_valid_out;
+    }
+    FEMTO_TRY(objective_rows(dtype, POLICY, p, N, s));
   }
   k_policy_sum<<<1, 1024, 0, s>>>(p, N, V, mean, loss_out, n_valid_out, n_clipped_out);
   KERNEL_CHECK();

@@ -5,9 +5,12 @@
 
 // Softmax statistics of a row.  With c = log2(e) / temperature, m = max(z) and u_j = c (z_j - m) <= 0:
 //   l = sum 2^u_j,  a = sum 2^u_j u_j,  log p_j = ln2 u_j - ln l,  H = ln l - ln2 a / l.
-// The difference comes before the product: logits of the type's lowest value stay finite, and a large common offset costs nothing.
 struct RowStats {
   float m = -INFINITY, l = 0.f, a = 0.f;
+};
+
+struct PolicyTerm {
+  float lo, hi, kl;
 };
 
 #ifdef __CUDACC__
@@ -21,6 +24,22 @@ __device__ __forceinline__ float exp2_fast(float x) {   // relative error 2^-22,
 }
 // What a maximum of -inf (nothing seen, or a row without any logit above -inf) is taken as: -inf - 0 gives 2^-inf = 0, where -inf + inf is NaN.
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
+
+// u_j as one fused product: u_j = fma(z_j, c, -r) + d with r = c m rounded and d = r - c m, the same for the whole row, so it is put into
+// what the exponentials are multiplied by.  Where c m leaves the range (rows of the type's lowest value), logits that are not m lie so far
+// below it that any scale gives 0 for them, and a power of two, which rounds nothing, gives 0 exactly for those that are.
+struct Exponent {
+  float c, r, d;
+};
+__device__ __forceinline__ Exponent exponent_of(float m, float c) {
+  Exponent x;
+  m = finite_or_zero(m);
+  const bool far = fabsf(m) > 1e30f && fabsf(m) < INFINITY;
+  x.c = far ? 0x1p-10f : c;
+  x.r = m * x.c;
+  x.d = -fmaf(m, x.c, -x.r);
+  return x;
+}
 
 // Moves statistics to a maximum that is no lower: with d = c (m_old - m_new) every 2^u scales by 2^d and every u moves by d.
 template <bool ENTROPY> __device__ __forceinline__ void rebase(RowStats& s, float m, float c) {
@@ -61,9 +80,6 @@ __device__ __forceinline__ float entropy(const RowStats& s) {
 // loss = w (-min(r A, clamp(r, lo, hi) A) + beta (e^g - g - 1)),  r = e^(lp - old),  g = ref - lp, and its derivative by lp.  The minimum is
 // the bounded product, which does not depend on lp, where A > 0 and r > hi or A < 0 and r < lo.  A weight of 0 counts nothing, whatever
 // the other numbers are.
-struct PolicyTerm {
-  float lo, hi, kl;
-};
 __device__ __forceinline__ bool policy_clipped(const PolicyTerm& t, float r, float A) { return (A > 0.f && r > t.hi) || (A < 0.f && r < t.lo); }
 __device__ __forceinline__ float policy_ratio(float lp, float old) { return expf(lp - old); }
 __device__ __forceinline__ void policy_token(const PolicyTerm& t, float lp, float old, float A, float ref, float w, float* loss, float* slope) {
@@ -81,3 +97,23 @@ __device__ __forceinline__ void policy_token(const PolicyTerm& t, float lp, floa
   *slope = w * d;
 }
 #endif
+
+// ---- passes over rows of logits (objective_rows.cu) ------------------------------------------------------------------------------------------
+enum RowsMode { LOGPROBS, GRADIENT, POLICY };
+
+struct RowsArgs {
+  const void* logits;
+  void* dlogits;                 // GRADIENT, POLICY (NULL there: the numbers only)
+  long long ldl, ldd;
+  const int* tgt0;
+  int V, N;
+  float c, inv_t;                // log2(e) / temperature, 1 / temperature
+  float *logp, *ent;             // LOGPROBS (ent may be NULL), POLICY: logp
+  const float *dlogp, *dent;     // GRADIENT (dent may be NULL)
+  const float *old, *ref, *adv, *w;      // POLICY
+  float* token_losses;
+  const int* n_valid;            // POLICY, mean: the slopes are divided by it
+  PolicyTerm term;
+};
+int objective_rows(int dtype, RowsMode mode, RowsArgs p, int N, cudaStream_t s);
+unsigned int objective_rows_status_word();

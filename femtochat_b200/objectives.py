@@ -87,12 +87,14 @@ def _code(t):
     return _lib.BF16 if t.dtype == torch.bfloat16 else _lib.F32
 
 
-def _gradient_of(logits, out):
-    """The tensor that takes the gradient, and its pitch."""
+def _gradient_of(logits, n, V, pitch, out):
+    """The tensor that takes the gradient, and its pitch: the logits' own where that wastes little, so that rows of both start alike."""
     import torch
     if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
+        if pitch == V or n == 0 or pitch - V > V // 8 + 64:
+            return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), V
+        return torch.empty((n, pitch), dtype=logits.dtype, device=logits.device)[:, :V].view(logits.shape), pitch
+    if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
         raise ValueError("out must have the logits' shape, type and device")
     return out, _rows("out", out)[2]
 
@@ -134,7 +136,7 @@ def token_logprobs_gradient(logits, targets0, dlogp, dentropy=None, temperature:
     shape, f32 = logits.shape[:-1], torch.float32
     targets0 = _on_device("targets0", targets0, torch.int32, shape, logits.device)
     dlogp, dentropy = _on_device("dlogp", dlogp, f32, shape, logits.device), _on_device("dentropy", dentropy, f32, shape, logits.device)
-    out, out_pitch = _gradient_of(logits, out)
+    out, out_pitch = _gradient_of(logits, n, V, pitch, out)
     with _Device(logits.device):
         _lib.check(_lib.lib().femto_token_logprobs_gradient(_code(logits), _lib.ptr(out), out_pitch, _lib.ptr(logits), pitch, _lib.ptr(targets0), n, V,
                                                             temperature, _lib.ptr(dlogp), _lib.ptr(dentropy), _lib.stream_ptr()))
@@ -159,7 +161,7 @@ def policy_loss(logits, targets0, old_logp, advantages, ref_logp=None, weights=N
     old_logp, advantages, ref_logp, weights = (_on_device(name, t, f32, shape, device) for name, t in
                                                (("old_logp", old_logp), ("advantages", advantages), ("ref_logp", ref_logp), ("weights", weights)))
     cfg = _policy_config(clip_low, clip_high, kl_coef, temperature, reduction)
-    d, d_pitch = _gradient_of(logits, out) if gradient else (None, V)
+    d, d_pitch = _gradient_of(logits, n, V, pitch, out) if gradient else (None, V)
     token_losses, logp = torch.empty((2,) + shape, dtype=f32, device=device)
     loss = torch.empty(1, dtype=f32, device=device)
     n_valid, n_clipped = torch.empty(2, 1, dtype=torch.int32, device=device)

@@ -63,8 +63,9 @@ def near(got, want, tol, what):
     assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()}, largest {float((got - want).abs().nan_to_num(1e300).max()):.3e}"
 
 
-# a row that fits a thread, a warp, a block; odd; past every size that one block, or eight together, hold of it
-SHAPES = [(1, 1), (3, 2), (5, 7), (2, 33), (7, 255), (4, 1000), (9, 4099), (150, 4096), (600, 300), (3, 50021), (2, 65536), (1, 131073), (2, 300007)]
+# a row that fits a thread, a warp, a block; odd; past every size that one block, or eight together, hold of it; many wide rows, which
+# come through a ring that holds them (20011, 40000) or not
+SHAPES = [(700, 20011), (310, 40000), (320, 150001), (1, 1), (3, 2), (5, 7), (2, 33), (7, 255), (4, 1000), (9, 4099), (150, 4096), (600, 300), (3, 50021), (2, 65536), (1, 131073), (2, 300007)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
