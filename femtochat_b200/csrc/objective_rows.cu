@@ -138,20 +138,24 @@ template <typename T, RowsMode MODE, bool ENTROPY> __device__ __forceinline__ Ro
 }
 // The row's numbers go out (where `write`), and (g, h) of its gradient come back.
 template <RowsMode MODE, bool ENTROPY>
-__device__ __forceinline__ float2 row_result(const RowsArgs& p, long long row, const RowStats& s, const RowNumbers& k, float scale, bool write) {
+__device__ __forceinline__ float2 row_result(const RowsArgs& p, long long row, const RowStats& s, const RowNumbers& k, bool write) {
   if (MODE == LOGPROBS) {
     if (write) {
-      p.logp[row] = log_prob(s, k.z, p.c);
+      p.logp[row] = log_prob(s, k.z, p.inv_t);
       if (ENTROPY) p.ent[row] = entropy(s);
     }
     return make_float2(0.f, 0.f);
   }
   if (MODE == GRADIENT) return make_float2(k.x[0] * p.inv_t, ENTROPY ? k.x[1] * p.inv_t * (float)LN2 : 0.f);
-  const float lp = log_prob(s, k.z, p.c);
+  const float lp = log_prob(s, k.z, p.inv_t);
   float loss, slope;
   policy_token(p.term, lp, k.x[0], k.x[1], k.x[2], k.x[3], &loss, &slope);
   if (write) { p.token_losses[row] = loss; p.logp[row] = lp; }
-  return make_float2(slope * scale * p.inv_t, 0.f);
+  if (p.n_valid) {      // a kernel of the same call counts the targets beside the first rows
+    pdl_wait();
+    slope *= 1.f / (float)*reinterpret_cast<const volatile int*>(p.n_valid);
+  }
+  return make_float2(slope * p.inv_t, 0.f);
 }
 template <RowsMode MODE, bool ENTROPY> __device__ __forceinline__ void row_without_target(const RowsArgs& p, long long row) {
   if (MODE == LOGPROBS) { p.logp[row] = 0.f; if (ENTROPY) p.ent[row] = 0.f; }
@@ -237,7 +241,6 @@ __global__ void __launch_bounds__(32 * ROWS_WARPS) k_rows(const RowsArgs p, cons
   const int threads = W * 32, tid = threadIdx.x - group * threads, first_warp = group * W;
   const bool one = warp == first_warp;      // of a group: it works the slopes out; of the first block: it writes the row's numbers
   if (C > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");      // this block runs: its shared memory may be written
-  const float scale = MODE == POLICY && p.n_valid ? 1.f / (float)p.n_valid[0] : 1.f;
   const long long step = (long long)(gridDim.x / C) * groups;
   long long row = (long long)(blockIdx.x / C) * groups + group;
   int t_next = row < p.N ? p.tgt0[row] : 0, turn = 0;
@@ -306,7 +309,7 @@ __global__ void __launch_bounds__(32 * ROWS_WARPS) k_rows(const RowsArgs p, cons
       if (STORE || one) s = merged_parts<ENTROPY>(mine, pitch, W * C, p.c);
     }
     float2 gh = make_float2(0.f, 0.f);
-    if (one) gh = row_result<MODE, ENTROPY>(p, row, s, numbers, scale, rank == 0 && lane == 0);
+    if (one) gh = row_result<MODE, ENTROPY>(p, row, s, numbers, rank == 0 && lane == 0);
     if (!STORE) continue;
     if (W > 1) {
       if (one && lane == 0) slope_s[group] = gh;
@@ -325,47 +328,46 @@ __global__ void __launch_bounds__(32 * ROWS_WARPS) k_rows(const RowsArgs p, cons
 }
 
 // ---- rows through a ring in shared memory -----------------------------------------------------------------------------------------------------
-// One block a multiprocessor: a warp brings the words of its rows in chunks (bulk copies, an mbarrier each), two groups of twelve warps take the
-// rows in turn, so that one's pass over a row goes on while the other works out its slopes or writes its gradient.  A row that the ring
-// holds (KEEP) is read once: its chunks are given back as its gradient is written.  A wider one is brought twice, the second time
-// behind the next row's first, from L2.
-constexpr int GROUP_WARPS = 12, GROUP_THREADS = 32 * GROUP_WARPS, CHUNK = 2 * GROUP_THREADS, SLOTS = 18;
-constexpr size_t RING_BYTES = (size_t)SLOTS * CHUNK * 16;
-
-__device__ __forceinline__ int next_slot(int slot) { return slot + 1 == SLOTS ? 0 : slot + 1; }
-
-template <typename T, RowsMode MODE, bool STORE, bool ENTROPY, bool KEEP>
-__global__ void __launch_bounds__(2 * GROUP_THREADS + 32) k_rows_ring(const RowsArgs p, const int chunks) {
+// One block a multiprocessor: a warp brings the words of its rows in chunks (bulk copies, an mbarrier each), and groups of warps take the rows
+// in turn, so that one's pass over a row goes on while another works out its slopes or writes its gradient.  Chunks stay where they are until
+// their gradient is written.  Of a row that the ring does not hold the first chunks are given back at once and brought `again`, behind the
+// row's last: two passes over the ring's length later they are still in L2.
+template <int GROUPS_, int WARPS_, int PER_, int SLOTS_> struct Ring {
+  static constexpr int GROUPS = GROUPS_, WARPS = WARPS_, THREADS = 32 * WARPS_, PER = PER_, CHUNK = PER_ * THREADS, SLOTS = SLOTS_;
+  static constexpr int SPARE = 2;      // slots that a row wider than the ring leaves to what follows
+  static constexpr int BLOCK = GROUPS * THREADS + 32;
+  static constexpr size_t BYTES = (size_t)SLOTS * CHUNK * 16;
+};
+template <typename T, RowsMode MODE, bool STORE, bool ENTROPY, class R>
+__global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const int chunks, const int again) {
+  constexpr int GROUPS = R::GROUPS, GROUP_WARPS = R::WARPS, GROUP_THREADS = R::THREADS, PER_CHUNK = R::PER, CHUNK = R::CHUNK, SLOTS = R::SLOTS;
+  auto next_slot = [](int slot) { return slot + 1 == SLOTS ? 0 : slot + 1; };
   pdl_trigger();
   extern __shared__ __align__(128) uint4 ring[];
-  __shared__ uint64_t full[2][SLOTS], empty[SLOTS];
-  __shared__ float part[2][2][3][GROUP_WARPS];
-  __shared__ float2 slope_s[2];
+  __shared__ uint64_t full[GROUPS][SLOTS], empty[SLOTS];
+  __shared__ float part[GROUPS][2][3][GROUP_WARPS];
+  __shared__ float2 slope_s[GROUPS];
   __shared__ int abort_flag;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < SLOTS; i++) { mbar_init(&full[0][i], 1); mbar_init(&full[1][i], 1); mbar_init(&empty[i], GROUP_WARPS); }
+    for (int i = 0; i < SLOTS; i++) {
+      for (int g = 0; g < GROUPS; g++) mbar_init(&full[g][i], 1);
+      mbar_init(&empty[i], GROUP_WARPS);
+    }
     abort_flag = 0;
     fence_barrier_init();
   }
   __syncthreads();
-  // Chunk numbers of a block's k-th row with a target.  Rows that are brought twice: 0, 1, 0 again, 2, 1 again, ..., the last again.
-  auto first_reading = [&](int k) { return KEEP || !STORE ? (long long)k * chunks : k == 0 ? 0ll : (long long)chunks * (2 * k - 1); };
-  auto second_reading = [&](int k, bool last) { return KEEP ? (long long)k * chunks : (long long)chunks * (2 * k + (last ? 1 : 2)); };
-
-  if (warp == 2 * GROUP_WARPS) {      // the warp that brings the rows
+  if (warp == GROUPS * GROUP_WARPS) {      // the warp that brings the rows
     if (lane != 0) return;
     int slot = 0, k = 0;
-    uint32_t round = 0, used[2] = {0, 0}, parity[2] = {0, 0};      // bits: slots that a group's barriers have been used for, and how often, modulo 2
+    uint32_t round = 0, used[GROUPS] = {}, parity[GROUPS] = {};      // bits: slots that a group's barriers have been used for, and how often, modulo 2
     bool alive = true;
-    auto bring = [&](long long row, int group) {
-      const T* z = reinterpret_cast<const T*>(p.logits) + row * p.ldl;
-      const RowShape r = row_shape<T>(z, p.V);
-      const uint4* words = reinterpret_cast<const uint4*>(z + r.head);
-      for (int c = 0; c < chunks; c++) {
+    auto bring = [&](const uint4* words, int nvec, int n_chunks, int group) {
+      for (int c = 0; c < n_chunks; c++) {
         if (round > 0) alive = mbar_wait(&empty[slot], (round - 1) & 1u, &abort_flag, &g_rows_status);
         if (!alive) return;
-        const int n = min(CHUNK, r.nvec - c * CHUNK);
+        const int n = min(CHUNK, nvec - c * CHUNK);
         if (n > 0) {
           mbar_expect_tx(&full[group][slot], (uint32_t)n * 16u);
           bulk_load_1d(ring + (size_t)slot * CHUNK, words + (size_t)c * CHUNK, (uint32_t)n * 16u, &full[group][slot]);
@@ -376,29 +378,26 @@ __global__ void __launch_bounds__(2 * GROUP_THREADS + 32) k_rows_ring(const Rows
         if (slot == 0) round++;
       }
     };
-    long long before = -1;      // the row whose second reading is due
     int t_next = blockIdx.x < p.N ? p.tgt0[blockIdx.x] : -1;
     for (long long row = blockIdx.x; row < p.N && alive; row += gridDim.x) {
       const int t = t_next;
       if (row + gridDim.x < p.N) t_next = p.tgt0[row + gridDim.x];
       if (t < 0 || t >= p.V) continue;
-      bring(row, k & 1);
-      if (STORE && !KEEP) {
-        if (before >= 0 && alive) bring(before, (k & 1) ^ 1);
-        before = row;
-      }
+      const T* z = reinterpret_cast<const T*>(p.logits) + row * p.ldl;
+      const RowShape r = row_shape<T>(z, p.V);
+      const uint4* words = reinterpret_cast<const uint4*>(z + r.head);
+      bring(words, r.nvec, chunks, k % GROUPS);
+      if (STORE && alive) bring(words, r.nvec, again, k % GROUPS);
       k++;
     }
-    if (STORE && !KEEP && before >= 0 && alive) bring(before, (k & 1) ^ 1);
     if (!alive)      // nothing may still be on its way to this block's memory when it ends
-      for (int i = 0; i < 2 * SLOTS; i++)
+      for (int i = 0; i < GROUPS * SLOTS; i++)
         if (used[i / SLOTS] >> (i % SLOTS) & 1u)
           for (uint32_t polls = 0; polls < WAIT_LIMIT && !mbar_try_wait(&full[i / SLOTS][i % SLOTS], (parity[i / SLOTS] >> (i % SLOTS) & 1u) ^ 1u); polls++) {}
     return;
   }
 
   const int group = warp / GROUP_WARPS, tid = threadIdx.x - group * GROUP_THREADS, gwarp = warp - group * GROUP_WARPS;
-  const float scale = MODE == POLICY && p.n_valid ? 1.f / (float)p.n_valid[0] : 1.f;
   bool alive = true;      // after a wait that ran out nothing is waited for any more; barriers of the group are
   // How often the group has waited for each slot, modulo 2.  A group's barriers are its own: of a barrier for both, a group that waits while the
   // other's row passes through the slot could not tell the phase it waits for from the one before the other's.
@@ -415,7 +414,7 @@ __global__ void __launch_bounds__(2 * GROUP_THREADS + 32) k_rows_ring(const Rows
     const T* z = reinterpret_cast<const T*>(p.logits) + row * p.ldl;
     T* d = reinterpret_cast<T*>(p.dlogits) + row * p.ldd;
     if (t < 0) {
-      if ((nth & 1) != group) continue;
+      if (nth % GROUPS != group) continue;
       if (tid == 0) row_without_target<MODE, ENTROPY>(p, row);
       if (STORE) {
         const RowShape r = row_shape<T>(d, p.V);
@@ -426,7 +425,7 @@ __global__ void __launch_bounds__(2 * GROUP_THREADS + 32) k_rows_ring(const Rows
       continue;
     }
     const int mine = k++;
-    if ((mine & 1) != group) continue;
+    if (mine % GROUPS != group) continue;
     const RowShape r = row_shape<T>(z, p.V);
     const int at = edge_of<T>(r, tid);
     RowNumbers numbers;
@@ -439,20 +438,23 @@ __global__ void __launch_bounds__(2 * GROUP_THREADS + 32) k_rows_ring(const Rows
     Adder<ENTROPY> sum;
     sum.at(x);
     if (at >= 0) sum.add(pack2(edge, -INFINITY));
-    int slot = (int)(first_reading(mine) % SLOTS);
+    const int first_slot = (int)((long long)mine * (chunks + (STORE ? again : 0)) % SLOTS);
+    int slot = first_slot;
     for (int c = 0; c < chunks; c++, slot = next_slot(slot)) {
       wait_full(slot);
-      uint4 q[2];
+      uint4 q[PER_CHUNK];
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
+      for (int h = 0; h < PER_CHUNK; h++) {
         q[h] = make_uint4(Word<T>::LEAST, Word<T>::LEAST, Word<T>::LEAST, Word<T>::LEAST);
         if (c * CHUNK + h * GROUP_THREADS + tid < r.nvec) q[h] = ring[(size_t)slot * CHUNK + h * GROUP_THREADS + tid];
       }
-      if (!(KEEP && STORE)) {
+      if (!STORE || c < again) {
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[slot]);
       }
-      const float m = fmaxf(Word<T>::most(q[0]), Word<T>::most(q[1]));
+      float m = Word<T>::most(q[0]);
+#pragma unroll
+      for (int h = 1; h < PER_CHUNK; h++) m = fmaxf(m, Word<T>::most(q[h]));
       if (m > s.m) {      // a thread's own maximum grows a few times in a row
         sum.join(s, x);
         rebase<ENTROPY>(s, m, p.c);
@@ -460,7 +462,7 @@ __global__ void __launch_bounds__(2 * GROUP_THREADS + 32) k_rows_ring(const Rows
         sum.at(x);
       }
 #pragma unroll
-      for (int h = 0; h < 2; h++)
+      for (int h = 0; h < PER_CHUNK; h++)
 #pragma unroll
         for (int i = 0; i < VecN<T>::n / 2; i++) sum.add(Word<T>::get(q[h], i));
     }
@@ -474,21 +476,19 @@ __global__ void __launch_bounds__(2 * GROUP_THREADS + 32) k_rows_ring(const Rows
     group_barrier(1 + group, GROUP_THREADS);
     if (STORE || gwarp == 0) s = merged_parts<ENTROPY>(parts, GROUP_WARPS, GROUP_WARPS, p.c);
     if (gwarp == 0) {
-      const float2 gh = row_result<MODE, ENTROPY>(p, row, s, numbers, scale, lane == 0);
+      const float2 gh = row_result<MODE, ENTROPY>(p, row, s, numbers, lane == 0);
       if (STORE && lane == 0) slope_s[group] = gh;
     }
     if (!STORE) continue;
     group_barrier(1 + group, GROUP_THREADS);
     const Slope<T, ENTROPY> slope(s, slope_s[group], p.c, t);
     const bool same = same_phase(z, d);
-    bool last = true;
-    if (!KEEP)
-      for (long long i = row + gridDim.x; last && i < p.N; i += gridDim.x) last = p.tgt0[i] < 0 || p.tgt0[i] >= p.V;
-    slot = (int)(second_reading(mine, last) % SLOTS);
-    for (int c = 0; c < chunks; c++, slot = next_slot(slot)) {
-      if (!KEEP) wait_full(slot);
+    slot = (first_slot + again) % SLOTS;
+    for (int i = 0; i < chunks; i++, slot = next_slot(slot)) {
+      const int c = i + again < chunks ? i + again : i + again - chunks;      // those that are still here first
+      if (i + again >= chunks) wait_full(slot);
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
+      for (int h = 0; h < PER_CHUNK; h++) {
         const int v = c * CHUNK + h * GROUP_THREADS + tid;
         if (v < r.nvec) slope.store_word(d, r.head, v, ring[(size_t)slot * CHUNK + h * GROUP_THREADS + tid], same);
       }
@@ -500,23 +500,40 @@ __global__ void __launch_bounds__(2 * GROUP_THREADS + 32) k_rows_ring(const Rows
 }
 
 // ---- launch -----------------------------------------------------------------------------------------------------------------------------------
+typedef Ring<3, 8, 4, 13> Reading;      // numbers only
+typedef Ring<2, 12, 4, 9> Writing;
+
+// Behind the kernel that counts the targets (n_valid) the rows may start at once: nothing else of theirs depends on it, and it started
+// itself when everything before the call was done.  Otherwise the launch is an ordinary one.
+template <typename... P, typename... A>
+int launch_kernel(const RowsArgs& p, void (*kernel)(P...), int C, dim3 grid, int threads, size_t smem, cudaStream_t s, const A&... args) {
+  if (p.n_valid) {
+    CUDA_TRY(launch_dependent_clusters(kernel, C, grid, dim3(threads), smem, s, args...));
+  } else {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = C; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
+    cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = s;
+    cfg.attrs = &at; cfg.numAttrs = C > 1;
+    CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
+  }
+  KERNEL_CHECK();
+  return 0;
+}
+template <typename T, RowsMode MODE, bool STORE, bool ENTROPY, class R> int launch_ring(const RowsArgs& p, int words, cudaStream_t s) {
+  constexpr auto kernel = k_rows_ring<T, MODE, STORE, ENTROPY, R>;
+  const int chunks = cdiv(words, R::CHUNK), again = chunks <= R::SLOTS ? 0 : chunks - (R::SLOTS - R::SPARE);
+  FEMTO_TRY(allow_smem<kernel>(R::BYTES));
+  return launch_kernel(p, kernel, 1, dim3((unsigned)std::min(p.N, device_sm_count())), R::BLOCK, R::BYTES, s, p, chunks, again);
+}
 template <typename T, RowsMode MODE, bool STORE, bool ENTROPY> int launch(const RowsArgs& p, cudaStream_t s) {
   const int words = std::max(1, p.V / VecN<T>::n), sms = device_sm_count();
   constexpr int NV = 8;
   const int most = ROWS_WARPS * 32 * NV;      // words that a block holds in registers
-  const int chunks = cdiv(words, CHUNK);
   if ((words > most && p.N >= sms) || words > MOST_CLUSTER * most) {
-    const unsigned grid = (unsigned)std::min(p.N, sms);
-    const bool keep = !STORE || chunks <= SLOTS;
-    if (keep) {
-      FEMTO_TRY((allow_smem<k_rows_ring<T, MODE, STORE, ENTROPY, true>>(RING_BYTES)));
-      k_rows_ring<T, MODE, STORE, ENTROPY, true><<<grid, 2 * GROUP_THREADS + 32, RING_BYTES, s>>>(p, chunks);
-    } else {
-      FEMTO_TRY((allow_smem<k_rows_ring<T, MODE, STORE, ENTROPY, false>>(RING_BYTES)));
-      k_rows_ring<T, MODE, STORE, ENTROPY, false><<<grid, 2 * GROUP_THREADS + 32, RING_BYTES, s>>>(p, chunks);
-    }
-    KERNEL_CHECK();
-    return 0;
+    if constexpr (STORE) return launch_ring<T, MODE, STORE, ENTROPY, Writing>(p, words, s);
+    else return launch_ring<T, MODE, STORE, ENTROPY, Reading>(p, words, s);
   }
   int C = 1;
   while (words > C * most) C *= 2;
@@ -526,24 +543,15 @@ template <typename T, RowsMode MODE, bool STORE, bool ENTROPY> int launch(const 
   while (W < ROWS_WARPS && cdiv(words, C) > W * 32 * NV) W *= 2;
   if (C > 1) W = ROWS_WARPS;
   const int groups = ROWS_WARPS / W;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute at;
-  at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim.x = C; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
-  cfg.gridDim = dim3(C > 1 ? (unsigned)(p.N * C) : (unsigned)std::min(cdiv(p.N, groups), sms * 4));
-  cfg.blockDim = dim3(32 * ROWS_WARPS); cfg.stream = s;
-  if (C > 1) { cfg.attrs = &at; cfg.numAttrs = 1; }
-  CUDA_TRY(cudaLaunchKernelEx(&cfg, k_rows<T, MODE, STORE, ENTROPY, NV>, p, W));
-  KERNEL_CHECK();
-  return 0;
+  const dim3 grid(C > 1 ? (unsigned)(p.N * C) : (unsigned)std::min(cdiv(p.N, groups), sms * 4));
+  return launch_kernel(p, k_rows<T, MODE, STORE, ENTROPY, NV>, C, grid, 32 * ROWS_WARPS, 0, s, p, W);
 }
 template <RowsMode MODE, bool STORE, bool ENTROPY> int typed(int dtype, const RowsArgs& p, cudaStream_t s) {
   return dtype == FEMTO_BF16 ? launch<bf16, MODE, STORE, ENTROPY>(p, s) : launch<float, MODE, STORE, ENTROPY>(p, s);
 }
 }  // namespace
 
-int objective_rows(int dtype, RowsMode mode, RowsArgs p, int N, cudaStream_t s) {
-  p.N = N;
+int objective_rows(int dtype, RowsMode mode, const RowsArgs& p, cudaStream_t s) {
   switch (mode) {
     case LOGPROBS: return p.ent ? typed<LOGPROBS, false, true>(dtype, p, s) : typed<LOGPROBS, false, false>(dtype, p, s);
     case GRADIENT: return p.dent ? typed<GRADIENT, true, true>(dtype, p, s) : typed<GRADIENT, true, false>(dtype, p, s);

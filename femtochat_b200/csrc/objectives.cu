@@ -33,17 +33,18 @@ __global__ void __launch_bounds__(1024) k_count_targets(const int* __restrict__ 
 }
 
 // Sum (or mean over the rows with a target) of the token losses, and how many tokens the clipping held.
-__global__ void __launch_bounds__(1024) k_policy_sum(const RowsArgs p, int N, int V, int mean, float* __restrict__ loss_out, int* __restrict__ n_valid_out,
-                                                     int* __restrict__ n_clipped_out) {
+__global__ void __launch_bounds__(1024) k_policy_sum(const RowsArgs p, int mean, float* loss_out, int* n_valid_out, int* n_clipped_out) {
   pdl_trigger();
+  pdl_wait();
   float sum = 0.f;
   int n = 0, clipped = 0;
-  for (long long i = threadIdx.x; i < N; i += 1024) {
+#pragma unroll 4
+  for (long long i = threadIdx.x; i < p.N; i += 1024) {
     const int t = p.tgt0[i];
-    if (t < 0 || t >= V) continue;
-    n++;
-    sum += p.token_losses[i];
-    if (n_clipped_out && policy_clipped(p.term, policy_ratio(p.logp[i], p.old[i]), p.adv[i])) clipped++;
+    const bool has = t >= 0 && t < p.V;
+    n += has;
+    sum += __ldcg(p.token_losses + i);      // 0 without a target
+    clipped += has && policy_clipped(p.term, policy_ratio(__ldcg(p.logp + i), p.old[i]), p.adv[i]);
   }
   sum = block_total(sum);
   n = block_total(n);
@@ -176,9 +177,9 @@ int check_temperature(float t) {
 }
 float log2e_over(float temperature) { return (float)(1.4426950408889634074 / (double)temperature); }
 
-RowsArgs rows_args(const void* logits, long long ldl, const int* tgt0, int V, float temperature) {
+RowsArgs rows_args(const void* logits, long long ldl, const int* tgt0, int N, int V, float temperature) {
   RowsArgs p = {};
-  p.logits = logits; p.ldl = ldl; p.tgt0 = tgt0; p.V = V;
+  p.logits = logits; p.ldl = ldl; p.tgt0 = tgt0; p.N = N; p.V = V;
   p.c = log2e_over(temperature); p.inv_t = 1.f / temperature;
   return p;
 }
@@ -190,9 +191,9 @@ extern "C" int32_t femto_token_logprobs(int32_t dtype, const void* logits, int64
   FEMTO_TRY(check_temperature(temperature));
   if (N == 0) return 0;
   if (!logp) return femto_fail(FEMTO_ERR_ARG, "NULL argument");
-  RowsArgs p = rows_args(logits, ldl, targets0, V, temperature);
+  RowsArgs p = rows_args(logits, ldl, targets0, N, V, temperature);
   p.logp = logp; p.ent = entropy_out;
-  return objective_rows(dtype, LOGPROBS, p, N, (cudaStream_t)stream);
+  return objective_rows(dtype, LOGPROBS, p, (cudaStream_t)stream);
 }
 
 extern "C" int32_t femto_token_logprobs_gradient(int32_t dtype, void* dlogits, int64_t ldd, const void* logits, int64_t ldl, const int32_t* targets0, int32_t N,
@@ -202,9 +203,9 @@ extern "C" int32_t femto_token_logprobs_gradient(int32_t dtype, void* dlogits, i
   FEMTO_TRY(check_gradient(dtype, dlogits, ldd, logits, ldl, N, V));
   if (N == 0) return 0;
   if (!dlogits || !dlogp) return femto_fail(FEMTO_ERR_ARG, "NULL argument");
-  RowsArgs p = rows_args(logits, ldl, targets0, V, temperature);
+  RowsArgs p = rows_args(logits, ldl, targets0, N, V, temperature);
   p.dlogits = dlogits; p.ldd = ldd; p.dlogp = dlogp; p.dent = dentropy;
-  return objective_rows(dtype, GRADIENT, p, N, (cudaStream_t)stream);
+  return objective_rows(dtype, GRADIENT, p, (cudaStream_t)stream);
 }
 
 int check_policy(const femto_policy_config* c, const float* ref_logp) {
@@ -229,7 +230,7 @@ extern "C" int32_t femto_policy_loss(int32_t dtype, const void* logits, int64_t 
   if (!loss_out || !n_valid_out || (N > 0 && (!old_logp || !advantages || !token_losses || !logp))) return femto_fail(FEMTO_ERR_ARG, "NULL argument");
   cudaStream_t s = (cudaStream_t)stream;
   const bool mean = h_cfg->reduction == FEMTO_REDUCTION_MEAN;
-  RowsArgs p = rows_args(logits, ldl, targets0, V, h_cfg->temperature);
+  RowsArgs p = rows_args(logits, ldl, targets0, N, V, h_cfg->temperature);
   p.dlogits = dlogits; p.ldd = ldd; p.logp = logp; p.token_losses = token_losses;
   p.old = old_logp; p.ref = ref_logp; p.adv = advantages; p.w = weights;
   p.term = {1.f - h_cfg->clip_low, 1.f + h_cfg->clip_high, h_cfg->kl_coef};
@@ -239,9 +240,9 @@ extern "C" int32_t femto_policy_loss(int32_t dtype, const void* logits, int64_t 
       KERNEL_CHECK();
       p.n_valid = n_valid_out;
     }
-    FEMTO_TRY(objective_rows(dtype, POLICY, p, N, s));
+    FEMTO_TRY(objective_rows(dtype, POLICY, p, s));
   }
-  k_policy_sum<<<1, 1024, 0, s>>>(p, N, V, mean, loss_out, n_valid_out, n_clipped_out);
+  CUDA_TRY(launch_dependent(k_policy_sum, dim3(1), dim3(1024), 0, s, p, (int)mean, loss_out, n_valid_out, n_clipped_out));
   KERNEL_CHECK();
   return 0;
 }

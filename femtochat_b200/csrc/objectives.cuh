@@ -58,22 +58,26 @@ template <bool ENTROPY> __device__ __forceinline__ RowStats merged(RowStats x, R
   if (ENTROPY) x.a += y.a;
   return x;
 }
-// l = 2^k f with f in [0.7, 1.4]: log l is k ln2 (in 64 bits) + log f, a small number.  log(l) in one piece has an error of 5e-7 at
-// l = 65536, and so has every log-probability then.
-__device__ __forceinline__ double log_sum(float l) {
-  if (!(l > 0.f && l < INFINITY)) return (double)logf(l);
-  int k;
-  float f = frexpf(l, &k);
-  if (f < 0.70710678f) { f *= 2.f; k--; }
-  return LN2 * k + (double)logf(f);
+// log l = k ln2 + log f of l = 2^k f, f in [0.7, 1.4]: with ln2 in two parts, the first of which gives k ln2 without rounding, the only error of
+// the size of log l is the last rounding.  log(l) in one piece is 5e-7 off at l = 65536.
+struct LogSum {
+  float k, log_f;
+  __device__ __forceinline__ float minus_from(float x) const { return fmaf(-k, 0.693145752f, x) - fmaf(k, 1.42860677e-6f, log_f); }      // x - log l
+};
+__device__ __forceinline__ LogSum log_sum(float l) {
+  LogSum r;
+  if (!(l < INFINITY)) { r.k = 0.f; r.log_f = logf(l); return r; }
+  const int bits = __float_as_int(l), k = (bits - 0x3f3504f3) >> 23;      // sqrt(1/2)
+  r.k = (float)k;
+  r.log_f = logf(__int_as_float(bits - (k << 23)));
+  return r;
 }
 // log p of a logit z; a row without any logit above -inf (l = 0) has no distribution: -inf.
-__device__ __forceinline__ float log_prob(const RowStats& s, float z, float c) {
-  if (s.l == 0.f) return -INFINITY;
-  return (float)(LN2 * c * ((double)z - (double)s.m) - log_sum(s.l));
+__device__ __forceinline__ float log_prob(const RowStats& s, float z, float inv_t) {
+  return s.l == 0.f ? -INFINITY : log_sum(s.l).minus_from((z - s.m) * inv_t);
 }
 __device__ __forceinline__ float entropy(const RowStats& s) {
-  return s.l == 0.f ? 0.f : (float)(log_sum(s.l) - LN2 * (double)s.a / (double)s.l);
+  return s.l == 0.f ? 0.f : -log_sum(s.l).minus_from(s.a / s.l * (float)LN2);
 }
 
 // ---- clipped policy term of one token ---------------------------------------------------------------------------------------------------
@@ -115,5 +119,5 @@ struct RowsArgs {
   const int* n_valid;            // POLICY, mean: the slopes are divided by it
   PolicyTerm term;
 };
-int objective_rows(int dtype, RowsMode mode, RowsArgs p, int N, cudaStream_t s);
+int objective_rows(int dtype, RowsMode mode, const RowsArgs& p, cudaStream_t s);
 unsigned int objective_rows_status_word();
