@@ -103,6 +103,42 @@ template <bool ENTROPY> struct Adder {
   }
 };
 
+// A thread's statistics, relative to a maximum of its own that grows a few times in a row.
+template <typename T, bool ENTROPY> struct Running {
+  RowStats s;
+  Exponent x;
+  Adder<ENTROPY> sum;
+  __device__ __forceinline__ Running(bool there, float edge, float c) {
+    s.m = there ? edge : -INFINITY;
+    x = exponent_of(s.m, c);
+    sum.at(x);
+    if (there) sum.add(pack2(edge, -INFINITY));
+  }
+  template <int K> __device__ __forceinline__ void add(const uint4 (&q)[K], float c) {
+    float m = Word<T>::most(q[0]);
+#pragma unroll
+    for (int h = 1; h < K; h++) m = fmaxf(m, Word<T>::most(q[h]));
+    if (m > s.m) {
+      sum.join(s, x);
+      rebase<ENTROPY>(s, m, c);
+      x = exponent_of(m, c);
+      sum.at(x);
+    }
+#pragma unroll
+    for (int h = 0; h < K; h++)
+#pragma unroll
+      for (int i = 0; i < VecN<T>::n / 2; i++) sum.add(Word<T>::get(q[h], i));
+  }
+  // The warp's statistics, in every lane.
+  __device__ __forceinline__ RowStats of_warp(float c) {
+    sum.join(s, x);
+    rebase<ENTROPY>(s, warp_max(s.m), c);
+    s.l = warp_sum(s.l);
+    if (ENTROPY) s.a = warp_sum(s.a);
+    return s;
+  }
+};
+
 // The statistics of `slots` warps (m, l, a in three runs of `pitch`), by every warp that calls it: fixed order, the same bits in all.
 template <bool ENTROPY> __device__ __forceinline__ RowStats merged_parts(const float* part, int pitch, int slots, float c) {
   const int lane = threadIdx.x & 31;
@@ -226,105 +262,168 @@ __device__ __forceinline__ void store_remote(const void* local, uint32_t rank, f
 }
 __device__ __forceinline__ void group_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
-// ---- rows in registers ------------------------------------------------------------------------------------------------------------------------
-// `W` warps share a row; a block has several such groups, which walk the rows in turn.  Clusters (few rows): one group a block, the cluster's
-// blocks share one row, and the statistics of all warps go to every block's shared memory.  A row takes at most C * W * 32 * NV words.
-constexpr int ROWS_WARPS = 8, MOST_CLUSTER = 8;
+// ---- few rows -----------------------------------------------------------------------------------------------------------------------------------
+// A cluster of blocks holds a row in registers, NV words a thread; the statistics of all its warps go to every block's shared memory.  There is
+// little to overlap: what counts is that a row is brought by many multiprocessors at once.
+constexpr int FEW_WARPS = 8, MOST_CLUSTER = 8, FEW_WORDS = 8;
 
 template <typename T, RowsMode MODE, bool STORE, bool ENTROPY, int NV>
-__global__ void __launch_bounds__(32 * ROWS_WARPS) k_rows(const RowsArgs p, const int W) {
+__global__ void __launch_bounds__(32 * FEW_WARPS) k_rows_few(const RowsArgs p) {
   pdl_trigger();
-  __shared__ float part[2][3][MOST_CLUSTER * ROWS_WARPS];
-  __shared__ float2 slope_s[ROWS_WARPS];
-  const int C = (int)cluster_size(), rank = (int)cluster_rank();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = warp / W, groups = (blockDim.x >> 5) / W;
+  constexpr int threads = 32 * FEW_WARPS, pitch = MOST_CLUSTER * FEW_WARPS;
+  __shared__ float part[3 * pitch];
+  __shared__ float2 slope_s;
+  const int C = (int)cluster_size(), rank = (int)cluster_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");      // this block runs: its shared memory may be written
+  const long long row = blockIdx.x / C;
+  const int t = checked_target(p, p.tgt0[row], rank == 0 && tid == 0);
+  const T* z = reinterpret_cast<const T*>(p.logits) + row * p.ldl;
+  T* d = reinterpret_cast<T*>(p.dlogits) + row * p.ldd;
+  const RowShape r = row_shape<T>(STORE && t < 0 ? d : z, p.V);      // the logits', or, where they are not read, the gradient's
+  const int per = (r.nvec + C - 1) / C, first = min(r.nvec, rank * per), last = min(r.nvec, first + per);
+  const int at = rank == 0 ? edge_of<T>(r, tid) : -1;
+  if (t < 0) {
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    if (rank == 0 && tid == 0) row_without_target<MODE, ENTROPY>(p, row);
+    if (STORE) {
+      for (int v = first + tid; v < last; v += threads) reinterpret_cast<uint4*>(d + r.head)[v] = make_uint4(0, 0, 0, 0);
+      if (at >= 0) d[at] = from_f<T>(0.f);
+    }
+    return;
+  }
+  const uint4* words = reinterpret_cast<const uint4*>(z + r.head);
+  uint4 q[NV];
+#pragma unroll
+  for (int k = 0; k < NV; k++) {
+    const int v = first + k * threads + tid;
+    q[k] = load_word(words + v, v < last, Word<T>::LEAST);
+  }
+  RowNumbers numbers;
+  if (warp == 0) numbers = row_numbers<T, MODE, ENTROPY>(p, row, z, t);      // in every block: each works the slopes out for itself
+  const float edge = at >= 0 ? to_f<T>(z[at]) : -INFINITY;
+  Running<T, ENTROPY> run(at >= 0, edge, p.c);
+  run.add(q, p.c);
+  RowStats s = run.of_warp(p.c);
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");      // all blocks run
+  const int slot = rank * FEW_WARPS + warp;
+  if (lane < C) {
+    store_remote(part + slot, lane, s.m); store_remote(part + pitch + slot, lane, s.l);
+    if (ENTROPY) store_remote(part + 2 * pitch + slot, lane, s.a);
+  }
+  asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+  if (!STORE && (rank != 0 || warp != 0)) return;
+  s = merged_parts<ENTROPY>(part, pitch, FEW_WARPS * C, p.c);
+  if (warp == 0) {
+    const float2 gh = row_result<MODE, ENTROPY>(p, row, s, numbers, rank == 0 && lane == 0);
+    if (lane == 0) slope_s = gh;
+  }
+  if (!STORE) return;
+  __syncthreads();
+  const Slope<T, ENTROPY> slope(s, slope_s, p.c, t);
+  const bool same = same_phase(z, d);
+#pragma unroll
+  for (int k = 0; k < NV; k++) {
+    const int v = first + k * threads + tid;
+    if (v < last) slope.store_word(d, r.head, v, q[k], same);
+  }
+  if (at >= 0) slope.store_edge(d, at, edge);
+}
+
+// ---- narrow rows --------------------------------------------------------------------------------------------------------------------------------
+// Groups of W warps walk the rows in turn.  A group has two buffers in shared memory: while it works on a row, a bulk copy brings its next one.
+constexpr int NEAR_WARPS = 8, NEAR_WORDS = 4;
+
+template <typename T, RowsMode MODE, bool STORE, bool ENTROPY>
+__global__ void __launch_bounds__(32 * NEAR_WARPS, 3) k_rows_near(const RowsArgs p, const int W, const int pitch) {
+  pdl_trigger();
+  extern __shared__ __align__(128) uint4 ring[];
+  __shared__ uint64_t full[NEAR_WARPS][2];
+  __shared__ float part[2][3][NEAR_WARPS];
+  __shared__ float2 slope_s[NEAR_WARPS];
+  __shared__ int abort_flag;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = warp / W, groups = NEAR_WARPS / W;
   const int threads = W * 32, tid = threadIdx.x - group * threads, first_warp = group * W;
-  const bool one = warp == first_warp;      // of a group: it works the slopes out; of the first block: it writes the row's numbers
-  if (C > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");      // this block runs: its shared memory may be written
-  const long long step = (long long)(gridDim.x / C) * groups;
-  long long row = (long long)(blockIdx.x / C) * groups + group;
-  int t_next = row < p.N ? p.tgt0[row] : 0, turn = 0;
-  for (; row < p.N; row += step, turn ^= 1) {
-    const int t = checked_target(p, t_next, rank == 0 && tid == 0);
-    if (row + step < p.N) t_next = p.tgt0[row + step];
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2 * NEAR_WARPS; i++) mbar_init(&full[i / 2][i % 2], 1);
+    abort_flag = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+  uint4* buffer = ring + (size_t)group * 2 * pitch;
+  // one thread of the group asks for a row's words
+  auto ask = [&](long long row, int which) {
+    const T* z = reinterpret_cast<const T*>(p.logits) + row * p.ldl;
+    const RowShape r = row_shape<T>(z, p.V);
+    if (r.nvec > 0) {
+      mbar_expect_tx(&full[group][which], (uint32_t)r.nvec * 16u);
+      bulk_load_1d(buffer + (size_t)which * pitch, z + r.head, (uint32_t)r.nvec * 16u, &full[group][which]);
+    } else mbar_arrive(&full[group][which]);
+  };
+  const long long step = (long long)gridDim.x * groups;
+  long long row = (long long)blockIdx.x * groups + group;
+  int t_next = row < p.N ? p.tgt0[row] : -1, k = 0;      // k: rows with a target so far
+  bool alive = true, asked = false;
+  for (; row < p.N; row += step) {
+    const int t = checked_target(p, t_next, tid == 0);
+    t_next = row + step < p.N ? p.tgt0[row + step] : -1;
     const T* z = reinterpret_cast<const T*>(p.logits) + row * p.ldl;
     T* d = reinterpret_cast<T*>(p.dlogits) + row * p.ldd;
     const RowShape r = row_shape<T>(STORE && t < 0 ? d : z, p.V);      // the logits', or, where they are not read, the gradient's
-    const int per = (r.nvec + C - 1) / C, first = min(r.nvec, rank * per), last = min(r.nvec, first + per);
-    const int at = rank == 0 ? edge_of<T>(r, tid) : -1;
+    const int at = edge_of<T>(r, tid);
     if (t < 0) {
-      if (C > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
-      if (rank == 0 && tid == 0) row_without_target<MODE, ENTROPY>(p, row);
+      if (tid == 0) row_without_target<MODE, ENTROPY>(p, row);
       if (STORE) {
-        for (int v = first + tid; v < last; v += threads) reinterpret_cast<uint4*>(d + r.head)[v] = make_uint4(0, 0, 0, 0);
+        for (int v = tid; v < r.nvec; v += threads) reinterpret_cast<uint4*>(d + r.head)[v] = make_uint4(0, 0, 0, 0);
         if (at >= 0) d[at] = from_f<T>(0.f);
       }
       continue;
     }
-    const uint4* words = reinterpret_cast<const uint4*>(z + r.head);
-    uint4 q[NV];
-#pragma unroll
-    for (int k = 0; k < NV; k++) {
-      const int v = first + k * threads + tid;
-      q[k] = load_word(words + v, v < last, Word<T>::LEAST);
-    }
+    const int which = k & 1;
+    const uint32_t parity = (uint32_t)(k >> 1) & 1u;
+    k++;
+    if (!asked && tid == 0 && alive) ask(row, which);      // the row before the last but one, which this buffer held, is done: a barrier lies between
     RowNumbers numbers;
-    if (one) numbers = row_numbers<T, MODE, ENTROPY>(p, row, z, t);
+    if (warp == first_warp) numbers = row_numbers<T, MODE, ENTROPY>(p, row, z, t);
     const float edge = at >= 0 ? to_f<T>(z[at]) : -INFINITY;
-
-    RowStats s;
-    s.m = edge;
+    Running<T, ENTROPY> run(at >= 0, edge, p.c);
+    const uint4* words = buffer + (size_t)which * pitch;
+    alive = alive && mbar_wait(&full[group][which], parity, &abort_flag, &g_rows_status);
+    for (int v0 = tid; v0 < r.nvec; v0 += NEAR_WORDS * threads) {
+      uint4 q[NEAR_WORDS];
 #pragma unroll
-    for (int k = 0; k < NV; k++) s.m = fmaxf(s.m, Word<T>::most(q[k]));
-    s.m = warp_max(s.m);
-    {
-      const Exponent x = exponent_of(s.m, p.c);
-      Adder<ENTROPY> sum;
-      sum.at(x);
-      if (at >= 0) sum.add(pack2(edge, -INFINITY));
-#pragma unroll
-      for (int k = 0; k < NV; k++)
-#pragma unroll
-        for (int i = 0; i < VecN<T>::n / 2; i++) sum.add(Word<T>::get(q[k], i));
-      sum.join(s, x);
-    }
-    s.l = warp_sum(s.l);
-    if (ENTROPY) s.a = warp_sum(s.a);
-    if (W * C > 1) {
-      float* mine = part[turn][0];      // two buffers in turn: warps that are done with a row may be one row ahead of the one that adds it up
-      constexpr int pitch = MOST_CLUSTER * ROWS_WARPS;
-      if (C > 1) {
-        asm volatile("barrier.cluster.wait.acquire;" ::: "memory");      // all blocks run
-        const int slot = rank * W + warp;
-        if (lane < C) {
-          store_remote(mine + slot, lane, s.m); store_remote(mine + pitch + slot, lane, s.l);
-          if (ENTROPY) store_remote(mine + 2 * pitch + slot, lane, s.a);
-        }
-        asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
-      } else {
-        if (lane == 0) { mine[warp] = s.m; mine[pitch + warp] = s.l; if (ENTROPY) mine[2 * pitch + warp] = s.a; }
-        group_barrier(1 + group, threads);
-        mine += first_warp;
+      for (int h = 0; h < NEAR_WORDS; h++) {
+        q[h] = make_uint4(Word<T>::LEAST, Word<T>::LEAST, Word<T>::LEAST, Word<T>::LEAST);
+        if (v0 + h * threads < r.nvec) q[h] = words[v0 + h * threads];
       }
-      if (STORE || one) s = merged_parts<ENTROPY>(mine, pitch, W * C, p.c);
+      run.add(q, p.c);
     }
+    RowStats s = run.of_warp(p.c);
+    if (W > 1) {
+      float* mine = part[which][0];
+      if (lane == 0) { mine[warp] = s.m; mine[NEAR_WARPS + warp] = s.l; if (ENTROPY) mine[2 * NEAR_WARPS + warp] = s.a; }
+      group_barrier(1 + group, threads);
+      if (STORE || warp == first_warp) s = merged_parts<ENTROPY>(mine + first_warp, NEAR_WARPS, W, p.c);
+    } else __syncwarp();
+    // all of the group are done with the row before this one: its buffer is free
+    asked = t_next >= 0 && t_next < p.V;
+    if (asked && tid == 0 && alive) ask(row + step, which ^ 1);
     float2 gh = make_float2(0.f, 0.f);
-    if (one) gh = row_result<MODE, ENTROPY>(p, row, s, numbers, rank == 0 && lane == 0);
+    if (warp == first_warp) gh = row_result<MODE, ENTROPY>(p, row, s, numbers, lane == 0);
     if (!STORE) continue;
     if (W > 1) {
-      if (one && lane == 0) slope_s[group] = gh;
+      if (warp == first_warp && lane == 0) slope_s[group] = gh;
       group_barrier(1 + group, threads);
       gh = slope_s[group];
     }
     const Slope<T, ENTROPY> slope(s, gh, p.c, t);
     const bool same = same_phase(z, d);
-#pragma unroll
-    for (int k = 0; k < NV; k++) {
-      const int v = first + k * threads + tid;
-      if (v < last) slope.store_word(d, r.head, v, q[k], same);
-    }
+#pragma unroll 2
+    for (int v = tid; v < r.nvec; v += threads) slope.store_word(d, r.head, v, words[v], same);
     if (at >= 0) slope.store_edge(d, at, edge);
   }
+  if (!alive && tid == 0)      // nothing may still be on its way to this block's memory when it ends
+    for (int b = 0; b < 2; b++)
+      for (uint32_t polls = 0; k > b && polls < WAIT_LIMIT && !mbar_try_wait(&full[group][b], (uint32_t)((k - b - 1) >> 1) & 1u); polls++) {}
 }
 
 // ---- rows through a ring in shared memory -----------------------------------------------------------------------------------------------------
@@ -432,12 +531,7 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
     if (gwarp == 0) numbers = row_numbers<T, MODE, ENTROPY>(p, row, z, t);
     const float edge = at >= 0 ? to_f<T>(z[at]) : -INFINITY;
 
-    RowStats s;
-    s.m = edge;
-    Exponent x = exponent_of(s.m, p.c);
-    Adder<ENTROPY> sum;
-    sum.at(x);
-    if (at >= 0) sum.add(pack2(edge, -INFINITY));
+    Running<T, ENTROPY> run(at >= 0, edge, p.c);
     const int first_slot = (int)((long long)mine * (chunks + (STORE ? again : 0)) % SLOTS);
     int slot = first_slot;
     for (int c = 0; c < chunks; c++, slot = next_slot(slot)) {
@@ -452,24 +546,9 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[slot]);
       }
-      float m = Word<T>::most(q[0]);
-#pragma unroll
-      for (int h = 1; h < PER_CHUNK; h++) m = fmaxf(m, Word<T>::most(q[h]));
-      if (m > s.m) {      // a thread's own maximum grows a few times in a row
-        sum.join(s, x);
-        rebase<ENTROPY>(s, m, p.c);
-        x = exponent_of(m, p.c);
-        sum.at(x);
-      }
-#pragma unroll
-      for (int h = 0; h < PER_CHUNK; h++)
-#pragma unroll
-        for (int i = 0; i < VecN<T>::n / 2; i++) sum.add(Word<T>::get(q[h], i));
+      run.add(q, p.c);
     }
-    sum.join(s, x);
-    rebase<ENTROPY>(s, warp_max(s.m), p.c);
-    s.l = warp_sum(s.l);
-    if (ENTROPY) s.a = warp_sum(s.a);
+    RowStats s = run.of_warp(p.c);
     float* parts = part[group][turn][0];
     turn ^= 1;
     if (lane == 0) { parts[gwarp] = s.m; parts[GROUP_WARPS + gwarp] = s.l; if (ENTROPY) parts[2 * GROUP_WARPS + gwarp] = s.a; }
@@ -500,8 +579,10 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
 }
 
 // ---- launch -----------------------------------------------------------------------------------------------------------------------------------
-typedef Ring<3, 8, 4, 13> Reading;      // numbers only
-typedef Ring<2, 12, 4, 9> Writing;
+constexpr int MOST_NEAR = 1280;
+typedef Ring<4, 6, 4, 18> Medium;
+typedef Ring<3, 8, 4, 13> WideReading;
+typedef Ring<2, 12, 4, 9> WideWriting;
 
 // Behind the kernel that counts the targets (n_valid) the rows may start at once: nothing else of theirs depends on it, and it started
 // itself when everything before the call was done.  Otherwise the launch is an ordinary one.
@@ -528,23 +609,28 @@ template <typename T, RowsMode MODE, bool STORE, bool ENTROPY, class R> int laun
   return launch_kernel(p, kernel, 1, dim3((unsigned)std::min(p.N, device_sm_count())), R::BLOCK, R::BYTES, s, p, chunks, again);
 }
 template <typename T, RowsMode MODE, bool STORE, bool ENTROPY> int launch(const RowsArgs& p, cudaStream_t s) {
-  const int words = std::max(1, p.V / VecN<T>::n), sms = device_sm_count();
-  constexpr int NV = 8;
-  const int most = ROWS_WARPS * 32 * NV;      // words that a block holds in registers
-  if ((words > most && p.N >= sms) || words > MOST_CLUSTER * most) {
-    if constexpr (STORE) return launch_ring<T, MODE, STORE, ENTROPY, Writing>(p, words, s);
-    else return launch_ring<T, MODE, STORE, ENTROPY, Reading>(p, words, s);
+  const int words = std::max(1, p.V / VecN<T>::n), sms = device_sm_count(), block = 32 * FEW_WARPS;
+  if (p.N < sms && words <= MOST_CLUSTER * block * FEW_WORDS) {
+    // as many blocks for a row as there is room for, while a thread keeps a word; and no fewer than hold it
+    int C = 1;
+    while (C < MOST_CLUSTER && (words > C * block * FEW_WORDS || ((long long)p.N * C < sms && words > C * block))) C *= 2;
+    const dim3 grid((unsigned)(p.N * C));
+    if (words <= C * block * 2) return launch_kernel(p, k_rows_few<T, MODE, STORE, ENTROPY, 2>, C, grid, block, 0, s, p);
+    return launch_kernel(p, k_rows_few<T, MODE, STORE, ENTROPY, FEW_WORDS>, C, grid, block, 0, s, p);
   }
-  int C = 1;
-  while (words > C * most) C *= 2;
-  // few rows: more blocks for each, while a thread keeps a word or more
-  while (C < MOST_CLUSTER && (long long)p.N * C < sms && words > C * 32 * ROWS_WARPS) C *= 2;
-  int W = 1;
-  while (W < ROWS_WARPS && cdiv(words, C) > W * 32 * NV) W *= 2;
-  if (C > 1) W = ROWS_WARPS;
-  const int groups = ROWS_WARPS / W;
-  const dim3 grid(C > 1 ? (unsigned)(p.N * C) : (unsigned)std::min(cdiv(p.N, groups), sms * 4));
-  return launch_kernel(p, k_rows<T, MODE, STORE, ENTROPY, NV>, C, grid, 32 * ROWS_WARPS, 0, s, p, W);
+  if (words <= MOST_NEAR) {
+    int W = 1;
+    while (W < NEAR_WARPS && words > W * 256) W *= 2;
+    const int groups = NEAR_WARPS / W;
+    const size_t smem = (size_t)groups * 2 * words * 16;
+    constexpr auto kernel = k_rows_near<T, MODE, STORE, ENTROPY>;
+    FEMTO_TRY(allow_smem<kernel>(smem));
+    const int blocks = std::max(1, std::min(3, (int)((220 << 10) / (smem + 2048))));
+    return launch_kernel(p, kernel, 1, dim3((unsigned)std::min(cdiv(p.N, groups), sms * blocks)), 32 * NEAR_WARPS, smem, s, p, W, words);
+  }
+  if (words <= 4096) return launch_ring<T, MODE, STORE, ENTROPY, Medium>(p, words, s);
+  if constexpr (STORE) return launch_ring<T, MODE, STORE, ENTROPY, WideWriting>(p, words, s);
+  else return launch_ring<T, MODE, STORE, ENTROPY, WideReading>(p, words, s);
 }
 template <RowsMode MODE, bool STORE, bool ENTROPY> int typed(int dtype, const RowsArgs& p, cudaStream_t s) {
   return dtype == FEMTO_BF16 ? launch<bf16, MODE, STORE, ENTROPY>(p, s) : launch<float, MODE, STORE, ENTROPY>(p, s);

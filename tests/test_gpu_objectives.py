@@ -65,7 +65,7 @@ def near(got, want, tol, what):
 
 # a row that fits a thread, a warp, a block; odd; past every size that one block, or eight together, hold of it; many wide rows, which
 # come through a ring that holds them (20011, 40000) or not
-SHAPES = [(700, 20011), (310, 40000), (320, 150001), (1, 1), (3, 2), (5, 7), (2, 33), (7, 255), (4, 1000), (9, 4099), (150, 4096), (600, 300), (3, 50021), (2, 65536), (1, 131073), (2, 300007)]
+SHAPES = [(200, 9001), (300, 1), (400, 5), (700, 20011), (310, 40000), (320, 150001), (1, 1), (3, 2), (5, 7), (2, 33), (7, 255), (4, 1000), (9, 4099), (150, 4096), (600, 300), (3, 50021), (2, 65536), (1, 131073), (2, 300007)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
