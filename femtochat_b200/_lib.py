@@ -149,6 +149,9 @@ SIGNATURES = {
     "femto_rmsnorm_bwd": (I32, [I32, P, P, P, P, I32, I32, P]),
     "femto_embed_gather": (I32, [I32, P, P, P, I32, I32, I32, P]),
     "femto_muon_direction": (I32, [I32, P, P, P, P, I32, I32, I32, F, F, F, C.POINTER(F), I32, P]),
+    "femto_forward_token_logprobs": (I32, [P, P, P, P, P, I32, F, P, P]),
+    "femto_policy_loss_and_gradient": (I32, [P, P, P, P, P, P, I32, P, P, P, P, C.POINTER(PolicyConfigC), I32, P, P, P, P, P]),
+    "femto_preference_loss_and_gradient": (I32, [P, P, P, P, P, P, I32, P, P, I32, C.POINTER(PreferenceConfigC), I32, P, P, P, P, P]),
     "femto_token_logprobs": (I32, [I32, P, I64, P, I32, I32, F, P, P, P]),
     "femto_token_logprobs_gradient": (I32, [I32, P, I64, P, I64, P, I32, I32, F, P, P, P]),
     "femto_policy_loss": (I32, [I32, P, I64, P, I32, I32, P, P, P, P, C.POINTER(PolicyConfigC), P, I64, P, P, P, P, P, P]),

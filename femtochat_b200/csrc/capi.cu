@@ -5,6 +5,7 @@
 
 #include "decoder.cuh"
 #include "model.cuh"
+#include "objectives.cuh"
 #include "streaming.cuh"
 
 struct femto_optimizer;
@@ -248,6 +249,71 @@ int32_t femto_forward_token_losses(femto_handle* h, const float* theta, const in
   // the scalar path also counts the valid targets; its sum goes to the handle's own loss scalar
   return model_step(h, theta, nullptr, tokens, targets, positions, B, FEMTO_REDUCTION_SUM, false, false, h->loss_dev,
                     n_valid_out ? n_valid_out : h->nvalid_dev, (cudaStream_t)stream, nullptr, losses_out);
+}
+
+int32_t femto_forward_token_logprobs(femto_handle* h, const float* theta, const int32_t* tokens, const int32_t* targets, const int32_t* positions,
+                                     int32_t B, float temperature, float* logp_out, void* stream) {
+  if (!h || !logp_out) return femto_fail(FEMTO_ERR_ARG, "NULL argument");
+  FEMTO_TRY(check_temperature(temperature));
+  StepExtra ex;
+  ex.temperature = temperature;
+  ex.as_step = true;
+  cudaStream_t s = (cudaStream_t)stream;
+  FEMTO_TRY(model_step(h, theta, nullptr, tokens, targets, positions, B, FEMTO_REDUCTION_SUM, false, false, h->loss_dev, h->nvalid_dev, s, nullptr,
+                       logp_out, &ex));
+  return objective_negate(logp_out, (long long)B * h->T, s);
+}
+
+// The workspace and the fields that every objective of a handle shares.
+static TokenObjective handle_objective(femto_handle* h, int32_t B, float temperature, float* logp_out) {
+  TokenObjective o;
+  const size_t N = (size_t)h->maxN;
+  o.logp = logp_out ? logp_out : h->objective_rows;
+  o.slopes = h->objective_rows + N;
+  RowsArgs& p = o.policy;
+  p.tgt0 = h->tgt0; p.N = B * h->T; p.V = h->V; p.logp = o.logp; p.token_losses = h->objective_rows + 2 * N;
+  p.inv_t = 1.f / temperature;
+  return o;
+}
+
+int32_t femto_policy_loss_and_gradient(femto_handle* h, const float* theta, float* delta, const int32_t* tokens, const int32_t* targets,
+                                       const int32_t* positions, int32_t B, const float* old_logp, const float* advantages, const float* ref_logp,
+                                       const float* weights, const femto_policy_config* cfg, int32_t accumulate, float* loss_out,
+                                       int32_t* n_valid_out, int32_t* n_clipped_out, float* logp_out, void* stream) {
+  if (!h) return femto_fail(FEMTO_ERR_ARG, "NULL handle");
+  if (h->dec) return femto_fail(FEMTO_ERR_UNSUPPORTED, "a decoder that lists its layers does not train");
+  FEMTO_TRY(check_policy(cfg, ref_logp));
+  if (!old_logp || !advantages || !loss_out || !n_valid_out) return femto_fail(FEMTO_ERR_ARG, "NULL argument");
+  if (B <= 0 || B > h->maxB) return femto_fail(FEMTO_ERR_SHAPE, "B=%d outside 1..max_batch=%d", B, h->maxB);
+  TokenObjective o = handle_objective(h, B, cfg->temperature, logp_out);
+  o.policy.old = old_logp; o.policy.adv = advantages; o.policy.ref = ref_logp; o.policy.w = weights;
+  o.policy.term = policy_term(*cfg);
+  StepExtra ex;
+  ex.objective = &o; ex.temperature = cfg->temperature; ex.n_clipped_out = n_clipped_out;
+  return model_step(h, theta, delta, tokens, targets, positions, B, cfg->reduction, true, accumulate != 0, loss_out, n_valid_out, (cudaStream_t)stream,
+                    nullptr, nullptr, &ex);
+}
+
+int32_t femto_preference_loss_and_gradient(femto_handle* h, const float* theta, float* delta, const int32_t* tokens, const int32_t* targets,
+                                           const int32_t* positions, int32_t B, const float* ref_logp, const int32_t* offsets, int32_t P,
+                                           const femto_preference_config* cfg, int32_t accumulate, float* loss_out, float* pair_losses,
+                                           float* ratios, float* logp_out, void* stream) {
+  if (!h) return femto_fail(FEMTO_ERR_ARG, "NULL handle");
+  if (h->dec) return femto_fail(FEMTO_ERR_UNSUPPORTED, "a decoder that lists its layers does not train");
+  FEMTO_TRY(check_preference(cfg));
+  if (!loss_out || P < 0 || P > (1 << 29) || (P > 0 && (!offsets || !pair_losses || !ratios))) return femto_fail(FEMTO_ERR_ARG, "bad argument");
+  if (B <= 0 || B > h->maxB) return femto_fail(FEMTO_ERR_SHAPE, "B=%d outside 1..max_batch=%d", B, h->maxB);
+  TokenObjective o = handle_objective(h, B, 1.f, logp_out);
+  o.pairs = true;
+  o.preference = preference_args(*cfg, B * h->T, P);
+  PreferenceArgs& p = o.preference;
+  p.logp = o.logp; p.ref = ref_logp; p.tgt0 = h->tgt0; p.offsets = offsets;
+  p.pair_losses = pair_losses; p.ratios = ratios; p.dlogp = o.slopes;
+  p.scale = -1.f;      // the slopes are those by -log p
+  StepExtra ex;
+  ex.objective = &o;
+  return model_step(h, theta, delta, tokens, targets, positions, B, FEMTO_REDUCTION_SUM, true, accumulate != 0, loss_out, nullptr, (cudaStream_t)stream,
+                    nullptr, nullptr, &ex);
 }
 
 int32_t femto_loss_and_gradient_host(femto_handle* h, const float* theta, float* delta, const int32_t* h_tokens,

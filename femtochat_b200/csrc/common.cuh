@@ -227,6 +227,8 @@ struct GemmArgs {
   float2* stats = nullptr;         // [M][2 * ntiles_n] partial (max, sumexp)
   float* tz = nullptr;             // [M] softcapped target logit
   int vocab = 0;                   // columns >= vocab are ignored
+  float cap = 15.f;                // 15 / temperature: the statistics are of cap tanh(x / 15)
+  bool stats_unrounded = false;    // with a destination: statistics from the products, not from what is stored of them
   // tensor-core path scratch
   void* ws = nullptr; size_t ws_bytes = 0;  // stream-K partials
   unsigned int* status = nullptr;
@@ -292,11 +294,15 @@ int standalone_status(unsigned int** out);
 // processed in token chunks; on the tensor-core path a forward-only call writes no logits at all, and a
 // call with the reverse pass keeps one chunk of bf16 logits, rewritten in place as d loss/d logit (the
 // operand of the two reverse GEMMs).
+struct TokenObjective;   // what the tail differentiates in place of the cross-entropy (objectives.cuh)
 struct XentArgs {
   const void* x = nullptr; const void* W = nullptr; long long ldw = 0; const int* targets0 = nullptr;
   int N = 0, D = 0, V = 0;
   float scale = 1.f; const float* scale_dev = nullptr;
   bool backward = false; void* dx = nullptr; float* dw = nullptr;
+  const TokenObjective* objective = nullptr;   // reverse pass: instead of the cross-entropy
+  float* objective_loss = nullptr;
+  float temperature = 1.f;      // the loss rows are those of softmax(z / temperature) (reverse pass: with an objective only)
   bool dw_overwrite = false;    // the first chunk's weight gradient overwrites dw instead of adding to it
   int chunk = 0;
   float* logits_f32 = nullptr;  // [chunk][ldw] fp32, SIMT path only

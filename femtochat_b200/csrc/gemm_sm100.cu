@@ -71,12 +71,12 @@ __device__ __forceinline__ float sqrt_approx(float x) {
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float softcap15(float x) {
-  // 15 * tanh(x/15) on the special-function unit (tanh.approx: relative error about 2^-11, below the
+__device__ __forceinline__ float softcap15(float x, float cap) {
+  // cap * tanh(x/15), cap = 15 / temperature, on the special-function unit (tanh.approx: relative error about 2^-11, below the
   // bf16 rounding of the logits that feed it)
   float t;
   asm("tanh.approx.f32 %0, %1;" : "=f"(t) : "f"(x * (1.f / 15.f)));
-  return 15.f * t;
+  return cap * t;
 }
 
 __device__ __forceinline__ float* f32_dst(const GemmArgs& g, long long bz, int m, int n) {
@@ -493,16 +493,18 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
           } break;
           case EPI_XENT_STATS: {
             // with a destination the raw logits are kept in bf16 (as the reference materialises them) and
-            // the statistics are taken from the rounded values, so a later pass over the stored chunk agrees
+            // the statistics are taken from the rounded values, so a later pass over the stored chunk agrees (or from
+            // the unrounded ones, as without a destination: log-probabilities that are compared with those of another call)
             if (tma_out) {
+              if (!g.stats_unrounded)
 #pragma unroll
-              for (int j = 0; j < 32; j++) v[j] = __bfloat162float(__float2bfloat16_rn(v[j]));
+                for (int j = 0; j < 32; j++) v[j] = __bfloat162float(__float2bfloat16_rn(v[j]));
               stage_store_bf16(v, sbuf, &tmC, sub, flush, nc_pair, m_tile0 + quad * 32, bz, lane);
             }
             float cm = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 32; j++) {
-              v[j] = (nc + j < g.vocab) ? softcap15(v[j]) : -INFINITY;
+              v[j] = (nc + j < g.vocab) ? softcap15(v[j], g.cap) : -INFINITY;
               cm = fmaxf(cm, v[j]);
             }
             if (tgt >= nc && tgt < nc + 32) {

@@ -8,6 +8,7 @@
 
 #include <algorithm>
 
+#include "objectives.cuh"
 #include "streaming.cuh"
 
 thread_local char g_femto_err[512] = {0};
@@ -199,6 +200,7 @@ void carve(femto_handle* h, Bump& b) {
   b.take(h->dlogit, es * xc * Vp);
   b.take(h->dlogit_b, es * xc * Vp);
   b.take(h->loss_dev, 256); b.take(h->nvalid_dev, 256);
+  b.take(h->objective_rows, 3 * 4 * N);
   h->gemm_ws_bytes = (size_t)160 << 20;
   b.take(h->gemm_ws, h->gemm_ws_bytes);
   b.take(h->gemm_ws2, h->gemm_ws_bytes);
@@ -350,8 +352,9 @@ static int step_t(femto_handle* h, const float* theta, float* delta, const int* 
   const int L = h->L;
   const float eps = h->eps;
   const bool mean = reduction == FEMTO_REDUCTION_MEAN;
+  const bool as_step = ex && ex->as_step;
   // with a side stream the GEMMs give up one ring stage (32 KB), so that streaming kernels of the other stream fit beside them
-  auto GA = [&]() { GemmArgs g; g.ws = h->gemm_ws; g.ws_bytes = h->gemm_ws_bytes; g.status = h->status; g.ring = (backward && side) ? 5 : 0; g.any_size = !backward; return g; };
+  auto GA = [&]() { GemmArgs g; g.ws = h->gemm_ws; g.ws_bytes = h->gemm_ws_bytes; g.status = h->status; g.ring = (backward && side) ? 5 : 0; g.any_size = !backward && !as_step; return g; };
   // (any_size: fewer rows than a tile still are faster on the tensor cores than in the SIMT kernel, whose blocks walk K alone:
   // 24 rows of d12 175 us a product, 17.4 us so.  A training step keeps the SIMT kernel's order of summation there, see attention_simt.cu)
   // Y[N][out] = X[N][in] * W[in][out]
@@ -452,7 +455,7 @@ static int step_t(femto_handle* h, const float* theta, float* delta, const int* 
     a.Q = l.qkv; a.K = (const T*)l.qkv + d; a.V = (const T*)l.qkv + d + kv; a.q_stride = dq; a.kv_stride = dq;
     a.O = l.att; a.o_stride = d; a.lse = l.lse; a.B = B; a.T = Tl; a.H = H; a.Hkv = Hkv; a.hd = hd;
     a.window_left = p.window; a.doc_start = docs; a.ws = h->attn_ws; a.ws_bytes = h->attn_ws_bytes; a.status = h->status;
-    a.reverse_follows = backward;
+    a.reverse_follows = backward || as_step;
     FEMTO_TRY(attention_fwd<T>(a, s));
     FEMTO_TRY(lin_fwd(l.att, d, l.sh_wo, d, h->xm, d, EPI_RESID, h->xm));
     FEMTO_TRY(S::norm((const T*)h->xm, (T*)l.xn2, l.r2, N, d, eps, s));
@@ -495,6 +498,7 @@ static int step_t(femto_handle* h, const float* theta, float* delta, const int* 
     x.scale_dev = mean ? h->inv_nvalid : nullptr; x.backward = backward; x.dx = dxnf;
     x.dw = backward ? delta + h->off_lm : nullptr; x.chunk = h->xchunk; x.logits_f32 = h->logits_f32;
     x.dw_overwrite = backward && !accumulate && lm_overwrite;
+    if (ex) { x.objective = ex->objective; x.objective_loss = loss_out; x.temperature = ex->temperature; }
     x.stats = h->xstats; x.tz = h->tz; x.lse_rows = h->lse_rows; x.loss_rows = h->loss_rows; x.dlogit = h->dlogit;
     x.ws = h->gemm_ws; x.ws_bytes = h->gemm_ws_bytes; x.status = h->status;
     if (two) {
@@ -507,7 +511,9 @@ static int step_t(femto_handle* h, const float* theta, float* delta, const int* 
   }
   if (token_losses_out)   // reduction=:none (src/gpt.jl:191-193): one loss per token slot, 0 where the target is ignored
     CUDA_TRY(cudaMemcpyAsync(token_losses_out, h->loss_rows, sizeof(float) * (size_t)N, cudaMemcpyDeviceToDevice, s));
-  if (loss_out) FEMTO_TRY(sum_rows_to_scalar(h->loss_rows, N, loss_out, h->tgt0, nvalid_out, mean ? 1.f : 0.f, s));
+  if (ex && ex->objective) {
+    if (!ex->objective->pairs) FEMTO_TRY(policy_sum(ex->objective->policy, mean, loss_out, nvalid_out, ex->n_clipped_out, s));
+  } else if (loss_out) FEMTO_TRY(sum_rows_to_scalar(h->loss_rows, N, loss_out, h->tgt0, nvalid_out, mean ? 1.f : 0.f, s));
   if (!backward) return 0;
 
   // ---- reverse ----

@@ -63,6 +63,7 @@ struct femto_handle {
   void* dlogit = nullptr;       // [xchunk][Vp] of T
   float* loss_dev = nullptr;
   int* nvalid_dev = nullptr;
+  float* objective_rows = nullptr;   // [3][maxN]: log-probabilities, slopes and losses of a step on another objective
   void* gemm_ws = nullptr;
   size_t gemm_ws_bytes = 0;
   // Two internal streams for the training step: `hi` (highest priority) carries the dependency chain of the
@@ -96,6 +97,11 @@ struct StepExtra {
   void* const *K = nullptr, * const *V = nullptr;   // the cache's keys and values of every block, maxT rows a column
   int maxT = 0;
   float* last_logits = nullptr;     // fp32 [B][vocab_size]: soft-capped logits of each column's last position
+  // a training step on another objective than the cross-entropy, or losses at a temperature
+  const TokenObjective* objective = nullptr;
+  int* n_clipped_out = nullptr;
+  float temperature = 1.f;
+  bool as_step = false;             // no reverse pass follows, but every sum is taken as a training step takes it
 };
 template <typename T> int kv_cache_store_prompt(femto_kv_cache* c, int B, int Tp, cudaStream_t s);
 template <typename T> int kv_cache_last_logits(femto_kv_cache* c, const T* xnf, int B, int Tp, float* logits_out, cudaStream_t s);

@@ -610,7 +610,7 @@ template <typename T, RowsMode MODE, bool STORE, bool ENTROPY, class R> int laun
 }
 template <typename T, RowsMode MODE, bool STORE, bool ENTROPY> int launch(const RowsArgs& p, cudaStream_t s) {
   const int words = std::max(1, p.V / VecN<T>::n), sms = device_sm_count(), block = 32 * FEW_WARPS;
-  if (p.N < sms && words <= MOST_CLUSTER * block * FEW_WORDS) {
+  if (2ll * p.N < 3 * sms && words <= MOST_CLUSTER * block * FEW_WORDS) {
     // as many blocks for a row as there is room for, while a thread keeps a word; and no fewer than hold it
     int C = 1;
     while (C < MOST_CLUSTER && (words > C * block * FEW_WORDS || ((long long)p.N * C < sms && words > C * block))) C *= 2;

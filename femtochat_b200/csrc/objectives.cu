@@ -57,13 +57,7 @@ __global__ void __launch_bounds__(1024) k_policy_sum(const RowsArgs p, int mean,
 }
 
 // ---- paired preference loss ---------------------------------------------------------------------------------------------------------------
-struct Preference {
-  const float *logp, *ref;
-  const int *tgt0, *offsets;
-  int N, P, kind, normalised;
-  float beta, margin, smoothing, scale;      // scale: of the slopes (1 / P for the mean)
-  float *pair_losses, *ratios, *dlogp;
-};
+typedef PreferenceArgs Preference;
 
 // The rows of one answer; offsets that leave the rows or descend make it empty.
 __device__ __forceinline__ int2 answer_rows(const Preference& p, int answer) {
@@ -113,7 +107,7 @@ __global__ void __launch_bounds__(1024) k_preference_pairs(const Preference p) {
       slope = 2.0 * u;
     }
     p.pair_losses[pair] = (float)loss;
-    slope *= (double)p.scale;
+    slope *= (double)p.scale / (p.mean ? p.P : 1);
     slope_s[0] = (float)(slope * per[0]);
     slope_s[1] = (float)(-slope * per[1]);
   }
@@ -124,13 +118,13 @@ __global__ void __launch_bounds__(1024) k_preference_pairs(const Preference p) {
 }
 
 // Sum or mean over the pairs, and zeros as the gradient of rows that belong to no answer.
-__global__ void __launch_bounds__(1024) k_preference_sum(const Preference p, int mean, float* __restrict__ loss_out) {
+__global__ void __launch_bounds__(1024) k_preference_sum(const Preference p, float* __restrict__ loss_out) {
   pdl_trigger();
   if (blockIdx.x == 0) {
     double sum = 0.0;
     for (int i = threadIdx.x; i < p.P; i += 1024) sum += (double)p.pair_losses[i];
     sum = block_total(sum);
-    if (threadIdx.x == 0) *loss_out = (float)(mean && p.P > 0 ? sum / p.P : sum);
+    if (threadIdx.x == 0) *loss_out = (float)(p.mean && p.P > 0 ? sum / p.P : sum);
   }
   if (!p.dlogp) return;
   const int first = p.P > 0 ? min(max(p.offsets[0], 0), p.N) : p.N, last = p.P > 0 ? min(max(p.offsets[2 * p.P], 0), p.N) : p.N;
@@ -147,6 +141,68 @@ unsigned int objectives_status_word() {
   if (w) cudaMemcpyToSymbol(g_objectives_status, &zero, sizeof(zero));
   return w | objective_rows_status_word();
 }
+
+int policy_sum(const RowsArgs& p, bool mean, float* loss_out, int* n_valid_out, int* n_clipped_out, cudaStream_t s) {
+  CUDA_TRY(launch_dependent(k_policy_sum, dim3(1), dim3(1024), 0, s, p, (int)mean, loss_out, n_valid_out, n_clipped_out));
+  KERNEL_CHECK();
+  return 0;
+}
+
+PreferenceArgs preference_args(const femto_preference_config& c, int N, int P) {
+  PreferenceArgs p = {};
+  p.N = N; p.P = P;
+  p.kind = c.kind; p.normalised = c.length_normalised != 0; p.mean = c.reduction == FEMTO_REDUCTION_MEAN;
+  p.beta = c.beta; p.margin = c.margin; p.smoothing = c.label_smoothing;
+  p.scale = 1.f;
+  return p;
+}
+int preference(const PreferenceArgs& p, float* loss_out, cudaStream_t s) {
+  if (p.P > 0) {
+    k_preference_pairs<<<p.P, 1024, 0, s>>>(p);
+    KERNEL_CHECK();
+  }
+  k_preference_sum<<<p.dlogp ? std::min(cdiv(p.N, 4096) + 1, 148) : 1, 1024, 0, s>>>(p, loss_out);
+  KERNEL_CHECK();
+  return 0;
+}
+
+// ---- behind the lm_head tail -------------------------------------------------------------------------------------------------------------------
+namespace {
+__global__ void __launch_bounds__(256) k_objective_rows(const RowsArgs p, const float* __restrict__ nll, float* __restrict__ logp, float* __restrict__ slopes,
+                                                        int row0, int n, const float* __restrict__ scale_dev, bool policy) {
+  pdl_trigger();
+  const int i = blockIdx.x * 256 + threadIdx.x, row = row0 + i;
+  if (i >= n) return;
+  const float lp = 0.f - nll[row];
+  logp[row] = lp;
+  if (!policy) { slopes[row] = 0.f; return; }
+  if (p.tgt0[row] < 0) { p.token_losses[row] = slopes[row] = 0.f; return; }
+  float loss, slope;
+  policy_token(p.term, lp, p.old[row], p.adv[row], p.term.kl != 0.f ? p.ref[row] : 0.f, p.w ? p.w[row] : 1.f, &loss, &slope);
+  p.token_losses[row] = loss;
+  slopes[row] = -slope * (scale_dev ? scale_dev[0] : 1.f) * p.inv_t;
+}
+__global__ void __launch_bounds__(256) k_negate(float* x, long long n) {
+  pdl_trigger();
+  const long long i = blockIdx.x * 256ll + threadIdx.x;
+  if (i < n) x[i] = 0.f - x[i];
+}
+}  // namespace
+int objective_negate(float* x, long long n, cudaStream_t s) {
+  k_negate<<<cdiv(n, 256), 256, 0, s>>>(x, n);
+  KERNEL_CHECK();
+  return 0;
+}
+int objective_slopes(const TokenObjective& o, const float* nll, int row0, int n, const float* scale_dev, float* loss_out, cudaStream_t s) {
+  k_objective_rows<<<cdiv(n, 256), 256, 0, s>>>(o.policy, nll, o.logp, o.slopes, row0, n, scale_dev, !o.pairs);
+  KERNEL_CHECK();
+  return o.pairs ? preference(o.preference, loss_out, s) : 0;
+}
+
+int check_temperature(float t) {
+  return t > 0.f && isfinite(t) ? 0 : femto_fail(FEMTO_ERR_ARG, "temperature must be positive and finite");
+}
+PolicyTerm policy_term(const femto_policy_config& c) { return {1.f - c.clip_low, 1.f + c.clip_high, c.kl_coef}; }
 
 // ---- checks of arguments ------------------------------------------------------------------------------------------------------------------
 namespace {
@@ -171,9 +227,6 @@ int check_gradient(int dtype, const void* dlogits, long long ldd, const void* lo
   const uintptr_t a_end = a + size * ((uintptr_t)(N - 1) * ldd + V), b_end = b + size * ((uintptr_t)(N - 1) * ldl + V);
   if (a < b_end && b < a_end) return femto_fail(FEMTO_ERR_ARG, "dlogits overlap the logits: give the same rows and pitch, or memory of their own");
   return 0;
-}
-int check_temperature(float t) {
-  return t > 0.f && isfinite(t) ? 0 : femto_fail(FEMTO_ERR_ARG, "temperature must be positive and finite");
 }
 float log2e_over(float temperature) { return (float)(1.4426950408889634074 / (double)temperature); }
 
@@ -233,7 +286,7 @@ extern "C" int32_t femto_policy_loss(int32_t dtype, const void* logits, int64_t 
   RowsArgs p = rows_args(logits, ldl, targets0, N, V, h_cfg->temperature);
   p.dlogits = dlogits; p.ldd = ldd; p.logp = logp; p.token_losses = token_losses;
   p.old = old_logp; p.ref = ref_logp; p.adv = advantages; p.w = weights;
-  p.term = {1.f - h_cfg->clip_low, 1.f + h_cfg->clip_high, h_cfg->kl_coef};
+  p.term = policy_term(*h_cfg);
   if (N > 0) {
     if (mean && dlogits) {
       k_count_targets<<<1, 1024, 0, s>>>(targets0, N, V, n_valid_out);
@@ -242,9 +295,7 @@ extern "C" int32_t femto_policy_loss(int32_t dtype, const void* logits, int64_t 
     }
     FEMTO_TRY(objective_rows(dtype, POLICY, p, s));
   }
-  CUDA_TRY(launch_dependent(k_policy_sum, dim3(1), dim3(1024), 0, s, p, (int)mean, loss_out, n_valid_out, n_clipped_out));
-  KERNEL_CHECK();
-  return 0;
+  return policy_sum(p, mean, loss_out, n_valid_out, n_clipped_out, s);
 }
 
 int check_preference(const femto_preference_config* c) {
@@ -268,14 +319,8 @@ extern "C" int32_t femto_preference_loss(const float* logp, const float* ref_log
   if (N < 0 || P < 0 || P > (1 << 29)) return femto_fail(FEMTO_ERR_SHAPE, "P = %d pairs of answers in N = %d rows", P, N);
   if (!loss_out || (N > 0 && !logp) || (P > 0 && (!offsets || !pair_losses || !ratios))) return femto_fail(FEMTO_ERR_ARG, "NULL argument");
   cudaStream_t s = (cudaStream_t)stream;
-  const bool mean = h_cfg->reduction == FEMTO_REDUCTION_MEAN;
-  const Preference p = {logp, ref_logp, targets0, offsets, N, P, h_cfg->kind, h_cfg->length_normalised != 0, h_cfg->beta, h_cfg->margin,
-                        h_cfg->label_smoothing, mean && P > 0 ? 1.f / (float)P : 1.f, pair_losses, ratios, dlogp};
-  if (P > 0) {
-    k_preference_pairs<<<P, 1024, 0, s>>>(p);
-    KERNEL_CHECK();
-  }
-  k_preference_sum<<<dlogp ? std::min(cdiv(N, 4096) + 1, 148) : 1, 1024, 0, s>>>(p, mean, loss_out);
-  KERNEL_CHECK();
-  return 0;
+  PreferenceArgs p = preference_args(*h_cfg, N, P);
+  p.logp = logp; p.ref = ref_logp; p.tgt0 = targets0; p.offsets = offsets;
+  p.pair_losses = pair_losses; p.ratios = ratios; p.dlogp = dlogp;
+  return preference(p, loss_out, s);
 }

@@ -121,3 +121,33 @@ struct RowsArgs {
 };
 int objective_rows(int dtype, RowsMode mode, const RowsArgs& p, cudaStream_t s);
 unsigned int objective_rows_status_word();
+int check_policy(const femto_policy_config* c, const float* ref_logp);
+int check_preference(const femto_preference_config* c);
+int check_temperature(float t);
+PolicyTerm policy_term(const femto_policy_config& c);
+int objective_negate(float* x, long long n, cudaStream_t s);      // x = -x
+// The reduced loss, the rows with a target and those that the clipping held, from token_losses and logp.
+int policy_sum(const RowsArgs& p, bool mean, float* loss_out, int* n_valid_out, int* n_clipped_out, cudaStream_t s);
+
+// ---- paired preference loss on log-probabilities -------------------------------------------------------------------------------------------------
+struct PreferenceArgs {
+  const float *logp, *ref;
+  const int *tgt0, *offsets;
+  int N, P, kind, normalised, mean;
+  float beta, margin, smoothing;
+  float scale;                   // of the slopes, beside the mean's 1 / P
+  float *pair_losses, *ratios, *dlogp;
+};
+PreferenceArgs preference_args(const femto_preference_config& c, int N, int P);
+int preference(const PreferenceArgs& p, float* loss_out, cudaStream_t s);
+
+// ---- behind the lm_head tail of a training step ---------------------------------------------------------------------------------------------------
+// The tail gives the cross-entropy of each row, -log p; the objective gives back the factors of its gradient, d loss / d (-log p) / temperature.
+struct TokenObjective {
+  bool pairs = false;            // preference (needs all rows at once), or policy (row by row)
+  RowsArgs policy = {};          // tgt0, N, V, old, ref, adv, w, token_losses, logp, term, inv_t
+  PreferenceArgs preference = {};      // logp and dlogp: the workspace below
+  float* logp = nullptr;         // [N]
+  float* slopes = nullptr;       // [N]
+};
+int objective_slopes(const TokenObjective& o, const float* nll, int row0, int n, const float* scale_dev, float* loss_out, cudaStream_t s);

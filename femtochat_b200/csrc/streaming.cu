@@ -762,23 +762,24 @@ __global__ void __launch_bounds__(256) k_embed_bwd(const T* __restrict__ dx0, co
   }
 }
 
-// One block per row of fp32 logits: z = 15 tanh(l/15), lse, loss, dlogit (src/gpt.jl:12,172-194;
-// src/kernels.jl:16-28; ext/FemtoChatEnzymeExt.jl:175-189).
+// One block per row of fp32 logits: z = cap tanh(l/15), lse, loss, dlogit (src/gpt.jl:12,172-194;
+// src/kernels.jl:16-28; ext/FemtoChatEnzymeExt.jl:175-189).  cap is 15 over a temperature; a factor for each row (w_rows) takes the
+// place of w; without dlogit only the loss is computed.
 template <typename T>
 __global__ void __launch_bounds__(256) k_xent_rows(const float* __restrict__ logits, long long ldl,
                                                    const int* __restrict__ tgt0, int V, float w_host,
                                                    const float* __restrict__ w_dev, T* __restrict__ dlogit,
                                                    long long lddl,
-                                                   float* __restrict__ loss_rows) {
+                                                   float* __restrict__ loss_rows, float cap, const float* __restrict__ w_rows) {
   pdl_trigger();
   __shared__ float red[8];
   __shared__ float bc;
   const long long row = blockIdx.x;
-  const float w = w_host * (w_dev ? w_dev[0] : 1.f);
+  const float w = w_rows ? w_rows[row] : w_host * (w_dev ? w_dev[0] : 1.f);
   const float* l = logits + row * ldl;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float mx = -INFINITY;
-  for (int v = threadIdx.x; v < V; v += 256) mx = fmaxf(mx, 15.f * tanhf(l[v] * (1.f / 15.f)));
+  for (int v = threadIdx.x; v < V; v += 256) mx = fmaxf(mx, cap * tanhf(l[v] * (1.f / 15.f)));
   mx = warp_max(mx);
   if (lane == 0) red[warp] = mx;
   __syncthreads();
@@ -786,7 +787,7 @@ __global__ void __launch_bounds__(256) k_xent_rows(const float* __restrict__ log
   __syncthreads();
   mx = bc;
   float sum = 0.f;
-  for (int v = threadIdx.x; v < V; v += 256) sum += expf(15.f * tanhf(l[v] * (1.f / 15.f)) - mx);
+  for (int v = threadIdx.x; v < V; v += 256) sum += expf(cap * tanhf(l[v] * (1.f / 15.f)) - mx);
   sum = warp_sum(sum);
   __syncthreads();
   if (lane == 0) red[warp] = sum;
@@ -795,11 +796,12 @@ __global__ void __launch_bounds__(256) k_xent_rows(const float* __restrict__ log
   __syncthreads();
   const float lse = mx + logf(bc);
   const int tg = tgt0[row];
-  if (threadIdx.x == 0) loss_rows[row] = tg >= 0 ? lse - 15.f * tanhf(l[tg] * (1.f / 15.f)) : 0.f;
+  if (threadIdx.x == 0) loss_rows[row] = tg >= 0 ? lse - cap * tanhf(l[tg] * (1.f / 15.f)) : 0.f;
+  if (!dlogit) return;
   T* dl = dlogit + row * lddl;
   for (int v = threadIdx.x; v < V; v += 256) {
     float th = tanhf(l[v] * (1.f / 15.f));
-    float z = 15.f * th;
+    float z = cap * th;
     float dz = tg >= 0 ? w * (expf(z - lse) - (v == tg ? 1.f : 0.f)) : 0.f;
     dl[v] = from_f<T>(dz * (1.f - th * th));
   }
@@ -910,19 +912,19 @@ __global__ void __launch_bounds__(256) k_xent_finalize(const float2* __restrict_
 }
 
 // In place on a chunk of stored bf16 logits l[row][col]: d loss / d logit = w (softmax(z) - onehot) (1 - tanh^2(l/15)),
-// z = 15 tanh(l/15), with the row's logsumexp from the statistics pass (src/kernels.jl:16-28;
+// z = cap tanh(l/15) (cap = 15 over a temperature; w may be one number for each row), with the row's logsumexp from the statistics pass (src/kernels.jl:16-28;
 // ext/FemtoChatEnzymeExt.jl:175-189).  Same tanh.approx / ex2 arithmetic as that pass, so softmax sums to 1 over
 // the stored values.  A thread takes four 8-column groups 2048 columns apart (all four loads in flight before the
 // arithmetic); rows with an ignored target become zero.
 __global__ void __launch_bounds__(256) k_xent_dlogit_inplace(bf16* __restrict__ buf, long long ld,
                                                              const float* __restrict__ lse_rows,
                                                              const int* __restrict__ tgt0, int V, float w_host,
-                                                             const float* __restrict__ w_dev) {
+                                                             const float* __restrict__ w_dev, float cap, const float* __restrict__ w_rows) {
   pdl_trigger();
   const long long row = blockIdx.y;
   const int col0 = blockIdx.x * 8192 + threadIdx.x * 8;
   const int tg = tgt0[row];
-  const float w = tg >= 0 ? w_host * (w_dev ? w_dev[0] : 1.f) : 0.f;
+  const float w = tg >= 0 ? (w_rows ? w_rows[row] : w_host * (w_dev ? w_dev[0] : 1.f)) : 0.f;
   const float lse = lse_rows[row];
   bf16* base = buf + row * ld;
   uint4 q[4];
@@ -938,7 +940,7 @@ __global__ void __launch_bounds__(256) k_xent_dlogit_inplace(bf16* __restrict__ 
     for (int e = 0; e < 8; e++) {
       float t;
       asm("tanh.approx.f32 %0, %1;" : "=f"(t) : "f"(__bfloat162float(h[e]) * (1.f / 15.f)));
-      const float z = 15.f * t;
+      const float z = cap * t;
       const float dz = w * (__expf(z - lse) - ((col + e) == tg ? 1.f : 0.f));
       h[e] = __float2bfloat16_rn(dz * (1.f - t * t));
     }
@@ -1097,8 +1099,8 @@ int Stream<T>::embed_bwd(const T* dx0, const T* table, const int* tok0, const T*
 }
 template <typename T>
 int Stream<T>::xent_rows(const float* logits, long long ldl, const int* tgt0, int n, int V, float w,
-                         const float* w_dev, T* dlogit, long long lddl, float* loss_rows, cudaStream_t s) {
-  k_xent_rows<T><<<n, 256, 0, s>>>(logits, ldl, tgt0, V, w, w_dev, dlogit, lddl, loss_rows);
+                         const float* w_dev, T* dlogit, long long lddl, float* loss_rows, cudaStream_t s, float cap, const float* w_rows) {
+  k_xent_rows<T><<<n, 256, 0, s>>>(logits, ldl, tgt0, V, w, w_dev, dlogit, lddl, loss_rows, cap, w_rows);
   KERNEL_CHECK();
   return 0;
 }
@@ -1130,9 +1132,9 @@ int xent_finalize(const float2* stats, int ntile, const float* tz, const int* tg
   return 0;
 }
 int xent_dlogit_inplace(void* logits_bf16, long long ld, const float* lse_rows, const int* tgt0, int n, int V, float w,
-                        const float* w_dev, cudaStream_t s) {
+                        const float* w_dev, cudaStream_t s, float cap, const float* w_rows) {
   if ((ld & 7) || (V & 7)) return femto_fail(FEMTO_ERR_ALIGN, "xent_dlogit_inplace: row pitch and vocabulary must be multiples of 8");
-  k_xent_dlogit_inplace<<<dim3(cdiv(V, 8192), n), 256, 0, s>>>(reinterpret_cast<bf16*>(logits_bf16), ld, lse_rows, tgt0, V, w, w_dev);
+  k_xent_dlogit_inplace<<<dim3(cdiv(V, 8192), n), 256, 0, s>>>(reinterpret_cast<bf16*>(logits_bf16), ld, lse_rows, tgt0, V, w, w_dev, cap, w_rows);
   KERNEL_CHECK();
   return 0;
 }

@@ -55,14 +55,14 @@ template <typename T> struct Stream {
                        float eps, T* dE, cudaStream_t s);
   static int xent_rows(const float* logits, long long ldl, const int* tgt0, int n, int V, float w,
                        const float* w_dev, T* dlogit,
-                       long long lddl, float* loss_rows, cudaStream_t s);
+                       long long lddl, float* loss_rows, cudaStream_t s, float cap = 15.f, const float* w_rows = nullptr);
   static int cast_all(const float* theta, const CastJob* jobs, int n_jobs, int from, int to, cudaStream_t s);      // blocks [from, to) of the jobs
 };
 
 int sum_rows_to_scalar(const float* rows, int n, float* out, const int* tgt0, int* n_valid_out, float scale_by_valid,
                        cudaStream_t s);
 int xent_dlogit_inplace(void* logits_bf16, long long ld, const float* lse_rows, const int* tgt0, int n, int V, float w,
-                        const float* w_dev, cudaStream_t s);
+                        const float* w_dev, cudaStream_t s, float cap = 15.f, const float* w_rows = nullptr);
 int softcap_inplace(float* x, long long n, cudaStream_t s, float cap = 15.f);   // x = cap tanh(x / cap)
 int xent_finalize(const float2* stats, int ntile, const float* tz, const int* tgt0, int n, float* lse,
                   float* loss_rows, cudaStream_t s);

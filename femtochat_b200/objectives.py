@@ -12,6 +12,7 @@ import math
 from typing import NamedTuple, Optional
 
 from . import _lib
+from .gpt import _dev_i32
 
 PREFERENCES = {"sigmoid": 0, "squared": 1}
 
@@ -99,6 +100,20 @@ def _gradient_of(logits, n, V, pitch, out):
     return out, _rows("out", out)[2]
 
 
+class PolicyStep(NamedTuple):
+    loss: object            # [1]
+    n_valid: object         # [1] int32
+    n_clipped: object       # [1] int32
+    logp: object            # [B][T]
+
+
+class PreferenceStep(NamedTuple):
+    loss: object            # [1]
+    pair_losses: object     # [P]
+    ratios: object          # [2 P]
+    logp: object            # [B][T]
+
+
 class _Device:
     """Makes the tensors' device the current one where it is not."""
 
@@ -181,6 +196,13 @@ def _preference_config(kind, beta, margin, label_smoothing, length_normalised, r
     return _lib.PreferenceConfigC(PREFERENCES[kind], beta, margin, label_smoothing, 1 if length_normalised else 0, _lib.REDUCTION[reduction])
 
 
+def _offsets(offsets, device):
+    import torch
+    if offsets.dim() != 1 or offsets.shape[0] % 2 != 1:
+        raise ValueError(f"offsets must be [2 P + 1], not {tuple(offsets.shape)}")
+    return _on_device("offsets", offsets, torch.int32, offsets.shape, device), offsets.shape[0] // 2
+
+
 def preference_loss(logp, offsets, targets0=None, ref_logp=None, kind: str = "sigmoid", beta: float = 0.1, margin: float = 0.0,
                     label_smoothing: float = 0.0, length_normalised: bool = False, reduction: str = "mean", gradient: bool = True) -> PreferenceLoss:
     """Preference loss of pairs of answers from their tokens' log-probabilities (any shape, taken in order): answer k is the rows
@@ -192,10 +214,8 @@ def preference_loss(logp, offsets, targets0=None, ref_logp=None, kind: str = "si
     f32, device, shape = torch.float32, logp.device, logp.shape
     logp, ref_logp = _on_device("logp", logp, f32, shape, device), _on_device("ref_logp", ref_logp, f32, shape, device)
     targets0 = _on_device("targets0", targets0, torch.int32, shape, device)
-    if offsets.dim() != 1 or offsets.shape[0] % 2 != 1:
-        raise ValueError(f"offsets must be [2 P + 1], not {tuple(offsets.shape)}")
-    offsets = _on_device("offsets", offsets, torch.int32, offsets.shape, device)
-    n, P = logp.numel(), offsets.shape[0] // 2
+    offsets, P = _offsets(offsets, device)
+    n = logp.numel()
     if n >= 1 << 31:
         raise ValueError(f"{n} tokens")
     cfg = _preference_config(kind, beta, margin, label_smoothing, length_normalised, reduction)
@@ -207,3 +227,55 @@ def preference_loss(logp, offsets, targets0=None, ref_logp=None, kind: str = "si
             _lib.ptr(logp), _lib.ptr(ref_logp), _lib.ptr(targets0), n, _lib.ptr(offsets), P, C.byref(cfg), _lib.ptr(loss), _lib.ptr(pair_losses),
             _lib.ptr(ratios), _lib.ptr(dlogp), _lib.stream_ptr()))
     return PreferenceLoss(loss, pair_losses, ratios, dlogp)
+
+
+# ---- the GPT's steps ----------------------------------------------------------------------------------------------------------------------
+def forward_token_logprobs(params, state, layout, tokens, targets, positions=None, temperature: float = 1.0):
+    """Log-probabilities [B][T] that the model gives the targets (0 where ignored), at a temperature: those of answers before an update, or
+    under a reference model.  Tokens, targets and positions as for `loss_and_gradient_`."""
+    import torch
+    tok, tgt, pos = _dev_i32(tokens), _dev_i32(targets), _dev_i32(positions)
+    logp = torch.empty(tok.shape, dtype=torch.float32, device=tok.device)
+    _lib.check(_lib.lib().femto_forward_token_logprobs(state.h, _lib.ptr(params.theta), _lib.ptr(tok), _lib.ptr(tgt), _lib.ptr(pos), tok.shape[0],
+                                                       temperature, _lib.ptr(logp), _lib.stream_ptr()))
+    return logp
+
+
+def policy_loss_and_gradient_(params, state, layout, tokens, targets, old_logp, advantages, positions=None, ref_logp=None, weights=None,
+                              clip_low: float = 0.2, clip_high: Optional[float] = 0.2, kl_coef: float = 0.0, temperature: float = 1.0,
+                              reduction: str = "sum", accumulate: bool = False) -> PolicyStep:
+    """A training step on `policy_loss`: fills params.delta (or adds to it), as `loss_and_gradient_` does for the cross-entropy.  old_logp,
+    advantages, ref_logp and weights are [B][T]."""
+    import torch
+    tok, tgt, pos = _dev_i32(tokens), _dev_i32(targets), _dev_i32(positions)
+    f32, device = torch.float32, tok.device
+    old_logp, advantages, ref_logp, weights = (_on_device(name, t, f32, tok.shape, device) for name, t in
+                                               (("old_logp", old_logp), ("advantages", advantages), ("ref_logp", ref_logp), ("weights", weights)))
+    cfg = _policy_config(clip_low, clip_high, kl_coef, temperature, reduction)
+    loss, logp = torch.empty(1, dtype=f32, device=device), torch.empty(tok.shape, dtype=f32, device=device)
+    n_valid, n_clipped = torch.empty(2, 1, dtype=torch.int32, device=device)
+    _lib.check(_lib.lib().femto_policy_loss_and_gradient(
+        state.h, _lib.ptr(params.theta), _lib.ptr(params.delta), _lib.ptr(tok), _lib.ptr(tgt), _lib.ptr(pos), tok.shape[0], _lib.ptr(old_logp),
+        _lib.ptr(advantages), _lib.ptr(ref_logp), _lib.ptr(weights), C.byref(cfg), 1 if accumulate else 0, _lib.ptr(loss), _lib.ptr(n_valid),
+        _lib.ptr(n_clipped), _lib.ptr(logp), _lib.stream_ptr()))
+    return PolicyStep(loss, n_valid, n_clipped, logp)
+
+
+def preference_loss_and_gradient_(params, state, layout, tokens, targets, offsets, positions=None, ref_logp=None, kind: str = "sigmoid",
+                                  beta: float = 0.1, margin: float = 0.0, label_smoothing: float = 0.0, length_normalised: bool = False,
+                                  reduction: str = "mean", accumulate: bool = False) -> PreferenceStep:
+    """A training step on `preference_loss`: fills params.delta (or adds to it).  offsets [2 P + 1] (int32) count rows of the flattened [B][T]
+    arrays; with one answer a column, chosen and rejected in turn, they are the multiples of T."""
+    import torch
+    tok, tgt, pos = _dev_i32(tokens), _dev_i32(targets), _dev_i32(positions)
+    f32, device = torch.float32, tok.device
+    ref_logp = _on_device("ref_logp", ref_logp, f32, tok.shape, device)
+    offsets, P = _offsets(offsets, device)
+    cfg = _preference_config(kind, beta, margin, label_smoothing, length_normalised, reduction)
+    loss, logp = torch.empty(1, dtype=f32, device=device), torch.empty(tok.shape, dtype=f32, device=device)
+    pair_losses, ratios = torch.empty(P, dtype=f32, device=device), torch.empty(2 * P, dtype=f32, device=device)
+    _lib.check(_lib.lib().femto_preference_loss_and_gradient(
+        state.h, _lib.ptr(params.theta), _lib.ptr(params.delta), _lib.ptr(tok), _lib.ptr(tgt), _lib.ptr(pos), tok.shape[0], _lib.ptr(ref_logp),
+        _lib.ptr(offsets), P, C.byref(cfg), 1 if accumulate else 0, _lib.ptr(loss), _lib.ptr(pair_losses), _lib.ptr(ratios), _lib.ptr(logp),
+        _lib.stream_ptr()))
+    return PreferenceStep(loss, pair_losses, ratios, logp)

@@ -130,6 +130,46 @@ int32_t femto_loss_and_gradient_host(femto_handle* h, const float* theta, float*
                                      const int32_t* h_positions, int32_t B, int32_t reduction,
                                      int32_t accumulate, float* h_loss, int32_t* h_n_valid, void* stream);
 
+/* ---- training on a model's own answers ------------------------------------------------------- */
+/* What follows pretraining: answers with rewards, or in pairs.  No counterpart in the reference.  The objectives are those of
+ * femto_policy_loss and femto_preference_loss below, of the log-probabilities that the model gives the targets; the step is that of
+ * femto_loss_and_gradient (weights, positions, accumulation, data parallelism) with them in the cross-entropy's place. */
+typedef struct femto_policy_config {
+  float temperature; /* > 0: at which the answers were sampled */
+  float clip_low, clip_high; /* the ratio r counts up to the range 1 - clip_low .. 1 + clip_high (infinity: no bound above) */
+  float kl_coef;     /* beta >= 0 */
+  int32_t reduction; /* FEMTO_REDUCTION_SUM, or _MEAN over the rows with a target */
+} femto_policy_config;
+#define FEMTO_PREFERENCE_SIGMOID 0
+#define FEMTO_PREFERENCE_SQUARED 1
+typedef struct femto_preference_config {
+  int32_t kind;
+  float beta;            /* > 0 */
+  float margin, label_smoothing; /* sigmoid only */
+  int32_t length_normalised; /* rho is divided by the number of the answer's counted rows */
+  int32_t reduction;     /* FEMTO_REDUCTION_SUM or _MEAN over the pairs */
+} femto_preference_config;
+/* Log-probabilities of the targets at a temperature, fp32 [B][T], 0 where the target is ignored: those of the answers before an update
+ * (old_logp), or under a reference model.  Every sum is taken as a training step takes it, so that the ratios of the first step are exactly 1
+ * (femto_forward_token_losses may take other kernels, and differs by roundings). */
+int32_t femto_forward_token_logprobs(femto_handle* h, const float* theta, const int32_t* tokens, const int32_t* targets,
+                                     const int32_t* positions, int32_t B, float temperature, float* logp_out, void* stream);
+/* old_logp, advantages, ref_logp, weights: fp32 [B][T] (the last two may be NULL, ref_logp when kl_coef is 0).  loss_out, n_valid_out and
+ * n_clipped_out (may be NULL) are device scalars; logp_out (may be NULL) [B][T] receives the log-probabilities of this step. */
+int32_t femto_policy_loss_and_gradient(femto_handle* h, const float* theta, float* delta, const int32_t* tokens,
+                                       const int32_t* targets, const int32_t* positions, int32_t B, const float* old_logp,
+                                       const float* advantages, const float* ref_logp, const float* weights,
+                                       const femto_policy_config* h_cfg, int32_t accumulate, float* loss_out,
+                                       int32_t* n_valid_out, int32_t* n_clipped_out, float* logp_out, void* stream);
+/* Answers are runs of the B * T rows taken in order: answer k is the rows offsets[k] .. offsets[k + 1] - 1 (int32 [2 P + 1], device), without
+ * those whose target is ignored.  ref_logp fp32 [B][T] or NULL; logp_out may be NULL.  With more rows than a chunk of the lm_head tail
+ * (16 384) the chunks' logits are computed twice. */
+int32_t femto_preference_loss_and_gradient(femto_handle* h, const float* theta, float* delta, const int32_t* tokens,
+                                           const int32_t* targets, const int32_t* positions, int32_t B, const float* ref_logp,
+                                           const int32_t* offsets, int32_t P, const femto_preference_config* h_cfg,
+                                           int32_t accumulate, float* loss_out, float* pair_losses, float* ratios,
+                                           float* logp_out, void* stream);
+
 /* ---- generation with a key/value cache (src/generation.jl:26-56) ----------------------------- */
 /* The reference's `generate` runs the whole context through the model for every new token (the cache is a TODO
  * at src/gpt.jl:81).  Here femto_prefill runs the prompt once and keeps every block's keys and values;
@@ -457,12 +497,6 @@ int32_t femto_token_logprobs_gradient(int32_t dtype, void* dlogits, int64_t ldd,
                                       const int32_t* targets0, int32_t N, int32_t V, float temperature, const float* dlogp,
                                       const float* dentropy, void* stream);
 
-typedef struct femto_policy_config {
-  float temperature; /* > 0: at which the answers were sampled */
-  float clip_low, clip_high; /* the ratio r counts up to the range 1 - clip_low .. 1 + clip_high (infinity: no bound above) */
-  float kl_coef;     /* beta >= 0 */
-  int32_t reduction; /* FEMTO_REDUCTION_SUM, or _MEAN over the rows with a target */
-} femto_policy_config;
 /* Clipped policy loss with a KL term.  Of a row with a target, with lp = log p(target) and r = exp(lp - old_logp):
  *   token_loss = weight (-min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A) + beta (e^(ref_logp - lp) - (ref_logp - lp) - 1))
  * advantages A [N]; ref_logp [N] (may be NULL when beta is 0); weights [N] (NULL = 1; where a weight is 0 loss and gradient are 0).
@@ -474,15 +508,6 @@ int32_t femto_policy_loss(int32_t dtype, const void* logits, int64_t ldl, const 
                           const femto_policy_config* h_cfg, void* dlogits, int64_t ldd, float* token_losses, float* logp,
                           float* loss_out, int32_t* n_valid_out, int32_t* n_clipped_out, void* stream);
 
-#define FEMTO_PREFERENCE_SIGMOID 0
-#define FEMTO_PREFERENCE_SQUARED 1
-typedef struct femto_preference_config {
-  int32_t kind;
-  float beta;            /* > 0 */
-  float margin, label_smoothing; /* sigmoid only */
-  int32_t length_normalised; /* rho is divided by the number of the answer's counted rows */
-  int32_t reduction;     /* FEMTO_REDUCTION_SUM or _MEAN over the pairs */
-} femto_preference_config;
 /* Preference loss of P pairs of answers.  Answer k is the rows offsets[k] .. offsets[k + 1] - 1 (int32 [2 P + 1], device, ascending), 2 p
  * the chosen and 2 p + 1 the rejected one of pair p; rho_k = sum over its rows of logp - ref_logp (ref_logp may be NULL = 0), without the
  * rows whose target is negative (targets0 may be NULL: all count).  With D = rho_2p - rho_2p+1 and h = beta D - margin:

@@ -105,3 +105,10 @@ def test_python_refuses_options():
     with pytest.raises(ValueError, match="kind"):
         objectives._preference_config("hinge", 0.1, 0.0, 0.0, False, "mean")
     assert objectives._policy_config(0.2, None, 0.0, 1.0, "sum").clip_high == math.inf
+
+
+def test_steps_refuse_without_a_handle():
+    L, c, q = _lib.lib(), C.byref(_lib.PolicyConfigC(1.0, 0.2, 0.2, 0.0, 0)), C.byref(_lib.PreferenceConfigC(0, 0.1, 0.0, 0.0, 0, 1))
+    assert L.femto_forward_token_logprobs(None, at(0), at(1), at(2), None, 1, 1.0, at(3), None) == ARG
+    assert L.femto_policy_loss_and_gradient(None, at(0), at(1), at(2), at(3), None, 1, at(4), at(5), None, None, c, 0, at(6), at(7), None, None, None) == ARG
+    assert L.femto_preference_loss_and_gradient(None, at(0), at(1), at(2), at(3), None, 1, None, at(4), 1, q, 0, at(5), at(6), at(7), None, None) == ARG
