@@ -191,5 +191,7 @@ def ptr(t):
 
 
 def stream_ptr():
+    """The current stream of the current device."""
     import torch
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # 0.2 us; through a Stream object 2 us
+    return C.c_void_p(raw(torch.cuda.current_device()) if raw is not None else torch.cuda.current_stream().cuda_stream)

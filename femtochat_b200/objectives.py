@@ -42,33 +42,40 @@ def _on_device(name, t, dtype, shape, device):
     """A contiguous array of `shape` on `device`, or an error that names it."""
     if t is None:
         return None
+    if t.dtype is dtype and t.shape == shape and t.device == device:
+        return t if t.is_contiguous() else t.contiguous()
     if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the logits on {device}")
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
     if t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
-    if t.shape != shape:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
-    return t if t.is_contiguous() else t.contiguous()
+    raise ValueError(f"{name} has shape {tuple(t.shape)}, not {tuple(shape)}")
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
 
 
 def _rows(name, t):
-    """(rows, V, pitch) of [..., V] logits whose rows lie one pitch apart."""
+    """(rows, V, pitch, type) of [..., V] logits whose rows lie one pitch apart."""
     import torch
-    if t.dtype not in (torch.float32, torch.bfloat16):
+    code = _lib.F32 if t.dtype is torch.float32 else _lib.BF16 if t.dtype is torch.bfloat16 else None
+    if code is None:
         raise ValueError(f"{name} must be float32 or bfloat16, not {t.dtype}")
     if not t.is_cuda:
         raise ValueError(f"{name} must be on a CUDA device")
-    if t.dim() < 1 or t.shape[-1] == 0:
+    shape = t.shape
+    if not shape or shape[-1] == 0:
         raise ValueError(f"{name} must be [..., V]")
-    V, n = t.shape[-1], t.numel() // t.shape[-1]
-    if n == 0:
-        return 0, V, V
+    V, n = shape[-1], t.numel() // shape[-1]
     if n >= 1 << 31 or V >= 1 << 31:
         raise ValueError(f"{name}: {n} rows of {V}")
-    if V > 1 and t.stride(-1) != 1:
+    if n == 0 or t.is_contiguous():
+        return n, V, V, code
+    strides = t.stride()
+    if V > 1 and strides[-1] != 1:
         raise ValueError(f"{name} must have unit stride along the vocabulary")
     pitch, reach = None, 1
-    for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+    for size, stride in zip(reversed(shape[:-1]), reversed(strides[:-1])):
         if size == 1:
             continue
         if pitch is None:
@@ -80,19 +87,16 @@ def _rows(name, t):
         pitch = V
     if pitch < V:
         raise ValueError(f"the rows of {name} overlap")
-    return n, V, pitch
-
-
-def _code(t):
-    import torch
-    return _lib.BF16 if t.dtype == torch.bfloat16 else _lib.F32
+    return n, V, pitch, code
 
 
 def _gradient_of(logits, n, V, pitch, out):
     """The tensor that takes the gradient, and its pitch: the logits' own where that wastes little, so that rows of both start alike."""
     import torch
     if out is None:
-        if pitch == V or n == 0 or pitch - V > V // 8 + 64:
+        if pitch == V:
+            return torch.empty_like(logits, memory_format=torch.contiguous_format), V
+        if pitch - V > V // 8 + 64:
             return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), V
         return torch.empty((n, pitch), dtype=logits.dtype, device=logits.device)[:, :V].view(logits.shape), pitch
     if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
@@ -114,47 +118,40 @@ class PreferenceStep(NamedTuple):
     logp: object            # [B][T]
 
 
-class _Device:
-    """Makes the tensors' device the current one where it is not."""
-
-    def __init__(self, device):
-        import torch
-        self.other = torch.cuda.device(device) if device.index != torch.cuda.current_device() else None
-
-    def __enter__(self):
-        if self.other is not None:
-            self.other.__enter__()
-
-    def __exit__(self, *exc):
-        if self.other is not None:
-            self.other.__exit__(*exc)
+def _call(device, name, *args):
+    """The library's call on the current stream of the tensors' device."""
+    import torch
+    if device.index == torch.cuda.current_device():
+        _lib.check(getattr(_lib.lib(), name)(*args, _lib.stream_ptr()))
+    else:
+        with torch.cuda.device(device):
+            _lib.check(getattr(_lib.lib(), name)(*args, _lib.stream_ptr()))
 
 
 def token_logprobs(logits, targets0, temperature: float = 1.0, entropy: bool = False) -> TokenLogprobs:
     """Log-probabilities of the targets under softmax(logits / temperature), and the entropy where asked for."""
     import torch
-    n, V, pitch = _rows("logits", logits)
-    shape = logits.shape[:-1]
-    targets0 = _on_device("targets0", targets0, torch.int32, shape, logits.device)
-    logp = torch.empty(shape, dtype=torch.float32, device=logits.device)
-    ent = torch.empty(shape, dtype=torch.float32, device=logits.device) if entropy else None
-    with _Device(logits.device):
-        _lib.check(_lib.lib().femto_token_logprobs(_code(logits), _lib.ptr(logits), pitch, _lib.ptr(targets0), n, V, temperature, _lib.ptr(logp),
-                                                   _lib.ptr(ent), _lib.stream_ptr()))
+    n, V, pitch, code = _rows("logits", logits)
+    shape, device = logits.shape[:-1], logits.device
+    targets0 = _on_device("targets0", targets0, torch.int32, shape, device)
+    if targets0 is None:
+        raise ValueError("targets0 is None")
+    logp = torch.empty_like(targets0, dtype=torch.float32)
+    ent = torch.empty_like(logp) if entropy else None
+    _call(device, "femto_token_logprobs", code, logits.data_ptr(), pitch, _address(targets0), n, V, temperature, logp.data_ptr(), _address(ent))
     return TokenLogprobs(logp, ent)
 
 
 def token_logprobs_gradient(logits, targets0, dlogp, dentropy=None, temperature: float = 1.0, out=None):
     """d objective / d logits from d objective / d logp (and / d entropy).  `out` may be the logits themselves."""
     import torch
-    n, V, pitch = _rows("logits", logits)
-    shape, f32 = logits.shape[:-1], torch.float32
-    targets0 = _on_device("targets0", targets0, torch.int32, shape, logits.device)
-    dlogp, dentropy = _on_device("dlogp", dlogp, f32, shape, logits.device), _on_device("dentropy", dentropy, f32, shape, logits.device)
+    n, V, pitch, code = _rows("logits", logits)
+    shape, f32, device = logits.shape[:-1], torch.float32, logits.device
+    targets0 = _on_device("targets0", targets0, torch.int32, shape, device)
+    dlogp, dentropy = _on_device("dlogp", dlogp, f32, shape, device), _on_device("dentropy", dentropy, f32, shape, device)
     out, out_pitch = _gradient_of(logits, n, V, pitch, out)
-    with _Device(logits.device):
-        _lib.check(_lib.lib().femto_token_logprobs_gradient(_code(logits), _lib.ptr(out), out_pitch, _lib.ptr(logits), pitch, _lib.ptr(targets0), n, V,
-                                                            temperature, _lib.ptr(dlogp), _lib.ptr(dentropy), _lib.stream_ptr()))
+    _call(device, "femto_token_logprobs_gradient", code, out.data_ptr(), out_pitch, logits.data_ptr(), pitch, _address(targets0), n, V, temperature,
+          _address(dlogp), _address(dentropy))
     return out
 
 
@@ -170,21 +167,21 @@ def policy_loss(logits, targets0, old_logp, advantages, ref_logp=None, weights=N
     weight (-min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (e^g - g - 1)) per token, r = exp(logp - old_logp) and
     g = ref_logp - logp.  clip_high=None bounds the ratio below only.  `out` may be the logits themselves."""
     import torch
-    n, V, pitch = _rows("logits", logits)
+    n, V, pitch, code = _rows("logits", logits)
     shape, f32, device = logits.shape[:-1], torch.float32, logits.device
     targets0 = _on_device("targets0", targets0, torch.int32, shape, device)
-    old_logp, advantages, ref_logp, weights = (_on_device(name, t, f32, shape, device) for name, t in
-                                               (("old_logp", old_logp), ("advantages", advantages), ("ref_logp", ref_logp), ("weights", weights)))
+    old_logp, advantages = _on_device("old_logp", old_logp, f32, shape, device), _on_device("advantages", advantages, f32, shape, device)
+    ref_logp, weights = _on_device("ref_logp", ref_logp, f32, shape, device), _on_device("weights", weights, f32, shape, device)
     cfg = _policy_config(clip_low, clip_high, kl_coef, temperature, reduction)
     d, d_pitch = _gradient_of(logits, n, V, pitch, out) if gradient else (None, V)
-    token_losses, logp = torch.empty((2,) + shape, dtype=f32, device=device)
+    if old_logp is None or advantages is None:
+        raise ValueError("old_logp or advantages is None")
+    token_losses, logp = torch.empty_like(old_logp), torch.empty_like(old_logp)
     loss = torch.empty(1, dtype=f32, device=device)
-    n_valid, n_clipped = torch.empty(2, 1, dtype=torch.int32, device=device)
-    with _Device(device):
-        _lib.check(_lib.lib().femto_policy_loss(
-            _code(logits), _lib.ptr(logits), pitch, _lib.ptr(targets0), n, V, _lib.ptr(old_logp), _lib.ptr(advantages), _lib.ptr(ref_logp),
-            _lib.ptr(weights), C.byref(cfg), _lib.ptr(d), d_pitch, _lib.ptr(token_losses), _lib.ptr(logp), _lib.ptr(loss), _lib.ptr(n_valid),
-            _lib.ptr(n_clipped), _lib.stream_ptr()))
+    n_valid, n_clipped = torch.empty(1, dtype=torch.int32, device=device), torch.empty(1, dtype=torch.int32, device=device)
+    _call(device, "femto_policy_loss", code, logits.data_ptr(), pitch, _address(targets0), n, V, _address(old_logp), _address(advantages),
+          _address(ref_logp), _address(weights), C.byref(cfg), _address(d), d_pitch, token_losses.data_ptr(), logp.data_ptr(), loss.data_ptr(),
+          n_valid.data_ptr(), n_clipped.data_ptr())
     return PolicyLoss(loss, n_valid, n_clipped, token_losses, logp, d)
 
 
@@ -221,11 +218,9 @@ def preference_loss(logp, offsets, targets0=None, ref_logp=None, kind: str = "si
     cfg = _preference_config(kind, beta, margin, label_smoothing, length_normalised, reduction)
     loss = torch.empty(1, dtype=f32, device=device)
     pair_losses, ratios = torch.empty(P, dtype=f32, device=device), torch.empty(2 * P, dtype=f32, device=device)
-    dlogp = torch.empty(shape, dtype=f32, device=device) if gradient else None
-    with _Device(device):
-        _lib.check(_lib.lib().femto_preference_loss(
-            _lib.ptr(logp), _lib.ptr(ref_logp), _lib.ptr(targets0), n, _lib.ptr(offsets), P, C.byref(cfg), _lib.ptr(loss), _lib.ptr(pair_losses),
-            _lib.ptr(ratios), _lib.ptr(dlogp), _lib.stream_ptr()))
+    dlogp = torch.empty_like(logp) if gradient else None
+    _call(device, "femto_preference_loss", logp.data_ptr(), _address(ref_logp), _address(targets0), n, offsets.data_ptr(), P, C.byref(cfg),
+          loss.data_ptr(), pair_losses.data_ptr(), ratios.data_ptr(), _address(dlogp))
     return PreferenceLoss(loss, pair_losses, ratios, dlogp)
 
 
@@ -253,7 +248,7 @@ def policy_loss_and_gradient_(params, state, layout, tokens, targets, old_logp, 
                                                (("old_logp", old_logp), ("advantages", advantages), ("ref_logp", ref_logp), ("weights", weights)))
     cfg = _policy_config(clip_low, clip_high, kl_coef, temperature, reduction)
     loss, logp = torch.empty(1, dtype=f32, device=device), torch.empty(tok.shape, dtype=f32, device=device)
-    n_valid, n_clipped = torch.empty(2, 1, dtype=torch.int32, device=device)
+    n_valid, n_clipped = torch.empty(1, dtype=torch.int32, device=device), torch.empty(1, dtype=torch.int32, device=device)
     _lib.check(_lib.lib().femto_policy_loss_and_gradient(
         state.h, _lib.ptr(params.theta), _lib.ptr(params.delta), _lib.ptr(tok), _lib.ptr(tgt), _lib.ptr(pos), tok.shape[0], _lib.ptr(old_logp),
         _lib.ptr(advantages), _lib.ptr(ref_logp), _lib.ptr(weights), C.byref(cfg), 1 if accumulate else 0, _lib.ptr(loss), _lib.ptr(n_valid),
