@@ -253,19 +253,12 @@ template <typename T> __device__ __forceinline__ bool same_phase(const T* z, con
   return ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0;
 }
 
-__device__ __forceinline__ uint32_t cluster_size() { uint32_t n; asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n)); return n; }
-__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
-__device__ __forceinline__ void store_remote(const void* local, uint32_t rank, float v) {
-  uint32_t there;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(smem_u32(local)), "r"(rank));
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(v) : "memory");
-}
 __device__ __forceinline__ void group_barrier(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
 // ---- few rows -----------------------------------------------------------------------------------------------------------------------------------
 // A cluster of blocks holds a row in registers, NV words a thread; the statistics of all its warps go to every block's shared memory.  There is
 // little to overlap: what counts is that a row is brought by many multiprocessors at once.
-constexpr int FEW_WARPS = 8, MOST_CLUSTER = 8, FEW_WORDS = 8;
+constexpr int FEW_WARPS = 8, FEW_WORDS = 8;
 
 template <typename T, RowsMode MODE, bool STORE, bool ENTROPY, int NV>
 __global__ void __launch_bounds__(32 * FEW_WARPS) k_rows_few(const RowsArgs p) {

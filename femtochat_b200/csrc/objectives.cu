@@ -60,39 +60,73 @@ __global__ void __launch_bounds__(1024) k_policy_sum(const RowsArgs p, int mean,
 typedef PreferenceArgs Preference;
 
 // The rows of one answer; offsets that leave the rows or descend make it empty.
-__device__ __forceinline__ int2 answer_rows(const Preference& p, int answer) {
+__device__ __forceinline__ int2 answer_rows(const Preference& p, int answer, bool flag) {
   const int a = p.offsets[answer], b = p.offsets[answer + 1];
   if (a >= 0 && a <= b && b <= p.N) return make_int2(a, b);
-  if (threadIdx.x == 0) atomicOr(&g_objectives_status, ST_BAD_RANGE);
+  if (flag) atomicOr(&g_objectives_status, ST_BAD_RANGE);
   return make_int2(0, 0);
 }
 
-// One block per pair.  Sums of log ratios of two long answers nearly cancel: they are held in 64 bits.
+// One block per pair, or a cluster of blocks for long answers; half of a block on each answer.  Sums of log ratios of two long answers nearly
+// cancel: they are held in 64 bits.  Bound by latency (two dependent loads, a reduction, one thread's logarithm) until there are some
+// thousands of pairs, by HBM behind that.
 __global__ void __launch_bounds__(1024) k_preference_pairs(const Preference p) {
   pdl_trigger();
+  __shared__ double sums[32], all_sums[2][MOST_CLUSTER];
+  __shared__ int counts[32], all_counts[2][MOST_CLUSTER];
   __shared__ float slope_s[2];
-  const int pair = blockIdx.x;
-  int2 rows[2];
-  double rho[2];
-  int count[2];
-  for (int side = 0; side < 2; side++) {
-    rows[side] = answer_rows(p, 2 * pair + side);
-    double sum = 0.0;
-    int n = 0;
-    for (int i = rows[side].x + threadIdx.x; i < rows[side].y; i += 1024) {
-      if (p.tgt0 && p.tgt0[i] < 0) continue;
-      n++;
-      sum += (double)(p.ref ? p.logp[i] - p.ref[i] : p.logp[i]);
+  const int C = (int)cluster_size(), rank = (int)cluster_rank();
+  if (C > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");      // this block runs: its shared memory may be written
+  const int pair = blockIdx.x / C, half = blockDim.x >> 1, side = threadIdx.x >= half, tid = threadIdx.x - side * half, warps = half >> 5;
+  const int2 rows = answer_rows(p, 2 * pair + side, rank == 0 && tid == 0);
+  const unsigned first = rows.x + rank * half + tid, end = rows.y, step = C * half;
+  double sum = 0.0;
+  int n = 0;
+  uint32_t seen = 0;      // which of the thread's first 32 rows count
+  int q = 0;
+  for (unsigned i0 = first; i0 < end; i0 += 4 * step, q += 4) {      // four rows a thread in flight
+    int t[4];
+    float lp[4], ref[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const unsigned i = min(i0 + k * step, end - 1);
+      t[k] = p.tgt0 ? p.tgt0[i] : 0;
+      lp[k] = p.logp[i];
+      ref[k] = p.ref ? p.ref[i] : 0.f;
     }
-    rho[side] = block_total(sum);
-    count[side] = block_total(n);
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const bool counted = t[k] >= 0 && i0 + k * step < end;
+      n += counted;
+      if (q < 32) seen |= (uint32_t)counted << (q + k);
+      sum += counted ? (double)(lp[k] - ref[k]) : 0.0;      // rows that do not count may hold anything
+    }
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) { sum += __shfl_xor_sync(0xffffffffu, sum, o); n += __shfl_xor_sync(0xffffffffu, n, o); }
+  if ((threadIdx.x & 31) == 0) { sums[threadIdx.x >> 5] = sum; counts[threadIdx.x >> 5] = n; }
+  __syncthreads();
+  if (C > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+  if (threadIdx.x < 2) {      // each answer's sum over the block, to every block
+    const int k = threadIdx.x;
+    double total = 0.0;
+    int count = 0;
+    for (int i = 0; i < warps; i++) { total += sums[k * warps + i]; count += counts[k * warps + i]; }
+    for (int to = 0; to < C; to++) {
+      store_remote(&all_sums[k][rank], to, total);
+      store_remote(&all_counts[k][rank], to, count);
+    }
+  }
+  if (C > 1) asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory"); else __syncthreads();
   if (threadIdx.x == 0) {
-    double per[2];
-    for (int side = 0; side < 2; side++) {
-      per[side] = p.normalised ? 1.0 / max(count[side], 1) : 1.0;
-      rho[side] *= per[side];
-      p.ratios[2 * pair + side] = (float)rho[side];
+    double rho[2], per[2];
+    for (int k = 0; k < 2; k++) {
+      int count = 0;
+      rho[k] = 0.0;
+      for (int i = 0; i < C; i++) { rho[k] += all_sums[k][i]; count += all_counts[k][i]; }
+      per[k] = p.normalised ? 1.0 / max(count, 1) : 1.0;
+      rho[k] *= per[k];
+      if (rank == 0) p.ratios[2 * pair + k] = (float)rho[k];
     }
     const double delta = rho[0] - rho[1], beta = p.beta;
     double loss, slope;      // slope: by delta
@@ -106,23 +140,27 @@ __global__ void __launch_bounds__(1024) k_preference_pairs(const Preference p) {
       loss = u * u;
       slope = 2.0 * u;
     }
-    p.pair_losses[pair] = (float)loss;
+    if (rank == 0) p.pair_losses[pair] = (float)loss;
     slope *= (double)p.scale / (p.mean ? p.P : 1);
     slope_s[0] = (float)(slope * per[0]);
     slope_s[1] = (float)(-slope * per[1]);
   }
   if (!p.dlogp) return;
   __syncthreads();
-  for (int side = 0; side < 2; side++)
-    for (int i = rows[side].x + threadIdx.x; i < rows[side].y; i += 1024) p.dlogp[i] = p.tgt0 && p.tgt0[i] < 0 ? 0.f : slope_s[side];
+  const float d = slope_s[side];
+  q = 0;
+#pragma unroll 4
+  for (unsigned i = first; i < end; i += step, q++) p.dlogp[i] = (q < 32 ? seen >> q & 1u : !p.tgt0 || p.tgt0[i] >= 0) ? d : 0.f;
 }
 
 // Sum or mean over the pairs, and zeros as the gradient of rows that belong to no answer.
 __global__ void __launch_bounds__(1024) k_preference_sum(const Preference p, float* __restrict__ loss_out) {
   pdl_trigger();
+  pdl_wait();
   if (blockIdx.x == 0) {
     double sum = 0.0;
-    for (int i = threadIdx.x; i < p.P; i += 1024) sum += (double)p.pair_losses[i];
+#pragma unroll 4
+    for (int i = threadIdx.x; i < p.P; i += 1024) sum += (double)__ldcg(p.pair_losses + i);
     sum = block_total(sum);
     if (threadIdx.x == 0) *loss_out = (float)(p.mean && p.P > 0 ? sum / p.P : sum);
   }
@@ -158,10 +196,21 @@ PreferenceArgs preference_args(const femto_preference_config& c, int N, int P) {
 }
 int preference(const PreferenceArgs& p, float* loss_out, cudaStream_t s) {
   if (p.P > 0) {
-    k_preference_pairs<<<p.P, 1024, 0, s>>>(p);
+    // A thread has some eight rows of an answer of average length; where pairs are few and long, a cluster shares one (one pair of 70000 rows
+    // each: 87 -> 12 us), and where they are many, small blocks let one's reduction pass behind others' loads (1024 pairs of 1536 rows each:
+    // 14.6 us with 128 threads, 15.9 with 256, 21.2 with 512).
+    int threads = 64, C = 1;
+    while (threads < (p.P < 4 * device_sm_count() ? 1024 : 128) && (long long)threads * p.P * 8 < p.N) threads *= 2;
+    while (C < MOST_CLUSTER && (long long)C * p.P < device_sm_count() && (long long)C * 1024 * p.P * 8 < p.N) C *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = C; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)(p.P * C)); cfg.blockDim = dim3(threads); cfg.stream = s; cfg.attrs = &at; cfg.numAttrs = C > 1;
+    CUDA_TRY(cudaLaunchKernelEx(&cfg, k_preference_pairs, p));
     KERNEL_CHECK();
   }
-  k_preference_sum<<<p.dlogp ? std::min(cdiv(p.N, 4096) + 1, 148) : 1, 1024, 0, s>>>(p, loss_out);
+  CUDA_TRY(launch_dependent(k_preference_sum, dim3(p.dlogp ? std::min(cdiv(p.N, 4096) + 1, 148) : 1), dim3(1024), 0, s, p, loss_out));
   KERNEL_CHECK();
   return 0;
 }

@@ -80,6 +80,26 @@ __device__ __forceinline__ float entropy(const RowStats& s) {
   return s.l == 0.f ? 0.f : -log_sum(s.l).minus_from(s.a / s.l * (float)LN2);
 }
 
+// ---- clusters ----------------------------------------------------------------------------------------------------------------------------------
+constexpr int MOST_CLUSTER = 8;
+__device__ __forceinline__ uint32_t cluster_size() { uint32_t n; asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n)); return n; }
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t remote_address(const void* local, uint32_t rank) {
+  uint32_t there;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"((uint32_t)__cvta_generic_to_shared(local)), "r"(rank));
+  return there;
+}
+// `v` to where `local` lies in another block's shared memory
+__device__ __forceinline__ void store_remote(const float* local, uint32_t rank, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote_address(local, rank)), "f"(v) : "memory");
+}
+__device__ __forceinline__ void store_remote(const double* local, uint32_t rank, double v) {
+  asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(remote_address(local, rank)), "d"(v) : "memory");
+}
+__device__ __forceinline__ void store_remote(const int* local, uint32_t rank, int v) {
+  asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(remote_address(local, rank)), "r"(v) : "memory");
+}
+
 // ---- clipped policy term of one token ---------------------------------------------------------------------------------------------------
 // loss = w (-min(r A, clamp(r, lo, hi) A) + beta (e^g - g - 1)),  r = e^(lp - old),  g = ref - lp, and its derivative by lp.  The minimum is
 // the bounded product, which does not depend on lp, where A > 0 and r > hi or A < 0 and r < lo.  A weight of 0 counts nothing, whatever
