@@ -32,24 +32,50 @@ __global__ void __launch_bounds__(1024) k_count_targets(const int* __restrict__ 
   if (threadIdx.x == 0) *out = n;
 }
 
-// Sum (or mean over the rows with a target) of the token losses, and how many tokens the clipping held.
+// Sum (or mean over the rows with a target) of the token losses, and how many tokens the clipping held.  One block, or a cluster for many
+// rows (60000 rows: 40 us with one block, 8 with eight).
 __global__ void __launch_bounds__(1024) k_policy_sum(const RowsArgs p, int mean, float* loss_out, int* n_valid_out, int* n_clipped_out) {
   pdl_trigger();
+  __shared__ float sums[MOST_CLUSTER];
+  __shared__ int counts[2][MOST_CLUSTER];
+  const int C = (int)cluster_size(), rank = (int)cluster_rank();
+  if (C > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
   pdl_wait();
   float sum = 0.f;
   int n = 0, clipped = 0;
-#pragma unroll 4
-  for (long long i = threadIdx.x; i < p.N; i += 1024) {
-    const int t = p.tgt0[i];
-    const bool has = t >= 0 && t < p.V;
-    n += has;
-    sum += __ldcg(p.token_losses + i);      // 0 without a target
-    clipped += has && policy_clipped(p.term, policy_ratio(__ldcg(p.logp + i), p.old[i]), p.adv[i]);
+  const unsigned N = p.N, step = C * 1024;
+  for (unsigned i0 = rank * 1024 + threadIdx.x; i0 < N; i0 += 4 * step) {
+    int t[4];
+    float loss[4], lp[4], old[4], A[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const unsigned i = min(i0 + k * step, N - 1);
+      t[k] = p.tgt0[i];
+      loss[k] = __ldcg(p.token_losses + i);      // 0 without a target
+      lp[k] = __ldcg(p.logp + i);
+      old[k] = p.old[i];
+      A[k] = p.adv[i];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const bool has = t[k] >= 0 && t[k] < p.V && i0 + k * step < N;
+      n += has;
+      sum += has ? loss[k] : 0.f;
+      clipped += has && policy_clipped(p.term, policy_ratio(lp[k], old[k]), A[k]);
+    }
   }
   sum = block_total(sum);
   n = block_total(n);
   clipped = block_total(clipped);
+  if (C > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
   if (threadIdx.x == 0) {
+    store_remote(&sums[rank], 0, sum);
+    store_remote(&counts[0][rank], 0, n);
+    store_remote(&counts[1][rank], 0, clipped);
+  }
+  if (C > 1) asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+  if (rank == 0 && threadIdx.x == 0) {
+    for (int i = 1; i < C; i++) { sum += sums[i]; n += counts[0][i]; clipped += counts[1][i]; }
     *loss_out = mean && n > 0 ? sum / (float)n : sum;
     *n_valid_out = n;
     if (n_clipped_out) *n_clipped_out = clipped;
@@ -181,7 +207,8 @@ unsigned int objectives_status_word() {
 }
 
 int policy_sum(const RowsArgs& p, bool mean, float* loss_out, int* n_valid_out, int* n_clipped_out, cudaStream_t s) {
-  CUDA_TRY(launch_dependent(k_policy_sum, dim3(1), dim3(1024), 0, s, p, (int)mean, loss_out, n_valid_out, n_clipped_out));
+  const int C = p.N > 2048 ? MOST_CLUSTER : 1;
+  CUDA_TRY(launch_dependent_clusters(k_policy_sum, C, dim3(C), dim3(1024), 0, s, p, (int)mean, loss_out, n_valid_out, n_clipped_out));
   KERNEL_CHECK();
   return 0;
 }
