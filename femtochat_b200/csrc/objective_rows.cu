@@ -1,9 +1,23 @@
 // Passes over rows of logits for the objectives on a model's own answers: softmax statistics, what they give for the row's token (its
 // log-probability, the entropy, the policy term), and the gradient by the logits, from one reading of the row.
 //
-// Two kernels.  k_rows holds a row in registers, of a few warps or (few rows) of a cluster of blocks; it takes narrow rows and few rows.
-// k_rows_ring brings wide rows through a ring in shared memory; it takes many wide rows.  Both give a warp's exponentials relative to a
-// maximum of its own, add the warps' (m, l, a) in a fixed order, and are bound by HBM: every logit is read once and its gradient written once.
+// Three kernels that differ in where a row lies between its reading and the writing of its gradient: in the registers of a cluster (k_rows_few),
+// in a buffer of the group of warps that works on it (k_rows_near), in a ring that a block's groups share (k_rows_ring); launch() says
+// which takes what.  A thread's exponentials are relative to a maximum of its own, the (m, l, a) of threads and warps are added in a fixed order.
+//
+// The floor is HBM: every logit is read once and its gradient written once.  Beside it stand two exponentials an element (16 a cycle and
+// multiprocessor: half of the time that bf16 takes to come and go) and some 17 instructions; one block's chain of load, statistics, exchange,
+// slopes and stores is ten times as long as a row's share of the bandwidth, so rows have to overlap.  Measured (time, share of the measured
+// copy rate; bytes of the floor):
+//   log-probabilities    gradient          policy loss and gradient
+//     77 us  0.80         172 us  0.83      185 us  0.78    4096 x 65536 bf16, a quarter of the rows without target   ring
+//     83     0.98         186     0.88      188     0.87    2048 x 65536 fp32                                         ring
+//     54     0.74         112     0.72      118     0.68    1000 x 131000 bf16                                        ring, a third of it twice
+//     28     0.66          50     0.73       55     0.66    2000 x 30000 bf16                                         ring
+//     30     0.68          45     0.91       51     0.80    8192 x 4096 fp32                                          near
+//     21     0.50          34     0.60       40     0.52    8192 x 4096 bf16                                          near
+//      3.7   0.17           5.0   0.26        6.9   0.18    16 x 65536 fp32                                           few
+// The exponential pipe is busy 68 % with 65536 logits in bf16.  Arithmetic in f32x2 pairs or in single floats takes the same time.
 #include <algorithm>
 
 #include "objectives.cuh"
@@ -80,26 +94,29 @@ template <typename T> __device__ __forceinline__ int edge_of(const RowShape& r, 
   return i < r.head ? i : i >= 16 && i < 16 + r.tail ? r.head + r.nvec * VecN<T>::n + i - 16 : -1;
 }
 
-// Adds pairs of logits to a thread's sums, relative to an exponent.
+// u = c (z - m) of a pair of logits.
+struct Exponent {
+  uint64_t c2, m2;
+  __device__ __forceinline__ Exponent(float m, float c) : c2(pack2(c, c)), m2(pack2(-finite_or_zero(m), -finite_or_zero(m))) {}
+  __device__ __forceinline__ void of(uint64_t z2, float& u0, float& u1) const { unpack2(mul2(add2(z2, m2), c2), u0, u1); }
+};
+// Adds pairs of logits to a thread's sums.
 template <bool ENTROPY> struct Adder {
-  uint64_t c2, r2, l2 = 0, a2 = 0;
-  __device__ __forceinline__ void at(const Exponent& x) { c2 = pack2(x.c, x.c); r2 = pack2(-x.r, -x.r); l2 = a2 = 0; }
-  __device__ __forceinline__ void add(uint64_t z2) {
+  uint64_t l2 = 0, a2 = 0;
+  __device__ __forceinline__ void add(const Exponent& x, uint64_t z2) {
     float u0, u1;
-    const uint64_t u2 = fma2(z2, c2, r2);
-    unpack2(u2, u0, u1);
+    x.of(z2, u0, u1);
     const uint64_t e2 = pack2(exp2_fast(u0), exp2_fast(u1));
     l2 = add2(l2, e2);
     if (ENTROPY) a2 = fma2(e2, pack2(fmaxf(u0, LEAST_U), fmaxf(u1, LEAST_U)), a2);
   }
-  // The sums so far join the statistics, which are rebased to m first; x is the exponent of m.
-  __device__ __forceinline__ void join(RowStats& s, const Exponent& x) {
-    float l0, l1, a0, a1;
-    unpack2(l2, l0, l1);
-    unpack2(a2, a0, a1);
-    const float f = exp2_fast(x.d), l = l0 + l1;
-    s.l = fmaf(f, l, s.l);
-    if (ENTROPY) s.a = fmaf(f, fmaf(l, x.d, a0 + a1), s.a);
+  // The sums so far join the statistics, whose maximum they are relative to.
+  __device__ __forceinline__ void join(RowStats& s) {
+    float v0, v1;
+    unpack2(l2, v0, v1);
+    s.l += v0 + v1;
+    if (ENTROPY) { unpack2(a2, v0, v1); s.a += v0 + v1; }
+    l2 = a2 = 0;
   }
 };
 
@@ -108,30 +125,27 @@ template <typename T, bool ENTROPY> struct Running {
   RowStats s;
   Exponent x;
   Adder<ENTROPY> sum;
-  __device__ __forceinline__ Running(bool there, float edge, float c) {
-    s.m = there ? edge : -INFINITY;
-    x = exponent_of(s.m, c);
-    sum.at(x);
-    if (there) sum.add(pack2(edge, -INFINITY));
+  __device__ __forceinline__ Running(bool there, float edge, float c) : x(edge, c) {
+    s.m = edge;
+    if (there) sum.add(x, pack2(edge, -INFINITY));
   }
   template <int K> __device__ __forceinline__ void add(const uint4 (&q)[K], float c) {
     float m = Word<T>::most(q[0]);
 #pragma unroll
     for (int h = 1; h < K; h++) m = fmaxf(m, Word<T>::most(q[h]));
     if (m > s.m) {
-      sum.join(s, x);
+      sum.join(s);
       rebase<ENTROPY>(s, m, c);
-      x = exponent_of(m, c);
-      sum.at(x);
+      x = Exponent(m, c);
     }
 #pragma unroll
     for (int h = 0; h < K; h++)
 #pragma unroll
-      for (int i = 0; i < VecN<T>::n / 2; i++) sum.add(Word<T>::get(q[h], i));
+      for (int i = 0; i < VecN<T>::n / 2; i++) sum.add(x, Word<T>::get(q[h], i));
   }
   // The warp's statistics, in every lane.
   __device__ __forceinline__ RowStats of_warp(float c) {
-    sum.join(s, x);
+    sum.join(s);
     rebase<ENTROPY>(s, warp_max(s.m), c);
     s.l = warp_sum(s.l);
     if (ENTROPY) s.a = warp_sum(s.a);
@@ -172,9 +186,9 @@ template <typename T, RowsMode MODE, bool ENTROPY> __device__ __forceinline__ Ro
   }
   return r;
 }
-// The row's numbers go out (where `write`), and (g, h) of its gradient come back.
+// The row's numbers go out (where `write`), and (g, h) of its gradient come back.  scale: 0 until the rows with a target have been counted.
 template <RowsMode MODE, bool ENTROPY>
-__device__ __forceinline__ float2 row_result(const RowsArgs& p, long long row, const RowStats& s, const RowNumbers& k, bool write) {
+__device__ __forceinline__ float2 row_result(const RowsArgs& p, long long row, const RowStats& s, const RowNumbers& k, float& scale, bool write) {
   if (MODE == LOGPROBS) {
     if (write) {
       p.logp[row] = log_prob(s, k.z, p.inv_t);
@@ -187,11 +201,11 @@ __device__ __forceinline__ float2 row_result(const RowsArgs& p, long long row, c
   float loss, slope;
   policy_token(p.term, lp, k.x[0], k.x[1], k.x[2], k.x[3], &loss, &slope);
   if (write) { p.token_losses[row] = loss; p.logp[row] = lp; }
-  if (p.n_valid) {      // a kernel of the same call counts the targets beside the first rows
+  if (p.n_valid && scale == 0.f) {      // a kernel of the same call counts the targets beside the first rows
     pdl_wait();
-    slope *= 1.f / (float)*reinterpret_cast<const volatile int*>(p.n_valid);
+    scale = 1.f / (float)*reinterpret_cast<const volatile int*>(p.n_valid);
   }
-  return make_float2(slope * p.inv_t, 0.f);
+  return make_float2((p.n_valid ? slope * scale : slope) * p.inv_t, 0.f);
 }
 template <RowsMode MODE, bool ENTROPY> __device__ __forceinline__ void row_without_target(const RowsArgs& p, long long row) {
   if (MODE == LOGPROBS) { p.logp[row] = 0.f; if (ENTROPY) p.ent[row] = 0.f; }
@@ -201,20 +215,20 @@ template <RowsMode MODE, bool ENTROPY> __device__ __forceinline__ void row_witho
 // dz_j = g (1[j = t] - p_j) - h p_j (u_j - a / l), where log p + H = ln2 (u - a / l).  A row without a distribution has no gradient.
 template <typename T, bool ENTROPY> struct Slope {
   static constexpr int n = VecN<T>::n;
-  uint64_t c2, r2, k2, h2;
+  Exponent x;
+  uint64_t k2, h2;
   float at_target;
   int t;
-  __device__ __forceinline__ Slope(const RowStats& s, float2 gh, float c, int target) : t(target) {
-    const Exponent x = exponent_of(s.m, c);
+  __device__ __forceinline__ Slope(const RowStats& s, float2 gh, float c, int target) : x(s.m, c), t(target) {
     const bool none = s.l == 0.f;
-    const float inv_l = exp2_fast(x.d) / s.l;
-    const float k = none ? 0.f : -(ENTROPY ? gh.x + gh.y * (x.d - s.a / s.l) : gh.x) * inv_l, h = none ? 0.f : -gh.y * inv_l;
-    c2 = pack2(x.c, x.c); r2 = pack2(-x.r, -x.r); k2 = pack2(k, k); h2 = pack2(h, h);
+    const float inv_l = 1.f / s.l;
+    const float k = none ? 0.f : -(ENTROPY ? gh.x - gh.y * (s.a / s.l) : gh.x) * inv_l, h = none ? 0.f : -gh.y * inv_l;
+    k2 = pack2(k, k); h2 = pack2(h, h);
     at_target = none ? 0.f : gh.x;
   }
   __device__ __forceinline__ uint64_t of(uint64_t z2) const {
     float u0, u1;
-    unpack2(fma2(z2, c2, r2), u0, u1);
+    x.of(z2, u0, u1);
     const uint64_t e2 = pack2(exp2_fast(u0), exp2_fast(u1));
     return mul2(e2, ENTROPY ? fma2(h2, pack2(fmaxf(u0, LEAST_U), fmaxf(u1, LEAST_U)), k2) : k2);
   }
@@ -257,7 +271,8 @@ __device__ __forceinline__ void group_barrier(int id, int threads) { asm volatil
 
 // ---- few rows -----------------------------------------------------------------------------------------------------------------------------------
 // A cluster of blocks holds a row in registers, NV words a thread; the statistics of all its warps go to every block's shared memory.  There is
-// little to overlap: what counts is that a row is brought by many multiprocessors at once.
+// little to overlap: what counts is that a row is brought by many multiprocessors at once (1 x 65536 in fp32: 3.0 us, of which a launch with
+// nothing to do is 2).
 constexpr int FEW_WARPS = 8, FEW_WORDS = 8;
 
 template <typename T, RowsMode MODE, bool STORE, bool ENTROPY, int NV>
@@ -307,7 +322,8 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) k_rows_few(const RowsArgs p) {
   if (!STORE && (rank != 0 || warp != 0)) return;
   s = merged_parts<ENTROPY>(part, pitch, FEW_WARPS * C, p.c);
   if (warp == 0) {
-    const float2 gh = row_result<MODE, ENTROPY>(p, row, s, numbers, rank == 0 && lane == 0);
+    float scale = 0.f;
+    const float2 gh = row_result<MODE, ENTROPY>(p, row, s, numbers, scale, rank == 0 && lane == 0);
     if (lane == 0) slope_s = gh;
   }
   if (!STORE) return;
@@ -323,7 +339,9 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) k_rows_few(const RowsArgs p) {
 }
 
 // ---- narrow rows --------------------------------------------------------------------------------------------------------------------------------
-// Groups of W warps walk the rows in turn.  A group has two buffers in shared memory: while it works on a row, a bulk copy brings its next one.
+// Groups of W warps walk the rows in turn.  A group has two buffers in shared memory: while it works on a row, a bulk copy brings its next one,
+// and three blocks a multiprocessor keep up to 24 rows going.  Rows in registers, one group of warps each, took 56 us where this takes 45
+// (8192 x 4096 in fp32, gradient): a row's loads could not start before the row ahead was written.
 constexpr int NEAR_WARPS = 8, NEAR_WORDS = 4;
 
 template <typename T, RowsMode MODE, bool STORE, bool ENTROPY>
@@ -356,6 +374,7 @@ __global__ void __launch_bounds__(32 * NEAR_WARPS, 3) k_rows_near(const RowsArgs
   long long row = (long long)blockIdx.x * groups + group;
   int t_next = row < p.N ? p.tgt0[row] : -1, k = 0;      // k: rows with a target so far
   bool alive = true, asked = false;
+  float scale = 0.f;
   for (; row < p.N; row += step) {
     const int t = checked_target(p, t_next, tid == 0);
     t_next = row + step < p.N ? p.tgt0[row + step] : -1;
@@ -401,7 +420,7 @@ __global__ void __launch_bounds__(32 * NEAR_WARPS, 3) k_rows_near(const RowsArgs
     asked = t_next >= 0 && t_next < p.V;
     if (asked && tid == 0 && alive) ask(row + step, which ^ 1);
     float2 gh = make_float2(0.f, 0.f);
-    if (warp == first_warp) gh = row_result<MODE, ENTROPY>(p, row, s, numbers, lane == 0);
+    if (warp == first_warp) gh = row_result<MODE, ENTROPY>(p, row, s, numbers, scale, lane == 0);
     if (!STORE) continue;
     if (W > 1) {
       if (warp == first_warp && lane == 0) slope_s[group] = gh;
@@ -499,6 +518,7 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
     parity ^= 1u << slot;
   };
   int k = 0, turn = 0, nth = 0;
+  float scale = 0.f;
   int t_next = blockIdx.x < p.N ? p.tgt0[blockIdx.x] : -1;
   for (long long row = blockIdx.x; row < p.N; row += gridDim.x, nth++) {
     const int t = checked_target(p, t_next, threadIdx.x == 0);
@@ -548,7 +568,7 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
     group_barrier(1 + group, GROUP_THREADS);
     if (STORE || gwarp == 0) s = merged_parts<ENTROPY>(parts, GROUP_WARPS, GROUP_WARPS, p.c);
     if (gwarp == 0) {
-      const float2 gh = row_result<MODE, ENTROPY>(p, row, s, numbers, lane == 0);
+      const float2 gh = row_result<MODE, ENTROPY>(p, row, s, numbers, scale, lane == 0);
       if (STORE && lane == 0) slope_s[group] = gh;
     }
     if (!STORE) continue;
@@ -572,7 +592,11 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
 }
 
 // ---- launch -----------------------------------------------------------------------------------------------------------------------------------
-constexpr int MOST_NEAR = 1280;
+// Where the kernels meet (gradient, us; the chosen one first).  few / others: 220 rows, where a block each leaves multiprocessors idle in the
+// second turn, 65536 fp32 27.0 / 30.7, 8000 fp32 5.7 / 7.6; 296 rows, 65536 bf16 27.3 / 22.6, so not there.  near / Medium: 1024 words (8192 x 4096
+// fp32) 45 / 65; 1500 words (4000 x 12000 bf16) 45 with Medium, 60 in registers.  Medium / WideWriting: 3750 words (2000 x 30000 bf16) 50 / 57;
+// 12505 words (999 x 50021 fp32) 75 / 64.  Numbers only, 4096 x 65536 bf16: WideReading 78, WideWriting's shape 84.
+constexpr int MOST_NEAR = 1280, MOST_MEDIUM = 4096;      // words of a row
 typedef Ring<4, 6, 4, 18> Medium;
 typedef Ring<3, 8, 4, 13> WideReading;
 typedef Ring<2, 12, 4, 9> WideWriting;
@@ -612,7 +636,7 @@ template <typename T, RowsMode MODE, bool STORE, bool ENTROPY> int launch(const 
     return launch_kernel(p, k_rows_few<T, MODE, STORE, ENTROPY, FEW_WORDS>, C, grid, block, 0, s, p);
   }
   if (words <= MOST_NEAR) {
-    int W = 1;
+    int W = 1;      // eight words a thread: with four, 8192 x 4096 in bf16 took 39 us for 34, more of it between the rows
     while (W < NEAR_WARPS && words > W * 256) W *= 2;
     const int groups = NEAR_WARPS / W;
     const size_t smem = (size_t)groups * 2 * words * 16;
@@ -621,7 +645,7 @@ template <typename T, RowsMode MODE, bool STORE, bool ENTROPY> int launch(const 
     const int blocks = std::max(1, std::min(3, (int)((220 << 10) / (smem + 2048))));
     return launch_kernel(p, kernel, 1, dim3((unsigned)std::min(cdiv(p.N, groups), sms * blocks)), 32 * NEAR_WARPS, smem, s, p, W, words);
   }
-  if (words <= 4096) return launch_ring<T, MODE, STORE, ENTROPY, Medium>(p, words, s);
+  if (words <= MOST_MEDIUM) return launch_ring<T, MODE, STORE, ENTROPY, Medium>(p, words, s);
   if constexpr (STORE) return launch_ring<T, MODE, STORE, ENTROPY, WideWriting>(p, words, s);
   else return launch_ring<T, MODE, STORE, ENTROPY, WideReading>(p, words, s);
 }

@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(1024) k_preference_pairs(const Preference p) {
 }
 
 // Sum or mean over the pairs, and zeros as the gradient of rows that belong to no answer.
-__global__ void __launch_bounds__(1024) k_preference_sum(const Preference p, float* __restrict__ loss_out) {
+__global__ void __launch_bounds__(1024) k_preference_sum(const Preference p, float* loss_out) {
   pdl_trigger();
   pdl_wait();
   if (blockIdx.x == 0) {
@@ -276,7 +276,7 @@ int objective_slopes(const TokenObjective& o, const float* nll, int row0, int n,
 }
 
 int check_temperature(float t) {
-  return t > 0.f && isfinite(t) ? 0 : femto_fail(FEMTO_ERR_ARG, "temperature must be positive and finite");
+  return t >= 1e-6f && t <= 1e6f ? 0 : femto_fail(FEMTO_ERR_ARG, "temperature must lie in 1e-6 .. 1e6");
 }
 PolicyTerm policy_term(const femto_policy_config& c) { return {1.f - c.clip_low, 1.f + c.clip_high, c.kl_coef}; }
 

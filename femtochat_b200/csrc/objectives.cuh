@@ -5,6 +5,8 @@
 
 // Softmax statistics of a row.  With c = log2(e) / temperature, m = max(z) and u_j = c (z_j - m) <= 0:
 //   l = sum 2^u_j,  a = sum 2^u_j u_j,  log p_j = ln2 u_j - ln l,  H = ln l - ln2 a / l.
+// The difference comes before the product.  (As one fused product, c z_j - c m, the rounding of c m would stand in every exponent: logits of the
+// type's lowest value, or of some millions, came out as 0 / 0.  It is no faster.)
 struct RowStats {
   float m = -INFINITY, l = 0.f, a = 0.f;
 };
@@ -24,22 +26,6 @@ __device__ __forceinline__ float exp2_fast(float x) {   // relative error 2^-22,
 }
 // What a maximum of -inf (nothing seen, or a row without any logit above -inf) is taken as: -inf - 0 gives 2^-inf = 0, where -inf + inf is NaN.
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
-
-// u_j as one fused product: u_j = fma(z_j, c, -r) + d with r = c m rounded and d = r - c m, the same for the whole row, so it is put into
-// what the exponentials are multiplied by.  Where c m leaves the range (rows of the type's lowest value), logits that are not m lie so far
-// below it that any scale gives 0 for them, and a power of two, which rounds nothing, gives 0 exactly for those that are.
-struct Exponent {
-  float c, r, d;
-};
-__device__ __forceinline__ Exponent exponent_of(float m, float c) {
-  Exponent x;
-  m = finite_or_zero(m);
-  const bool far = fabsf(m) > 1e30f && fabsf(m) < INFINITY;
-  x.c = far ? 0x1p-10f : c;
-  x.r = m * x.c;
-  x.d = -fmaf(m, x.c, -x.r);
-  return x;
-}
 
 // Moves statistics to a maximum that is no lower: with d = c (m_old - m_new) every 2^u scales by 2^d and every u moves by d.
 template <bool ENTROPY> __device__ __forceinline__ void rebase(RowStats& s, float m, float c) {

@@ -174,11 +174,10 @@ def policy_loss(logits, targets0, old_logp, advantages, ref_logp=None, weights=N
     ref_logp, weights = _on_device("ref_logp", ref_logp, f32, shape, device), _on_device("weights", weights, f32, shape, device)
     cfg = _policy_config(clip_low, clip_high, kl_coef, temperature, reduction)
     d, d_pitch = _gradient_of(logits, n, V, pitch, out) if gradient else (None, V)
-    if old_logp is None or advantages is None:
-        raise ValueError("old_logp or advantages is None")
+    if targets0 is None or old_logp is None or advantages is None:
+        raise ValueError("targets0, old_logp or advantages is None")
     token_losses, logp = torch.empty_like(old_logp), torch.empty_like(old_logp)
-    loss = torch.empty(1, dtype=f32, device=device)
-    n_valid, n_clipped = torch.empty(1, dtype=torch.int32, device=device), torch.empty(1, dtype=torch.int32, device=device)
+    loss, n_valid, n_clipped = old_logp.new_empty(1), targets0.new_empty(1), targets0.new_empty(1)
     _call(device, "femto_policy_loss", code, logits.data_ptr(), pitch, _address(targets0), n, V, _address(old_logp), _address(advantages),
           _address(ref_logp), _address(weights), C.byref(cfg), _address(d), d_pitch, token_losses.data_ptr(), logp.data_ptr(), loss.data_ptr(),
           n_valid.data_ptr(), n_clipped.data_ptr())
@@ -216,8 +215,7 @@ def preference_loss(logp, offsets, targets0=None, ref_logp=None, kind: str = "si
     if n >= 1 << 31:
         raise ValueError(f"{n} tokens")
     cfg = _preference_config(kind, beta, margin, label_smoothing, length_normalised, reduction)
-    loss = torch.empty(1, dtype=f32, device=device)
-    pair_losses, ratios = torch.empty(P, dtype=f32, device=device), torch.empty(2 * P, dtype=f32, device=device)
+    loss, pair_losses, ratios = logp.new_empty(1), logp.new_empty(P), logp.new_empty(2 * P)
     dlogp = torch.empty_like(logp) if gradient else None
     _call(device, "femto_preference_loss", logp.data_ptr(), _address(ref_logp), _address(targets0), n, offsets.data_ptr(), P, C.byref(cfg),
           loss.data_ptr(), pair_losses.data_ptr(), ratios.data_ptr(), _address(dlogp))

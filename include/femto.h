@@ -135,7 +135,7 @@ int32_t femto_loss_and_gradient_host(femto_handle* h, const float* theta, float*
  * femto_policy_loss and femto_preference_loss below, of the log-probabilities that the model gives the targets; the step is that of
  * femto_loss_and_gradient (weights, positions, accumulation, data parallelism) with them in the cross-entropy's place. */
 typedef struct femto_policy_config {
-  float temperature; /* > 0: at which the answers were sampled */
+  float temperature; /* at which the answers were sampled, 1e-6 .. 1e6 */
   float clip_low, clip_high; /* the ratio r counts up to the range 1 - clip_low .. 1 + clip_high (infinity: no bound above) */
   float kl_coef;     /* beta >= 0 */
   int32_t reduction; /* FEMTO_REDUCTION_SUM, or _MEAN over the rows with a target */
@@ -163,7 +163,7 @@ int32_t femto_policy_loss_and_gradient(femto_handle* h, const float* theta, floa
                                        int32_t* n_valid_out, int32_t* n_clipped_out, float* logp_out, void* stream);
 /* Answers are runs of the B * T rows taken in order: answer k is the rows offsets[k] .. offsets[k + 1] - 1 (int32 [2 P + 1], device), without
  * those whose target is ignored.  ref_logp fp32 [B][T] or NULL; logp_out may be NULL.  With more rows than a chunk of the lm_head tail
- * (16 384) the chunks' logits are computed twice. */
+ * (16 384) the chunks' logits are computed twice.  Bad offsets are reported as those of femto_preference_loss are. */
 int32_t femto_preference_loss_and_gradient(femto_handle* h, const float* theta, float* delta, const int32_t* tokens,
                                            const int32_t* targets, const int32_t* positions, int32_t B, const float* ref_logp,
                                            const int32_t* offsets, int32_t P, const femto_preference_config* h_cfg,
@@ -487,7 +487,8 @@ int32_t femto_muon_direction(int32_t dtype, float* X_out, const float* G, float*
  * aligned to their type only.  targets0: 0-based, or negative where a row counts for nothing: neither its logits nor its entries in other
  * arrays are then read, and its results are 0.  A target of V or more counts as none and raises bit 1 of the word that
  * femto_status_word(NULL, ..) reads.  Logits of -inf are tokens that cannot be chosen; a row with nothing else has no distribution: its
- * log-probability is -inf, its entropy and its gradient are 0.  NaN or +inf in a counted row give NaN there.  N = 0 is allowed. */
+ * log-probability is -inf, its entropy and its gradient are 0.  NaN or +inf in a counted row give NaN there.  N = 0 is allowed.
+ * temperature: 1e-6 .. 1e6.  Outputs lie apart from inputs and from one another, but for dlogits where it says so. */
 /* Log-probabilities log p(target) of softmax(logits / temperature): logp [N]; entropy [N] (may be NULL). */
 int32_t femto_token_logprobs(int32_t dtype, const void* logits, int64_t ldl, const int32_t* targets0, int32_t N, int32_t V,
                              float temperature, float* logp, float* entropy, void* stream);

@@ -187,6 +187,41 @@ def test_a_policy_step_trains_a_model():
     assert st.status_word() == 0
 
 
+def test_the_step_and_the_call_on_the_model_s_logits_agree():
+    """The model's logits through `policy_loss` and `preference_loss`, against the steps that never hold them all."""
+    cfg, lay, th, batch, params, st, M = setup(MID, 2, "float32", seed=8, short_window=32)
+    tok, tgt, pos = batch
+    z = fb.GPT(params, cfg, lay, short_window=32).logits(tok, pos)
+    t0 = (torch.where(tgt > 0, tgt - 1, tgt)).int().cuda()
+    old, A, ref, w = (x.cuda() for x in numbers(fb.token_logprobs(z, t0).logp.cpu(), 9))
+    args = dict(ref_logp=ref, weights=w, clip_low=0.2, clip_high=0.28, kl_coef=0.125, reduction="mean")
+    a = fb.policy_loss(z, t0, old, A, **args)
+    b = fb.policy_loss_and_gradient_(params, st, lay, tok, tgt, old, A, positions=pos, **args)
+    assert torch.equal(a.n_valid, b.n_valid) and torch.equal(a.n_clipped, b.n_clipped)
+    assert float((a.logp - b.logp).abs().max()) < 2e-5 and float(a.loss) == pytest.approx(float(b.loss), rel=1e-4, abs=1e-6)
+    offsets = torch.tensor([0, 60, 150], dtype=torch.int32, device="cuda")
+    p = fb.preference_loss(a.logp, offsets, targets0=t0, ref_logp=ref, beta=0.5)
+    q = fb.preference_loss_and_gradient_(params, st, lay, tok, tgt, offsets, positions=pos, ref_logp=ref, beta=0.5)
+    assert float(p.loss) == pytest.approx(float(q.loss), rel=1e-3)
+    # one token of a request: its logits from the cache, its log-probability as the whole text has it
+    cache = fb.KVCache(st, 2, MID["sequence_len"])
+    one = fb.prefill(fb.GPT(params, cfg, lay, short_window=32), cache, tok[:, :10], pos[:, :10])
+    assert float((fb.token_logprobs(one, t0[:, 9].contiguous()).logp - b.logp[:, 9]).abs().max()) < 1e-3
+
+
+def test_steps_refuse_a_decoder():
+    layers = [fb.LayerConfig(mixer="lightning", heads=2, dim=16, vdim=16, decay=(0.9, 0.8), ff=64)]
+    cfg = fb.DecoderConfig(vocab_size=50, width=32, norm_eps=1e-5, layers=layers)
+    st = fb.DecoderState(cfg, max_batch=1, max_rows=8)
+    x = torch.zeros(1024, device="cuda")
+    i = torch.zeros(8, dtype=torch.int32, device="cuda")
+    L, p = _lib.lib(), _lib.ptr
+    c, q = C.byref(_lib.PolicyConfigC(1.0, 0.2, 0.2, 0.0, 0)), C.byref(_lib.PreferenceConfigC(0, 0.1, 0.0, 0.0, 0, 1))
+    assert L.femto_policy_loss_and_gradient(st.h, p(x), p(x), p(i), p(i), None, 1, p(x), p(x), None, None, c, 0, p(x), p(i), None, None, None) == -5
+    assert L.femto_preference_loss_and_gradient(st.h, p(x), p(x), p(i), p(i), None, 1, None, p(i), 1, q, 0, p(x), p(x), p(x), None, None) == -5
+    assert L.femto_forward_token_logprobs(st.h, p(x), p(i), p(i), None, 1, 1.0, p(x), None) == -5
+
+
 def test_steps_refuse():
     cfg, lay, th, batch, params, st, M = setup(MID, 2, "float32")
     z = torch.zeros(2, MID["sequence_len"], device="cuda")

@@ -325,6 +325,42 @@ def test_streams_and_graphs():
         assert torch.equal(d, fb.token_logprobs_gradient(y, u, old, dentropy=A))
 
 
+def test_first_call_of_a_process_inside_a_capture():
+    """Nothing is allocated or looked up on a call's way that a capture would refuse, not even the first time."""
+    import subprocess
+    import sys
+    code = """
+import torch, femtochat_b200 as fb
+z = torch.randn(300, 70000, device="cuda"); t = torch.zeros(300, device="cuda", dtype=torch.int32); f = torch.randn(300, device="cuda")
+o = torch.tensor([0, 100, 300], device="cuda", dtype=torch.int32)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    p = fb.policy_loss(z, t, f, f, reduction="mean")
+    a = fb.token_logprobs(z[:, :3000], t, entropy=True)
+    d = fb.token_logprobs_gradient(z[:9], t[:9], f[:9])
+    q = fb.preference_loss(a.logp, o)
+g.replay(); torch.cuda.synchronize()
+r = fb.policy_loss(z, t, f, f, reduction="mean")
+assert all(torch.equal(x, y) for x, y in zip(p, r)) and torch.equal(q.loss, fb.preference_loss(a.logp, o).loss)
+assert torch.equal(d, fb.token_logprobs_gradient(z[:9], t[:9], f[:9]))
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=__file__.rsplit("/tests/", 1)[0], timeout=300)
+
+
+def test_temperatures_at_the_ends_of_their_range():
+    z, t = make(5, 700, torch.float32, seed=11)
+    for temperature in (1e-6, 1e6):
+        r = fb.token_logprobs(z, t, temperature=temperature, entropy=True)
+        T = float(torch.tensor(temperature, dtype=torch.float32))
+        lp, h, _ = reference(z, t, T)
+        near(r.logp, lp, slack(700) + 2.0 ** -22 * (lp.abs() + h + 1), "logp")
+        assert bool(fb.token_logprobs_gradient(z, t, torch.ones(5, device="cuda"), temperature=temperature).isfinite().all())
+    low = torch.full((1, 700), torch.finfo(torch.float32).min, device="cuda")
+    near(fb.token_logprobs(low, t[:1], temperature=1e-6).logp, torch.tensor([-math.log(700)], device="cuda", dtype=torch.float64), slack(700) + 1e-6, "lowest")
+    high = torch.full((1, 700), 1e30, device="cuda")
+    near(fb.token_logprobs(high, t[:1], temperature=1e-6).logp, torch.tensor([-math.log(700)], device="cuda", dtype=torch.float64), slack(700) + 1e-6, "highest")
+
+
 def test_gradient_against_differences():
     """The gradient of the reduced loss against central differences of the definition in 64 bits."""
     N, V, kl = 4, 11, 0.125
@@ -449,6 +485,7 @@ def test_preference_from_logits_to_logits(dtype):
     gap = torch.where(t >= 0, ls - ref.double(), 0.0).view(B, T).sum(1)
     loss = -torch.nn.functional.logsigmoid(0.375 * (gap[0::2] - gap[1::2])).mean()
     want, = torch.autograd.grad(loss, x)
+    loss = loss.detach()
     p, onehot = torch.softmax(x.detach() / 0.875, 1), torch.nn.functional.one_hot(t.clamp(min=0).long(), V)
     size = 0.125 / 0.875 * (p + onehot)      # |d loss / d lp| <= beta / pairs
     dlp = T * 2 * (slack(V) + 2.0 ** -23 * 30)

@@ -56,7 +56,7 @@ def test_rows_that_are_refused(call, change, code):
 
 
 def test_log_probabilities_refuse():
-    for t in (0.0, -1.0, math.inf, math.nan):
+    for t in (0.0, -1.0, 1e-7, 1e7, math.inf, math.nan):
         assert logprobs(temperature=t) == ARG and gradient(temperature=t) == ARG
     assert logprobs(logp=None) == ARG
     assert gradient(dlogits=None) == ARG and gradient(dlogp=None) == ARG
