@@ -18,6 +18,8 @@
 //     21     0.50          34     0.60       40     0.52    8192 x 4096 bf16                                          near
 //      3.7   0.17           5.0   0.26        6.9   0.18    16 x 65536 fp32                                           few
 // The exponential pipe is busy 68 % with 65536 logits in bf16.  Arithmetic in f32x2 pairs or in single floats takes the same time.
+#include <limits.h>
+
 #include <algorithm>
 
 #include "objectives.cuh"
@@ -35,6 +37,24 @@ __device__ __forceinline__ int checked_target(const RowsArgs& p, int t, bool fla
   if (t >= p.V) { if (flag) atomicOr(&g_rows_status, ST_BAD_TOKEN); return -1; }
   return t < 0 ? -1 : t;
 }
+
+// The targets of the rows that a block (or group) walks, every `step`-th from its first: a warp holds 32 of them, so that one load serves 32
+// rows.  (One row ahead at a time, a run of 14 rows without target cost a block 7 us.)  Called by whole warps.
+struct Targets {
+  const int* tgt0;
+  long long first, step;
+  int N, held;
+  __device__ __forceinline__ Targets(const RowsArgs& p, long long first, long long step) : tgt0(p.tgt0), first(first), step(step), N(p.N) { load(0); }
+  __device__ __forceinline__ void load(int k) {
+    const long long row = first + (long long)(k + (threadIdx.x & 31)) * step;
+    held = row < N ? tgt0[row] : -1;
+  }
+  // of the k-th row; asked for in order
+  __device__ __forceinline__ int operator()(int k) {
+    if (k > 0 && (k & 31) == 0) load(k);
+    return __shfl_sync(0xffffffffu, held, k & 31);
+  }
+};
 
 __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) { uint64_t v; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b)); return v; }
 
@@ -372,12 +392,13 @@ __global__ void __launch_bounds__(32 * NEAR_WARPS, 3) k_rows_near(const RowsArgs
   };
   const long long step = (long long)gridDim.x * groups;
   long long row = (long long)blockIdx.x * groups + group;
-  int t_next = row < p.N ? p.tgt0[row] : -1, k = 0;      // k: rows with a target so far
+  Targets targets(p, row, step);
+  int t_next = targets(0), k = 0;      // k: rows with a target so far
   bool alive = true, asked = false;
   float scale = 0.f;
-  for (; row < p.N; row += step) {
+  for (int nth = 1; row < p.N; row += step, nth++) {
     const int t = checked_target(p, t_next, tid == 0);
-    t_next = row + step < p.N ? p.tgt0[row + step] : -1;
+    t_next = targets(nth);
     const T* z = reinterpret_cast<const T*>(p.logits) + row * p.ldl;
     T* d = reinterpret_cast<T*>(p.dlogits) + row * p.ldd;
     const RowShape r = row_shape<T>(STORE && t < 0 ? d : z, p.V);      // the logits', or, where they are not read, the gradient's
@@ -442,13 +463,19 @@ __global__ void __launch_bounds__(32 * NEAR_WARPS, 3) k_rows_near(const RowsArgs
 // One block a multiprocessor: a warp brings the words of its rows in chunks (bulk copies, an mbarrier each), and groups of warps take the rows
 // in turn, so that one's pass over a row goes on while another works out its slopes or writes its gradient.  Chunks stay where they are until
 // their gradient is written.  Of a row that the ring does not hold the first chunks are given back at once and brought `again`, behind the
-// row's last: two passes over the ring's length later they are still in L2.
+// row's last: two passes over the ring's length later they are still in L2.  The warp that brings rows also writes the zeros of those without
+// target, by bulk copies, one such row behind each that it brings: all at once in their turn they took the reads' place (4096 x 65536 in bf16, the
+// first half of the rows without target, gradient: 157 -> 145 us).
 template <int GROUPS_, int WARPS_, int PER_, int SLOTS_> struct Ring {
   static constexpr int GROUPS = GROUPS_, WARPS = WARPS_, THREADS = 32 * WARPS_, PER = PER_, CHUNK = PER_ * THREADS, SLOTS = SLOTS_;
   static constexpr int SPARE = 2;      // slots that a row wider than the ring leaves to what follows
   static constexpr int BLOCK = GROUPS * THREADS + 32;
-  static constexpr size_t BYTES = (size_t)SLOTS * CHUNK * 16;
+  static constexpr int ZEROS = 512;      // words of zeros behind the ring, the source of the gradient of rows without target
+  static constexpr size_t BYTES = ((size_t)SLOTS * CHUNK + ZEROS) * 16;
 };
+__device__ __forceinline__ void bulk_store_1d(void* gdst, const void* smem_src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(gdst), "r"(smem_u32(smem_src)), "r"(bytes) : "memory");
+}
 template <typename T, RowsMode MODE, bool STORE, bool ENTROPY, class R>
 __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const int chunks, const int again) {
   constexpr int GROUPS = R::GROUPS, GROUP_WARPS = R::WARPS, GROUP_THREADS = R::THREADS, PER_CHUNK = R::PER, CHUNK = R::CHUNK, SLOTS = R::SLOTS;
@@ -468,13 +495,17 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
     abort_flag = 0;
     fence_barrier_init();
   }
+  uint4* zeros = ring + (size_t)SLOTS * CHUNK;
+  if (STORE) {
+    for (int i = threadIdx.x; i < R::ZEROS; i += R::BLOCK) zeros[i] = make_uint4(0, 0, 0, 0);
+    fence_proxy_async();
+  }
   __syncthreads();
   if (warp == GROUPS * GROUP_WARPS) {      // the warp that brings the rows
-    if (lane != 0) return;
-    int slot = 0, k = 0;
+    int slot = 0, k = 0, nth = 0;
     uint32_t round = 0, used[GROUPS] = {}, parity[GROUPS] = {};      // bits: slots that a group's barriers have been used for, and how often, modulo 2
     bool alive = true;
-    auto bring = [&](const uint4* words, int nvec, int n_chunks, int group) {
+    auto bring = [&](const uint4* words, int nvec, int n_chunks, int group) {      // by one lane
       for (int c = 0; c < n_chunks; c++) {
         if (round > 0) alive = mbar_wait(&empty[slot], (round - 1) & 1u, &abort_flag, &g_rows_status);
         if (!alive) return;
@@ -489,19 +520,47 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
         if (slot == 0) round++;
       }
     };
-    int t_next = blockIdx.x < p.N ? p.tgt0[blockIdx.x] : -1;
-    for (long long row = blockIdx.x; row < p.N && alive; row += gridDim.x) {
-      const int t = t_next;
-      if (row + gridDim.x < p.N) t_next = p.tgt0[row + gridDim.x];
+    // the next row without target among the block's first `end`, behind those that have been dealt with
+    Targets masked(p, blockIdx.x, gridDim.x);
+    int masked_nth = 0;
+    auto clear_next = [&](int end) -> bool {
+      for (long long row; masked_nth < end && (row = blockIdx.x + (long long)masked_nth * gridDim.x) < p.N;) {
+        const int t = masked(masked_nth++);
+        if (t >= 0 && t < p.V) continue;
+        if (lane == 0) row_without_target<MODE, ENTROPY>(p, row);
+        if (STORE) {
+          T* d = reinterpret_cast<T*>(p.dlogits) + row * p.ldd;
+          const RowShape r = row_shape<T>(d, p.V);
+          if (lane == 0) {
+            uint4* words = reinterpret_cast<uint4*>(d + r.head);
+            for (int v = 0; v < r.nvec; v += R::ZEROS) bulk_store_1d(words + v, zeros, (uint32_t)min(R::ZEROS, r.nvec - v) * 16u);
+            bulk_commit();
+          }
+          const int at = edge_of<T>(r, lane);
+          if (at >= 0) d[at] = from_f<T>(0.f);
+        }
+        return true;
+      }
+      return false;
+    };
+    Targets targets(p, blockIdx.x, gridDim.x);
+    for (long long row = blockIdx.x; row < p.N; row += gridDim.x) {
+      const int t = targets(nth++);
       if (t < 0 || t >= p.V) continue;
       const T* z = reinterpret_cast<const T*>(p.logits) + row * p.ldl;
       const RowShape r = row_shape<T>(z, p.V);
       const uint4* words = reinterpret_cast<const uint4*>(z + r.head);
-      bring(words, r.nvec, chunks, k % GROUPS);
-      if (STORE && alive) bring(words, r.nvec, again, k % GROUPS);
+      if (lane == 0) {
+        if (alive) bring(words, r.nvec, chunks, k % GROUPS);
+        if (STORE && alive) bring(words, r.nvec, again, k % GROUPS);
+      }
+      __syncwarp();
+      clear_next(nth);
       k++;
     }
-    if (!alive)      // nothing may still be on its way to this block's memory when it ends
+    while (clear_next(INT_MAX)) {}
+    if (STORE && lane == 0) bulk_wait_all();
+    if (lane == 0 && !alive)      // nothing may still be on its way to this block's memory when it ends
       for (int i = 0; i < GROUPS * SLOTS; i++)
         if (used[i / SLOTS] >> (i % SLOTS) & 1u)
           for (uint32_t polls = 0; polls < WAIT_LIMIT && !mbar_try_wait(&full[i / SLOTS][i % SLOTS], (parity[i / SLOTS] >> (i % SLOTS) & 1u) ^ 1u); polls++) {}
@@ -519,25 +578,14 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
   };
   int k = 0, turn = 0, nth = 0;
   float scale = 0.f;
-  int t_next = blockIdx.x < p.N ? p.tgt0[blockIdx.x] : -1;
-  for (long long row = blockIdx.x; row < p.N; row += gridDim.x, nth++) {
-    const int t = checked_target(p, t_next, threadIdx.x == 0);
-    if (row + gridDim.x < p.N) t_next = p.tgt0[row + gridDim.x];
-    const T* z = reinterpret_cast<const T*>(p.logits) + row * p.ldl;
-    T* d = reinterpret_cast<T*>(p.dlogits) + row * p.ldd;
-    if (t < 0) {
-      if (nth % GROUPS != group) continue;
-      if (tid == 0) row_without_target<MODE, ENTROPY>(p, row);
-      if (STORE) {
-        const RowShape r = row_shape<T>(d, p.V);
-        for (int v = tid; v < r.nvec; v += GROUP_THREADS) reinterpret_cast<uint4*>(d + r.head)[v] = make_uint4(0, 0, 0, 0);
-        const int at = edge_of<T>(r, tid);
-        if (at >= 0) d[at] = from_f<T>(0.f);
-      }
-      continue;
-    }
+  Targets targets(p, blockIdx.x, gridDim.x);
+  for (long long row = blockIdx.x; row < p.N; row += gridDim.x) {
+    const int t = checked_target(p, targets(nth++), threadIdx.x == 0);
+    if (t < 0) continue;
     const int mine = k++;
     if (mine % GROUPS != group) continue;
+    const T* z = reinterpret_cast<const T*>(p.logits) + row * p.ldl;
+    T* d = reinterpret_cast<T*>(p.dlogits) + row * p.ldd;
     const RowShape r = row_shape<T>(z, p.V);
     const int at = edge_of<T>(r, tid);
     RowNumbers numbers;
@@ -593,13 +641,14 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
 
 // ---- launch -----------------------------------------------------------------------------------------------------------------------------------
 // Where the kernels meet (gradient, us; the chosen one first).  few / others: 220 rows, where a block each leaves multiprocessors idle in the
-// second turn, 65536 fp32 27.0 / 30.7, 8000 fp32 5.7 / 7.6; 296 rows, 65536 bf16 27.3 / 22.6, so not there.  near / Medium: 1024 words (8192 x 4096
-// fp32) 45 / 65; 1500 words (4000 x 12000 bf16) 45 with Medium, 60 in registers.  Medium / WideWriting: 3750 words (2000 x 30000 bf16) 50 / 57;
-// 12505 words (999 x 50021 fp32) 75 / 64.  Numbers only, 4096 x 65536 bf16: WideReading 78, WideWriting's shape 84.
-constexpr int MOST_NEAR = 1280, MOST_MEDIUM = 4096;      // words of a row
-typedef Ring<4, 6, 4, 18> Medium;
-typedef Ring<3, 8, 4, 13> WideReading;
-typedef Ring<2, 12, 4, 9> WideWriting;
+// second turn, 65536 fp32 27.0 / 30.7, 8000 fp32 5.7 / 7.6; 296 rows, 65536 bf16 27.3 / 22.6, so not there.  near / a ring: 1024 words (8192 x 4096
+// fp32) 45 / 65.  Medium / Broad: 1500 words (4000 x 12000 bf16) 44 / 51.  Broad / Medium / Wide: 3750 words (2000 x 30000 bf16) 51 / 56 / 57.
+// Wide / Broad: 8192 words (2048 x 65536 bf16) 107 / 111, 12505 (999 x 50021 fp32) 78 / 88; numbers only, the same 53 / 47, 36 / 35.  Eight words a thread
+// and wait where a thread took four before: numbers only, 2048 x 65536 bf16, 51 -> 47.
+constexpr int MOST_NEAR = 1280, MOST_MEDIUM = 2048, MOST_BROAD = 4096;      // words of a row
+typedef Ring<4, 6, 8, 9> Medium;
+typedef Ring<3, 8, 8, 6> Broad;
+typedef Ring<2, 12, 4, 9> Wide;
 
 // Behind the kernel that counts the targets (n_valid) the rows may start at once: nothing else of theirs depends on it, and it started
 // itself when everything before the call was done.  Otherwise the launch is an ordinary one.
@@ -646,8 +695,9 @@ template <typename T, RowsMode MODE, bool STORE, bool ENTROPY> int launch(const 
     return launch_kernel(p, kernel, 1, dim3((unsigned)std::min(cdiv(p.N, groups), sms * blocks)), 32 * NEAR_WARPS, smem, s, p, W, words);
   }
   if (words <= MOST_MEDIUM) return launch_ring<T, MODE, STORE, ENTROPY, Medium>(p, words, s);
-  if constexpr (STORE) return launch_ring<T, MODE, STORE, ENTROPY, WideWriting>(p, words, s);
-  else return launch_ring<T, MODE, STORE, ENTROPY, WideReading>(p, words, s);
+  if constexpr (STORE)
+    if (words > MOST_BROAD) return launch_ring<T, MODE, STORE, ENTROPY, Wide>(p, words, s);
+  return launch_ring<T, MODE, STORE, ENTROPY, Broad>(p, words, s);
 }
 template <RowsMode MODE, bool STORE, bool ENTROPY> int typed(int dtype, const RowsArgs& p, cudaStream_t s) {
   return dtype == FEMTO_BF16 ? launch<bf16, MODE, STORE, ENTROPY>(p, s) : launch<float, MODE, STORE, ENTROPY>(p, s);
