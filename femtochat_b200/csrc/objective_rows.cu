@@ -10,13 +10,13 @@
 // slopes and stores is ten times as long as a row's share of the bandwidth, so rows have to overlap.  Measured (time, share of the measured
 // copy rate; bytes of the floor):
 //   log-probabilities    gradient          policy loss and gradient
-//     77 us  0.80         172 us  0.83      185 us  0.78    4096 x 65536 bf16, a quarter of the rows without target   ring
-//     83     0.98         186     0.88      188     0.87    2048 x 65536 fp32                                         ring
-//     54     0.74         112     0.72      118     0.68    1000 x 131000 bf16                                        ring, a third of it twice
-//     28     0.66          50     0.73       55     0.66    2000 x 30000 bf16                                         ring
-//     30     0.68          45     0.91       51     0.80    8192 x 4096 fp32                                          near
-//     21     0.50          34     0.60       40     0.52    8192 x 4096 bf16                                          near
-//      3.7   0.17           5.0   0.26        6.9   0.18    16 x 65536 fp32                                           few
+//     70 us  0.88         174 us  0.83      180 us  0.80    4096 x 65536 bf16, a quarter of the rows without target   ring
+//     88     0.93         182     0.90      186     0.88    2048 x 65536 fp32                                         ring
+//     50     0.80         115     0.70      121     0.66    1000 x 131000 bf16                                        ring, a third of it twice
+//     28     0.65          51     0.72       55     0.66    2000 x 30000 bf16                                         ring
+//     30     0.69          45     0.91       54     0.75    8192 x 4096 fp32                                          near
+//     21     0.49          34     0.60       41     0.50    8192 x 4096 bf16                                          near
+//      4.0   0.16           5.0   0.26        7.0   0.18    16 x 65536 fp32                                           few
 // The exponential pipe is busy 68 % with 65536 logits in bf16.  Arithmetic in f32x2 pairs or in single floats takes the same time.
 #include <limits.h>
 
@@ -211,16 +211,16 @@ template <RowsMode MODE, bool ENTROPY>
 __device__ __forceinline__ float2 row_result(const RowsArgs& p, long long row, const RowStats& s, const RowNumbers& k, float& scale, bool write) {
   if (MODE == LOGPROBS) {
     if (write) {
-      p.logp[row] = log_prob(s, k.z, p.inv_t);
+      p.logp[row] = (float)log_prob(s, k.z, p.inv_t64);
       if (ENTROPY) p.ent[row] = entropy(s);
     }
     return make_float2(0.f, 0.f);
   }
   if (MODE == GRADIENT) return make_float2(k.x[0] * p.inv_t, ENTROPY ? k.x[1] * p.inv_t * (float)LN2 : 0.f);
-  const float lp = log_prob(s, k.z, p.inv_t);
+  const double lp = log_prob(s, k.z, p.inv_t64);
   float loss, slope;
   policy_token(p.term, lp, k.x[0], k.x[1], k.x[2], k.x[3], &loss, &slope);
-  if (write) { p.token_losses[row] = loss; p.logp[row] = lp; }
+  if (write) { p.token_losses[row] = loss; p.logp[row] = (float)lp; }
   if (p.n_valid && scale == 0.f) {      // a kernel of the same call counts the targets beside the first rows
     pdl_wait();
     scale = 1.f / (float)*reinterpret_cast<const volatile int*>(p.n_valid);

@@ -36,12 +36,12 @@ __global__ void __launch_bounds__(1024) k_count_targets(const int* __restrict__ 
 // rows (60000 rows: 40 us with one block, 8 with eight).
 __global__ void __launch_bounds__(1024) k_policy_sum(const RowsArgs p, int mean, float* loss_out, int* n_valid_out, int* n_clipped_out) {
   pdl_trigger();
-  __shared__ float sums[MOST_CLUSTER];
+  __shared__ double sums[MOST_CLUSTER];      // token losses have both signs: their sum is held in 64 bits
   __shared__ int counts[2][MOST_CLUSTER];
   const int C = (int)cluster_size(), rank = (int)cluster_rank();
   if (C > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
   pdl_wait();
-  float sum = 0.f;
+  double sum = 0.0;
   int n = 0, clipped = 0;
   const unsigned N = p.N, step = C * 1024;
   for (unsigned i0 = rank * 1024 + threadIdx.x; i0 < N; i0 += 4 * step) {
@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(1024) k_policy_sum(const RowsArgs p, int mean,
     for (int k = 0; k < 4; k++) {
       const bool has = t[k] >= 0 && t[k] < p.V && i0 + k * step < N;
       n += has;
-      sum += has ? loss[k] : 0.f;
+      sum += has ? (double)loss[k] : 0.0;
       clipped += has && policy_clipped(p.term, policy_ratio(lp[k], old[k]), A[k]);
     }
   }
@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(1024) k_policy_sum(const RowsArgs p, int mean,
   if (C > 1) asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
   if (rank == 0 && threadIdx.x == 0) {
     for (int i = 1; i < C; i++) { sum += sums[i]; n += counts[0][i]; clipped += counts[1][i]; }
-    *loss_out = mean && n > 0 ? sum / (float)n : sum;
+    *loss_out = (float)(mean && n > 0 ? sum / n : sum);
     *n_valid_out = n;
     if (n_clipped_out) *n_clipped_out = clipped;
   }
@@ -309,7 +309,7 @@ float log2e_over(float temperature) { return (float)(1.4426950408889634074 / (do
 RowsArgs rows_args(const void* logits, long long ldl, const int* tgt0, int N, int V, float temperature) {
   RowsArgs p = {};
   p.logits = logits; p.ldl = ldl; p.tgt0 = tgt0; p.N = N; p.V = V;
-  p.c = log2e_over(temperature); p.inv_t = 1.f / temperature;
+  p.c = log2e_over(temperature); p.inv_t = 1.f / temperature; p.inv_t64 = 1.0 / (double)temperature;
   return p;
 }
 }  // namespace

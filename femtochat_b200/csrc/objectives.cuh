@@ -44,26 +44,19 @@ template <bool ENTROPY> __device__ __forceinline__ RowStats merged(RowStats x, R
   if (ENTROPY) x.a += y.a;
   return x;
 }
-// log l = k ln2 + log f of l = 2^k f, f in [0.7, 1.4]: with ln2 in two parts, the first of which gives k ln2 without rounding, the only error of
-// the size of log l is the last rounding.  log(l) in one piece is 5e-7 off at l = 65536.
-struct LogSum {
-  float k, log_f;
-  __device__ __forceinline__ float minus_from(float x) const { return fmaf(-k, 0.693145752f, x) - fmaf(k, 1.42860677e-6f, log_f); }      // x - log l
-};
-__device__ __forceinline__ LogSum log_sum(float l) {
-  LogSum r;
-  if (!(l < INFINITY)) { r.k = 0.f; r.log_f = logf(l); return r; }
+// l = 2^k f with f in [0.7, 1.4]: log l is k ln2 + log f, a small number.  A log-probability is put together in 64 bits, a few instructions of one
+// warp a row: log(l) in one piece is 5e-7 off at l = 65536, and so would every ratio of two log-probabilities be.
+__device__ __forceinline__ double log_sum(float l) {
+  if (!(l < INFINITY)) return (double)logf(l);
   const int bits = __float_as_int(l), k = (bits - 0x3f3504f3) >> 23;      // sqrt(1/2)
-  r.k = (float)k;
-  r.log_f = logf(__int_as_float(bits - (k << 23)));
-  return r;
+  return LN2 * k + (double)logf(__int_as_float(bits - (k << 23)));
 }
 // log p of a logit z; a row without any logit above -inf (l = 0) has no distribution: -inf.
-__device__ __forceinline__ float log_prob(const RowStats& s, float z, float inv_t) {
-  return s.l == 0.f ? -INFINITY : log_sum(s.l).minus_from((z - s.m) * inv_t);
+__device__ __forceinline__ double log_prob(const RowStats& s, float z, double inv_t) {
+  return s.l == 0.f ? -(double)INFINITY : ((double)z - (double)s.m) * inv_t - log_sum(s.l);
 }
 __device__ __forceinline__ float entropy(const RowStats& s) {
-  return s.l == 0.f ? 0.f : -log_sum(s.l).minus_from(s.a / s.l * (float)LN2);
+  return s.l == 0.f ? 0.f : (float)(log_sum(s.l) - LN2 * (double)s.a / (double)s.l);
 }
 
 // ---- clusters ----------------------------------------------------------------------------------------------------------------------------------
@@ -91,15 +84,15 @@ __device__ __forceinline__ void store_remote(const int* local, uint32_t rank, in
 // the bounded product, which does not depend on lp, where A > 0 and r > hi or A < 0 and r < lo.  A weight of 0 counts nothing, whatever
 // the other numbers are.
 __device__ __forceinline__ bool policy_clipped(const PolicyTerm& t, float r, float A) { return (A > 0.f && r > t.hi) || (A < 0.f && r < t.lo); }
-__device__ __forceinline__ float policy_ratio(float lp, float old) { return expf(lp - old); }
-__device__ __forceinline__ void policy_token(const PolicyTerm& t, float lp, float old, float A, float ref, float w, float* loss, float* slope) {
+__device__ __forceinline__ float policy_ratio(double lp, float old) { return expf((float)(lp - (double)old)); }
+__device__ __forceinline__ void policy_token(const PolicyTerm& t, double lp, float old, float A, float ref, float w, float* loss, float* slope) {
   if (w == 0.f) { *loss = *slope = 0.f; return; }
   const float r = policy_ratio(lp, old);
   const float gain = A == 0.f ? 0.f : r * A;      // r may be inf
   const bool clipped = policy_clipped(t, r, A);
   float l = clipped ? -(A > 0.f ? t.hi : t.lo) * A : -gain, d = clipped ? 0.f : -gain;
   if (t.kl != 0.f) {
-    const float g = ref - lp, e = expm1f(g);
+    const float g = (float)((double)ref - lp), e = expm1f(g);
     l += t.kl * (e - g);
     d -= t.kl * e;
   }
@@ -118,6 +111,7 @@ struct RowsArgs {
   const int* tgt0;
   int V, N;
   float c, inv_t;                // log2(e) / temperature, 1 / temperature
+  double inv_t64;
   float *logp, *ent;             // LOGPROBS (ent may be NULL), POLICY: logp
   const float *dlogp, *dent;     // GRADIENT (dent may be NULL)
   const float *old, *ref, *adv, *w;      // POLICY
