@@ -27,7 +27,13 @@ template <typename S> __device__ S block_total(S v) {
 __global__ void __launch_bounds__(1024) k_count_targets(const int* __restrict__ tgt0, int N, int V, int* __restrict__ out) {
   pdl_trigger();
   int n = 0;
-  for (long long i = threadIdx.x; i < N; i += 1024) n += tgt0[i] >= 0 && tgt0[i] < V;
+  for (unsigned i0 = threadIdx.x; i0 < (unsigned)N; i0 += 8 * 1024) {      // eight in flight: the first rows' slopes wait for this
+    int t[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) t[k] = i0 + k * 1024 < (unsigned)N ? tgt0[i0 + k * 1024] : -1;
+#pragma unroll
+    for (int k = 0; k < 8; k++) n += t[k] >= 0 && t[k] < V;
+  }
   n = block_total(n);
   if (threadIdx.x == 0) *out = n;
 }

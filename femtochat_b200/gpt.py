@@ -187,6 +187,13 @@ class GPT:
             _lib.REDUCTION[reduction], _lib.ptr(st._loss), _lib.ptr(st._nvalid), _lib.stream_ptr()))
         return float(st._loss.item())
 
+    def token_logprobs(self, tokens, targets, positions=None, temperature: float = 1.0):
+        """Log-probabilities [B][T] of the targets (0 where ignored), e.g. under a reference model; see objectives.py."""
+        from .objectives import forward_token_logprobs
+        st = self.state(tokens.shape[0])
+        st.refresh_for(self.params.theta)
+        return forward_token_logprobs(self.params, st, self.layout, tokens, targets, positions, temperature)
+
     def logits(self, tokens, positions=None):
         import torch
         tok, pos = _dev_i32(tokens), _dev_i32(positions)

@@ -195,6 +195,8 @@ def test_the_step_and_the_call_on_the_model_s_logits_agree():
     t0 = (torch.where(tgt > 0, tgt - 1, tgt)).int().cuda()
     old, A, ref, w = (x.cuda() for x in numbers(fb.token_logprobs(z, t0).logp.cpu(), 9))
     args = dict(ref_logp=ref, weights=w, clip_low=0.2, clip_high=0.28, kl_coef=0.125, reduction="mean")
+    reference = fb.GPT(fb.Params(params.theta.clone()), cfg, lay, short_window=32)      # a model of its own, whose weights it casts itself
+    assert torch.equal(reference.token_logprobs(tok, tgt, pos, temperature=0.75), fb.forward_token_logprobs(params, st, lay, tok, tgt, pos, temperature=0.75))
     a = fb.policy_loss(z, t0, old, A, **args)
     b = fb.policy_loss_and_gradient_(params, st, lay, tok, tgt, old, A, positions=pos, **args)
     assert torch.equal(a.n_valid, b.n_valid) and torch.equal(a.n_clipped, b.n_clipped)

@@ -202,8 +202,9 @@ def test_rows_around_the_gradient_stay(V):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("V", [9, 3001, 66000])
-def test_masked_rows_and_masked_tokens(dtype, V):
+@pytest.mark.parametrize("V", [9, 3001, 12001, 66000, 140001])
+@pytest.mark.parametrize("copies", [1, 51])      # few rows and many take different kernels
+def test_masked_rows_and_masked_tokens(dtype, V, copies):
     """Rows without a target may hold anything; logits of -inf are tokens that cannot be chosen; a row of them has no distribution."""
     N = 6
     z, t = make(N, V, dtype, seed=3)
@@ -218,33 +219,40 @@ def test_masked_rows_and_masked_tokens(dtype, V):
     z[3, int(t[3])] = 1.0                # one token left: it is certain
     t[4] = -5
     numbers = torch.tensor([math.nan, 0.5, -0.5, 1.0, math.inf, 0.25], device="cuda")
-    r = fb.token_logprobs(z, t, entropy=True)
     lp, h, ls = reference(z, t)
     lp[2], h[2] = -math.log(V), math.log(V)
-    near(r.logp, lp, slack(V) + 2.0 ** -23 * (lp.abs() + h + 1), "logp")
-    near(r.entropy, h, 3 * slack(V) * (h + 1), "entropy")
-    assert float(r.logp[1]) == -math.inf and float(r.logp[3]) == 0.0 and float(r.entropy[3]) == 0.0
-    d = fb.token_logprobs_gradient(z, t, numbers, dentropy=numbers)
+    many_z, many_t, many_numbers = z.repeat(copies, 1), t.repeat(copies), numbers.repeat(copies)
+
+    def every(x):      # [copies][row]...
+        return x.unflatten(0, (copies, N))
+
+    r = fb.token_logprobs(many_z, many_t, entropy=True)
+    near(r.logp, lp.repeat(copies), slack(V) + 2.0 ** -23 * (lp.abs() + h + 1).repeat(copies), "logp")
+    near(r.entropy, h.repeat(copies), 3 * slack(V) * (h + 1).repeat(copies), "entropy")
+    assert bool((every(r.logp)[:, 1] == -math.inf).all() and (every(r.logp)[:, 3] == 0.0).all() and (every(r.entropy)[:, 3] == 0.0).all())
+    d = fb.token_logprobs_gradient(many_z, many_t, many_numbers, dentropy=many_numbers)
     assert not d.isnan().any()
-    for row in (0, 1, 4):
-        assert bool((d[row] == 0).all())
-    assert bool((d[hidden & (t >= 0)[:, None] & (torch.arange(N, device="cuda") != 2)[:, None]] == 0).all())
+    assert bool((every(d)[:, [0, 1, 4]] == 0).all())
+    impossible = hidden & (t >= 0)[:, None] & (torch.arange(N, device="cuda") != 2)[:, None]
+    assert bool((every(d)[:, impossible] == 0).all())
     finite = torch.tensor([math.nan, 0.0, 0.0, 0.0, math.nan, -2.0], device="cuda")
-    q = fb.policy_loss(z, t, finite, numbers, ref_logp=torch.where(t < 0, math.nan, -3.0), weights=torch.where(t < 0, math.nan, 1.0))
-    for row in (0, 1, 4):
-        assert bool((q.dlogits[row] == 0).all()) and float(q.token_losses[row]) == 0
-    assert not q.dlogits.isnan().any() and math.isfinite(float(q.loss)) and int(q.n_valid) == 4
+    q = fb.policy_loss(many_z, many_t, finite.repeat(copies), many_numbers, ref_logp=torch.where(many_t < 0, math.nan, -3.0),
+                       weights=torch.where(many_t < 0, math.nan, 1.0))
+    assert bool((every(q.dlogits)[:, [0, 1, 4]] == 0).all() and (every(q.token_losses)[:, [0, 1, 4]] == 0).all())
+    assert not q.dlogits.isnan().any() and math.isfinite(float(q.loss)) and int(q.n_valid) == 4 * copies
     assert status() == 0
 
 
 def test_not_a_number_stays_in_its_row():
-    for V in (50, 40000):
-        z, t = make(4, V, torch.float32, seed=4)
+    for N, V in ((4, 50), (4, 40000), (300, 50), (300, 9000), (300, 40000), (300, 140000)):
+        z, t = make(N, V, torch.float32, seed=4)
         z[1, 3], z[2, 4] = math.nan, math.inf
+        rest = torch.arange(N, device="cuda") % N
+        rest = rest[(rest != 1) & (rest != 2)]
         r = fb.token_logprobs(z, t, entropy=True)
-        assert r.logp[1:3].isnan().all() and r.entropy[1:3].isnan().all() and not r.logp[[0, 3]].isnan().any()
-        q = fb.policy_loss(z, t, torch.zeros(4, device="cuda"), torch.ones(4, device="cuda"), clip_high=None)
-        assert q.dlogits[1:3].isnan().all() and not q.dlogits[[0, 3]].isnan().any()
+        assert r.logp[1:3].isnan().all() and r.entropy[1:3].isnan().all() and not r.logp[rest].isnan().any()
+        q = fb.policy_loss(z, t, torch.zeros(N, device="cuda"), torch.ones(N, device="cuda"), clip_high=None)
+        assert q.dlogits[1:3].isnan().all() and not q.dlogits[rest].isnan().any()
 
 
 def test_no_rows_and_rows_without_targets():
@@ -255,9 +263,12 @@ def test_no_rows_and_rows_without_targets():
     for reduction in ("sum", "mean"):
         r = fb.policy_loss(empty, i32, f32, f32, reduction=reduction)
         assert float(r.loss) == 0 and int(r.n_valid) == 0 and int(r.n_clipped) == 0
-        z = torch.randn(3, 4000, device="cuda")
-        r = fb.policy_loss(z, torch.full((3,), -1, device="cuda", dtype=torch.int32), torch.zeros(3, device="cuda"), torch.ones(3, device="cuda"), reduction=reduction)
-        assert float(r.loss) == 0 and int(r.n_valid) == 0 and bool((r.dlogits == 0).all())
+        for N, V in ((3, 4000), (300, 1000), (700, 9001), (333, 70003)):
+            z = torch.randn(N, V, device="cuda")
+            out = torch.full_like(z, 3.0)
+            r = fb.policy_loss(z, torch.full((N,), -1, device="cuda", dtype=torch.int32), torch.zeros(N, device="cuda"), torch.ones(N, device="cuda"),
+                               reduction=reduction, out=out)
+            assert float(r.loss) == 0 and int(r.n_valid) == 0 and bool((out == 0).all()) and bool((r.logp == 0).all())
 
 
 def test_target_outside_the_vocabulary():
@@ -287,11 +298,12 @@ def test_rows_past_32_bits():
     assert torch.equal(fb.policy_loss(z, t, old, A, out=z).dlogits, want)
 
 
-def test_streams_and_graphs():
+@pytest.mark.parametrize("N,V", [(64, 9000), (320, 2000), (320, 9000), (320, 70000)])
+def test_streams_and_graphs(N, V):
     """Two calls at once on two streams, and a captured call replayed on other inputs while another graph of the same call lives."""
-    z, t = make(64, 9000, torch.bfloat16, seed=6)
-    y, u = make(64, 9000, torch.bfloat16, seed=7)
-    old, A = torch.full((64,), -4.0, device="cuda"), torch.linspace(-1, 1, 64, device="cuda")
+    z, t = make(N, V, torch.bfloat16, seed=6, masked=0.2)
+    y, u = make(N, V, torch.bfloat16, seed=7, masked=0.2)
+    old, A = torch.full((N,), -4.0, device="cuda"), torch.linspace(-1, 1, N, device="cuda")
     want, other = (fb.policy_loss(a, b, old, A, reduction="mean") for a, b in ((z, t), (y, u)))
     torch.cuda.synchronize()
     s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
@@ -303,7 +315,7 @@ def test_streams_and_graphs():
         torch.cuda.synchronize()
         for got, ref in ((a, want), (b, other)):
             assert all(torch.equal(x, y) for x, y in zip(got, ref))
-    x, v, runs = z.clone(), t.clone(), torch.arange(0, 65, 16, device="cuda", dtype=torch.int32)
+    x, v, runs = z.clone(), t.clone(), torch.arange(0, N + 1, N // 4, device="cuda", dtype=torch.int32)
     graphs = []
     for _ in range(2):
         g = torch.cuda.CUDAGraph()
