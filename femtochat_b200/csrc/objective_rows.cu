@@ -120,6 +120,12 @@ struct Exponent {
   __device__ __forceinline__ Exponent(float m, float c) : c2(pack2(c, c)), m2(pack2(-finite_or_zero(m), -finite_or_zero(m))) {}
   __device__ __forceinline__ void of(uint64_t z2, float& u0, float& u1) const { unpack2(mul2(add2(z2, m2), c2), u0, u1); }
 };
+// The word that holds the target, or -1 where it lies outside the words.
+template <typename T> __device__ __forceinline__ int word_of_target(const RowShape& r, int t) {
+  const int v = (t - r.head) / VecN<T>::n;
+  return t >= r.head && v < r.nvec ? v : -1;
+}
+
 // Adds pairs of logits to a thread's sums.
 template <bool ENTROPY> struct Adder {
   uint64_t l2 = 0, a2 = 0;
@@ -197,7 +203,7 @@ struct RowNumbers {
 };
 template <typename T, RowsMode MODE, bool ENTROPY> __device__ __forceinline__ RowNumbers row_numbers(const RowsArgs& p, long long row, const T* z, int t) {
   RowNumbers r;
-  if (MODE != GRADIENT) r.z = to_f<T>(z[t]);
+  r.z = to_f<T>(z[t]);
   if (MODE == GRADIENT) { r.x[0] = p.dlogp[row]; if (ENTROPY) r.x[1] = p.dent[row]; }
   if (MODE == POLICY) {
     r.x[0] = p.old[row]; r.x[1] = p.adv[row];
@@ -206,17 +212,17 @@ template <typename T, RowsMode MODE, bool ENTROPY> __device__ __forceinline__ Ro
   }
   return r;
 }
-// The row's numbers go out (where `write`), and (g, h) of its gradient come back.  scale: 0 until the rows with a target have been counted.
+// The row's numbers go out (where `write`), and (g, h) of its gradient and the target's logit come back.  scale: 0 until the rows with a target have been counted.
 template <RowsMode MODE, bool ENTROPY>
-__device__ __forceinline__ float2 row_result(const RowsArgs& p, long long row, const RowStats& s, const RowNumbers& k, float& scale, bool write) {
+__device__ __forceinline__ float4 row_result(const RowsArgs& p, long long row, const RowStats& s, const RowNumbers& k, float& scale, bool write) {
   if (MODE == LOGPROBS) {
     if (write) {
       p.logp[row] = (float)log_prob(s, k.z, p.inv_t64);
       if (ENTROPY) p.ent[row] = entropy(s);
     }
-    return make_float2(0.f, 0.f);
+    return make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  if (MODE == GRADIENT) return make_float2(k.x[0] * p.inv_t, ENTROPY ? k.x[1] * p.inv_t * (float)LN2 : 0.f);
+  if (MODE == GRADIENT) return make_float4(k.x[0] * p.inv_t, ENTROPY ? k.x[1] * p.inv_t * (float)LN2 : 0.f, k.z, 0.f);
   const double lp = log_prob(s, k.z, p.inv_t64);
   float loss, slope;
   policy_token(p.term, lp, k.x[0], k.x[1], k.x[2], k.x[3], &loss, &slope);
@@ -225,7 +231,7 @@ __device__ __forceinline__ float2 row_result(const RowsArgs& p, long long row, c
     pdl_wait();
     scale = 1.f / (float)*reinterpret_cast<const volatile int*>(p.n_valid);
   }
-  return make_float2((p.n_valid ? slope * scale : slope) * p.inv_t, 0.f);
+  return make_float4((p.n_valid ? slope * scale : slope) * p.inv_t, 0.f, k.z, 0.f);
 }
 template <RowsMode MODE, bool ENTROPY> __device__ __forceinline__ void row_without_target(const RowsArgs& p, long long row) {
   if (MODE == LOGPROBS) { p.logp[row] = 0.f; if (ENTROPY) p.ent[row] = 0.f; }
@@ -239,7 +245,7 @@ template <typename T, bool ENTROPY> struct Slope {
   uint64_t k2, h2;
   float at_target;
   int t;
-  __device__ __forceinline__ Slope(const RowStats& s, float2 gh, float c, int target) : x(s.m, c), t(target) {
+  __device__ __forceinline__ Slope(const RowStats& s, float4 gh, float c, int target) : x(s.m, c), t(target) {
     const bool none = s.l == 0.f;
     const float inv_l = 1.f / s.l;
     const float k = none ? 0.f : -(ENTROPY ? gh.x - gh.y * (s.a / s.l) : gh.x) * inv_l, h = none ? 0.f : -gh.y * inv_l;
@@ -252,29 +258,28 @@ template <typename T, bool ENTROPY> struct Slope {
     const uint64_t e2 = pack2(exp2_fast(u0), exp2_fast(u1));
     return mul2(e2, ENTROPY ? fma2(h2, pack2(fmaxf(u0, LEAST_U), fmaxf(u1, LEAST_U)), k2) : k2);
   }
-  // word v of the row, whose first element is j
-  __device__ __forceinline__ void store_word(T* d, int head, int v, const uint4& q, bool same) const {
-    const int j = head + v * n;
-    uint64_t y[n / 2];
+  __device__ __forceinline__ uint4 word(const uint4& q) const {
+    uint4 o;
 #pragma unroll
-    for (int i = 0; i < n / 2; i++) y[i] = of(Word<T>::get(q, i));
-    if ((unsigned)(t - j) < (unsigned)n)
+    for (int i = 0; i < n / 2; i++) Word<T>::put(o, i, of(Word<T>::get(q, i)));
+    return o;
+  }
+  // a word that does not lie in the gradient as it does in the logits
+  __device__ __forceinline__ void scatter(T* d, const uint4& q) const {
 #pragma unroll
-      for (int i = 0; i < n / 2; i++) y[i] = add2(y[i], pack2(j + 2 * i == t ? at_target : 0.f, j + 2 * i + 1 == t ? at_target : 0.f));
-    if (same) {
-      uint4 o;
-#pragma unroll
-      for (int i = 0; i < n / 2; i++) Word<T>::put(o, i, y[i]);
-      reinterpret_cast<uint4*>(d + head)[v] = o;
-    } else {
-#pragma unroll
-      for (int i = 0; i < n / 2; i++) {
-        float lo, hi;
-        unpack2(y[i], lo, hi);
-        d[j + 2 * i] = from_f<T>(lo);
-        d[j + 2 * i + 1] = from_f<T>(hi);
-      }
+    for (int i = 0; i < n / 2; i++) {
+      float lo, hi;
+      unpack2(of(Word<T>::get(q, i)), lo, hi);
+      d[2 * i] = from_f<T>(lo);
+      d[2 * i + 1] = from_f<T>(hi);
     }
+  }
+  // The target's element, over what stands there of its word, by the thread that stored the word.  (A comparison with the target at every word was
+  // a third of the instructions.)
+  __device__ __forceinline__ void store_target(T* d, float z) const {
+    float lo, hi;
+    unpack2(of(pack2(z, z)), lo, hi);
+    d[t] = from_f<T>(lo + at_target);
   }
   __device__ __forceinline__ void store_edge(T* d, int at, float z) const {
     float lo, hi;
@@ -300,7 +305,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) k_rows_few(const RowsArgs p) {
   pdl_trigger();
   constexpr int threads = 32 * FEW_WARPS, pitch = MOST_CLUSTER * FEW_WARPS;
   __shared__ float part[3 * pitch];
-  __shared__ float2 slope_s;
+  __shared__ float4 slope_s;
   const int C = (int)cluster_size(), rank = (int)cluster_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");      // this block runs: its shared memory may be written
   const long long row = blockIdx.x / C;
@@ -343,18 +348,23 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) k_rows_few(const RowsArgs p) {
   s = merged_parts<ENTROPY>(part, pitch, FEW_WARPS * C, p.c);
   if (warp == 0) {
     float scale = 0.f;
-    const float2 gh = row_result<MODE, ENTROPY>(p, row, s, numbers, scale, rank == 0 && lane == 0);
+    const float4 gh = row_result<MODE, ENTROPY>(p, row, s, numbers, scale, rank == 0 && lane == 0);
     if (lane == 0) slope_s = gh;
   }
   if (!STORE) return;
   __syncthreads();
-  const Slope<T, ENTROPY> slope(s, slope_s, p.c, t);
+  const float4 gh = slope_s;
+  const Slope<T, ENTROPY> slope(s, gh, p.c, t);
   const bool same = same_phase(z, d);
 #pragma unroll
   for (int k = 0; k < NV; k++) {
     const int v = first + k * threads + tid;
-    if (v < last) slope.store_word(d, r.head, v, q[k], same);
+    if (v >= last) continue;
+    if (same) reinterpret_cast<uint4*>(d + r.head)[v] = slope.word(q[k]);
+    else slope.scatter(d + r.head + v * VecN<T>::n, q[k]);
   }
+  const int vt = word_of_target<T>(r, t);
+  if (vt >= first && vt < last && (vt - first) % threads == tid) slope.store_target(d, gh.z);
   if (at >= 0) slope.store_edge(d, at, edge);
 }
 
@@ -370,7 +380,7 @@ __global__ void __launch_bounds__(32 * NEAR_WARPS, 3) k_rows_near(const RowsArgs
   extern __shared__ __align__(128) uint4 ring[];
   __shared__ uint64_t full[NEAR_WARPS][2];
   __shared__ float part[2][3][NEAR_WARPS];
-  __shared__ float2 slope_s[NEAR_WARPS];
+  __shared__ float4 slope_s[NEAR_WARPS];
   __shared__ int abort_flag;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = warp / W, groups = NEAR_WARPS / W;
   const int threads = W * 32, tid = threadIdx.x - group * threads, first_warp = group * W;
@@ -440,7 +450,7 @@ __global__ void __launch_bounds__(32 * NEAR_WARPS, 3) k_rows_near(const RowsArgs
     // all of the group are done with the row before this one: its buffer is free
     asked = t_next >= 0 && t_next < p.V;
     if (asked && tid == 0 && alive) ask(row + step, which ^ 1);
-    float2 gh = make_float2(0.f, 0.f);
+    float4 gh = make_float4(0.f, 0.f, 0.f, 0.f);
     if (warp == first_warp) gh = row_result<MODE, ENTROPY>(p, row, s, numbers, scale, lane == 0);
     if (!STORE) continue;
     if (W > 1) {
@@ -450,8 +460,15 @@ __global__ void __launch_bounds__(32 * NEAR_WARPS, 3) k_rows_near(const RowsArgs
     }
     const Slope<T, ENTROPY> slope(s, gh, p.c, t);
     const bool same = same_phase(z, d);
-#pragma unroll 2
-    for (int v = tid; v < r.nvec; v += threads) slope.store_word(d, r.head, v, words[v], same);
+    if (same) {
+      uint4* out = reinterpret_cast<uint4*>(d + r.head);
+#pragma unroll 4
+      for (int v = tid; v < r.nvec; v += threads) out[v] = slope.word(words[v]);
+    } else {
+      for (int v = tid; v < r.nvec; v += threads) slope.scatter(d + r.head + v * VecN<T>::n, words[v]);
+    }
+    const int vt = word_of_target<T>(r, t);
+    if (vt >= 0 && vt % threads == tid) slope.store_target(d, gh.z);
     if (at >= 0) slope.store_edge(d, at, edge);
   }
   if (!alive && tid == 0)      // nothing may still be on its way to this block's memory when it ends
@@ -484,7 +501,7 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
   extern __shared__ __align__(128) uint4 ring[];
   __shared__ uint64_t full[GROUPS][SLOTS], empty[SLOTS];
   __shared__ float part[GROUPS][2][3][GROUP_WARPS];
-  __shared__ float2 slope_s[GROUPS];
+  __shared__ float4 slope_s[GROUPS];
   __shared__ int abort_flag;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
@@ -598,10 +615,16 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
     for (int c = 0; c < chunks; c++, slot = next_slot(slot)) {
       wait_full(slot);
       uint4 q[PER_CHUNK];
+      const uint4* from = ring + slot * CHUNK + tid;
+      if ((c + 1) * CHUNK <= r.nvec) {
 #pragma unroll
-      for (int h = 0; h < PER_CHUNK; h++) {
-        q[h] = make_uint4(Word<T>::LEAST, Word<T>::LEAST, Word<T>::LEAST, Word<T>::LEAST);
-        if (c * CHUNK + h * GROUP_THREADS + tid < r.nvec) q[h] = ring[(size_t)slot * CHUNK + h * GROUP_THREADS + tid];
+        for (int h = 0; h < PER_CHUNK; h++) q[h] = from[h * GROUP_THREADS];
+      } else {
+#pragma unroll
+        for (int h = 0; h < PER_CHUNK; h++) {
+          q[h] = make_uint4(Word<T>::LEAST, Word<T>::LEAST, Word<T>::LEAST, Word<T>::LEAST);
+          if (c * CHUNK + h * GROUP_THREADS + tid < r.nvec) q[h] = from[h * GROUP_THREADS];
+        }
       }
       if (!STORE || c < again) {
         __syncwarp();
@@ -616,25 +639,34 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
     group_barrier(1 + group, GROUP_THREADS);
     if (STORE || gwarp == 0) s = merged_parts<ENTROPY>(parts, GROUP_WARPS, GROUP_WARPS, p.c);
     if (gwarp == 0) {
-      const float2 gh = row_result<MODE, ENTROPY>(p, row, s, numbers, scale, lane == 0);
+      const float4 gh = row_result<MODE, ENTROPY>(p, row, s, numbers, scale, lane == 0);
       if (STORE && lane == 0) slope_s[group] = gh;
     }
     if (!STORE) continue;
     group_barrier(1 + group, GROUP_THREADS);
-    const Slope<T, ENTROPY> slope(s, slope_s[group], p.c, t);
+    const float4 gh = slope_s[group];
+    const Slope<T, ENTROPY> slope(s, gh, p.c, t);
     const bool same = same_phase(z, d);
     slot = (first_slot + again) % SLOTS;
     for (int i = 0; i < chunks; i++, slot = next_slot(slot)) {
       const int c = i + again < chunks ? i + again : i + again - chunks;      // those that are still here first
       if (i + again >= chunks) wait_full(slot);
+      const uint4* from = ring + slot * CHUNK + tid;
+      if (same && (c + 1) * CHUNK <= r.nvec) {
+        uint4* out = reinterpret_cast<uint4*>(d + r.head) + c * CHUNK + tid;
 #pragma unroll
-      for (int h = 0; h < PER_CHUNK; h++) {
-        const int v = c * CHUNK + h * GROUP_THREADS + tid;
-        if (v < r.nvec) slope.store_word(d, r.head, v, ring[(size_t)slot * CHUNK + h * GROUP_THREADS + tid], same);
+        for (int h = 0; h < PER_CHUNK; h++) out[h * GROUP_THREADS] = slope.word(from[h * GROUP_THREADS]);
+      } else {
+        for (int h = 0, v = c * CHUNK + tid; v < r.nvec && h < PER_CHUNK; h++, v += GROUP_THREADS) {
+          if (same) reinterpret_cast<uint4*>(d + r.head)[v] = slope.word(from[h * GROUP_THREADS]);
+          else slope.scatter(d + r.head + v * VecN<T>::n, from[h * GROUP_THREADS]);
+        }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[slot]);
     }
+    const int vt = word_of_target<T>(r, t);
+    if (vt >= 0 && vt % CHUNK % GROUP_THREADS == tid) slope.store_target(d, gh.z);
     if (at >= 0) slope.store_edge(d, at, edge);
   }
 }
