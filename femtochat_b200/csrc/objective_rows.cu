@@ -10,13 +10,14 @@
 // slopes and stores is ten times as long as a row's share of the bandwidth, so rows have to overlap.  Measured (time, share of the measured
 // copy rate; bytes of the floor):
 //   log-probabilities    gradient          policy loss and gradient
-//     70 us  0.88         174 us  0.83      180 us  0.80    4096 x 65536 bf16, a quarter of the rows without target   ring
-//     88     0.93         182     0.90      186     0.88    2048 x 65536 fp32                                         ring
-//     50     0.80         115     0.70      121     0.66    1000 x 131000 bf16                                        ring, a third of it twice
-//     28     0.65          51     0.72       55     0.66    2000 x 30000 bf16                                         ring
-//     30     0.69          45     0.91       54     0.75    8192 x 4096 fp32                                          near
-//     21     0.49          34     0.60       41     0.50    8192 x 4096 bf16                                          near
-//      4.0   0.16           5.0   0.26        7.0   0.18    16 x 65536 fp32                                           few
+//     67 us  0.92         170 us  0.84      176 us  0.82    4096 x 65536 bf16, a quarter of the rows without target   ring, a row to two blocks (*)
+//     86     0.96         181     0.91      176     0.93    2048 x 65536 fp32                                         ring, the same
+//     49     0.81         100     0.80      108     0.74    1000 x 131000 bf16                                        ring, the same
+//     29     0.63          50     0.73       57     0.65    2000 x 30000 bf16                                         ring
+//     30     0.69          45     0.91       54     0.76    8192 x 4096 fp32                                          near
+//     21     0.49          33     0.63       39     0.52    8192 x 4096 bf16                                          near
+//      4.0   0.16           5.1   0.25        7.6   0.17    16 x 65536 fp32                                           few
+// (* log-probabilities: to one.)
 // The exponential pipe is busy 68 % with 65536 logits in bf16.  Arithmetic in f32x2 pairs or in single floats takes the same time.
 #include <limits.h>
 
@@ -480,35 +481,59 @@ __global__ void __launch_bounds__(32 * NEAR_WARPS, 3) k_rows_near(const RowsArgs
 // One block a multiprocessor: a warp brings the words of its rows in chunks (bulk copies, an mbarrier each), and groups of warps take the rows
 // in turn, so that one's pass over a row goes on while another works out its slopes or writes its gradient.  Chunks stay where they are until
 // their gradient is written.  Of a row that the ring does not hold the first chunks are given back at once and brought `again`, behind the
-// row's last: two passes over the ring's length later they are still in L2.  The warp that brings rows also writes the zeros of those without
+// row's last: two passes over the ring's length later they are still in L2.  Wide rows are shared by the two blocks of a cluster, half a row each, so
+// that a ring holds more of the rows that follow; their groups exchange statistics.  The warp that brings rows also writes the zeros of those without
 // target, by bulk copies, one such row behind each that it brings: all at once in their turn they took the reads' place (4096 x 65536 in bf16, the
 // first half of the rows without target, gradient: 157 -> 145 us).
-template <int GROUPS_, int WARPS_, int PER_, int SLOTS_> struct Ring {
-  static constexpr int GROUPS = GROUPS_, WARPS = WARPS_, THREADS = 32 * WARPS_, PER = PER_, CHUNK = PER_ * THREADS, SLOTS = SLOTS_;
+template <int BLOCKS_, int GROUPS_, int WARPS_, int PER_, int SLOTS_> struct Ring {
+  static constexpr int BLOCKS = BLOCKS_, GROUPS = GROUPS_, WARPS = WARPS_, THREADS = 32 * WARPS_, PER = PER_, CHUNK = PER_ * THREADS, SLOTS = SLOTS_;
   static constexpr int SPARE = 2;      // slots that a row wider than the ring leaves to what follows
   static constexpr int BLOCK = GROUPS * THREADS + 32;
   static constexpr int ZEROS = 512;      // words of zeros behind the ring, the source of the gradient of rows without target
   static constexpr size_t BYTES = ((size_t)SLOTS * CHUNK + ZEROS) * 16;
 };
+// Four numbers to where `local` lies in another block of the cluster, 16 bytes that its barrier counts.
+__device__ __forceinline__ void send_remote(const float4* local, const uint64_t* barrier, uint32_t rank, float4 v) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];"
+               ::"r"(remote_address(local, rank)), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(remote_address(barrier, rank)) : "memory");
+}
+// As mbar_wait, for what another block of the cluster sends.
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  for (uint32_t polls = 0; polls < WAIT_LIMIT; polls++) {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    if (ok) return true;
+    if ((polls & 255u) == 255u && *abort_flag) return false;
+  }
+  *abort_flag = 1;
+  atomicOr(&g_rows_status, ST_WAIT_TIMEOUT);
+  return false;
+}
 __device__ __forceinline__ void bulk_store_1d(void* gdst, const void* smem_src, uint32_t bytes) {
   asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(gdst), "r"(smem_u32(smem_src)), "r"(bytes) : "memory");
 }
 template <typename T, RowsMode MODE, bool STORE, bool ENTROPY, class R>
 __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const int chunks, const int again) {
-  constexpr int GROUPS = R::GROUPS, GROUP_WARPS = R::WARPS, GROUP_THREADS = R::THREADS, PER_CHUNK = R::PER, CHUNK = R::CHUNK, SLOTS = R::SLOTS;
+  constexpr int C = R::BLOCKS, GROUPS = R::GROUPS, GROUP_WARPS = R::WARPS, GROUP_THREADS = R::THREADS, PER_CHUNK = R::PER, CHUNK = R::CHUNK, SLOTS = R::SLOTS;
   auto next_slot = [](int slot) { return slot + 1 == SLOTS ? 0 : slot + 1; };
   pdl_trigger();
   extern __shared__ __align__(128) uint4 ring[];
   __shared__ uint64_t full[GROUPS][SLOTS], empty[SLOTS];
-  __shared__ float part[GROUPS][2][3][GROUP_WARPS];
+  __shared__ float part[GROUPS][3][GROUP_WARPS];
   __shared__ float4 slope_s[GROUPS];
+  __shared__ RowStats stats_s[GROUPS];
+  __shared__ uint64_t met[GROUPS][2];      // a group's statistics of a row from the other block of the cluster, two rows in turn
+  __shared__ __align__(16) float4 theirs[GROUPS][2];
   __shared__ int abort_flag;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = C > 1 ? (int)cluster_rank() : 0;
+  const long long first_row = blockIdx.x / C, step = gridDim.x / C;
   if (threadIdx.x == 0) {
     for (int i = 0; i < SLOTS; i++) {
       for (int g = 0; g < GROUPS; g++) mbar_init(&full[g][i], 1);
       mbar_init(&empty[i], GROUP_WARPS);
     }
+    for (int g = 0; g < GROUPS; g++) { mbar_init(&met[g][0], 1); mbar_init(&met[g][1], 1); }
     abort_flag = 0;
     fence_barrier_init();
   }
@@ -518,6 +543,13 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
     fence_proxy_async();
   }
   __syncthreads();
+  if (C > 1) asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");      // the other block's barriers are there
+  // the words of a row that are this block's
+  auto mine_of = [&](const RowShape& r, int& from) {
+    const int per = (r.nvec + C - 1) / C;
+    from = min(r.nvec, rank * per);
+    return min(r.nvec, from + per) - from;
+  };
   if (warp == GROUPS * GROUP_WARPS) {      // the warp that brings the rows
     int slot = 0, k = 0, nth = 0;
     uint32_t round = 0, used[GROUPS] = {}, parity[GROUPS] = {};      // bits: slots that a group's barriers have been used for, and how often, modulo 2
@@ -538,38 +570,42 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
       }
     };
     // the next row without target among the block's first `end`, behind those that have been dealt with
-    Targets masked(p, blockIdx.x, gridDim.x);
+    Targets masked(p, first_row, step);
     int masked_nth = 0;
     auto clear_next = [&](int end) -> bool {
-      for (long long row; masked_nth < end && (row = blockIdx.x + (long long)masked_nth * gridDim.x) < p.N;) {
+      for (long long row; masked_nth < end && (row = first_row + (long long)masked_nth * step) < p.N;) {
         const int t = masked(masked_nth++);
         if (t >= 0 && t < p.V) continue;
-        if (lane == 0) row_without_target<MODE, ENTROPY>(p, row);
+        if (rank == 0 && lane == 0) row_without_target<MODE, ENTROPY>(p, row);
         if (STORE) {
           T* d = reinterpret_cast<T*>(p.dlogits) + row * p.ldd;
           const RowShape r = row_shape<T>(d, p.V);
           if (lane == 0) {
-            uint4* words = reinterpret_cast<uint4*>(d + r.head);
-            for (int v = 0; v < r.nvec; v += R::ZEROS) bulk_store_1d(words + v, zeros, (uint32_t)min(R::ZEROS, r.nvec - v) * 16u);
+            int from;
+            const int n = mine_of(r, from);
+            uint4* words = reinterpret_cast<uint4*>(d + r.head) + from;
+            for (int v = 0; v < n; v += R::ZEROS) bulk_store_1d(words + v, zeros, (uint32_t)min(R::ZEROS, n - v) * 16u);
             bulk_commit();
           }
-          const int at = edge_of<T>(r, lane);
+          const int at = rank == 0 ? edge_of<T>(r, lane) : -1;
           if (at >= 0) d[at] = from_f<T>(0.f);
         }
         return true;
       }
       return false;
     };
-    Targets targets(p, blockIdx.x, gridDim.x);
-    for (long long row = blockIdx.x; row < p.N; row += gridDim.x) {
+    Targets targets(p, first_row, step);
+    for (long long row = first_row; row < p.N; row += step) {
       const int t = targets(nth++);
       if (t < 0 || t >= p.V) continue;
       const T* z = reinterpret_cast<const T*>(p.logits) + row * p.ldl;
       const RowShape r = row_shape<T>(z, p.V);
-      const uint4* words = reinterpret_cast<const uint4*>(z + r.head);
+      int from;
+      const int n = mine_of(r, from);
+      const uint4* words = reinterpret_cast<const uint4*>(z + r.head) + from;
       if (lane == 0) {
-        if (alive) bring(words, r.nvec, chunks, k % GROUPS);
-        if (STORE && alive) bring(words, r.nvec, again, k % GROUPS);
+        if (alive) bring(words, n, chunks, k % GROUPS);
+        if (STORE && alive) bring(words, n, again, k % GROUPS);
       }
       __syncwarp();
       clear_next(nth);
@@ -581,6 +617,8 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
       for (int i = 0; i < GROUPS * SLOTS; i++)
         if (used[i / SLOTS] >> (i % SLOTS) & 1u)
           for (uint32_t polls = 0; polls < WAIT_LIMIT && !mbar_try_wait(&full[i / SLOTS][i % SLOTS], (parity[i / SLOTS] >> (i % SLOTS) & 1u) ^ 1u); polls++) {}
+    __syncwarp();
+    if (C > 1) asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
     return;
   }
 
@@ -593,18 +631,21 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
     alive = alive && mbar_wait(&full[group][slot], parity >> slot & 1u, &abort_flag, &g_rows_status);
     parity ^= 1u << slot;
   };
-  int k = 0, turn = 0, nth = 0;
+  int k = 0, nth = 0;
+  uint32_t rows = 0;      // that the group has worked on
   float scale = 0.f;
-  Targets targets(p, blockIdx.x, gridDim.x);
-  for (long long row = blockIdx.x; row < p.N; row += gridDim.x) {
-    const int t = checked_target(p, targets(nth++), threadIdx.x == 0);
+  Targets targets(p, first_row, step);
+  for (long long row = first_row; row < p.N; row += step) {
+    const int t = checked_target(p, targets(nth++), rank == 0 && threadIdx.x == 0);
     if (t < 0) continue;
     const int mine = k++;
     if (mine % GROUPS != group) continue;
     const T* z = reinterpret_cast<const T*>(p.logits) + row * p.ldl;
     T* d = reinterpret_cast<T*>(p.dlogits) + row * p.ldd;
     const RowShape r = row_shape<T>(z, p.V);
-    const int at = edge_of<T>(r, tid);
+    int from_word;
+    const int nvec = mine_of(r, from_word);
+    const int at = rank == 0 ? edge_of<T>(r, tid) : -1;
     RowNumbers numbers;
     if (gwarp == 0) numbers = row_numbers<T, MODE, ENTROPY>(p, row, z, t);
     const float edge = at >= 0 ? to_f<T>(z[at]) : -INFINITY;
@@ -616,14 +657,14 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
       wait_full(slot);
       uint4 q[PER_CHUNK];
       const uint4* from = ring + slot * CHUNK + tid;
-      if ((c + 1) * CHUNK <= r.nvec) {
+      if ((c + 1) * CHUNK <= nvec) {
 #pragma unroll
         for (int h = 0; h < PER_CHUNK; h++) q[h] = from[h * GROUP_THREADS];
       } else {
 #pragma unroll
         for (int h = 0; h < PER_CHUNK; h++) {
           q[h] = make_uint4(Word<T>::LEAST, Word<T>::LEAST, Word<T>::LEAST, Word<T>::LEAST);
-          if (c * CHUNK + h * GROUP_THREADS + tid < r.nvec) q[h] = from[h * GROUP_THREADS];
+          if (c * CHUNK + h * GROUP_THREADS + tid < nvec) q[h] = from[h * GROUP_THREADS];
         }
       }
       if (!STORE || c < again) {
@@ -633,17 +674,33 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
       run.add(q, p.c);
     }
     RowStats s = run.of_warp(p.c);
-    float* parts = part[group][turn][0];
-    turn ^= 1;
+    float* parts = part[group][0];
     if (lane == 0) { parts[gwarp] = s.m; parts[GROUP_WARPS + gwarp] = s.l; if (ENTROPY) parts[2 * GROUP_WARPS + gwarp] = s.a; }
     group_barrier(1 + group, GROUP_THREADS);
-    if (STORE || gwarp == 0) s = merged_parts<ENTROPY>(parts, GROUP_WARPS, GROUP_WARPS, p.c);
     if (gwarp == 0) {
-      const float4 gh = row_result<MODE, ENTROPY>(p, row, s, numbers, scale, lane == 0);
-      if (STORE && lane == 0) slope_s[group] = gh;
+      s = merged_parts<ENTROPY>(parts, GROUP_WARPS, GROUP_WARPS, p.c);
+      if (C > 1) {
+        // Two rows in turn: the other block sends a row's statistics when it has this block's of the row before, and those go out ahead of the wait.
+        const int turn = rows & 1u;
+        if (lane == 0) {
+          mbar_expect_tx(&met[group][turn], 16);
+          // the target's logit goes along: it has been read then, and the other block may write over it
+          send_remote(&theirs[group][turn], &met[group][turn], rank ^ 1, make_float4(s.m, s.l, s.a, numbers.z));
+        }
+        alive = alive && mbar_wait_cluster(&met[group][turn], rows >> 1 & 1u, &abort_flag);
+        __syncwarp();
+        const float4 o = theirs[group][turn];
+        RowStats other;
+        other.m = o.x; other.l = o.y; other.a = o.z;
+        s = rank == 0 ? merged<ENTROPY>(s, other, p.c) : merged<ENTROPY>(other, s, p.c);      // the same order, the same bits, in both
+      }
+      const float4 gh = row_result<MODE, ENTROPY>(p, row, s, numbers, scale, rank == 0 && lane == 0);
+      if (STORE && lane == 0) { slope_s[group] = gh; stats_s[group] = s; }
     }
+    rows++;
+    group_barrier(1 + group, GROUP_THREADS);      // the parts are read, the slopes are there
     if (!STORE) continue;
-    group_barrier(1 + group, GROUP_THREADS);
+    s = stats_s[group];
     const float4 gh = slope_s[group];
     const Slope<T, ENTROPY> slope(s, gh, p.c, t);
     const bool same = same_phase(z, d);
@@ -652,35 +709,38 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
       const int c = i + again < chunks ? i + again : i + again - chunks;      // those that are still here first
       if (i + again >= chunks) wait_full(slot);
       const uint4* from = ring + slot * CHUNK + tid;
-      if (same && (c + 1) * CHUNK <= r.nvec) {
-        uint4* out = reinterpret_cast<uint4*>(d + r.head) + c * CHUNK + tid;
+      if (same && (c + 1) * CHUNK <= nvec) {
+        uint4* out = reinterpret_cast<uint4*>(d + r.head) + from_word + c * CHUNK + tid;
 #pragma unroll
         for (int h = 0; h < PER_CHUNK; h++) out[h * GROUP_THREADS] = slope.word(from[h * GROUP_THREADS]);
       } else {
-        for (int h = 0, v = c * CHUNK + tid; v < r.nvec && h < PER_CHUNK; h++, v += GROUP_THREADS) {
-          if (same) reinterpret_cast<uint4*>(d + r.head)[v] = slope.word(from[h * GROUP_THREADS]);
-          else slope.scatter(d + r.head + v * VecN<T>::n, from[h * GROUP_THREADS]);
+        for (int h = 0, v = c * CHUNK + tid; v < nvec && h < PER_CHUNK; h++, v += GROUP_THREADS) {
+          if (same) reinterpret_cast<uint4*>(d + r.head)[from_word + v] = slope.word(from[h * GROUP_THREADS]);
+          else slope.scatter(d + r.head + (from_word + v) * VecN<T>::n, from[h * GROUP_THREADS]);
         }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[slot]);
     }
-    const int vt = word_of_target<T>(r, t);
-    if (vt >= 0 && vt % CHUNK % GROUP_THREADS == tid) slope.store_target(d, gh.z);
+    const int vt = word_of_target<T>(r, t) - from_word;
+    if (vt >= 0 && vt < nvec && vt % CHUNK % GROUP_THREADS == tid) slope.store_target(d, gh.z);
     if (at >= 0) slope.store_edge(d, at, edge);
   }
+  if (C > 1) asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");      // nothing is on its way to a block that has ended
 }
 
 // ---- launch -----------------------------------------------------------------------------------------------------------------------------------
 // Where the kernels meet (gradient, us; the chosen one first).  few / others: 220 rows, where a block each leaves multiprocessors idle in the
 // second turn, 65536 fp32 27.0 / 30.7, 8000 fp32 5.7 / 7.6; 296 rows, 65536 bf16 27.3 / 22.6, so not there.  near / a ring: 1024 words (8192 x 4096
-// fp32) 45 / 65.  Medium / Broad: 1500 words (4000 x 12000 bf16) 44 / 51.  Broad / Medium / Wide: 3750 words (2000 x 30000 bf16) 51 / 56 / 57.
-// Wide / Broad: 8192 words (2048 x 65536 bf16) 107 / 111, 12505 (999 x 50021 fp32) 78 / 88; numbers only, the same 53 / 47, 36 / 35.  Eight words a thread
-// and wait where a thread took four before: numbers only, 2048 x 65536 bf16, 51 -> 47.
-constexpr int MOST_NEAR = 1280, MOST_MEDIUM = 2048, MOST_BROAD = 4096;      // words of a row
-typedef Ring<4, 6, 8, 9> Medium;
-typedef Ring<3, 8, 8, 6> Broad;
-typedef Ring<2, 12, 4, 9> Wide;
+// fp32) 45 / 65.  Medium / Wide: 1500 words (4000 x 12000 bf16) 45 / 51, 5000 (1000 x 40000 bf16) 37 / 39, 6250 (1500 x 25000 fp32) 54 / 59.
+// Wide / Medium: 8192 words (1000 x 32768 fp32) 46 / 48, (2048 x 65536 bf16) 93 / 105, 12505 (999 x 50021 fp32) 62 / 71; two groups of twelve warps
+// 112 at 2048 x 65536 bf16, a row to each block (two groups of twelve) 103.  Numbers only: nothing waits for its gradient, so a row to a block, in fewer
+// and larger groups, 2048 x 65536 bf16 46 / 53 with Medium, 1500 x 25000 fp32 the same 28.  Eight words a thread and wait where a thread took four
+// before: numbers only, 2048 x 65536 bf16, 51 -> 47; the gradient of Wide rows keeps four, eight spill.
+constexpr int MOST_NEAR = 1280, MOST_MEDIUM = 7168;      // words of a row
+typedef Ring<1, 4, 6, 8, 9> Medium;
+typedef Ring<1, 3, 8, 8, 6> WideReading;
+typedef Ring<2, 3, 8, 4, 13> WideWriting;
 
 // Behind the kernel that counts the targets (n_valid) the rows may start at once: nothing else of theirs depends on it, and it started
 // itself when everything before the call was done.  Otherwise the launch is an ordinary one.
@@ -702,9 +762,9 @@ int launch_kernel(const RowsArgs& p, void (*kernel)(P...), int C, dim3 grid, int
 }
 template <typename T, RowsMode MODE, bool STORE, bool ENTROPY, class R> int launch_ring(const RowsArgs& p, int words, cudaStream_t s) {
   constexpr auto kernel = k_rows_ring<T, MODE, STORE, ENTROPY, R>;
-  const int chunks = cdiv(words, R::CHUNK), again = chunks <= R::SLOTS ? 0 : chunks - (R::SLOTS - R::SPARE);
+  const int chunks = cdiv(cdiv(words, R::BLOCKS), R::CHUNK), again = chunks <= R::SLOTS ? 0 : chunks - (R::SLOTS - R::SPARE);
   FEMTO_TRY(allow_smem<kernel>(R::BYTES));
-  return launch_kernel(p, kernel, 1, dim3((unsigned)std::min(p.N, device_sm_count())), R::BLOCK, R::BYTES, s, p, chunks, again);
+  return launch_kernel(p, kernel, R::BLOCKS, dim3((unsigned)(std::min(p.N, device_sm_count() / R::BLOCKS) * R::BLOCKS)), R::BLOCK, R::BYTES, s, p, chunks, again);
 }
 template <typename T, RowsMode MODE, bool STORE, bool ENTROPY> int launch(const RowsArgs& p, cudaStream_t s) {
   const int words = std::max(1, p.V / VecN<T>::n), sms = device_sm_count(), block = 32 * FEW_WARPS;
@@ -727,9 +787,8 @@ template <typename T, RowsMode MODE, bool STORE, bool ENTROPY> int launch(const 
     return launch_kernel(p, kernel, 1, dim3((unsigned)std::min(cdiv(p.N, groups), sms * blocks)), 32 * NEAR_WARPS, smem, s, p, W, words);
   }
   if (words <= MOST_MEDIUM) return launch_ring<T, MODE, STORE, ENTROPY, Medium>(p, words, s);
-  if constexpr (STORE)
-    if (words > MOST_BROAD) return launch_ring<T, MODE, STORE, ENTROPY, Wide>(p, words, s);
-  return launch_ring<T, MODE, STORE, ENTROPY, Broad>(p, words, s);
+  if constexpr (STORE) return launch_ring<T, MODE, STORE, ENTROPY, WideWriting>(p, words, s);
+  else return launch_ring<T, MODE, STORE, ENTROPY, WideReading>(p, words, s);
 }
 template <RowsMode MODE, bool STORE, bool ENTROPY> int typed(int dtype, const RowsArgs& p, cudaStream_t s) {
   return dtype == FEMTO_BF16 ? launch<bf16, MODE, STORE, ENTROPY>(p, s) : launch<float, MODE, STORE, ENTROPY>(p, s);

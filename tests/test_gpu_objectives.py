@@ -255,6 +255,32 @@ def test_not_a_number_stays_in_its_row():
         assert q.dlogits[1:3].isnan().all() and not q.dlogits[rest].isnan().any()
 
 
+@pytest.mark.parametrize("dtype,V", [(torch.bfloat16, 60007), (torch.bfloat16, 214001), (torch.float32, 33001), (torch.float32, 110003)])
+@pytest.mark.parametrize("pitch,offset", [(0, 0), (7, 5)])
+def test_wide_rows_in_place(dtype, V, pitch, offset):
+    """A row that two blocks share, written over its logits: the target in either half and where they meet; rows that their ring holds, and wider."""
+    N = 260
+    z, t = make(N, V, dtype, pitch, offset, seed=6, masked=0.3)
+    half = V // 2
+    t[:12] = torch.tensor([0, V - 1, half, half - 1, half + 1, half - 9, half + 9, half - 17, half + 17, -1, 1, V - 2], device="cuda", dtype=t.dtype)
+    g = torch.Generator(device="cuda").manual_seed(V)
+    lp = reference(z, t, 1.0)[0]
+    old, A, _, w = tokens_of(N, lp, 6)
+    apart = fb.policy_loss(z, t, old, A, weights=w, out=torch.full_like(z, 3.0))
+    dlogp, dent = torch.randn(2, N, device="cuda", generator=g)
+    want = fb.token_logprobs_gradient(z, t, dlogp, dentropy=dent)
+    over = z.as_strided(z.shape, z.stride(), z.storage_offset())
+    keep = z.clone()
+    r = fb.policy_loss(over, t, old, A, weights=w, out=over)
+    assert torch.equal(r.logp, apart.logp) and torch.equal(r.loss, apart.loss)
+    near(over, apart.dlogits.double(), 0, "the same pass")
+    z.copy_(keep)
+    d = fb.token_logprobs_gradient(over, t, dlogp, dentropy=dent, out=over)
+    near(d, want.double(), 0, "the same pass, with the entropy")
+    near(r.logp, torch.where(t >= 0, lp, 0.0), slack(V) + 2.0 ** -23 * (lp.abs() + 13), "logp")
+    assert status() == 0
+
+
 def test_no_rows_and_rows_without_targets():
     empty = torch.empty(0, 5, device="cuda")
     i32, f32 = torch.empty(0, device="cuda", dtype=torch.int32), torch.empty(0, device="cuda")
