@@ -912,20 +912,24 @@ __global__ void __launch_bounds__(256) k_xent_finalize(const float2* __restrict_
 }
 
 // In place on a chunk of stored bf16 logits l[row][col]: d loss / d logit = w (softmax(z) - onehot) (1 - tanh^2(l/15)),
-// z = cap tanh(l/15) (cap = 15 over a temperature; w may be one number for each row), with the row's logsumexp from the statistics pass (src/kernels.jl:16-28;
+// z = 15 tanh(l/15), with the row's logsumexp from the statistics pass (src/kernels.jl:16-28;
 // ext/FemtoChatEnzymeExt.jl:175-189).  Same tanh.approx / ex2 arithmetic as that pass, so softmax sums to 1 over
 // the stored values.  A thread takes four 8-column groups 2048 columns apart (all four loads in flight before the
 // arithmetic); rows with an ignored target become zero.
-__global__ void __launch_bounds__(256) k_xent_dlogit_inplace(bf16* __restrict__ buf, long long ld,
+// OBJECTIVE: cap is 15 over a temperature, w one number for each row, and the logsumexp that of the logits before their rounding to bf16.  A
+// stored logit is off by up to 0.02 then, every e^(z - lse) by as much of itself, but softmax - 1 at a target of p = 0.99 by twice its size: that
+// element is taken from the row's -log p (loss_rows).
+template <bool OBJECTIVE> __global__ void __launch_bounds__(256) k_xent_dlogit_inplace(bf16* __restrict__ buf, long long ld,
                                                              const float* __restrict__ lse_rows,
                                                              const int* __restrict__ tgt0, int V, float w_host,
-                                                             const float* __restrict__ w_dev, float cap, const float* __restrict__ w_rows) {
+                                                             const float* __restrict__ w_dev, float cap, const float* __restrict__ w_rows,
+                                                             const float* __restrict__ loss_rows) {
   pdl_trigger();
   const long long row = blockIdx.y;
   const int col0 = blockIdx.x * 8192 + threadIdx.x * 8;
   const int tg = tgt0[row];
-  const float w = tg >= 0 ? (w_rows ? w_rows[row] : w_host * (w_dev ? w_dev[0] : 1.f)) : 0.f;
-  const float lse = lse_rows[row];
+  const float w = tg >= 0 ? (OBJECTIVE ? w_rows[row] : w_host * (w_dev ? w_dev[0] : 1.f)) : 0.f;
+  const float lse = lse_rows[row], at_target = OBJECTIVE ? expm1f(-loss_rows[row]) : 0.f;
   bf16* base = buf + row * ld;
   uint4 q[4];
 #pragma unroll
@@ -941,7 +945,8 @@ __global__ void __launch_bounds__(256) k_xent_dlogit_inplace(bf16* __restrict__ 
       float t;
       asm("tanh.approx.f32 %0, %1;" : "=f"(t) : "f"(__bfloat162float(h[e]) * (1.f / 15.f)));
       const float z = cap * t;
-      const float dz = w * (__expf(z - lse) - ((col + e) == tg ? 1.f : 0.f));
+      const float p = __expf(z - lse);
+      const float dz = w * (OBJECTIVE ? ((col + e) == tg ? at_target : fminf(p, 1.f)) : p - ((col + e) == tg ? 1.f : 0.f));
       h[e] = __float2bfloat16_rn(dz * (1.f - t * t));
     }
     *reinterpret_cast<uint4*>(base + col) = q[u];
@@ -1132,9 +1137,12 @@ int xent_finalize(const float2* stats, int ntile, const float* tz, const int* tg
   return 0;
 }
 int xent_dlogit_inplace(void* logits_bf16, long long ld, const float* lse_rows, const int* tgt0, int n, int V, float w,
-                        const float* w_dev, cudaStream_t s, float cap, const float* w_rows) {
+                        const float* w_dev, cudaStream_t s, float cap, const float* w_rows, const float* loss_rows) {
   if ((ld & 7) || (V & 7)) return femto_fail(FEMTO_ERR_ALIGN, "xent_dlogit_inplace: row pitch and vocabulary must be multiples of 8");
-  k_xent_dlogit_inplace<<<dim3(cdiv(V, 8192), n), 256, 0, s>>>(reinterpret_cast<bf16*>(logits_bf16), ld, lse_rows, tgt0, V, w, w_dev, cap, w_rows);
+  const dim3 grid(cdiv(V, 8192), n);
+  bf16* buf = reinterpret_cast<bf16*>(logits_bf16);
+  if (w_rows) k_xent_dlogit_inplace<true><<<grid, 256, 0, s>>>(buf, ld, lse_rows, tgt0, V, w, w_dev, cap, w_rows, loss_rows);
+  else k_xent_dlogit_inplace<false><<<grid, 256, 0, s>>>(buf, ld, lse_rows, tgt0, V, w, w_dev, cap, nullptr, nullptr);
   KERNEL_CHECK();
   return 0;
 }

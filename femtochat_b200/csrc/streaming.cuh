@@ -62,7 +62,7 @@ template <typename T> struct Stream {
 int sum_rows_to_scalar(const float* rows, int n, float* out, const int* tgt0, int* n_valid_out, float scale_by_valid,
                        cudaStream_t s);
 int xent_dlogit_inplace(void* logits_bf16, long long ld, const float* lse_rows, const int* tgt0, int n, int V, float w,
-                        const float* w_dev, cudaStream_t s, float cap = 15.f, const float* w_rows = nullptr);
+                        const float* w_dev, cudaStream_t s, float cap = 15.f, const float* w_rows = nullptr, const float* loss_rows = nullptr);
 int softcap_inplace(float* x, long long n, cudaStream_t s, float cap = 15.f);   // x = cap tanh(x / cap)
 int xent_finalize(const float2* stats, int ntile, const float* tz, const int* tgt0, int n, float* lse,
                   float* loss_rows, cudaStream_t s);

@@ -48,7 +48,8 @@ template <typename T> int xent_tail(const XentArgs& x, cudaStream_t s) {
                               x.loss_rows + c0, s));
       if (x.objective && !first_pass) FEMTO_TRY(objective_slopes(*x.objective, x.loss_rows, c0, cn, x.scale_dev, x.objective_loss, s));
       if (x.backward)
-        FEMTO_TRY(xent_dlogit_inplace(dlogit, ld, x.lse_rows + c0, x.targets0 + c0, cn, V, x.scale, x.scale_dev, s, cap, w_rows ? w_rows + c0 : nullptr));
+        FEMTO_TRY(xent_dlogit_inplace(dlogit, ld, x.lse_rows + c0, x.targets0 + c0, cn, V, x.scale, x.scale_dev, s, cap,
+                                      w_rows ? w_rows + c0 : nullptr, x.loss_rows + c0));
     } else {
       if (!x.logits_f32) return femto_fail(FEMTO_ERR_UNSUPPORTED, "lm_head tail: no fp32 logits workspace for this shape");
       g.epi = EPI_F32; g.beta = 0.f; g.C = x.logits_f32; g.ldc = ld;

@@ -169,6 +169,42 @@ def test_first_update_is_the_plain_policy_gradient(kw, dtype):
         assert cosine(want, params.delta) >= 0.9999
 
 
+def test_confident_tokens_in_bf16():
+    """Of tokens that the model is all but sure of, softmax - 1 is smaller than the rounding of a stored logit.  With unit advantages and the answers' own
+    log-probabilities the step is the cross-entropy's, whose softmax is that of the stored logits.  These are off by half a bf16 step, 2^-9 of x, which
+    softcap15 scales by 1 - tanh^2(x / 15): at most 6.8 2^-9 = 0.014, and tanh.approx by 15 2^-11 = 0.008.  A factor e^(z - lse) takes the error of
+    two logits, so an element of the two gradients differs by at most 0.044 of itself in either, 0.09 together; its parts of one sign add up in dx, and the
+    cosine is 1 - 0.09^2 / 2 at the least where they do not cancel."""
+    cfg, lay, th, batch, params, st, M = setup(TC, 8, "bfloat16", seed=10)
+    tok, tgt, pos = batch
+    g = torch.Generator().manual_seed(11)
+    head = slice(lay.lm_head.offset, lay.lm_head.offset + lay.lm_head.size)
+    D, V = TC["n_embed"], lay.lm_head.size // TC["n_embed"]
+    # the rows that enter the lm_head, read through a head that is the identity; the head that is used gives 64 of them a token each
+    th[head] = torch.eye(D, V).flatten()
+    x = 15 * torch.atanh(fb.GPT(fb.Params(th.cuda()), cfg, lay, compute_type="bfloat16").logits(tok, pos)[..., :D].cpu().flatten(0, 1) / 15)
+    W = D ** -0.5 * torch.randn(D, V, generator=g)
+    rows = torch.randperm(x.shape[0], generator=g)[:64]
+    W[:, :64] = ((16 + 10 * torch.rand(64, 1, generator=g)) * torch.nn.functional.normalize(x[rows], dim=1)).T * D ** -0.5
+    th[head] = W.flatten()
+    best = torch.full((x.shape[0],), -1, dtype=torch.int32)
+    best[rows] = torch.arange(1, 65, dtype=torch.int32)
+    best = best.view(tok.shape)
+    params = fb.Params(th.cuda())
+    st = fb.gradient_state(params, cfg, lay, tok, tgt, pos, compute_type="bfloat16")
+    logp = fb.forward_token_logprobs(params, st, lay, tok, best, pos)
+    left = -torch.expm1(logp.double()).cpu()
+    chosen = torch.where((left > 2e-4) & (left < 8e-3), best, -1).int()
+    assert int((chosen > 0).sum()) >= 8
+    fb.loss_and_gradient_(params, st, lay, tok, chosen, pos)
+    want = params.delta.clone()
+    r = fb.policy_loss_and_gradient_(params, st, lay, tok, chosen, logp, torch.ones_like(logp), positions=pos)
+    got = params.delta
+    assert int(r.n_valid) == int((chosen > 0).sum()) and int(r.n_clipped) == 0
+    assert cosine(want[head], got[head]) >= 0.99 and abs(float(got[head].norm() / want[head].norm()) - 1) < 0.09
+    assert cosine(want, got) >= 0.98
+
+
 def test_a_policy_step_trains_a_model():
     """Log-probabilities, steps and updates in turn, as a training loop calls them, on another stream than the default."""
     cfg, lay, th, batch, params, st, M = setup(TC, 4, "bfloat16", seed=7)
