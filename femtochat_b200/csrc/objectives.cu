@@ -91,12 +91,14 @@ __global__ void __launch_bounds__(1024) k_policy_sum(const RowsArgs p, int mean,
 // ---- paired preference loss ---------------------------------------------------------------------------------------------------------------
 typedef PreferenceArgs Preference;
 
-// The rows of one answer; offsets that leave the rows or descend make it empty.
-__device__ __forceinline__ int2 answer_rows(const Preference& p, int answer, bool flag) {
+// The rows of one answer, and whether they count: none of an answer does whose offsets leave the rows or descend.  Its rows still get a gradient
+// of 0: a row from offsets[0] on that no good answer holds lies between the offsets of a bad one.
+__device__ __forceinline__ int3 answer_rows(const Preference& p, int answer, bool flag) {
   const int a = p.offsets[answer], b = p.offsets[answer + 1];
-  if (a >= 0 && a <= b && b <= p.N) return make_int2(a, b);
+  if (a >= 0 && a <= b && b <= p.N) return make_int3(a, b, 1);
   if (flag) atomicOr(&g_objectives_status, ST_BAD_RANGE);
-  return make_int2(0, 0);
+  const int first = min(max(a, 0), p.N);
+  return make_int3(first, max(first, min(b, p.N)), 0);
 }
 
 // One block per pair, or a cluster of blocks for long answers; half of a block on each answer.  Sums of log ratios of two long answers nearly
@@ -110,13 +112,13 @@ __global__ void __launch_bounds__(1024) k_preference_pairs(const Preference p) {
   const int C = (int)cluster_size(), rank = (int)cluster_rank();
   if (C > 1) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");      // this block runs: its shared memory may be written
   const int pair = blockIdx.x / C, half = blockDim.x >> 1, side = threadIdx.x >= half, tid = threadIdx.x - side * half, warps = half >> 5;
-  const int2 rows = answer_rows(p, 2 * pair + side, rank == 0 && tid == 0);
+  const int3 rows = answer_rows(p, 2 * pair + side, rank == 0 && tid == 0);
   const unsigned first = rows.x + rank * half + tid, end = rows.y, step = C * half;
   double sum = 0.0;
   int n = 0;
   uint32_t seen = 0;      // which of the thread's first 32 rows count
   int q = 0;
-  for (unsigned i0 = first; i0 < end; i0 += 4 * step, q += 4) {      // four rows a thread in flight
+  for (unsigned i0 = first, counted_end = rows.z ? end : 0; i0 < counted_end; i0 += 4 * step, q += 4) {      // four rows a thread in flight
     int t[4];
     float lp[4], ref[4];
 #pragma unroll
@@ -179,7 +181,7 @@ __global__ void __launch_bounds__(1024) k_preference_pairs(const Preference p) {
   }
   if (!p.dlogp) return;
   __syncthreads();
-  const float d = slope_s[side];
+  const float d = rows.z ? slope_s[side] : 0.f;
   q = 0;
 #pragma unroll 4
   for (unsigned i = first; i < end; i += step, q++) p.dlogp[i] = (q < 32 ? seen >> q & 1u : !p.tgt0 || p.tgt0[i] >= 0) ? d : 0.f;

@@ -515,7 +515,7 @@ int32_t femto_policy_loss(int32_t dtype, const void* logits, int64_t ldl, const 
  *   sigmoid: -(1 - label_smoothing) log sigma(h) - label_smoothing log sigma(-h)        squared: (D - 1 / (2 beta))^2
  * Outputs: the reduced loss, pair_losses [P], ratios [2 P] = rho, dlogp [N] (may be NULL) = the gradient of the reduced loss, 0 in rows that
  * count for nothing or belong to no answer.  Offsets that leave 0 .. N or descend make an answer empty and raise bit 8 of the word that
- * femto_status_word(NULL, ..) reads; dlogp is then not complete. */
+ * femto_status_word(NULL, ..) reads; where answers then lie over one another, a row's dlogp is that of one of them, or 0. */
 int32_t femto_preference_loss(const float* logp, const float* ref_logp, const int32_t* targets0, int32_t N, const int32_t* offsets,
                               int32_t P, const femto_preference_config* h_cfg, float* loss_out, float* pair_losses, float* ratios,
                               float* dlogp, void* stream);

@@ -508,6 +508,27 @@ def test_bad_offsets_are_flagged():
     assert status() == 0
 
 
+@pytest.mark.parametrize("N,offsets", [(10, [0, 4, 11]), (10, [0, 6, 5]), (10, [-1, 4, 6]), (12, [0, -5, 8, 10, 12]), (12, [3, 2147483647, 5, 6, 7]), (12, [-2147483648, 2147483647, -1]),
+                                       (60000, [100, 70000, 50000]), (60000, [0, 20000, 70000])])
+def test_every_row_gets_a_gradient_behind_bad_offsets(N, offsets):
+    """The output's memory held something else before: a row that no good answer holds gets 0, one that a good answer holds a finite number."""
+    logp = -torch.rand(N, device="cuda")
+    o = torch.tensor(offsets, device="cuda", dtype=torch.int32)
+    P = len(offsets) // 2
+    dlogp, losses, ratios, loss = torch.full((N,), math.nan, device="cuda"), torch.empty(P, device="cuda"), torch.empty(2 * P, device="cuda"), torch.empty(1, device="cuda")
+    cfg = _lib.PreferenceConfigC(0, 0.1, 0.0, 0.0, 0, 0)
+    _lib.check(_lib.lib().femto_preference_loss(logp.data_ptr(), None, None, N, o.data_ptr(), P, C.byref(cfg), loss.data_ptr(), losses.data_ptr(), ratios.data_ptr(),
+                                                dlogp.data_ptr(), _lib.stream_ptr()))
+    held = torch.zeros(N, dtype=torch.bool, device="cuda")
+    for k, (a, b) in enumerate(zip(offsets, offsets[1:])):
+        if 0 <= a <= b <= N:
+            held[a:b] = True
+        else:
+            assert float(ratios[k]) == 0
+    assert status() == 8
+    assert bool(dlogp.isfinite().all()) and bool((dlogp[~held] == 0).all())
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_preference_from_logits_to_logits(dtype):
     """The three calls in a row, as a step makes them, against the gradient of the whole by differentiation in 64 bits."""
