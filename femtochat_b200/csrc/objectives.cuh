@@ -89,7 +89,7 @@ __device__ __forceinline__ void policy_token(const PolicyTerm& t, double lp, flo
   if (w == 0.f) { *loss = *slope = 0.f; return; }
   const float r = policy_ratio(lp, old);
   const float gain = A == 0.f ? 0.f : r * A;      // r may be inf
-  const bool clipped = policy_clipped(t, r, A);
+  const bool clipped = policy_clipped(t, policy_ratio((float)lp, old), A);      // of the number that goes out: the count of clipped tokens is taken from it
   float l = clipped ? -(A > 0.f ? t.hi : t.lo) * A : -gain, d = clipped ? 0.f : -gain;
   if (t.kl != 0.f) {
     const float g = (float)((double)ref - lp), e = expm1f(g);

@@ -529,6 +529,20 @@ def test_every_row_gets_a_gradient_behind_bad_offsets(N, offsets):
     assert bool(dlogp.isfinite().all()) and bool((dlogp[~held] == 0).all())
 
 
+def test_the_count_of_clipped_tokens_is_that_of_the_gradient():
+    """Ratios within a rounding of the bound: a token counts as clipped where, and only where, it has no gradient."""
+    N, V = 4000, 50
+    z, t = make(N, V, torch.float32, seed=12)
+    lp = fb.token_logprobs(z, t).logp
+    old = lp - math.log(1.25)
+    turn = torch.arange(N, device="cuda") % 3
+    for way in (1, 2):
+        old = torch.where(turn == way, torch.nextafter(old, torch.full_like(old, 90.0 if way == 1 else -90.0)), old)
+    r = fb.policy_loss(z, t, old, torch.ones(N, device="cuda"), clip_high=0.25)
+    none = (r.dlogits == 0).all(1)
+    assert 0 < int(none.sum()) < N and int(r.n_clipped) == int(none.sum())
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_preference_from_logits_to_logits(dtype):
     """The three calls in a row, as a step makes them, against the gradient of the whole by differentiation in 64 bits."""
