@@ -213,6 +213,12 @@ template <typename T, RowsMode MODE, bool ENTROPY> __device__ __forceinline__ Ro
   }
   return r;
 }
+// A kernel that started beside the one that counts the targets does not end before it, even if no row of its has asked for the count: what follows
+// in the stream waits for this kernel alone.
+template <RowsMode MODE> __device__ __forceinline__ void end_behind_the_count(const RowsArgs& p) {
+  if (MODE == POLICY && p.n_valid) pdl_wait();
+}
+
 // The row's numbers go out (where `write`), and (g, h) of its gradient and the target's logit come back.  scale: 0 until the rows with a target have been counted.
 template <RowsMode MODE, bool ENTROPY>
 __device__ __forceinline__ float4 row_result(const RowsArgs& p, long long row, const RowStats& s, const RowNumbers& k, float& scale, bool write) {
@@ -323,6 +329,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) k_rows_few(const RowsArgs p) {
       for (int v = first + tid; v < last; v += threads) reinterpret_cast<uint4*>(d + r.head)[v] = make_uint4(0, 0, 0, 0);
       if (at >= 0) d[at] = from_f<T>(0.f);
     }
+    end_behind_the_count<MODE>(p);
     return;
   }
   const uint4* words = reinterpret_cast<const uint4*>(z + r.head);
@@ -472,6 +479,7 @@ __global__ void __launch_bounds__(32 * NEAR_WARPS, 3) k_rows_near(const RowsArgs
     if (vt >= 0 && vt % threads == tid) slope.store_target(d, gh.z);
     if (at >= 0) slope.store_edge(d, at, edge);
   }
+  end_behind_the_count<MODE>(p);
   if (!alive && tid == 0)      // nothing may still be on its way to this block's memory when it ends
     for (int b = 0; b < 2; b++)
       for (uint32_t polls = 0; k > b && polls < WAIT_LIMIT && !mbar_try_wait(&full[group][b], (uint32_t)((k - b - 1) >> 1) & 1u); polls++) {}
@@ -726,6 +734,7 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
     if (vt >= 0 && vt < nvec && vt % CHUNK % GROUP_THREADS == tid) slope.store_target(d, gh.z);
     if (at >= 0) slope.store_edge(d, at, edge);
   }
+  end_behind_the_count<MODE>(p);
   if (C > 1) asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");      // nothing is on its way to a block that has ended
 }
 
