@@ -15,7 +15,8 @@
 //     49     0.81         100     0.80      108     0.74    1000 x 131000 bf16                                        ring, the same
 //     29     0.63          50     0.73       57     0.65    2000 x 30000 bf16                                         ring
 //     30     0.69          45     0.91       54     0.76    8192 x 4096 fp32                                          near
-//     21     0.49          33     0.63       39     0.52    8192 x 4096 bf16                                          near
+//     21     0.49          33     0.63       40     0.52    8192 x 4096 bf16                                          near
+//     31     0.48          49     0.60       58     0.50    20000 x 2400 bf16                                         near
 //      4.0   0.16           5.1   0.25        7.6   0.17    16 x 65536 fp32                                           few
 // (* log-probabilities: to one.)
 // The exponential pipe is busy 68 % with 65536 logits in bf16.  Arithmetic in f32x2 pairs or in single floats takes the same time.
@@ -390,7 +391,7 @@ __global__ void __launch_bounds__(32 * NEAR_WARPS, 3) k_rows_near(const RowsArgs
   __shared__ float part[2][3][NEAR_WARPS];
   __shared__ float4 slope_s[NEAR_WARPS];
   __shared__ int abort_flag;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = warp / W, groups = NEAR_WARPS / W;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = warp / W, groups = blockDim.x / (32 * W);
   const int threads = W * 32, tid = threadIdx.x - group * threads, first_warp = group * W;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2 * NEAR_WARPS; i++) mbar_init(&full[i / 2][i % 2], 1);
@@ -741,12 +742,12 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
 // ---- launch -----------------------------------------------------------------------------------------------------------------------------------
 // Where the kernels meet (gradient, us; the chosen one first).  few / others: 220 rows, where a block each leaves multiprocessors idle in the
 // second turn, 65536 fp32 27.0 / 30.7, 8000 fp32 5.7 / 7.6; 296 rows, 65536 bf16 27.3 / 22.6, so not there.  near / a ring: 1024 words (8192 x 4096
-// fp32) 45 / 65.  Medium / Wide: 1500 words (4000 x 12000 bf16) 45 / 51, 5000 (1000 x 40000 bf16) 37 / 39, 6250 (1500 x 25000 fp32) 54 / 59.
+// fp32) 45 / 62, 1250 (8000 x 10000 bf16) 78 / 80, 1500 (4000 x 12000 bf16) 45 / 45.  Medium / Wide: 1500 words (4000 x 12000 bf16) 45 / 51, 5000 (1000 x 40000 bf16) 37 / 39, 6250 (1500 x 25000 fp32) 54 / 59.
 // Wide / Medium: 8192 words (1000 x 32768 fp32) 46 / 48, (2048 x 65536 bf16) 93 / 105, 12505 (999 x 50021 fp32) 62 / 71; two groups of twelve warps
 // 112 at 2048 x 65536 bf16, a row to each block (two groups of twelve) 103.  Numbers only: nothing waits for its gradient, so a row to a block, in fewer
 // and larger groups, 2048 x 65536 bf16 46 / 53 with Medium, 1500 x 25000 fp32 the same 28.  Eight words a thread and wait where a thread took four
 // before: numbers only, 2048 x 65536 bf16, 51 -> 47; the gradient of Wide rows keeps four, eight spill.
-constexpr int MOST_NEAR = 1280, MOST_MEDIUM = 7168;      // words of a row
+constexpr int MOST_NEAR = 1400, MOST_MEDIUM = 7168;      // words of a row
 typedef Ring<1, 4, 6, 8, 9> Medium;
 typedef Ring<1, 3, 8, 8, 6> WideReading;
 typedef Ring<2, 3, 8, 4, 13> WideWriting;
@@ -786,14 +787,22 @@ template <typename T, RowsMode MODE, bool STORE, bool ENTROPY> int launch(const 
     return launch_kernel(p, k_rows_few<T, MODE, STORE, ENTROPY, FEW_WORDS>, C, grid, block, 0, s, p);
   }
   if (words <= MOST_NEAR) {
-    int W = 1;      // eight words a thread: with four, 8192 x 4096 in bf16 took 39 us for 34, more of it between the rows
-    while (W < NEAR_WARPS && words > W * 256) W *= 2;
-    const int groups = NEAR_WARPS / W;
-    const size_t smem = (size_t)groups * 2 * words * 16;
+    // W warps a row, `groups` of them a block: most rows in flight on a multiprocessor, if 16 warps work on them.  (8000 rows, gradient, us: 300 words
+    // of bf16 21 rows of a warp 48, 12 of two warps 62; 450 words 15 of one 54, 12 of two 60; 1150 words of fp32 6 of two 50, 3 of eight 67; but 1280
+    // words of bf16 5 of one 98, 4 of four 78.)
+    auto smem_of = [&](int n) { return (size_t)n * 2 * words * 16; };
+    auto blocks_of = [&](int n) { return std::min(3, (int)((220 << 10) / (smem_of(n) + 2048))); };
+    int W = 1, groups = 1, best = 0;
+    for (int w = 1; w <= NEAR_WARPS; w *= 2)
+      for (int n = 1; n <= NEAR_WARPS / w; n++) {
+        const int rows = n * blocks_of(n), score = rows * std::min(16, w * rows);
+        if (score >= best) { W = w; groups = n; best = score; }
+      }
+    const int blocks = blocks_of(groups);
+    const size_t smem = smem_of(groups);
     constexpr auto kernel = k_rows_near<T, MODE, STORE, ENTROPY>;
     FEMTO_TRY(allow_smem<kernel>(smem));
-    const int blocks = std::max(1, std::min(3, (int)((220 << 10) / (smem + 2048))));
-    return launch_kernel(p, kernel, 1, dim3((unsigned)std::min(cdiv(p.N, groups), sms * blocks)), 32 * NEAR_WARPS, smem, s, p, W, words);
+    return launch_kernel(p, kernel, 1, dim3((unsigned)std::min(cdiv(p.N, groups), sms * blocks)), 32 * W * groups, smem, s, p, W, words);
   }
   if (words <= MOST_MEDIUM) return launch_ring<T, MODE, STORE, ENTROPY, Medium>(p, words, s);
   if constexpr (STORE) return launch_ring<T, MODE, STORE, ENTROPY, WideWriting>(p, words, s);
