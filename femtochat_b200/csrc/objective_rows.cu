@@ -23,6 +23,7 @@
 #include <limits.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "objectives.cuh"
 #include "sm100_ptx.cuh"
@@ -171,6 +172,28 @@ template <typename T, bool ENTROPY> struct Running {
 #pragma unroll
       for (int i = 0; i < VecN<T>::n / 2; i++) sum.add(x, Word<T>::get(q[h], i));
   }
+  // The words that are left of a row, fewer than K for each of `threads`: `rest`, and counted from this thread on `mine`.  Where few are left, no
+  // exponentials of what is not there (16000 x 3200 in bf16, gradient: 47 -> 43 us).  `loaded` is called when the words have been read.
+  template <int K, class F> __device__ __forceinline__ void add_rest(const uint4* words, int threads, int mine, int rest, float c, const F& loaded) {
+    if (rest > K / 2 * threads) {
+      uint4 q[K];
+#pragma unroll
+      for (int h = 0; h < K; h++) q[h] = word_or_none(words + h * threads, h * threads < mine);
+      loaded();
+      add(q, c);
+    } else {
+      for (; rest > 0; rest -= threads, mine -= threads, words += threads) {
+        uint4 q[1] = {word_or_none(words, mine > 0)};
+        add(q, c);
+      }
+      loaded();
+    }
+  }
+  static __device__ __forceinline__ uint4 word_or_none(const uint4* word, bool there) {
+    uint4 q = make_uint4(Word<T>::LEAST, Word<T>::LEAST, Word<T>::LEAST, Word<T>::LEAST);
+    if (there) q = *word;
+    return q;
+  }
   // The warp's statistics, in every lane.
   __device__ __forceinline__ RowStats of_warp(float c) {
     sum.join(s);
@@ -212,6 +235,28 @@ template <typename T, RowsMode MODE, bool ENTROPY> __device__ __forceinline__ Ro
     if (p.term.kl != 0.f) r.x[2] = p.ref[row];
     if (p.w) r.x[3] = p.w[row];
   }
+  return r;
+}
+// The same in one register while the row is read: a number for each of a warp's first lanes, from one load.  (With four more registers the
+// narrow rows' policy kernel spaced its loads out: 8000 x 4600 in fp32 66 us for 57.)  By whole warps.
+struct LaneNumbers {
+  float z = 0.f, v = 1.f;
+  __device__ __forceinline__ RowNumbers all() const {
+    RowNumbers r;
+    r.z = z;
+#pragma unroll
+    for (int i = 0; i < 4; i++) r.x[i] = __shfl_sync(0xffffffffu, v, i);
+    return r;
+  }
+};
+template <typename T, RowsMode MODE, bool ENTROPY> __device__ __forceinline__ LaneNumbers lane_numbers(const RowsArgs& p, long long row, const T* z, int t) {
+  LaneNumbers r;
+  r.z = to_f<T>(z[t]);
+  const int lane = threadIdx.x & 31;
+  const float* from = nullptr;
+  if (MODE == GRADIENT) from = lane == 0 ? p.dlogp : ENTROPY && lane == 1 ? p.dent : nullptr;
+  if (MODE == POLICY) from = lane == 0 ? p.old : lane == 1 ? p.adv : lane == 2 && p.term.kl != 0.f ? p.ref : lane == 3 ? p.w : nullptr;
+  if (from) r.v = from[row];
   return r;
 }
 // A kernel that started beside the one that counts the targets does not end before it, even if no row of its has asked for the count: what follows
@@ -434,21 +479,20 @@ __global__ void __launch_bounds__(32 * NEAR_WARPS, 3) k_rows_near(const RowsArgs
     const uint32_t parity = (uint32_t)(k >> 1) & 1u;
     k++;
     if (!asked && tid == 0 && alive) ask(row, which);      // the row before the last but one, which this buffer held, is done: a barrier lies between
-    RowNumbers numbers;
-    if (warp == first_warp) numbers = row_numbers<T, MODE, ENTROPY>(p, row, z, t);
+    LaneNumbers numbers;
+    if (warp == first_warp) numbers = lane_numbers<T, MODE, ENTROPY>(p, row, z, t);
     const float edge = at >= 0 ? to_f<T>(z[at]) : -INFINITY;
     Running<T, ENTROPY> run(at >= 0, edge, p.c);
     const uint4* words = buffer + (size_t)which * pitch;
     alive = alive && mbar_wait(&full[group][which], parity, &abort_flag, &g_rows_status);
-    for (int v0 = tid; v0 < r.nvec; v0 += NEAR_WORDS * threads) {
+    int v0 = 0;
+    for (; v0 + NEAR_WORDS * threads <= r.nvec; v0 += NEAR_WORDS * threads) {
       uint4 q[NEAR_WORDS];
 #pragma unroll
-      for (int h = 0; h < NEAR_WORDS; h++) {
-        q[h] = make_uint4(Word<T>::LEAST, Word<T>::LEAST, Word<T>::LEAST, Word<T>::LEAST);
-        if (v0 + h * threads < r.nvec) q[h] = words[v0 + h * threads];
-      }
+      for (int h = 0; h < NEAR_WORDS; h++) q[h] = words[v0 + h * threads + tid];
       run.add(q, p.c);
     }
+    run.template add_rest<NEAR_WORDS>(words + v0 + tid, threads, r.nvec - v0 - tid, r.nvec - v0, p.c, [] {});
     RowStats s = run.of_warp(p.c);
     if (W > 1) {
       float* mine = part[which][0];
@@ -460,7 +504,7 @@ __global__ void __launch_bounds__(32 * NEAR_WARPS, 3) k_rows_near(const RowsArgs
     asked = t_next >= 0 && t_next < p.V;
     if (asked && tid == 0 && alive) ask(row + step, which ^ 1);
     float4 gh = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (warp == first_warp) gh = row_result<MODE, ENTROPY>(p, row, s, numbers, scale, lane == 0);
+    if (warp == first_warp) gh = row_result<MODE, ENTROPY>(p, row, s, numbers.all(), scale, lane == 0);
     if (!STORE) continue;
     if (W > 1) {
       if (warp == first_warp && lane == 0) slope_s[group] = gh;
@@ -471,8 +515,18 @@ __global__ void __launch_bounds__(32 * NEAR_WARPS, 3) k_rows_near(const RowsArgs
     const bool same = same_phase(z, d);
     if (same) {
       uint4* out = reinterpret_cast<uint4*>(d + r.head);
-#pragma unroll 4
-      for (int v = tid; v < r.nvec; v += threads) out[v] = slope.word(words[v]);
+      // Four words at a time while every thread has as many, and one by one from there: unrolled with a remainder for each thread, the code of
+      // 24 warps that are at different places of it took more time than its instructions (30000 x 1000 in bf16: 38 -> 32 us).
+      int v = 0;
+      for (; v + 4 * threads <= r.nvec; v += 4 * threads) {
+        uint4 q[4];
+#pragma unroll
+        for (int h = 0; h < 4; h++) q[h] = words[v + h * threads + tid];
+#pragma unroll
+        for (int h = 0; h < 4; h++) out[v + h * threads + tid] = slope.word(q[h]);
+      }
+#pragma unroll 1
+      for (v += tid; v < r.nvec; v += threads) out[v] = slope.word(words[v]);
     } else {
       for (int v = tid; v < r.nvec; v += threads) slope.scatter(d + r.head + v * VecN<T>::n, words[v]);
     }
@@ -664,23 +718,21 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
     int slot = first_slot;
     for (int c = 0; c < chunks; c++, slot = next_slot(slot)) {
       wait_full(slot);
-      uint4 q[PER_CHUNK];
       const uint4* from = ring + slot * CHUNK + tid;
-      if ((c + 1) * CHUNK <= nvec) {
-#pragma unroll
-        for (int h = 0; h < PER_CHUNK; h++) q[h] = from[h * GROUP_THREADS];
-      } else {
-#pragma unroll
-        for (int h = 0; h < PER_CHUNK; h++) {
-          q[h] = make_uint4(Word<T>::LEAST, Word<T>::LEAST, Word<T>::LEAST, Word<T>::LEAST);
-          if (c * CHUNK + h * GROUP_THREADS + tid < nvec) q[h] = from[h * GROUP_THREADS];
-        }
-      }
-      if (!STORE || c < again) {
+      auto done = [&]() {
+        if (STORE && c >= again) return;
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[slot]);
+      };
+      if ((c + 1) * CHUNK <= nvec) {
+        uint4 q[PER_CHUNK];
+#pragma unroll
+        for (int h = 0; h < PER_CHUNK; h++) q[h] = from[h * GROUP_THREADS];
+        done();
+        run.add(q, p.c);
+      } else {      // a row's last
+        run.template add_rest<PER_CHUNK>(from, GROUP_THREADS, nvec - c * CHUNK - tid, nvec - c * CHUNK, p.c, done);
       }
-      run.add(q, p.c);
     }
     RowStats s = run.of_warp(p.c);
     float* parts = part[group][0];
@@ -742,13 +794,17 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
 // ---- launch -----------------------------------------------------------------------------------------------------------------------------------
 // Where the kernels meet (gradient, us; the chosen one first).  few / others: 220 rows, where a block each leaves multiprocessors idle in the
 // second turn, 65536 fp32 27.0 / 30.7, 8000 fp32 5.7 / 7.6; 296 rows, 65536 bf16 27.3 / 22.6, so not there.  near / a ring: 1024 words (8192 x 4096
-// fp32) 45 / 62, 1250 (8000 x 10000 bf16) 78 / 80, 1500 (4000 x 12000 bf16) 45 / 45.  Medium / Wide: 1500 words (4000 x 12000 bf16) 45 / 51, 5000 (1000 x 40000 bf16) 37 / 39, 6250 (1500 x 25000 fp32) 54 / 59.
-// Wide / Medium: 8192 words (1000 x 32768 fp32) 46 / 48, (2048 x 65536 bf16) 93 / 105, 12505 (999 x 50021 fp32) 62 / 71; two groups of twelve warps
-// 112 at 2048 x 65536 bf16, a row to each block (two groups of twelve) 103.  Numbers only: nothing waits for its gradient, so a row to a block, in fewer
-// and larger groups, 2048 x 65536 bf16 46 / 53 with Medium, 1500 x 25000 fp32 the same 28.  Eight words a thread and wait where a thread took four
-// before: numbers only, 2048 x 65536 bf16, 51 -> 47; the gradient of Wide rows keeps four, eight spill.
+// fp32) 45 / 62, 1250 (8000 x 10000 bf16) 78 / 80, 1500 (4000 x 12000 bf16) 45 / 45.  Medium / Wide: 1500 words (4000 x 12000 bf16) 45 / 51,
+// 5000 (1000 x 40000 bf16) 37 / 39, 6250 (1500 x 25000 fp32) 53 / 59.  Wide / Medium: 8192 words (1000 x 32768 fp32) 46 / 48, (2048 x 65536 bf16)
+// 93 / 105, 12505 (999 x 50021 fp32) 62 / 71.
+// Medium and writing: 20 warps that may have 80 registers; with 24, as for numbers only, the policy's kernels spill (4000 x 12000 bf16 53 / 56, 3000 x
+// 20000 bf16 46 / 50, 1500 x 25000 fp32 57 / 59; numbers only, the first, 30 / 28).  Wide and writing: a row to two blocks; two groups of twelve warps 112 at
+// 2048 x 65536 bf16, four of six 108, a row to each block (two groups of twelve) 103.  Numbers only: nothing waits for its gradient, so a row to a
+// block, in fewer and larger groups, 2048 x 65536 bf16 46 / 53 with Medium, 1500 x 25000 fp32 the same 28.  Eight words a thread and wait where a thread
+// took four before: numbers only, 2048 x 65536 bf16, 51 -> 47; the gradient of Wide rows keeps four, eight spill.
 constexpr int MOST_NEAR = 1400, MOST_MEDIUM = 7168;      // words of a row
-typedef Ring<1, 4, 6, 8, 9> Medium;
+typedef Ring<1, 4, 6, 8, 9> MediumReading;
+typedef Ring<1, 4, 5, 8, 10> MediumWriting;
 typedef Ring<1, 3, 8, 8, 6> WideReading;
 typedef Ring<2, 3, 8, 4, 13> WideWriting;
 
@@ -787,7 +843,7 @@ template <typename T, RowsMode MODE, bool STORE, bool ENTROPY> int launch(const 
     return launch_kernel(p, k_rows_few<T, MODE, STORE, ENTROPY, FEW_WORDS>, C, grid, block, 0, s, p);
   }
   if (words <= MOST_NEAR) {
-    // W warps a row, `groups` of them a block: most rows in flight on a multiprocessor, if 16 warps work on them.  (8000 rows, gradient, us: 300 words
+    // W warps a row, `groups` of them a block: most rows in flight on a multiprocessor, if 16 warps work on them.  (Gradient, us, each pair at one size: 300 words
     // of bf16 21 rows of a warp 48, 12 of two warps 62; 450 words 15 of one 54, 12 of two 60; 1150 words of fp32 6 of two 50, 3 of eight 67; but 1280
     // words of bf16 5 of one 98, 4 of four 78.)
     auto smem_of = [&](int n) { return (size_t)n * 2 * words * 16; };
@@ -804,9 +860,9 @@ template <typename T, RowsMode MODE, bool STORE, bool ENTROPY> int launch(const 
     FEMTO_TRY(allow_smem<kernel>(smem));
     return launch_kernel(p, kernel, 1, dim3((unsigned)std::min(cdiv(p.N, groups), sms * blocks)), 32 * W * groups, smem, s, p, W, words);
   }
-  if (words <= MOST_MEDIUM) return launch_ring<T, MODE, STORE, ENTROPY, Medium>(p, words, s);
-  if constexpr (STORE) return launch_ring<T, MODE, STORE, ENTROPY, WideWriting>(p, words, s);
-  else return launch_ring<T, MODE, STORE, ENTROPY, WideReading>(p, words, s);
+  typedef typename std::conditional<STORE, MediumWriting, MediumReading>::type Medium;
+  typedef typename std::conditional<STORE, WideWriting, WideReading>::type Wide;
+  return words <= MOST_MEDIUM ? launch_ring<T, MODE, STORE, ENTROPY, Medium>(p, words, s) : launch_ring<T, MODE, STORE, ENTROPY, Wide>(p, words, s);
 }
 template <RowsMode MODE, bool STORE, bool ENTROPY> int typed(int dtype, const RowsArgs& p, cudaStream_t s) {
   return dtype == FEMTO_BF16 ? launch<bf16, MODE, STORE, ENTROPY>(p, s) : launch<float, MODE, STORE, ENTROPY>(p, s);
