@@ -13,10 +13,10 @@
 //     67 us  0.92         170 us  0.84      176 us  0.82    4096 x 65536 bf16, a quarter of the rows without target   ring, a row to two blocks (*)
 //     86     0.96         181     0.91      176     0.93    2048 x 65536 fp32                                         ring, the same
 //     49     0.81         100     0.80      108     0.74    1000 x 131000 bf16                                        ring, the same
-//     29     0.63          50     0.73       57     0.65    2000 x 30000 bf16                                         ring
-//     30     0.69          45     0.91       54     0.76    8192 x 4096 fp32                                          near
-//     21     0.49          33     0.63       40     0.52    8192 x 4096 bf16                                          near
-//     31     0.48          49     0.60       58     0.50    20000 x 2400 bf16                                         near
+//     30     0.61          48     0.77       52     0.70    2000 x 30000 bf16                                         ring
+//     30     0.69          45     0.91       50     0.81    8192 x 4096 fp32                                          near
+//     21     0.49          32     0.64       39     0.53    8192 x 4096 bf16                                          near
+//     28     0.52          45     0.65       54     0.54    20000 x 2400 bf16                                         near
 //      4.0   0.16           5.1   0.25        7.6   0.17    16 x 65536 fp32                                           few
 // (* log-probabilities: to one.)
 // The exponential pipe is busy 68 % with 65536 logits in bf16.  Arithmetic in f32x2 pairs or in single floats takes the same time.
@@ -794,15 +794,15 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
 // ---- launch -----------------------------------------------------------------------------------------------------------------------------------
 // Where the kernels meet (gradient, us; the chosen one first).  few / others: 220 rows, where a block each leaves multiprocessors idle in the
 // second turn, 65536 fp32 27.0 / 30.7, 8000 fp32 5.7 / 7.6; 296 rows, 65536 bf16 27.3 / 22.6, so not there.  near / a ring: 1024 words (8192 x 4096
-// fp32) 45 / 62, 1250 (8000 x 10000 bf16) 78 / 80, 1500 (4000 x 12000 bf16) 45 / 45.  Medium / Wide: 1500 words (4000 x 12000 bf16) 45 / 51,
-// 5000 (1000 x 40000 bf16) 37 / 39, 6250 (1500 x 25000 fp32) 53 / 59.  Wide / Medium: 8192 words (1000 x 32768 fp32) 46 / 48, (2048 x 65536 bf16)
-// 93 / 105, 12505 (999 x 50021 fp32) 62 / 71.
-// Medium and writing: 20 warps that may have 80 registers; with 24, as for numbers only, the policy's kernels spill (4000 x 12000 bf16 53 / 56, 3000 x
-// 20000 bf16 46 / 50, 1500 x 25000 fp32 57 / 59; numbers only, the first, 30 / 28).  Wide and writing: a row to two blocks; two groups of twelve warps 112 at
-// 2048 x 65536 bf16, four of six 108, a row to each block (two groups of twelve) 103.  Numbers only: nothing waits for its gradient, so a row to a
-// block, in fewer and larger groups, 2048 x 65536 bf16 46 / 53 with Medium, 1500 x 25000 fp32 the same 28.  Eight words a thread and wait where a thread
-// took four before: numbers only, 2048 x 65536 bf16, 51 -> 47; the gradient of Wide rows keeps four, eight spill.
-constexpr int MOST_NEAR = 1400, MOST_MEDIUM = 7168;      // words of a row
+// fp32) 45 / 62, 1500 (4000 x 6000 fp32) 35 / 42, (4000 x 12000 bf16) 44 / 46, 1700 (4000 x 13600 bf16, a quarter masked) 43 / 42.  Medium / Wide:
+// 2500 words (3000 x 20000 bf16, masked alike) 41 / 48, 5000 (1000 x 40000 bf16) 36 / 39, 6250 (1500 x 25000 fp32) 53 / 59.  Wide / Medium: 8192 words
+// (1000 x 32768 fp32) 46 / 48, (2048 x 65536 bf16) 93 / 105, 12505 (999 x 50021 fp32) 62 / 71.
+// Medium and writing: 20 warps that may have 80 registers; with 24, as for numbers only, the policy's kernels spill (8000 x 16000 bf16 94 / 105,
+// 2000 x 30000 52 / 56, 1500 x 25000 fp32 57 / 61; numbers only, 2000 x 16000 fp32, 29 to the 26 of 24).  Wide and writing: a row to two blocks;
+// two groups of twelve warps 112 at 2048 x 65536 bf16, four of six 108, a row to each block (two groups of twelve) 103.  Numbers only: nothing waits for
+// its gradient, so a row to a block, in fewer and larger groups, 2048 x 65536 bf16 46 / 53 with Medium, 1500 x 25000 fp32 the same 28.  Eight words a
+// thread and wait where a thread took four before: numbers only, 2048 x 65536 bf16, 51 -> 47; the gradient of Wide rows keeps four, eight spill.
+constexpr int MOST_NEAR = 1700, MOST_MEDIUM = 7168;      // words of a row
 typedef Ring<1, 4, 6, 8, 9> MediumReading;
 typedef Ring<1, 4, 5, 8, 10> MediumWriting;
 typedef Ring<1, 3, 8, 8, 6> WideReading;

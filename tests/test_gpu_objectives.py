@@ -182,7 +182,7 @@ def test_policy_loss(dtype, N, V, pitch, offset, temperature, kl, reduction):
 # every number of warps a row and of rows a block that narrow rows have, each group with several rows in turn
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("N,words", [(7200, 40), (7000, 255), (6500, 301), (5500, 341), (5000, 401), (4700, 450), (3700, 513), (2900, 641), (2500, 801), (1900, 902), (1900, 1050),
-                                     (1900, 1151), (1300, 1281), (1300, 1399), (1300, 1401)])
+                                     (1900, 1151), (1300, 1281), (1300, 1399), (1300, 1401), (1100, 1699), (1100, 1701)])
 def test_narrow_rows(dtype, N, words):
     V = words * 16 // torch.finfo(dtype).bits * 8 + 1
     N = N if V < 2000 else N // 2
