@@ -100,6 +100,30 @@ def _dev_i32(x):
     return x.to(torch.int32).contiguous()
 
 
+def _check_batch(config, device, tokens, targets, positions) -> None:
+    """The library is told B alone and walks B x sequence_len entries of every array: a batch of any other shape is refused, before anything
+    is copied or launched."""
+    T = config.sequence_len
+    if tokens.dim() != 2 or tokens.shape[1] != T:
+        raise ValueError(f"tokens must be [B][{T}], as long as the model's sequence_len, not {tuple(tokens.shape)}")
+    for name, x in (("tokens", tokens), ("targets", targets), ("positions", positions)):
+        if x is None:
+            continue
+        if x.shape != tokens.shape:
+            raise ValueError(f"{name} has shape {tuple(x.shape)}, not {tuple(tokens.shape)}")
+        if x.is_cuda and x.device != device:
+            raise ValueError(f"{name} is on {x.device}, not on {device}")
+
+
+def _batch(config, device, tokens, targets, positions):
+    """Tokens, targets and positions (or None) as int32 on the model's device."""
+    import torch
+    if targets is None:
+        raise ValueError("targets is None")
+    _check_batch(config, device, tokens, targets, positions)
+    return [None if x is None else x.to(device, non_blocking=True).to(torch.int32).contiguous() for x in (tokens, targets, positions)]
+
+
 def loss_and_gradient_(params: Params, state: GradientState, layout: Layout, tokens, targets, positions=None,
                        reduction: str = "sum", accumulate: bool = False, sync: bool = True, batch: int = None):
     """`loss_and_gradient!` (ext/FemtoChatEnzymeExt.jl:38-44): fills params.δ (or adds to it, as
@@ -190,6 +214,7 @@ class GPT:
     def token_logprobs(self, tokens, targets, positions=None, temperature: float = 1.0):
         """Log-probabilities [B][T] of the targets (0 where ignored), e.g. under a reference model; see objectives.py."""
         from .objectives import forward_token_logprobs
+        _check_batch(self.config, self.params.theta.device, tokens, targets, positions)
         st = self.state(tokens.shape[0])
         st.refresh_for(self.params.theta)
         return forward_token_logprobs(self.params, st, self.layout, tokens, targets, positions, temperature)

@@ -12,7 +12,7 @@ import math
 from typing import NamedTuple, Optional
 
 from . import _lib
-from .gpt import _dev_i32
+from .gpt import _batch
 
 PREFERENCES = {"sigmoid": 0, "squared": 1}
 
@@ -225,12 +225,13 @@ def preference_loss(logp, offsets, targets0=None, ref_logp=None, kind: str = "si
 # ---- the GPT's steps ----------------------------------------------------------------------------------------------------------------------
 def forward_token_logprobs(params, state, layout, tokens, targets, positions=None, temperature: float = 1.0):
     """Log-probabilities [B][T] that the model gives the targets (0 where ignored), at a temperature: those of answers before an update, or
-    under a reference model.  Tokens, targets and positions as for `loss_and_gradient_`."""
+    under a reference model.  Tokens, targets and positions as for `loss_and_gradient_`: [B][sequence_len]; shorter answers are padded, their targets
+    ignored there."""
     import torch
-    tok, tgt, pos = _dev_i32(tokens), _dev_i32(targets), _dev_i32(positions)
+    tok, tgt, pos = _batch(state.config, params.theta.device, tokens, targets, positions)
     logp = torch.empty(tok.shape, dtype=torch.float32, device=tok.device)
-    _lib.check(_lib.lib().femto_forward_token_logprobs(state.h, _lib.ptr(params.theta), _lib.ptr(tok), _lib.ptr(tgt), _lib.ptr(pos), tok.shape[0],
-                                                       temperature, _lib.ptr(logp), _lib.stream_ptr()))
+    _call(tok.device, "femto_forward_token_logprobs", state.h, _lib.ptr(params.theta), _lib.ptr(tok), _lib.ptr(tgt), _lib.ptr(pos), tok.shape[0],
+          temperature, _lib.ptr(logp))
     return logp
 
 
@@ -240,17 +241,16 @@ def policy_loss_and_gradient_(params, state, layout, tokens, targets, old_logp, 
     """A training step on `policy_loss`: fills params.delta (or adds to it), as `loss_and_gradient_` does for the cross-entropy.  old_logp,
     advantages, ref_logp and weights are [B][T]."""
     import torch
-    tok, tgt, pos = _dev_i32(tokens), _dev_i32(targets), _dev_i32(positions)
+    tok, tgt, pos = _batch(state.config, params.theta.device, tokens, targets, positions)
     f32, device = torch.float32, tok.device
     old_logp, advantages, ref_logp, weights = (_on_device(name, t, f32, tok.shape, device) for name, t in
                                                (("old_logp", old_logp), ("advantages", advantages), ("ref_logp", ref_logp), ("weights", weights)))
     cfg = _policy_config(clip_low, clip_high, kl_coef, temperature, reduction)
     loss, logp = torch.empty(1, dtype=f32, device=device), torch.empty(tok.shape, dtype=f32, device=device)
     n_valid, n_clipped = torch.empty(1, dtype=torch.int32, device=device), torch.empty(1, dtype=torch.int32, device=device)
-    _lib.check(_lib.lib().femto_policy_loss_and_gradient(
-        state.h, _lib.ptr(params.theta), _lib.ptr(params.delta), _lib.ptr(tok), _lib.ptr(tgt), _lib.ptr(pos), tok.shape[0], _lib.ptr(old_logp),
-        _lib.ptr(advantages), _lib.ptr(ref_logp), _lib.ptr(weights), C.byref(cfg), 1 if accumulate else 0, _lib.ptr(loss), _lib.ptr(n_valid),
-        _lib.ptr(n_clipped), _lib.ptr(logp), _lib.stream_ptr()))
+    _call(device, "femto_policy_loss_and_gradient", state.h, _lib.ptr(params.theta), _lib.ptr(params.delta), _lib.ptr(tok), _lib.ptr(tgt), _lib.ptr(pos),
+          tok.shape[0], _lib.ptr(old_logp), _lib.ptr(advantages), _lib.ptr(ref_logp), _lib.ptr(weights), C.byref(cfg), 1 if accumulate else 0,
+          _lib.ptr(loss), _lib.ptr(n_valid), _lib.ptr(n_clipped), _lib.ptr(logp))
     return PolicyStep(loss, n_valid, n_clipped, logp)
 
 
@@ -260,15 +260,14 @@ def preference_loss_and_gradient_(params, state, layout, tokens, targets, offset
     """A training step on `preference_loss`: fills params.delta (or adds to it).  offsets [2 P + 1] (int32) count rows of the flattened [B][T]
     arrays; with one answer a column, chosen and rejected in turn, they are the multiples of T."""
     import torch
-    tok, tgt, pos = _dev_i32(tokens), _dev_i32(targets), _dev_i32(positions)
+    tok, tgt, pos = _batch(state.config, params.theta.device, tokens, targets, positions)
     f32, device = torch.float32, tok.device
     ref_logp = _on_device("ref_logp", ref_logp, f32, tok.shape, device)
     offsets, P = _offsets(offsets, device)
     cfg = _preference_config(kind, beta, margin, label_smoothing, length_normalised, reduction)
     loss, logp = torch.empty(1, dtype=f32, device=device), torch.empty(tok.shape, dtype=f32, device=device)
     pair_losses, ratios = torch.empty(P, dtype=f32, device=device), torch.empty(2 * P, dtype=f32, device=device)
-    _lib.check(_lib.lib().femto_preference_loss_and_gradient(
-        state.h, _lib.ptr(params.theta), _lib.ptr(params.delta), _lib.ptr(tok), _lib.ptr(tgt), _lib.ptr(pos), tok.shape[0], _lib.ptr(ref_logp),
-        _lib.ptr(offsets), P, C.byref(cfg), 1 if accumulate else 0, _lib.ptr(loss), _lib.ptr(pair_losses), _lib.ptr(ratios), _lib.ptr(logp),
-        _lib.stream_ptr()))
+    _call(device, "femto_preference_loss_and_gradient", state.h, _lib.ptr(params.theta), _lib.ptr(params.delta), _lib.ptr(tok), _lib.ptr(tgt), _lib.ptr(pos),
+          tok.shape[0], _lib.ptr(ref_logp), _lib.ptr(offsets), P, C.byref(cfg), 1 if accumulate else 0, _lib.ptr(loss), _lib.ptr(pair_losses),
+          _lib.ptr(ratios), _lib.ptr(logp))
     return PreferenceStep(loss, pair_losses, ratios, logp)

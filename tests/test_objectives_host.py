@@ -112,3 +112,38 @@ def test_steps_refuse_without_a_handle():
     assert L.femto_forward_token_logprobs(None, at(0), at(1), at(2), None, 1, 1.0, at(3), None) == ARG
     assert L.femto_policy_loss_and_gradient(None, at(0), at(1), at(2), at(3), None, 1, at(4), at(5), None, None, c, 0, at(6), at(7), None, None, None) == ARG
     assert L.femto_preference_loss_and_gradient(None, at(0), at(1), at(2), at(3), None, 1, None, at(4), 1, q, 0, at(5), at(6), at(7), None, None) == ARG
+
+
+T = 8
+
+
+def steps_of(tokens, targets, positions=None):
+    """The three steps on a batch; the model is one without a handle, so that a call that is not refused cannot launch anything."""
+    from types import SimpleNamespace
+    params = SimpleNamespace(theta=torch.zeros(16), delta=torch.zeros(16))
+    state = SimpleNamespace(h=None, config=SimpleNamespace(sequence_len=T))
+    rows, offsets = torch.zeros(tokens.shape), torch.tensor([0, 1, 2], dtype=torch.int32)
+    return (lambda: fb.forward_token_logprobs(params, state, None, tokens, targets, positions),
+            lambda: fb.policy_loss_and_gradient_(params, state, None, tokens, targets, rows, rows, positions=positions),
+            lambda: fb.preference_loss_and_gradient_(params, state, None, tokens, targets, offsets, positions=positions))
+
+
+def ids(*shape):
+    return torch.ones(shape, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("tokens,targets,positions,match", [
+    (ids(2, T - 1), ids(2, T - 1), None, "tokens must be"), (ids(2, T + 1), ids(2, T + 1), None, "tokens must be"), (ids(2 * T), ids(2 * T), None, "tokens must be"),
+    (ids(1, 2, T), ids(1, 2, T), None, "tokens must be"), (ids(2, T), ids(2, T - 1), None, "targets has shape"), (ids(2, T), ids(1, T), None, "targets has shape"),
+    (ids(2, T), ids(2 * T), None, "targets has shape"), (ids(2, T), ids(2, T), ids(2, T - 1), "positions has shape"), (ids(2, T), ids(2, T), ids(T), "positions has shape")])
+def test_steps_refuse_a_batch_of_another_shape(tokens, targets, positions, match):
+    """The library reads and writes B x sequence_len entries of every array."""
+    for step in steps_of(tokens, targets, positions):
+        with pytest.raises(ValueError, match=match):
+            step()
+
+
+def test_steps_refuse_no_targets():
+    for step in steps_of(ids(2, T), None):
+        with pytest.raises(ValueError, match="targets is None"):
+            step()
