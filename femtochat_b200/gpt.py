@@ -115,10 +115,10 @@ def _check_batch(config, device, tokens, targets, positions) -> None:
             raise ValueError(f"{name} is on {x.device}, not on {device}")
 
 
-def _batch(config, device, tokens, targets, positions):
+def _batch(config, device, tokens, targets, positions, needs_targets: bool = True):
     """Tokens, targets and positions (or None) as int32 on the model's device."""
     import torch
-    if targets is None:
+    if targets is None and needs_targets:
         raise ValueError("targets is None")
     _check_batch(config, device, tokens, targets, positions)
     return [None if x is None else x.to(device, non_blocking=True).to(torch.int32).contiguous() for x in (tokens, targets, positions)]
@@ -134,7 +134,7 @@ def loss_and_gradient_(params: Params, state: GradientState, layout: Layout, tok
             raise ValueError("pass batch= with raw device pointers")
         ptok, ptgt, ppos, B = tokens, targets, positions, batch
     else:
-        tok, tgt, pos = _dev_i32(tokens), _dev_i32(targets), _dev_i32(positions)
+        tok, tgt, pos = _batch(state.config, params.theta.device, tokens, targets, positions)
         ptok, ptgt, ppos, B = _lib.ptr(tok), _lib.ptr(tgt), _lib.ptr(pos), tok.shape[0]
     _lib.check(_lib.lib().femto_loss_and_gradient(
         state.h, _lib.ptr(params.theta), _lib.ptr(params.delta), ptok, ptgt, ppos, B,
@@ -149,6 +149,7 @@ def loss_and_gradient_host_(params: Params, state: GradientState, tokens_pinned,
                             reduction: str = "sum", accumulate: bool = False):
     """End-to-end call with HOST int32 [B][T] buffers: host→device copies, the step, and the read
     back of (loss, n_valid) all happen inside the library call."""
+    _check_batch(state.config, None, tokens_pinned, targets_pinned, positions_pinned)
     B = tokens_pinned.shape[0]
     loss, nv = C.c_float(0), C.c_int32(0)
     _lib.check(_lib.lib().femto_loss_and_gradient_host(
@@ -196,7 +197,7 @@ class GPT:
         [B][T][vocab_size] tensor, the reference's (V,T,B) array (src/gpt.jl:129-170)."""
         if targets is None:
             return self.logits(tokens, positions)
-        tok, tgt, pos = _dev_i32(tokens), _dev_i32(targets), _dev_i32(positions)
+        tok, tgt, pos = _batch(self.config, self.params.theta.device, tokens, targets, positions)
         st = self.state(tok.shape[0])
         st.refresh_for(self.params.theta)
         if reduction == "none":   # per-token losses [B][T] (src/gpt.jl:191-193)
@@ -221,7 +222,7 @@ class GPT:
 
     def logits(self, tokens, positions=None):
         import torch
-        tok, pos = _dev_i32(tokens), _dev_i32(positions)
+        tok, _, pos = _batch(self.config, self.params.theta.device, tokens, None, positions, needs_targets=False)
         st = self.state(tok.shape[0])
         st.refresh_for(self.params.theta)
         out = torch.empty(tok.shape[0], tok.shape[1], self.config.vocab_size, device="cuda", dtype=torch.float32)

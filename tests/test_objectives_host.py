@@ -143,6 +143,27 @@ def test_steps_refuse_a_batch_of_another_shape(tokens, targets, positions, match
             step()
 
 
+@pytest.mark.parametrize("tokens,targets,positions,match", [
+    (ids(2, T - 1), ids(2, T - 1), None, "tokens must be"), (ids(2, T + 1), ids(2, T + 1), None, "tokens must be"), (ids(2, T), ids(2, T - 1), None, "targets has shape"),
+    (ids(2, T), ids(2, T), ids(2, T - 1), "positions has shape")])
+def test_model_calls_refuse_a_batch_of_another_shape(tokens, targets, positions, match):
+    """As above: the losses of all tokens and the logits have B x sequence_len entries too."""
+    from types import SimpleNamespace
+    params = SimpleNamespace(theta=torch.zeros(16), delta=torch.zeros(16))
+    config = SimpleNamespace(sequence_len=T, vocab_size=9)
+    state = SimpleNamespace(h=None, config=config)
+    model = fb.GPT(params, config, None)
+    model.state = lambda B: pytest.fail("the batch was not refused")
+    calls = [lambda: fb.loss_and_gradient_(params, state, None, tokens, targets, positions), lambda: model(tokens, targets, positions),
+             lambda: model(tokens, targets, positions, reduction="none"), lambda: model.token_logprobs(tokens, targets, positions),
+             lambda: fb.loss_and_gradient_host_(params, state, tokens, targets, positions)]
+    if "targets" not in match:
+        calls.append(lambda: model.logits(tokens, positions))
+    for call in calls:
+        with pytest.raises(ValueError, match=match):
+            call()
+
+
 def test_steps_refuse_no_targets():
     for step in steps_of(ids(2, T), None):
         with pytest.raises(ValueError, match="targets is None"):
