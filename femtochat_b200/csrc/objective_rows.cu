@@ -128,6 +128,12 @@ template <typename T> __device__ __forceinline__ int word_of_target(const RowSha
   const int v = (t - r.head) / VecN<T>::n;
   return t >= r.head && v < r.nvec ? v : -1;
 }
+// Takes the target's element out of its word in shared memory, by the thread that reads the word, ahead of its reading.  (In registers, a selection for every
+// word in flight: 8000 x 16000 in bf16, gradient, 97 us for 87.)  The next copy to this memory is another proxy's.
+template <typename T> __device__ __forceinline__ void take_out(uint4* word, int e) {
+  reinterpret_cast<T*>(word)[e] = from_f<T>(-INFINITY);
+  fence_proxy_async();
+}
 
 // Adds pairs of logits to a thread's sums.
 template <bool ENTROPY> struct Adder {
@@ -149,7 +155,8 @@ template <bool ENTROPY> struct Adder {
   }
 };
 
-// A thread's statistics, relative to a maximum of its own that grows a few times in a row.
+// A thread's statistics, relative to a maximum of its own that grows a few times in a row.  They are those of the row without its target, which
+// with_token() adds.
 template <typename T, bool ENTROPY> struct Running {
   RowStats s;
   Exponent x;
@@ -265,18 +272,40 @@ template <RowsMode MODE> __device__ __forceinline__ void end_behind_the_count(co
   if (MODE == POLICY && p.n_valid) pdl_wait();
 }
 
-// The row's numbers go out (where `write`), and (g, h) of its gradient and the target's logit come back.  scale: 0 until the rows with a target have been counted.
+// What the gradient of a row needs: dz_j = 2^u_j (k + h u_j) for j other than the target, u_j = c (z_j - m), and the target's.
+struct RowSlope {
+  float m = 0.f, k = 0.f, h = 0.f, target = 0.f;
+};
+// dz_j = g (1[j = t] - p_j) - y p_j (u_j - a / l), where log p + H = ln2 (u - a / l) and y has the factor ln2.  At the target 1 - p comes from the
+// other tokens' part of l.  A row without a distribution has no gradient.
+template <bool ENTROPY> __device__ __forceinline__ RowSlope row_slope(const TokenStats& s, float g, float y, float c) {
+  RowSlope r;
+  if (s.all.l == 0.f) return r;
+  const float inv_l = 1.f / s.all.l, mean = ENTROPY ? s.all.a / s.all.l : 0.f;
+  r.m = s.all.m;
+  r.k = -(ENTROPY ? g - y * mean : g) * inv_l;
+  r.h = ENTROPY ? -y * inv_l : 0.f;
+  r.target = g * (s.others * inv_l);
+  if (ENTROPY) {
+    const float u = fmaxf((s.z - s.all.m) * c, LEAST_U);
+    r.target += exp2_fast(u) * inv_l * (y * (mean - u));
+  }
+  return r;
+}
+// The row's numbers go out (where `write`), and what its gradient needs comes back, from the statistics of the tokens other than its target.
+// scale: 0 until the rows with a target have been counted.
 template <RowsMode MODE, bool ENTROPY>
-__device__ __forceinline__ float4 row_result(const RowsArgs& p, long long row, const RowStats& s, const RowNumbers& k, float& scale, bool write) {
+__device__ __forceinline__ RowSlope row_result(const RowsArgs& p, long long row, const RowStats& others, const RowNumbers& k, float& scale, bool write) {
+  const TokenStats s = with_token<ENTROPY>(others, k.z, p.c);
   if (MODE == LOGPROBS) {
     if (write) {
-      p.logp[row] = (float)log_prob(s, k.z, p.inv_t64);
+      p.logp[row] = (float)log_prob(s, p.inv_t64);
       if (ENTROPY) p.ent[row] = entropy(s);
     }
-    return make_float4(0.f, 0.f, 0.f, 0.f);
+    return RowSlope();
   }
-  if (MODE == GRADIENT) return make_float4(k.x[0] * p.inv_t, ENTROPY ? k.x[1] * p.inv_t * (float)LN2 : 0.f, k.z, 0.f);
-  const double lp = log_prob(s, k.z, p.inv_t64);
+  if (MODE == GRADIENT) return row_slope<ENTROPY>(s, k.x[0] * p.inv_t, ENTROPY ? k.x[1] * p.inv_t * (float)LN2 : 0.f, p.c);
+  const double lp = log_prob(s, p.inv_t64);
   float loss, slope;
   policy_token(p.term, lp, k.x[0], k.x[1], k.x[2], k.x[3], &loss, &slope);
   if (write) { p.token_losses[row] = loss; p.logp[row] = (float)lp; }
@@ -284,27 +313,21 @@ __device__ __forceinline__ float4 row_result(const RowsArgs& p, long long row, c
     pdl_wait();
     scale = 1.f / (float)*reinterpret_cast<const volatile int*>(p.n_valid);
   }
-  return make_float4((p.n_valid ? slope * scale : slope) * p.inv_t, 0.f, k.z, 0.f);
+  return row_slope<false>(s, (p.n_valid ? slope * scale : slope) * p.inv_t, 0.f, p.c);
 }
 template <RowsMode MODE, bool ENTROPY> __device__ __forceinline__ void row_without_target(const RowsArgs& p, long long row) {
   if (MODE == LOGPROBS) { p.logp[row] = 0.f; if (ENTROPY) p.ent[row] = 0.f; }
   if (MODE == POLICY) p.logp[row] = p.token_losses[row] = 0.f;
 }
 
-// dz_j = g (1[j = t] - p_j) - h p_j (u_j - a / l), where log p + H = ln2 (u - a / l).  A row without a distribution has no gradient.
 template <typename T, bool ENTROPY> struct Slope {
   static constexpr int n = VecN<T>::n;
   Exponent x;
   uint64_t k2, h2;
   float at_target;
   int t;
-  __device__ __forceinline__ Slope(const RowStats& s, float4 gh, float c, int target) : x(s.m, c), t(target) {
-    const bool none = s.l == 0.f;
-    const float inv_l = 1.f / s.l;
-    const float k = none ? 0.f : -(ENTROPY ? gh.x - gh.y * (s.a / s.l) : gh.x) * inv_l, h = none ? 0.f : -gh.y * inv_l;
-    k2 = pack2(k, k); h2 = pack2(h, h);
-    at_target = none ? 0.f : gh.x;
-  }
+  __device__ __forceinline__ Slope(const RowSlope& s, float c, int target)
+      : x(s.m, c), k2(pack2(s.k, s.k)), h2(pack2(s.h, s.h)), at_target(s.target), t(target) {}
   __device__ __forceinline__ uint64_t of(uint64_t z2) const {
     float u0, u1;
     x.of(z2, u0, u1);
@@ -329,15 +352,13 @@ template <typename T, bool ENTROPY> struct Slope {
   }
   // The target's element, over what stands there of its word, by the thread that stored the word.  (A comparison with the target at every word was
   // a third of the instructions.)
-  __device__ __forceinline__ void store_target(T* d, float z) const {
-    float lo, hi;
-    unpack2(of(pack2(z, z)), lo, hi);
-    d[t] = from_f<T>(lo + at_target);
-  }
+  // The target's element, over what stands there of its word, by the thread that stored the word.  (A comparison with the target at every word was
+  // a third of the instructions.)
+  __device__ __forceinline__ void store_target(T* d) const { d[t] = from_f<T>(at_target); }
   __device__ __forceinline__ void store_edge(T* d, int at, float z) const {
     float lo, hi;
     unpack2(of(pack2(z, z)), lo, hi);
-    d[at] = from_f<T>(lo + (at == t ? at_target : 0.f));
+    d[at] = from_f<T>(at == t ? at_target : lo);
   }
 };
 // Words of the gradient may be stored whole where they lie as the logits' do.
@@ -349,16 +370,17 @@ __device__ __forceinline__ void group_barrier(int id, int threads) { asm volatil
 
 // ---- few rows -----------------------------------------------------------------------------------------------------------------------------------
 // A cluster of blocks holds a row in registers, NV words a thread; the statistics of all its warps go to every block's shared memory.  There is
-// little to overlap: what counts is that a row is brought by many multiprocessors at once (1 x 65536 in fp32: 3.0 us, of which a launch with
-// nothing to do is 2).
+// little to overlap: what counts is that a row is brought by many multiprocessors at once (1 x 65536 in fp32: 3.1 us, of which a launch with
+// nothing to do is 2).  Four blocks a multiprocessor in fp32: left to the compiler, 220 rows of 50021 take 32 us for 24 (gradient, three blocks), 150 of 8000
+// 4.2 for 3.7 (numbers only, fewer words on their way).
 constexpr int FEW_WARPS = 8, FEW_WORDS = 8;
 
 template <typename T, RowsMode MODE, bool STORE, bool ENTROPY, int NV>
-__global__ void __launch_bounds__(32 * FEW_WARPS) k_rows_few(const RowsArgs p) {
+__global__ void __launch_bounds__(32 * FEW_WARPS, sizeof(T) == 4 && NV == FEW_WORDS ? 4 : 0) k_rows_few(const RowsArgs p) {
   pdl_trigger();
   constexpr int threads = 32 * FEW_WARPS, pitch = MOST_CLUSTER * FEW_WARPS;
   __shared__ float part[3 * pitch];
-  __shared__ float4 slope_s;
+  __shared__ RowSlope slope_s;
   const int C = (int)cluster_size(), rank = (int)cluster_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");      // this block runs: its shared memory may be written
   const long long row = blockIdx.x / C;
@@ -367,7 +389,9 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) k_rows_few(const RowsArgs p) {
   T* d = reinterpret_cast<T*>(p.dlogits) + row * p.ldd;
   const RowShape r = row_shape<T>(STORE && t < 0 ? d : z, p.V);      // the logits', or, where they are not read, the gradient's
   const int per = (r.nvec + C - 1) / C, first = min(r.nvec, rank * per), last = min(r.nvec, first + per);
-  const int at = rank == 0 ? edge_of<T>(r, tid) : -1;
+  // the word that holds the target goes with the elements outside the words, one to a thread
+  const int vt = t >= 0 ? word_of_target<T>(r, t) : -1;
+  const int at = rank != 0 ? -1 : vt >= 0 && tid >= 8 && tid < 8 + VecN<T>::n ? r.head + vt * VecN<T>::n + tid - 8 : edge_of<T>(r, tid);
   if (t < 0) {
     asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
     if (rank == 0 && tid == 0) row_without_target<MODE, ENTROPY>(p, row);
@@ -383,14 +407,15 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) k_rows_few(const RowsArgs p) {
 #pragma unroll
   for (int k = 0; k < NV; k++) {
     const int v = first + k * threads + tid;
-    q[k] = load_word(words + v, v < last, Word<T>::LEAST);
+    q[k] = load_word(words + v, v < last && v != vt, Word<T>::LEAST);
   }
   RowNumbers numbers;
   if (warp == 0) numbers = row_numbers<T, MODE, ENTROPY>(p, row, z, t);      // in every block: each works the slopes out for itself
-  const float edge = at >= 0 ? to_f<T>(z[at]) : -INFINITY;
-  Running<T, ENTROPY> run(at >= 0, edge, p.c);
+  const bool there = at >= 0 && at != t;
+  const float edge = there ? to_f<T>(z[at]) : -INFINITY;
+  Running<T, ENTROPY> run(there, edge, p.c);
   run.add(q, p.c);
-  RowStats s = run.of_warp(p.c);
+  const RowStats s = run.of_warp(p.c);
   asm volatile("barrier.cluster.wait.acquire;" ::: "memory");      // all blocks run
   const int slot = rank * FEW_WARPS + warp;
   if (lane < C) {
@@ -399,26 +424,22 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) k_rows_few(const RowsArgs p) {
   }
   asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
   if (!STORE && (rank != 0 || warp != 0)) return;
-  s = merged_parts<ENTROPY>(part, pitch, FEW_WARPS * C, p.c);
   if (warp == 0) {
     float scale = 0.f;
-    const float4 gh = row_result<MODE, ENTROPY>(p, row, s, numbers, scale, rank == 0 && lane == 0);
-    if (lane == 0) slope_s = gh;
+    const RowSlope given = row_result<MODE, ENTROPY>(p, row, merged_parts<ENTROPY>(part, pitch, FEW_WARPS * C, p.c), numbers, scale, rank == 0 && lane == 0);
+    if (lane == 0) slope_s = given;
   }
   if (!STORE) return;
   __syncthreads();
-  const float4 gh = slope_s;
-  const Slope<T, ENTROPY> slope(s, gh, p.c, t);
+  const Slope<T, ENTROPY> slope(slope_s, p.c, t);
   const bool same = same_phase(z, d);
 #pragma unroll
   for (int k = 0; k < NV; k++) {
     const int v = first + k * threads + tid;
-    if (v >= last) continue;
+    if (v >= last || v == vt) continue;
     if (same) reinterpret_cast<uint4*>(d + r.head)[v] = slope.word(q[k]);
     else slope.scatter(d + r.head + v * VecN<T>::n, q[k]);
   }
-  const int vt = word_of_target<T>(r, t);
-  if (vt >= first && vt < last && (vt - first) % threads == tid) slope.store_target(d, gh.z);
   if (at >= 0) slope.store_edge(d, at, edge);
 }
 
@@ -434,7 +455,7 @@ __global__ void __launch_bounds__(32 * NEAR_WARPS, 3) k_rows_near(const RowsArgs
   extern __shared__ __align__(128) uint4 ring[];
   __shared__ uint64_t full[NEAR_WARPS][2];
   __shared__ float part[2][3][NEAR_WARPS];
-  __shared__ float4 slope_s[NEAR_WARPS];
+  __shared__ RowSlope slope_s[NEAR_WARPS];
   __shared__ int abort_flag;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = warp / W, groups = blockDim.x / (32 * W);
   const int threads = W * 32, tid = threadIdx.x - group * threads, first_warp = group * W;
@@ -481,10 +502,14 @@ __global__ void __launch_bounds__(32 * NEAR_WARPS, 3) k_rows_near(const RowsArgs
     if (!asked && tid == 0 && alive) ask(row, which);      // the row before the last but one, which this buffer held, is done: a barrier lies between
     LaneNumbers numbers;
     if (warp == first_warp) numbers = lane_numbers<T, MODE, ENTROPY>(p, row, z, t);
-    const float edge = at >= 0 ? to_f<T>(z[at]) : -INFINITY;
-    Running<T, ENTROPY> run(at >= 0, edge, p.c);
-    const uint4* words = buffer + (size_t)which * pitch;
+    const bool there = at >= 0 && at != t;
+    const float edge = there ? to_f<T>(z[at]) : -INFINITY;
+    Running<T, ENTROPY> run(there, edge, p.c);
+    const int vt = word_of_target<T>(r, t);
+    const bool own = vt >= 0 && (vt & (threads - 1)) == tid;      // the target's word is this thread's (W is a power of two)
+    uint4* words = buffer + (size_t)which * pitch;
     alive = alive && mbar_wait(&full[group][which], parity, &abort_flag, &g_rows_status);
+    if (own) take_out<T>(words + vt, (t - r.head) % VecN<T>::n);
     int v0 = 0;
     for (; v0 + NEAR_WORDS * threads <= r.nvec; v0 += NEAR_WORDS * threads) {
       uint4 q[NEAR_WORDS];
@@ -498,20 +523,20 @@ __global__ void __launch_bounds__(32 * NEAR_WARPS, 3) k_rows_near(const RowsArgs
       float* mine = part[which][0];
       if (lane == 0) { mine[warp] = s.m; mine[NEAR_WARPS + warp] = s.l; if (ENTROPY) mine[2 * NEAR_WARPS + warp] = s.a; }
       group_barrier(1 + group, threads);
-      if (STORE || warp == first_warp) s = merged_parts<ENTROPY>(mine + first_warp, NEAR_WARPS, W, p.c);
+      if (warp == first_warp) s = merged_parts<ENTROPY>(mine + first_warp, NEAR_WARPS, W, p.c);
     } else __syncwarp();
     // all of the group are done with the row before this one: its buffer is free
     asked = t_next >= 0 && t_next < p.V;
     if (asked && tid == 0 && alive) ask(row + step, which ^ 1);
-    float4 gh = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (warp == first_warp) gh = row_result<MODE, ENTROPY>(p, row, s, numbers.all(), scale, lane == 0);
+    RowSlope given;
+    if (warp == first_warp) given = row_result<MODE, ENTROPY>(p, row, s, numbers.all(), scale, lane == 0);
     if (!STORE) continue;
     if (W > 1) {
-      if (warp == first_warp && lane == 0) slope_s[group] = gh;
+      if (warp == first_warp && lane == 0) slope_s[group] = given;
       group_barrier(1 + group, threads);
-      gh = slope_s[group];
+      given = slope_s[group];
     }
-    const Slope<T, ENTROPY> slope(s, gh, p.c, t);
+    const Slope<T, ENTROPY> slope(given, p.c, t);
     const bool same = same_phase(z, d);
     if (same) {
       uint4* out = reinterpret_cast<uint4*>(d + r.head);
@@ -530,8 +555,7 @@ __global__ void __launch_bounds__(32 * NEAR_WARPS, 3) k_rows_near(const RowsArgs
     } else {
       for (int v = tid; v < r.nvec; v += threads) slope.scatter(d + r.head + v * VecN<T>::n, words[v]);
     }
-    const int vt = word_of_target<T>(r, t);
-    if (vt >= 0 && vt % threads == tid) slope.store_target(d, gh.z);
+    if (own) slope.store_target(d);
     if (at >= 0) slope.store_edge(d, at, edge);
   }
   end_behind_the_count<MODE>(p);
@@ -584,8 +608,7 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
   extern __shared__ __align__(128) uint4 ring[];
   __shared__ uint64_t full[GROUPS][SLOTS], empty[SLOTS];
   __shared__ float part[GROUPS][3][GROUP_WARPS];
-  __shared__ float4 slope_s[GROUPS];
-  __shared__ RowStats stats_s[GROUPS];
+  __shared__ RowSlope slope_s[GROUPS];
   __shared__ uint64_t met[GROUPS][2];      // a group's statistics of a row from the other block of the cluster, two rows in turn
   __shared__ __align__(16) float4 theirs[GROUPS][2];
   __shared__ int abort_flag;
@@ -711,13 +734,18 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
     const int at = rank == 0 ? edge_of<T>(r, tid) : -1;
     RowNumbers numbers;
     if (gwarp == 0) numbers = row_numbers<T, MODE, ENTROPY>(p, row, z, t);
-    const float edge = at >= 0 ? to_f<T>(z[at]) : -INFINITY;
+    const bool there = at >= 0 && at != t;
+    const float edge = there ? to_f<T>(z[at]) : -INFINITY;
 
-    Running<T, ENTROPY> run(at >= 0, edge, p.c);
+    Running<T, ENTROPY> run(there, edge, p.c);
+    const int vt = word_of_target<T>(r, t) - from_word;
+    const bool own = vt >= 0 && vt < nvec && vt % CHUNK % GROUP_THREADS == tid;      // the target's word is this thread's
+    const int target_chunk = own ? vt / CHUNK : -1;
     const int first_slot = (int)((long long)mine * (chunks + (STORE ? again : 0)) % SLOTS);
     int slot = first_slot;
     for (int c = 0; c < chunks; c++, slot = next_slot(slot)) {
       wait_full(slot);
+      if (c == target_chunk) take_out<T>(ring + slot * CHUNK + vt % CHUNK, (t - r.head) % VecN<T>::n);
       const uint4* from = ring + slot * CHUNK + tid;
       auto done = [&]() {
         if (STORE && c >= again) return;
@@ -755,15 +783,13 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
         other.m = o.x; other.l = o.y; other.a = o.z;
         s = rank == 0 ? merged<ENTROPY>(s, other, p.c) : merged<ENTROPY>(other, s, p.c);      // the same order, the same bits, in both
       }
-      const float4 gh = row_result<MODE, ENTROPY>(p, row, s, numbers, scale, rank == 0 && lane == 0);
-      if (STORE && lane == 0) { slope_s[group] = gh; stats_s[group] = s; }
+      const RowSlope given = row_result<MODE, ENTROPY>(p, row, s, numbers, scale, rank == 0 && lane == 0);
+      if (STORE && lane == 0) slope_s[group] = given;
     }
     rows++;
     group_barrier(1 + group, GROUP_THREADS);      // the parts are read, the slopes are there
     if (!STORE) continue;
-    s = stats_s[group];
-    const float4 gh = slope_s[group];
-    const Slope<T, ENTROPY> slope(s, gh, p.c, t);
+    const Slope<T, ENTROPY> slope(slope_s[group], p.c, t);
     const bool same = same_phase(z, d);
     slot = (first_slot + again) % SLOTS;
     for (int i = 0; i < chunks; i++, slot = next_slot(slot)) {
@@ -783,8 +809,7 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[slot]);
     }
-    const int vt = word_of_target<T>(r, t) - from_word;
-    if (vt >= 0 && vt < nvec && vt % CHUNK % GROUP_THREADS == tid) slope.store_target(d, gh.z);
+    if (own) slope.store_target(d);
     if (at >= 0) slope.store_edge(d, at, edge);
   }
   end_behind_the_count<MODE>(p);

@@ -51,12 +51,40 @@ __device__ __forceinline__ double log_sum(float l) {
   const int bits = __float_as_int(l), k = (bits - 0x3f3504f3) >> 23;      // sqrt(1/2)
   return LN2 * k + (double)logf(__int_as_float(bits - (k << 23)));
 }
-// log p of a logit z; a row without any logit above -inf (l = 0) has no distribution: -inf.
-__device__ __forceinline__ double log_prob(const RowStats& s, float z, double inv_t) {
-  return s.l == 0.f ? -(double)INFINITY : ((double)z - (double)s.m) * inv_t - log_sum(s.l);
+// The statistics of a row's other tokens, with its own token's logit z added.  The others' part of l is kept beside the sum: of a token that the
+// model is all but sure of, 1 - p = others / l and -log p = log(1 + others) are small numbers, of which the rounding of l = 1 + others leaves little
+// (1 - p = 1e-6: 6 %).
+struct TokenStats {
+  RowStats all;
+  float others, z;
+};
+template <bool ENTROPY> __device__ __forceinline__ TokenStats with_token(const RowStats& others, float z, float c) {
+  TokenStats s;
+  const float d = fminf(fabsf(z - others.m) * c, -LEAST_U), f = exp2_fast(-d);
+  float own = z == -INFINITY ? 0.f : 1.f + (z - z), own_a = 0.f;      // NaN and +inf give NaN
+  s.z = z; s.others = others.l; s.all.a = others.a;
+  if (z >= others.m) {
+    s.others = others.l * f;
+    if (ENTROPY) s.all.a = f * fmaf(-others.l, d, others.a);
+  } else {
+    own *= f;
+    own_a = -own * d;
+  }
+  s.all.m = fmaxf(others.m, z);
+  s.all.l = s.others + own;
+  if (ENTROPY) s.all.a += own_a;
+  return s;
 }
-__device__ __forceinline__ float entropy(const RowStats& s) {
-  return s.l == 0.f ? 0.f : (float)(log_sum(s.l) - LN2 * (double)s.a / (double)s.l);
+// log l, where the token is the row's maximum and its others are few from what they are
+__device__ __forceinline__ double log_total(const TokenStats& s) {
+  return s.z == s.all.m && s.others < 0.5f ? (double)log1pf(s.others) : log_sum(s.all.l);
+}
+// log p of the token; a row without any logit above -inf (l = 0) has no distribution: -inf.
+__device__ __forceinline__ double log_prob(const TokenStats& s, double inv_t) {
+  return s.all.l == 0.f ? -(double)INFINITY : ((double)s.z - (double)s.all.m) * inv_t - log_total(s);
+}
+__device__ __forceinline__ float entropy(const TokenStats& s) {
+  return s.all.l == 0.f ? 0.f : (float)(log_total(s) - LN2 * (double)s.all.a / (double)s.all.l);
 }
 
 // ---- clusters ----------------------------------------------------------------------------------------------------------------------------------

@@ -589,3 +589,46 @@ def test_tensors_as_the_model_gives_them():
     assert r.dlogits.shape == z3.shape and torch.equal(r.dlogits.flatten(0, 1), want.dlogits) and torch.equal(r.loss, want.loss)
     one = fb.token_logprobs(z[0], t[0])
     assert one.logp.shape == () and torch.equal(one.logp, fb.token_logprobs(z, t).logp[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,V", [(7, 300), (9, 9001), (5, 66001), (300, 37), (300, 701), (400, 4003), (300, 9001), (310, 20011), (300, 60007), (300, 140001)])
+@pytest.mark.parametrize("offset,temperature", [(0, 1.0), (3, 0.75)])
+def test_confident_tokens(dtype, N, V, offset, temperature):
+    """Of a token that the model is all but sure of, 1 - p and -log p are small numbers, right to some roundings of their own.  With q the sum of the
+    others' exponentials over the token's: q has the relative error of l above, and that of the scale's rounding, 2^-24 of the exponent (|u| < 64, so
+    2^-24 48); with_token() takes one more exponential, log1p, the quotient and the products some roundings: `rel` for each number that is made of q."""
+    z, t = make(N, V, dtype, 5, offset, seed=21)
+    g = torch.Generator(device="cuda").manual_seed(V + N)
+    t = torch.randint(0, V, (N,), device="cuda", generator=g).int()
+    t[:4] = torch.tensor([0, V - 1, 1, V // 2], device="cuda", dtype=torch.int32)
+    rows = torch.arange(N, device="cuda")
+    s = z.double() / temperature
+    s[rows, t.long()] = -math.inf
+    left = torch.logspace(-7, -3, N, device="cuda", dtype=torch.float64)[torch.randperm(N, device="cuda", generator=g)]      # 1 - p
+    z[rows, t.long()] = (temperature * (torch.logsumexp(s, 1) + torch.log1p(-left) - left.log())).to(dtype)
+    lp, h, ls = reference(z, t, temperature)
+    q = torch.where(torch.nn.functional.one_hot(t.long(), V) > 0, 0.0, ls.exp()).sum(1)      # 1 - p
+    assert float(q.max()) < 0.01
+    rel = slack(V) + 2.0 ** -24 * 48 + 2.0 ** -20
+    r = fb.token_logprobs(z, t, temperature=temperature, entropy=True)
+    near(r.logp, lp, rel * lp.abs(), "logp")
+    near(r.entropy, h, 3 * rel * h, "entropy")
+    near(fb.token_logprobs(z, t, temperature=temperature).logp, r.logp, 0, "logp without the entropy")
+    dlogp, dent = torch.randn(2, N, device="cuda", generator=g)
+    inv, at = 1 / temperature, (rows, t.long())
+    d = fb.token_logprobs_gradient(z, t, dlogp, temperature=temperature)[at]
+    want = inv * dlogp.double() * q
+    near(d, want, (half_step(dtype) * 1.01 + rel) * want.abs(), "at the target")
+    d = fb.token_logprobs_gradient(z, t, dlogp, dentropy=dent, temperature=temperature)[at]
+    second = inv * dent.double() * lp.exp() * (lp + h)
+    near(d, want - second, half_step(dtype) * 1.01 * (want - second).abs() + 3 * rel * (want.abs() + inv * dent.double().abs() * h), "with the entropy")
+    # ratios of 1: the slope by log p is -A, right to the error of log p and of the exponential
+    A = torch.randn(N, device="cuda", generator=g)
+    keep = z.clone()
+    for out in (None, z):
+        got = fb.policy_loss(z, t, r.logp, A, temperature=temperature, out=out).dlogits[at]
+        want = -inv * A.double() * q
+        near(got, want, (half_step(dtype) * 1.01 + 2 * rel) * want.abs(), "policy")
+    z.copy_(keep)
+    assert status() == 0
