@@ -309,6 +309,7 @@ __device__ __forceinline__ RowSlope row_result(const RowsArgs& p, long long row,
   float loss, slope;
   policy_token(p.term, lp, k.x[0], k.x[1], k.x[2], k.x[3], &loss, &slope);
   if (write) { p.token_losses[row] = loss; p.logp[row] = (float)lp; }
+  if (k.x[3] == 0.f) return RowSlope();      // whatever the logits are
   if (p.n_valid && scale == 0.f) {      // a kernel of the same call counts the targets beside the first rows
     pdl_wait();
     scale = 1.f / (float)*reinterpret_cast<const volatile int*>(p.n_valid);
@@ -320,32 +321,36 @@ template <RowsMode MODE, bool ENTROPY> __device__ __forceinline__ void row_witho
   if (MODE == POLICY) p.logp[row] = p.token_losses[row] = 0.f;
 }
 
-template <typename T, bool ENTROPY> struct Slope {
+// POLICY: rows with k = 0 (clipped, or of weight 0) have zeros, whatever their logits are.
+template <typename T, bool ENTROPY, bool POLICY> struct Slope {
   static constexpr int n = VecN<T>::n;
   Exponent x;
   uint64_t k2, h2;
   float at_target;
   int t;
+  bool zero;
   __device__ __forceinline__ Slope(const RowSlope& s, float c, int target)
-      : x(s.m, c), k2(pack2(s.k, s.k)), h2(pack2(s.h, s.h)), at_target(s.target), t(target) {}
+      : x(s.m, c), k2(pack2(s.k, s.k)), h2(pack2(s.h, s.h)), at_target(s.target), t(target), zero(POLICY && s.k == 0.f) {}
   __device__ __forceinline__ uint64_t of(uint64_t z2) const {
     float u0, u1;
     x.of(z2, u0, u1);
     const uint64_t e2 = pack2(exp2_fast(u0), exp2_fast(u1));
     return mul2(e2, ENTROPY ? fma2(h2, pack2(fmaxf(u0, LEAST_U), fmaxf(u1, LEAST_U)), k2) : k2);
   }
+  // (Rows of zeros take a loop of their own: with the question at every word the policy's kernel for medium rows took 56 us for 53.)
   __device__ __forceinline__ uint4 word(const uint4& q) const {
     uint4 o;
 #pragma unroll
     for (int i = 0; i < n / 2; i++) Word<T>::put(o, i, of(Word<T>::get(q, i)));
     return o;
   }
+  __device__ __forceinline__ uint4 word_or_zeros(const uint4& q) const { return zero ? make_uint4(0, 0, 0, 0) : word(q); }
   // a word that does not lie in the gradient as it does in the logits
   __device__ __forceinline__ void scatter(T* d, const uint4& q) const {
 #pragma unroll
     for (int i = 0; i < n / 2; i++) {
       float lo, hi;
-      unpack2(of(Word<T>::get(q, i)), lo, hi);
+      unpack2(zero ? 0 : of(Word<T>::get(q, i)), lo, hi);
       d[2 * i] = from_f<T>(lo);
       d[2 * i + 1] = from_f<T>(hi);
     }
@@ -357,7 +362,7 @@ template <typename T, bool ENTROPY> struct Slope {
   __device__ __forceinline__ void store_target(T* d) const { d[t] = from_f<T>(at_target); }
   __device__ __forceinline__ void store_edge(T* d, int at, float z) const {
     float lo, hi;
-    unpack2(of(pack2(z, z)), lo, hi);
+    unpack2(zero ? 0 : of(pack2(z, z)), lo, hi);
     d[at] = from_f<T>(at == t ? at_target : lo);
   }
 };
@@ -431,13 +436,13 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, sizeof(T) == 4 && NV == FEW_WO
   }
   if (!STORE) return;
   __syncthreads();
-  const Slope<T, ENTROPY> slope(slope_s, p.c, t);
+  const Slope<T, ENTROPY, MODE == POLICY> slope(slope_s, p.c, t);
   const bool same = same_phase(z, d);
 #pragma unroll
   for (int k = 0; k < NV; k++) {
     const int v = first + k * threads + tid;
     if (v >= last || v == vt) continue;
-    if (same) reinterpret_cast<uint4*>(d + r.head)[v] = slope.word(q[k]);
+    if (same) reinterpret_cast<uint4*>(d + r.head)[v] = slope.word_or_zeros(q[k]);
     else slope.scatter(d + r.head + v * VecN<T>::n, q[k]);
   }
   if (at >= 0) slope.store_edge(d, at, edge);
@@ -536,14 +541,14 @@ __global__ void __launch_bounds__(32 * NEAR_WARPS, 3) k_rows_near(const RowsArgs
       group_barrier(1 + group, threads);
       given = slope_s[group];
     }
-    const Slope<T, ENTROPY> slope(given, p.c, t);
+    const Slope<T, ENTROPY, MODE == POLICY> slope(given, p.c, t);
     const bool same = same_phase(z, d);
     if (same) {
       uint4* out = reinterpret_cast<uint4*>(d + r.head);
       // Four words at a time while every thread has as many, and one by one from there: unrolled with a remainder for each thread, the code of
       // 24 warps that are at different places of it took more time than its instructions (30000 x 1000 in bf16: 38 -> 32 us).
       int v = 0;
-      for (; v + 4 * threads <= r.nvec; v += 4 * threads) {
+      for (; !slope.zero && v + 4 * threads <= r.nvec; v += 4 * threads) {
         uint4 q[4];
 #pragma unroll
         for (int h = 0; h < 4; h++) q[h] = words[v + h * threads + tid];
@@ -551,7 +556,7 @@ __global__ void __launch_bounds__(32 * NEAR_WARPS, 3) k_rows_near(const RowsArgs
         for (int h = 0; h < 4; h++) out[v + h * threads + tid] = slope.word(q[h]);
       }
 #pragma unroll 1
-      for (v += tid; v < r.nvec; v += threads) out[v] = slope.word(words[v]);
+      for (v += tid; v < r.nvec; v += threads) out[v] = slope.word_or_zeros(words[v]);
     } else {
       for (int v = tid; v < r.nvec; v += threads) slope.scatter(d + r.head + v * VecN<T>::n, words[v]);
     }
@@ -789,20 +794,20 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
     rows++;
     group_barrier(1 + group, GROUP_THREADS);      // the parts are read, the slopes are there
     if (!STORE) continue;
-    const Slope<T, ENTROPY> slope(slope_s[group], p.c, t);
+    const Slope<T, ENTROPY, MODE == POLICY> slope(slope_s[group], p.c, t);
     const bool same = same_phase(z, d);
     slot = (first_slot + again) % SLOTS;
     for (int i = 0; i < chunks; i++, slot = next_slot(slot)) {
       const int c = i + again < chunks ? i + again : i + again - chunks;      // those that are still here first
       if (i + again >= chunks) wait_full(slot);
       const uint4* from = ring + slot * CHUNK + tid;
-      if (same && (c + 1) * CHUNK <= nvec) {
+      if (same && !slope.zero && (c + 1) * CHUNK <= nvec) {
         uint4* out = reinterpret_cast<uint4*>(d + r.head) + from_word + c * CHUNK + tid;
 #pragma unroll
         for (int h = 0; h < PER_CHUNK; h++) out[h * GROUP_THREADS] = slope.word(from[h * GROUP_THREADS]);
       } else {
         for (int h = 0, v = c * CHUNK + tid; v < nvec && h < PER_CHUNK; h++, v += GROUP_THREADS) {
-          if (same) reinterpret_cast<uint4*>(d + r.head)[from_word + v] = slope.word(from[h * GROUP_THREADS]);
+          if (same) reinterpret_cast<uint4*>(d + r.head)[from_word + v] = slope.word_or_zeros(from[h * GROUP_THREADS]);
           else slope.scatter(d + r.head + (from_word + v) * VecN<T>::n, from[h * GROUP_THREADS]);
         }
       }

@@ -632,3 +632,30 @@ def test_confident_tokens(dtype, N, V, offset, temperature):
         near(got, want, (half_step(dtype) * 1.01 + 2 * rel) * want.abs(), "policy")
     z.copy_(keep)
     assert status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,V", [(6, 50), (6, 9001), (6, 66001), (330, 50), (330, 4003), (330, 20011), (330, 70001), (330, 300001)])
+@pytest.mark.parametrize("reduction", ["sum", "mean"])
+def test_a_weight_of_0_counts_nothing(dtype, N, V, reduction):
+    """Rows that a user drops by their weight, an overflow in their logits or in another of their numbers: no loss, no gradient."""
+    z, t = make(N, V, dtype, 3, 1, seed=22)
+    lp, _, _ = reference(z, t)
+    old, A, ref, w = tokens_of(N, lp, V)
+    w = torch.where(torch.arange(N, device="cuda") % 3 == 0, w + 0.25, 0.0)
+    args = dict(clip_low=LO, clip_high=HI, kl_coef=0.125, reduction=reduction)
+    clean = fb.policy_loss(z, t, old, A, ref_logp=ref, weights=w, **args)
+    dropped = w == 0
+    g = torch.Generator(device="cuda").manual_seed(V)
+    kind = torch.randint(0, 5, (N,), device="cuda", generator=g)
+    spot = torch.randint(0, V, (N,), device="cuda", generator=g)
+    rows = torch.arange(N, device="cuda")
+    z[rows[dropped & (kind == 0)], spot[dropped & (kind == 0)]] = math.nan
+    z[rows[dropped & (kind == 1)], t.long()[dropped & (kind == 1)]] = math.inf
+    z[rows[dropped & (kind == 2)]] = math.nan
+    old, A, ref = (torch.where(dropped & (kind >= 3 - i), bad, x) for i, (x, bad) in enumerate(((old, math.nan), (A, math.inf), (ref, -math.inf))))
+    for out in (None, z):
+        r = fb.policy_loss(z, t, old, A, ref_logp=ref, weights=w, out=out, **args)
+        assert torch.equal(r.loss, clean.loss) and torch.equal(r.token_losses, clean.token_losses) and torch.equal(r.n_valid, clean.n_valid)
+        assert bool((r.dlogits[dropped] == 0).all()) and torch.equal(r.dlogits[~dropped], clean.dlogits[~dropped])
+    assert status() == 0
