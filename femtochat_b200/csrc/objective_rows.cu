@@ -321,21 +321,34 @@ template <RowsMode MODE, bool ENTROPY> __device__ __forceinline__ void row_witho
   if (MODE == POLICY) p.logp[row] = p.token_losses[row] = 0.f;
 }
 
-// POLICY: rows with k = 0 (clipped, or of weight 0) have zeros, whatever their logits are.
+// POLICY: rows with k = 0 (clipped, or of weight 0) have zeros, whatever their logits are.  Where k is infinite (the KL term of a token that the model
+// rules out, or all but) tokens of p = 0 still have no gradient: such rows are written element by element.
 template <typename T, bool ENTROPY, bool POLICY> struct Slope {
   static constexpr int n = VecN<T>::n;
   Exponent x;
   uint64_t k2, h2;
   float at_target;
   int t;
-  bool zero;
+  bool zero, unbounded;
   __device__ __forceinline__ Slope(const RowSlope& s, float c, int target)
-      : x(s.m, c), k2(pack2(s.k, s.k)), h2(pack2(s.h, s.h)), at_target(s.target), t(target), zero(POLICY && s.k == 0.f) {}
+      : x(s.m, c), k2(pack2(s.k, s.k)), h2(pack2(s.h, s.h)), at_target(s.target), t(target), zero(POLICY && s.k == 0.f),
+        unbounded(POLICY && fabsf(s.k) == INFINITY) {}
   __device__ __forceinline__ uint64_t of(uint64_t z2) const {
     float u0, u1;
     x.of(z2, u0, u1);
     const uint64_t e2 = pack2(exp2_fast(u0), exp2_fast(u1));
     return mul2(e2, ENTROPY ? fma2(h2, pack2(fmaxf(u0, LEAST_U), fmaxf(u1, LEAST_U)), k2) : k2);
+  }
+  __device__ __forceinline__ void elements(uint64_t z2, float& lo, float& hi) const {
+    float k, unused;
+    unpack2(of(z2), lo, hi);
+    if (zero) lo = hi = 0.f;
+    if (unbounded) {
+      x.of(z2, lo, hi);
+      unpack2(k2, k, unused);
+      lo = exp2_fast(lo) == 0.f ? 0.f : exp2_fast(lo) * k;
+      hi = exp2_fast(hi) == 0.f ? 0.f : exp2_fast(hi) * k;
+    }
   }
   // (Rows of zeros take a loop of their own: with the question at every word the policy's kernel for medium rows took 56 us for 53.)
   __device__ __forceinline__ uint4 word(const uint4& q) const {
@@ -350,19 +363,17 @@ template <typename T, bool ENTROPY, bool POLICY> struct Slope {
 #pragma unroll
     for (int i = 0; i < n / 2; i++) {
       float lo, hi;
-      unpack2(zero ? 0 : of(Word<T>::get(q, i)), lo, hi);
+      elements(Word<T>::get(q, i), lo, hi);
       d[2 * i] = from_f<T>(lo);
       d[2 * i + 1] = from_f<T>(hi);
     }
   }
   // The target's element, over what stands there of its word, by the thread that stored the word.  (A comparison with the target at every word was
   // a third of the instructions.)
-  // The target's element, over what stands there of its word, by the thread that stored the word.  (A comparison with the target at every word was
-  // a third of the instructions.)
   __device__ __forceinline__ void store_target(T* d) const { d[t] = from_f<T>(at_target); }
   __device__ __forceinline__ void store_edge(T* d, int at, float z) const {
     float lo, hi;
-    unpack2(zero ? 0 : of(pack2(z, z)), lo, hi);
+    elements(pack2(z, z), lo, hi);
     d[at] = from_f<T>(at == t ? at_target : lo);
   }
 };
@@ -437,7 +448,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, sizeof(T) == 4 && NV == FEW_WO
   if (!STORE) return;
   __syncthreads();
   const Slope<T, ENTROPY, MODE == POLICY> slope(slope_s, p.c, t);
-  const bool same = same_phase(z, d);
+  const bool same = same_phase(z, d) && !slope.unbounded;
 #pragma unroll
   for (int k = 0; k < NV; k++) {
     const int v = first + k * threads + tid;
@@ -542,7 +553,7 @@ __global__ void __launch_bounds__(32 * NEAR_WARPS, 3) k_rows_near(const RowsArgs
       given = slope_s[group];
     }
     const Slope<T, ENTROPY, MODE == POLICY> slope(given, p.c, t);
-    const bool same = same_phase(z, d);
+    const bool same = same_phase(z, d) && !slope.unbounded;
     if (same) {
       uint4* out = reinterpret_cast<uint4*>(d + r.head);
       // Four words at a time while every thread has as many, and one by one from there: unrolled with a remainder for each thread, the code of
@@ -795,7 +806,7 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
     group_barrier(1 + group, GROUP_THREADS);      // the parts are read, the slopes are there
     if (!STORE) continue;
     const Slope<T, ENTROPY, MODE == POLICY> slope(slope_s[group], p.c, t);
-    const bool same = same_phase(z, d);
+    const bool same = same_phase(z, d) && !slope.unbounded;
     slot = (first_slot + again) % SLOTS;
     for (int i = 0; i < chunks; i++, slot = next_slot(slot)) {
       const int c = i + again < chunks ? i + again : i + again - chunks;      // those that are still here first

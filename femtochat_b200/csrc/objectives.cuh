@@ -121,7 +121,7 @@ __device__ __forceinline__ void policy_token(const PolicyTerm& t, double lp, flo
   float l = clipped ? -(A > 0.f ? t.hi : t.lo) * A : -gain, d = clipped ? 0.f : -gain;
   if (t.kl != 0.f) {
     const float g = (float)((double)ref - lp), e = expm1f(g);
-    l += t.kl * (e - g);
+    l += t.kl * (e == INFINITY ? e : e - g);      // of a token that the model rules out infinite, and not inf - inf
     d -= t.kl * e;
   }
   *loss = w * l;

@@ -659,3 +659,46 @@ def test_a_weight_of_0_counts_nothing(dtype, N, V, reduction):
         assert torch.equal(r.loss, clean.loss) and torch.equal(r.token_losses, clean.token_losses) and torch.equal(r.n_valid, clean.n_valid)
         assert bool((r.dlogits[dropped] == 0).all()) and torch.equal(r.dlogits[~dropped], clean.dlogits[~dropped])
     assert status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [9, 3001, 12001, 66000, 140001])
+@pytest.mark.parametrize("copies", [1, 51])      # few rows and many take different kernels
+@pytest.mark.parametrize("offset", [0, 1])       # of the gradient: rows that lie as the logits do, or not
+def test_kl_term_of_tokens_that_the_model_rules_out(dtype, V, copies, offset):
+    """A chosen token of probability 0 has g = ref - log p = +inf: its KL term and the loss are +inf by the definition, e^g - g - 1, and no NaN.  Its row's
+    gradient is -inf at the token, +inf at tokens of p > 0, and 0 where p = 0; a row without a distribution has none."""
+    N, kl = 6, 0.125
+    z, t = make(N, V, dtype, seed=23)
+    g = torch.Generator(device="cuda").manual_seed(V)
+    hidden = torch.rand(N, V, device="cuda", generator=g) < 0.5
+    hidden[:, V - 1] = False
+    t[:] = torch.tensor([V // 2, -1, 0, 3, V // 3, 5], device="cuda", dtype=torch.int32)
+    hidden.scatter_(1, t.clamp(min=0).long()[:, None], False)
+    hidden[0, V // 2] = hidden[4, V // 3] = True      # ruled out
+    z.masked_fill_(hidden, -math.inf)
+    z[3], z[1] = -math.inf, math.nan                  # a row without a distribution; one without a target
+    lp, _, ls = reference(z, t)
+    ref = torch.tensor([-3.0, math.nan, -2.0, -4.0, -0.5, -1.0], device="cuda")
+    old = torch.tensor([-3.0, math.nan, -2.5, -4.0, -0.5, -1.5], device="cuda")
+    A = torch.tensor([1.0, math.nan, 0.5, -1.0, -2.0, 1.5], device="cuda")
+    many = lambda x: x.repeat(copies, *[1] * (x.dim() - 1))
+    buf = torch.full((offset + N * copies * V,), 5.0, device="cuda", dtype=dtype)
+    r = fb.policy_loss(many(z), many(t), many(old), many(A), ref_logp=many(ref), clip_low=LO, clip_high=HI, kl_coef=kl, out=buf[offset:].view(-1, V))
+    losses, d, logp = r.token_losses.view(copies, N), r.dlogits.view(copies, N, V), r.logp.view(copies, N)
+    assert float(r.loss) == math.inf and not losses.isnan().any() and not d.isnan().any()
+    assert bool((losses[:, [0, 3, 4]] == math.inf).all()) and bool((logp[:, [0, 3, 4]] == -math.inf).all()) and bool((losses[:, 1] == 0).all())
+    assert bool((d[:, [1, 3]] == 0).all())
+    for i in (0, 4):
+        at = int(t[i])
+        assert bool((d[:, i, at] == -math.inf).all())
+        rest = torch.arange(V, device="cuda") != at
+        assert bool((d[:, i, rest & hidden[i]] == 0).all()) and bool((d[:, i, rest & ~hidden[i]] == math.inf).all())
+    # the other rows are what they are without these
+    keep = torch.tensor([2, 5], device="cuda")
+    alone = fb.policy_loss(z[keep], t[keep], old[keep], A[keep], ref_logp=ref[keep], clip_low=LO, clip_high=HI, kl_coef=kl)
+    h = -torch.where(ls[keep] == -math.inf, 0.0, ls[keep].exp() * ls[keep]).sum(1)
+    term = policy_reference(lp[keep], t[keep] >= 0, old[keep], A[keep], ref[keep], None, kl)[3] * (2 * (slack(V) + 2.0 ** -23 * (lp[keep].abs() + h + 1)) + 2.0 ** -21)
+    near(losses[:, keep], alone.token_losses.expand(copies, 2).double(), 2 * term, "other rows")
+    assert bool(alone.dlogits.isfinite().all()) and bool(d[:, keep].isfinite().all())
+    assert status() == 0
