@@ -44,6 +44,15 @@ extern long long g_femto_launches;  // host counter of kernel launches issued by
 #define ST_NONFINITE 4u
 #define ST_BAD_RANGE 8u      // a run of rows that leaves the array or ends before it starts (taken as empty, flagged)
 
+// tanh(y) from one exponential: 1 - 2 / (1 + e^2y).  With ex2 and rcp of the special-function unit (2^-22 and 2^-23 of their values) it is at most 5e-7
+// off; tanh.approx is 2^-11 of tanh off, which softcapping makes 0.007 of a logit.
+__device__ __forceinline__ float tanh_fp32(float y) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(y * 2.8853900817779268f));      // 2 log2(e)
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return fmaf(-2.f, r, 1.f);
+}
+
 // ---- dtype helpers ----------------------------------------------------------------------------
 template <typename T> __device__ __forceinline__ float to_f(T v);
 template <> __device__ __forceinline__ float to_f<float>(float v) { return v; }
@@ -228,7 +237,9 @@ struct GemmArgs {
   float* tz = nullptr;             // [M] softcapped target logit
   int vocab = 0;                   // columns >= vocab are ignored
   float cap = 15.f;                // 15 / temperature: the statistics are of cap tanh(x / 15)
-  bool stats_unrounded = false;    // with a destination: statistics from the products, not from what is stored of them
+  // Log-probabilities, which are compared with those of another call and exponentiated: the statistics are those of the tokens other than the target, from
+  // the products themselves, with tanh to fp32; a destination receives the logits in fp16.
+  bool logprobs = false;
   // tensor-core path scratch
   void* ws = nullptr; size_t ws_bytes = 0;  // stream-K partials
   unsigned int* status = nullptr;
@@ -302,7 +313,8 @@ struct XentArgs {
   bool backward = false; void* dx = nullptr; float* dw = nullptr;
   const TokenObjective* objective = nullptr;   // reverse pass: instead of the cross-entropy
   float* objective_loss = nullptr;
-  float temperature = 1.f;      // the loss rows are those of softmax(z / temperature) (reverse pass: with an objective only)
+  bool logprobs = false;        // the loss rows are log-probabilities that go out, or into an objective (GemmArgs::logprobs)
+  float temperature = 1.f;      // of softmax(z / temperature); with logprobs only
   bool dw_overwrite = false;    // the first chunk's weight gradient overwrites dw instead of adding to it
   int chunk = 0;
   float* logits_f32 = nullptr;  // [chunk][ldw] fp32, SIMT path only

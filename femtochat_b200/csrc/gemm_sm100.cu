@@ -9,6 +9,7 @@
 // gradient M/N-contiguous); the difference is only in the tensor maps and the matrix descriptors.
 // Replaces the library GEMMs behind `W*X` (src/gpt.jl:28), the Linear/MLP reverse rules
 // (ext/FemtoChatEnzymeExt.jl:83-134) and batched_mul! (ext/FemtoChatCUDAExt.jl:121-125).
+#include <cuda_fp16.h>
 #include <stdlib.h>
 
 #include <algorithm>
@@ -71,12 +72,12 @@ __device__ __forceinline__ float sqrt_approx(float x) {
   asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float softcap15(float x, float cap) {
-  // cap * tanh(x/15), cap = 15 / temperature, on the special-function unit (tanh.approx: relative error about 2^-11, below the
+__device__ __forceinline__ float softcap15(float x) {
+  // 15 * tanh(x/15) on the special-function unit (tanh.approx: relative error about 2^-11, below the
   // bf16 rounding of the logits that feed it)
   float t;
   asm("tanh.approx.f32 %0, %1;" : "=f"(t) : "f"(x * (1.f / 15.f)));
-  return cap * t;
+  return 15.f * t;
 }
 
 __device__ __forceinline__ float* f32_dst(const GemmArgs& g, long long bz, int m, int n) {
@@ -92,6 +93,8 @@ __device__ __forceinline__ float* f32_dst(const GemmArgs& g, long long bz, int m
 // banks) and one TMA tiled store writes whole 128-byte lines, clipping rows >= M and columns >= N.
 // sub: 0 = first chunk of the pair (waits until the previous store has read the buffer), 1 = second;
 // flush: this chunk is the last valid one of its pair.
+// HALF: in fp16.
+template <bool HALF = false>
 __device__ __forceinline__ void stage_store_bf16(const float (&v)[32], uint8_t* stage_buf, const CUtensorMap* tmC, int sub, bool flush,
                                                  int nc_pair, int m_warp0, int bz, int lane) {
   if (sub == 0) {
@@ -103,7 +106,10 @@ __device__ __forceinline__ void stage_store_bf16(const float (&v)[32], uint8_t* 
     uint4 q;
     __nv_bfloat162* hq = reinterpret_cast<__nv_bfloat162*>(&q);
 #pragma unroll
-    for (int e = 0; e < 4; e++) hq[e] = __floats2bfloat162_rn(v[8 * j + 2 * e], v[8 * j + 2 * e + 1]);
+    for (int e = 0; e < 4; e++) {
+      if constexpr (HALF) reinterpret_cast<__half2*>(&q)[e] = __floats2half2_rn(v[8 * j + 2 * e], v[8 * j + 2 * e + 1]);
+      else hq[e] = __floats2bfloat162_rn(v[8 * j + 2 * e], v[8 * j + 2 * e + 1]);
+    }
     *reinterpret_cast<uint4*>(stage_buf + lane * 128 + (((sub * 4 + j) ^ (lane & 7)) << 4)) = q;
   }
   if (flush) {
@@ -493,18 +499,42 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
           } break;
           case EPI_XENT_STATS: {
             // with a destination the raw logits are kept in bf16 (as the reference materialises them) and
-            // the statistics are taken from the rounded values, so a later pass over the stored chunk agrees (or from
-            // the unrounded ones, as without a destination: log-probabilities that are compared with those of another call)
-            if (tma_out) {
-              if (!g.stats_unrounded)
+            // the statistics are taken from the rounded values, so a later pass over the stored chunk agrees
+            if (g.logprobs) {
+              if (tma_out) stage_store_bf16<true>(v, sbuf, &tmC, sub, flush, nc_pair, m_tile0 + quad * 32, bz, lane);
+              // the maximum may be the target's: of others that far below it, what underflows does not count
+              float cm = -INFINITY;
+              if (full_chunk && nc + 32 <= g.vocab) {
 #pragma unroll
-                for (int j = 0; j < 32; j++) v[j] = __bfloat162float(__float2bfloat16_rn(v[j]));
+                for (int j = 0; j < 32; j++) v[j] = g.cap * tanh_fp32(v[j] * (1.f / 15.f));
+              } else {
+#pragma unroll
+                for (int j = 0; j < 32; j++) v[j] = nc + j < g.vocab ? g.cap * tanh_fp32(v[j] * (1.f / 15.f)) : -INFINITY;
+              }
+#pragma unroll
+              for (int j = 0; j < 32; j++) cm = fmaxf(cm, v[j]);
+              if (tgt >= nc && tgt < nc + 32) {
+#pragma unroll
+                for (int j = 0; j < 32; j++)
+                  if (nc + j == tgt) { g.tz[m] = v[j]; v[j] = -INFINITY; }
+              }
+              const float nm = fmaxf(rmax, cm);
+              float cs = 0.f;
+#pragma unroll
+              for (int j = 0; j < 32; j++) cs += __expf(v[j] - nm);
+              rsum = rsum * __expf(rmax - nm) + cs;
+              rmax = nm;
+              break;
+            }
+            if (tma_out) {
+#pragma unroll
+              for (int j = 0; j < 32; j++) v[j] = __bfloat162float(__float2bfloat16_rn(v[j]));
               stage_store_bf16(v, sbuf, &tmC, sub, flush, nc_pair, m_tile0 + quad * 32, bz, lane);
             }
             float cm = -INFINITY;
 #pragma unroll
             for (int j = 0; j < 32; j++) {
-              v[j] = (nc + j < g.vocab) ? softcap15(v[j], g.cap) : -INFINITY;
+              v[j] = (nc + j < g.vocab) ? softcap15(v[j]) : -INFINITY;
               cm = fmaxf(cm, v[j]);
             }
             if (tgt >= nc && tgt < nc + 32) {

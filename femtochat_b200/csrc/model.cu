@@ -498,7 +498,7 @@ static int step_t(femto_handle* h, const float* theta, float* delta, const int* 
     x.scale_dev = mean ? h->inv_nvalid : nullptr; x.backward = backward; x.dx = dxnf;
     x.dw = backward ? delta + h->off_lm : nullptr; x.chunk = h->xchunk; x.logits_f32 = h->logits_f32;
     x.dw_overwrite = backward && !accumulate && lm_overwrite;
-    if (ex) { x.objective = ex->objective; x.objective_loss = loss_out; x.temperature = ex->temperature; }
+    if (ex) { x.objective = ex->objective; x.objective_loss = loss_out; x.temperature = ex->temperature; x.logprobs = ex->objective || ex->as_step; }
     x.stats = h->xstats; x.tz = h->tz; x.lse_rows = h->lse_rows; x.loss_rows = h->loss_rows; x.dlogit = h->dlogit;
     x.ws = h->gemm_ws; x.ws_bytes = h->gemm_ws_bytes; x.status = h->status;
     if (two) {

@@ -17,6 +17,7 @@ struct PolicyTerm {
 
 #ifdef __CUDACC__
 constexpr double LN2 = 0.69314718055994530942;
+constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LEAST_U = -200.f;      // 2^u is 0 there, and u stays finite beside it
 
 __device__ __forceinline__ float exp2_fast(float x) {   // relative error 2^-22, 0 for -inf

@@ -6,7 +6,11 @@
 // QK-norm src/gpt.jl:105-106, value-embedding gate src/gpt.jl:95-99.
 #include "streaming.cuh"
 
+#include <cuda_fp16.h>
+
 #include <algorithm>
+
+#include "objectives.cuh"
 
 namespace {
 
@@ -763,9 +767,10 @@ __global__ void __launch_bounds__(256) k_embed_bwd(const T* __restrict__ dx0, co
 }
 
 // One block per row of fp32 logits: z = cap tanh(l/15), lse, loss, dlogit (src/gpt.jl:12,172-194;
-// src/kernels.jl:16-28; ext/FemtoChatEnzymeExt.jl:175-189).  cap is 15 over a temperature; a factor for each row (w_rows) takes the
-// place of w; without dlogit only the loss is computed.
-template <typename T>
+// src/kernels.jl:16-28; ext/FemtoChatEnzymeExt.jl:175-189).
+// LOGPROBS: cap is 15 over a temperature, and the sum is that of the tokens other than the target, which with_token() adds: 1 - p and -log p of
+// a confident token hold their own precision.  A factor for each row (w_rows) takes the place of w; without dlogit only the loss is computed.
+template <typename T, bool LOGPROBS>
 __global__ void __launch_bounds__(256) k_xent_rows(const float* __restrict__ logits, long long ldl,
                                                    const int* __restrict__ tgt0, int V, float w_host,
                                                    const float* __restrict__ w_dev, T* __restrict__ dlogit,
@@ -778,8 +783,10 @@ __global__ void __launch_bounds__(256) k_xent_rows(const float* __restrict__ log
   const float w = w_rows ? w_rows[row] : w_host * (w_dev ? w_dev[0] : 1.f);
   const float* l = logits + row * ldl;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int tg = tgt0[row], apart = LOGPROBS ? tg : -1;
   float mx = -INFINITY;
-  for (int v = threadIdx.x; v < V; v += 256) mx = fmaxf(mx, cap * tanhf(l[v] * (1.f / 15.f)));
+  for (int v = threadIdx.x; v < V; v += 256)
+    if (v != apart) mx = fmaxf(mx, cap * tanhf(l[v] * (1.f / 15.f)));
   mx = warp_max(mx);
   if (lane == 0) red[warp] = mx;
   __syncthreads();
@@ -787,22 +794,31 @@ __global__ void __launch_bounds__(256) k_xent_rows(const float* __restrict__ log
   __syncthreads();
   mx = bc;
   float sum = 0.f;
-  for (int v = threadIdx.x; v < V; v += 256) sum += expf(cap * tanhf(l[v] * (1.f / 15.f)) - mx);
+  for (int v = threadIdx.x; v < V; v += 256)
+    if (v != apart) sum += expf(cap * tanhf(l[v] * (1.f / 15.f)) - mx);
   sum = warp_sum(sum);
   __syncthreads();
   if (lane == 0) red[warp] = sum;
   __syncthreads();
   if (threadIdx.x == 0) { float a = 0.f; for (int i = 0; i < 8; i++) a += red[i]; bc = a; }
   __syncthreads();
-  const float lse = mx + logf(bc);
-  const int tg = tgt0[row];
-  if (threadIdx.x == 0) loss_rows[row] = tg >= 0 ? lse - cap * tanhf(l[tg] * (1.f / 15.f)) : 0.f;
+  float lse = mx + logf(bc), at_target = 0.f;
+  if (LOGPROBS) {
+    if (tg >= 0) {
+      RowStats others;
+      others.m = mx; others.l = bc;
+      const TokenStats s = with_token<false>(others, cap * tanhf(l[tg] * (1.f / 15.f)), LOG2E);
+      lse = (float)((double)s.all.m + log_total(s));
+      at_target = -(s.others / s.all.l);
+      if (threadIdx.x == 0) loss_rows[row] = (float)-log_prob(s, 1.0);
+    } else if (threadIdx.x == 0) loss_rows[row] = 0.f;
+  } else if (threadIdx.x == 0) loss_rows[row] = tg >= 0 ? lse - cap * tanhf(l[tg] * (1.f / 15.f)) : 0.f;
   if (!dlogit) return;
   T* dl = dlogit + row * lddl;
   for (int v = threadIdx.x; v < V; v += 256) {
     float th = tanhf(l[v] * (1.f / 15.f));
     float z = cap * th;
-    float dz = tg >= 0 ? w * (expf(z - lse) - (v == tg ? 1.f : 0.f)) : 0.f;
+    float dz = tg >= 0 ? w * (LOGPROBS && v == tg ? at_target : expf(z - lse) - (v == tg ? 1.f : 0.f)) : 0.f;
     dl[v] = from_f<T>(dz * (1.f - th * th));
   }
 }
@@ -888,6 +904,8 @@ __global__ void __launch_bounds__(256) k_reduce_partials(const float* __restrict
 }
 
 // One warp per row: merge the row's (max, sum exp) partials into its logsumexp.
+// LOGPROBS: the statistics are those of the tokens other than the target.
+template <bool LOGPROBS>
 __global__ void __launch_bounds__(256) k_xent_finalize(const float2* __restrict__ stats, int ntile,
                                                        const float* __restrict__ tz, const int* __restrict__ tgt0,
                                                        int n, float* __restrict__ lse, float* __restrict__ loss_rows) {
@@ -901,10 +919,17 @@ __global__ void __launch_bounds__(256) k_xent_finalize(const float2* __restrict_
   float s = 0.f;
   for (int i = lane; i < ntile; i += 32) {
     const float2 v = st[i];
-    s += v.y * expf(v.x - m);
+    s += v.y * expf(v.x - (LOGPROBS ? finite_or_zero(m) : m));
   }
   s = warp_sum(s);
-  if (lane == 0) {
+  if (LOGPROBS && lane == 0) {
+    const bool has = tgt0[row] >= 0;
+    RowStats others;
+    others.m = m; others.l = s;
+    const TokenStats t = with_token<false>(others, has ? tz[row] : -INFINITY, LOG2E);
+    lse[row] = (float)((double)t.all.m + log_total(t));
+    loss_rows[row] = has ? (float)-log_prob(t, 1.0) : 0.f;
+  } else if (lane == 0) {
     const float l = m + logf(s);
     lse[row] = l;
     loss_rows[row] = tgt0[row] >= 0 ? l - tz[row] : 0.f;
@@ -916,9 +941,9 @@ __global__ void __launch_bounds__(256) k_xent_finalize(const float2* __restrict_
 // ext/FemtoChatEnzymeExt.jl:175-189).  Same tanh.approx / ex2 arithmetic as that pass, so softmax sums to 1 over
 // the stored values.  A thread takes four 8-column groups 2048 columns apart (all four loads in flight before the
 // arithmetic); rows with an ignored target become zero.
-// OBJECTIVE: cap is 15 over a temperature, w one number for each row, and the logsumexp that of the logits before their rounding to bf16.  A
-// stored logit is off by up to 0.02 then, every e^(z - lse) by as much of itself, but softmax - 1 at a target of p = 0.99 by twice its size: that
-// element is taken from the row's -log p (loss_rows).
+// OBJECTIVE: cap is 15 over a temperature, w one number for each row, the logits are stored in fp16 and the logsumexp is that of what they were before.  A
+// stored logit is half a step off, 2^-11 of x or after softcapping 0.0033 at most (in bf16 0.027); with tanh_fp32's 8e-6 every e^(z - lse) is off by that over
+// the temperature, of itself.  The target's element is taken from the row's -log p (loss_rows): softmax - 1 would be off by as much of p.
 template <bool OBJECTIVE> __global__ void __launch_bounds__(256) k_xent_dlogit_inplace(bf16* __restrict__ buf, long long ld,
                                                              const float* __restrict__ lse_rows,
                                                              const int* __restrict__ tgt0, int V, float w_host,
@@ -943,10 +968,11 @@ template <bool OBJECTIVE> __global__ void __launch_bounds__(256) k_xent_dlogit_i
 #pragma unroll
     for (int e = 0; e < 8; e++) {
       float t;
-      asm("tanh.approx.f32 %0, %1;" : "=f"(t) : "f"(__bfloat162float(h[e]) * (1.f / 15.f)));
+      if (OBJECTIVE) t = tanh_fp32(__half2float(reinterpret_cast<const __half*>(h)[e]) * (1.f / 15.f));
+      else asm("tanh.approx.f32 %0, %1;" : "=f"(t) : "f"(__bfloat162float(h[e]) * (1.f / 15.f)));
       const float z = cap * t;
       const float p = __expf(z - lse);
-      const float dz = w * (OBJECTIVE ? ((col + e) == tg ? at_target : fminf(p, 1.f)) : p - ((col + e) == tg ? 1.f : 0.f));
+      const float dz = w * (OBJECTIVE ? ((col + e) == tg ? at_target : p > 1.f ? 1.f : p) : p - ((col + e) == tg ? 1.f : 0.f));
       h[e] = __float2bfloat16_rn(dz * (1.f - t * t));
     }
     *reinterpret_cast<uint4*>(base + col) = q[u];
@@ -1104,8 +1130,10 @@ int Stream<T>::embed_bwd(const T* dx0, const T* table, const int* tok0, const T*
 }
 template <typename T>
 int Stream<T>::xent_rows(const float* logits, long long ldl, const int* tgt0, int n, int V, float w,
-                         const float* w_dev, T* dlogit, long long lddl, float* loss_rows, cudaStream_t s, float cap, const float* w_rows) {
-  k_xent_rows<T><<<n, 256, 0, s>>>(logits, ldl, tgt0, V, w, w_dev, dlogit, lddl, loss_rows, cap, w_rows);
+                         const float* w_dev, T* dlogit, long long lddl, float* loss_rows, cudaStream_t s, bool logprobs, float cap,
+                         const float* w_rows) {
+  if (logprobs) k_xent_rows<T, true><<<n, 256, 0, s>>>(logits, ldl, tgt0, V, w, w_dev, dlogit, lddl, loss_rows, cap, w_rows);
+  else k_xent_rows<T, false><<<n, 256, 0, s>>>(logits, ldl, tgt0, V, w, w_dev, dlogit, lddl, loss_rows, 15.f, nullptr);
   KERNEL_CHECK();
   return 0;
 }
@@ -1131,8 +1159,9 @@ int reduce_partials(const float* partial, int nrow, int ncol, float* out, const 
   return 0;
 }
 int xent_finalize(const float2* stats, int ntile, const float* tz, const int* tgt0, int n, float* lse,
-                  float* loss_rows, cudaStream_t s) {
-  k_xent_finalize<<<cdiv(n, 8), 256, 0, s>>>(stats, ntile, tz, tgt0, n, lse, loss_rows);
+                  float* loss_rows, cudaStream_t s, bool logprobs) {
+  if (logprobs) k_xent_finalize<true><<<cdiv(n, 8), 256, 0, s>>>(stats, ntile, tz, tgt0, n, lse, loss_rows);
+  else k_xent_finalize<false><<<cdiv(n, 8), 256, 0, s>>>(stats, ntile, tz, tgt0, n, lse, loss_rows);
   KERNEL_CHECK();
   return 0;
 }

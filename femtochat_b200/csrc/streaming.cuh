@@ -55,7 +55,7 @@ template <typename T> struct Stream {
                        float eps, T* dE, cudaStream_t s);
   static int xent_rows(const float* logits, long long ldl, const int* tgt0, int n, int V, float w,
                        const float* w_dev, T* dlogit,
-                       long long lddl, float* loss_rows, cudaStream_t s, float cap = 15.f, const float* w_rows = nullptr);
+                       long long lddl, float* loss_rows, cudaStream_t s, bool logprobs = false, float cap = 15.f, const float* w_rows = nullptr);
   static int cast_all(const float* theta, const CastJob* jobs, int n_jobs, int from, int to, cudaStream_t s);      // blocks [from, to) of the jobs
 };
 
@@ -65,5 +65,5 @@ int xent_dlogit_inplace(void* logits_bf16, long long ld, const float* lse_rows, 
                         const float* w_dev, cudaStream_t s, float cap = 15.f, const float* w_rows = nullptr, const float* loss_rows = nullptr);
 int softcap_inplace(float* x, long long n, cudaStream_t s, float cap = 15.f);   // x = cap tanh(x / cap)
 int xent_finalize(const float2* stats, int ntile, const float* tz, const int* tgt0, int n, float* lse,
-                  float* loss_rows, cudaStream_t s);
+                  float* loss_rows, cudaStream_t s, bool logprobs = false);
 int fill_zero(void* p, size_t bytes, cudaStream_t s);

@@ -13,7 +13,7 @@
 template <typename T> int xent_tail(const XentArgs& x, cudaStream_t s) {
   const int N = x.N, d = x.D, V = x.V;
   const long long ld = x.ldw;
-  const float cap = x.temperature == 1.f ? 15.f : (float)(15.0 / (double)x.temperature);
+  const float cap = x.logprobs ? (float)(15.0 / (double)x.temperature) : 15.f;
   const float* w_rows = x.objective ? x.objective->slopes : nullptr;
   // An objective on pairs of answers needs every row's log-probability before the first gradient: with more rows than a chunk holds they are
   // computed in a pass of their own, and the chunks' logits twice.
@@ -37,7 +37,7 @@ template <typename T> int xent_tail(const XentArgs& x, cudaStream_t s) {
     g.ws = x.ws; g.ws_bytes = x.ws_bytes; g.status = x.status; g.ring = two ? 5 : 0;
     g.A = xc; g.lda = d; g.B = x.W; g.ldb = ld; g.b_kmajor = false; g.M = cn; g.N = V; g.K = d;
     g.targets0 = x.targets0 + c0; g.vocab = V;
-    g.epi = EPI_XENT_STATS; g.stats = x.stats; g.tz = x.tz + c0; g.cap = cap; g.stats_unrounded = x.objective != nullptr;
+    g.epi = EPI_XENT_STATS; g.stats = x.stats; g.tz = x.tz + c0; g.cap = cap; g.logprobs = x.logprobs;
     // reverse pass: the statistics GEMM also keeps the chunk's logits in bf16 (as the reference materialises
     // them) and a streaming pass turns them into d loss/d logit in place
     if (x.backward) { g.C = dlogit; g.ldc = ld; }
@@ -45,7 +45,7 @@ template <typename T> int xent_tail(const XentArgs& x, cudaStream_t s) {
     if (tc) {
       FEMTO_TRY(gemm_tc_bf16(g, s));
       FEMTO_TRY(xent_finalize(x.stats, 2 * ((V + 255) / 256), x.tz + c0, x.targets0 + c0, cn, x.lse_rows + c0,
-                              x.loss_rows + c0, s));
+                              x.loss_rows + c0, s, x.logprobs));
       if (x.objective && !first_pass) FEMTO_TRY(objective_slopes(*x.objective, x.loss_rows, c0, cn, x.scale_dev, x.objective_loss, s));
       if (x.backward)
         FEMTO_TRY(xent_dlogit_inplace(dlogit, ld, x.lse_rows + c0, x.targets0 + c0, cn, V, x.scale, x.scale_dev, s, cap,
@@ -55,11 +55,11 @@ template <typename T> int xent_tail(const XentArgs& x, cudaStream_t s) {
       g.epi = EPI_F32; g.beta = 0.f; g.C = x.logits_f32; g.ldc = ld;
       FEMTO_TRY(gemm<T>(g, s));
       if (x.objective && !first_pass) {
-        FEMTO_TRY(Stream<T>::xent_rows(x.logits_f32, ld, x.targets0 + c0, cn, V, x.scale, x.scale_dev, (T*)nullptr, ld, x.loss_rows + c0, s, cap));
+        FEMTO_TRY(Stream<T>::xent_rows(x.logits_f32, ld, x.targets0 + c0, cn, V, x.scale, x.scale_dev, (T*)nullptr, ld, x.loss_rows + c0, s, true, cap));
         FEMTO_TRY(objective_slopes(*x.objective, x.loss_rows, c0, cn, x.scale_dev, x.objective_loss, s));
       }
       FEMTO_TRY(Stream<T>::xent_rows(x.logits_f32, ld, x.targets0 + c0, cn, V, x.scale, x.scale_dev, (T*)dlogit, ld,
-                                     x.loss_rows + c0, s, cap, w_rows ? w_rows + c0 : nullptr));
+                                     x.loss_rows + c0, s, x.logprobs, cap, w_rows ? w_rows + c0 : nullptr));
     }
     if (x.backward) {
       cudaStream_t sw = s;

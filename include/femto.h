@@ -151,7 +151,10 @@ typedef struct femto_preference_config {
 } femto_preference_config;
 /* Log-probabilities of the targets at a temperature, fp32 [B][T], 0 where the target is ignored: those of the answers before an update
  * (old_logp), or under a reference model.  Every sum is taken as a training step takes it, so that the ratios of the first step are exactly 1
- * (femto_forward_token_losses may take other kernels, and differs by roundings). */
+ * (femto_forward_token_losses may take other kernels, and differs by roundings).  Behind the rows that enter the lm_head, which have the compute
+ * type's roundings, a logit is some 1e-5 off (its fp32 product and the softcap), and a log-probability that over the temperature; log p of a confident
+ * token is right relative to itself.  In bf16 the step keeps its logits in fp16: an element of their gradient is up to 0.0033 / temperature of itself off
+ * (3 % at a temperature of 0.1), the target's not. */
 int32_t femto_forward_token_logprobs(femto_handle* h, const float* theta, const int32_t* tokens, const int32_t* targets,
                                      const int32_t* positions, int32_t B, float temperature, float* logp_out, void* stream);
 /* old_logp, advantages, ref_logp, weights: fp32 [B][T] (the last two may be NULL, ref_logp when kl_coef is 0).  loss_out, n_valid_out and

@@ -205,6 +205,137 @@ def test_confident_tokens_in_bf16():
     assert cosine(want, got) >= 0.98
 
 
+def rows_of_the_head(params, st, lay, cfg, batch, targets, rows):
+    """The bf16 rows that enter the lm_head of a step, as it has them (another pass, as the model call's, may take other kernels and differ by roundings).
+    With one target in the batch, in row r, the head's gradient is x_r d, each product of two bf16 numbers exact in fp32: of the numbers that d may be
+    at the target, by the row's norm, which is 1 per element within some percent, one makes every x_r a bf16 number."""
+    D, Vp = cfg.n_embed, lay.lm_head.size // cfg.n_embed
+    out = []
+    for r in rows:
+        only = torch.full_like(targets, -1).flatten()
+        only[r] = targets.flatten()[r]
+        only = only.view(targets.shape)
+        old = fb.forward_token_logprobs(params, st, lay, batch[0], only, batch[2])
+        fb.policy_loss_and_gradient_(params, st, lay, batch[0], only, old, torch.ones_like(old), positions=batch[2])
+        column = params.delta[lay.lm_head.offset:lay.lm_head.offset + lay.lm_head.size].view(D, Vp)[:, int(only.flatten()[r]) - 1].cpu().double()
+        guess = -float(column.norm()) / D ** 0.5      # the gradient at the target is negative
+        first = torch.tensor(1.03 * guess).bfloat16()
+        found, d = [], first
+        while abs(float(d)) > 0.97 * abs(guess):
+            x = column / float(d)      # correctly rounded on the host
+            if torch.equal(x, x.bfloat16().double()):
+                found.append(x)
+            d = torch.nextafter(d, torch.zeros_like(d))
+        assert len(found) == 1, (r, len(found))
+        out.append(found[0])
+    return torch.stack(out).cuda()
+
+
+@pytest.mark.parametrize("chunk", ["", "256"])
+@pytest.mark.parametrize("temperature", [1.0, 0.125, 0.03125])
+def test_log_probabilities_and_gradient_at_low_temperatures_in_bf16(chunk, temperature, monkeypatch):
+    """The lm_head's product of bf16 numbers, softcapped and divided by the temperature, against 64 bits.  Tolerances: a product's sum of D exact terms has
+    at most D / 8 roundings of 2^-23 of sum |x w| in the tensor cores; tanh_fp32 is 5e-7 off, 8e-6 of a logit: `dz` together, divided by the temperature
+    in a log-probability, of the target and of the others.  An element of the gradient is made from a logit stored in fp16: half a step, 2^-11 of x,
+    or x (1 - tanh^2) 2^-11 behind the softcap; and twice that relative to x in 1 - tanh^2.  It is rounded to bf16, 2^-8."""
+    if chunk:
+        monkeypatch.setenv("FEMTO_XENT_CHUNK", chunk)
+    cfg, lay, th, batch, params, st, M = setup(TC, 2, "bfloat16", seed=12)
+    tok, tgt, pos = batch
+    D, Vp, V = TC["n_embed"], lay.lm_head.size // TC["n_embed"], TC["vocab_size"]
+    head = slice(lay.lm_head.offset, lay.lm_head.offset + lay.lm_head.size)
+    rows = [0, 1, 130, 255, 256, 300, 301, 511]
+    targets = torch.randint(1, V + 1, tok.shape, generator=torch.Generator().manual_seed(3), dtype=torch.int32).cuda()
+    x = rows_of_the_head(params, st, lay, cfg, batch, targets, rows)
+    W = th[head].view(D, Vp)[:, :V].cuda().bfloat16().double()
+    y = x @ W
+    th15 = torch.tanh(y / 15)
+    ls = torch.log_softmax(15 * th15 / temperature, 1)
+    # half of the tokens are the likeliest, the others what was drawn
+    t0 = targets.flatten()[rows].long() - 1
+    t0[::2] = torch.argmax(y, 1)[::2]
+    targets.view(-1)[rows] = t0.int() + 1
+    lp = ls.gather(1, t0[:, None])[:, 0]
+    dz = float((x.abs() @ W.abs()).max()) * D / 8 * 2.0 ** -23 + 8e-6
+    got = fb.forward_token_logprobs(params, st, lay, tok, targets, pos, temperature=temperature)
+    error = (got.double().flatten()[rows] - lp).abs()
+    tol = 2 * dz / temperature + 2.0 ** -23 * (lp.abs() + 16) + 1e-6
+    assert not bool((error > tol).any()), (float(error.max()), float(tol.min()))
+    # one row at a time has a target: with ratios of 1 and an advantage of 1 its column of the head's gradient is x (p - 1[target]) (1 - tanh^2) / temperature
+    for k, r in enumerate(rows):
+        only = torch.full_like(targets, -1).flatten()
+        only[r] = targets.flatten()[r]
+        only = only.view(tok.shape)
+        q = fb.policy_loss_and_gradient_(params, st, lay, tok, only, got, torch.ones_like(got), positions=pos, temperature=temperature)
+        assert float(q.loss) == -1 and int(q.n_valid) == 1 and float(q.logp.flatten()[r]) == float(got.flatten()[r])
+        i, t = int(torch.argmax(x[k].abs())), int(t0[k])
+        d = params.delta[head].view(D, Vp)[i, :V].double() / x[k, i]
+        slope = 1 - th15[k] ** 2
+        want = ls[k].exp() * slope / temperature
+        want[t] = torch.expm1(lp[k]) * slope[t] / temperature
+        off = (y[k].abs() * slope * 2.0 ** -11 + 2 * dz) / temperature      # of the exponent
+        rel = torch.expm1(off) + 2 * 2.0 ** -11 * y[k].abs() / 15 + 2.0 ** -8 * 1.01 + 1e-5
+        rel[t] = 2 * 2.0 ** -11 * y[k, t].abs() / 15 + 2.0 ** -8 * 1.01 + 1e-5
+        tol = rel * want.abs() + 1e-30
+        tol[t] += tolerance_of_p(lp[k], 2 * dz / temperature) * slope[t] / temperature
+        bad = (d - want).abs() > tol
+        assert not bad.any(), (r, int(bad.sum()), float(((d - want).abs() / (want.abs() + 1e-30))[bad].max()))
+    assert st.status_word() == 0
+
+
+def tolerance_of_p(lp, off):
+    """How far p is off where log p + log(1 / (1 - p)), the target's logit relative to the others', is `off`: p (1 - p) off, and the second order."""
+    p = torch.exp(lp)
+    return p * (1 - p) * torch.expm1(torch.tensor(off))
+
+
+@pytest.mark.parametrize("kw,dtype", [(MID, "float32"), (TC, "bfloat16")])
+def test_steps_on_confident_tokens(kw, dtype):
+    """Tokens of 1 - p from 1e-8 to 1e-2: the step's -log p has its own precision, where a difference of logsumexp and logit in fp32 would leave 1e-6.  The
+    head gives chosen rows a token each; what the model then gives them is compared with 64 bits for the rows that enter the head in bf16, or in fp32 for the
+    logits of the model call: another pass in fp32, whose logits, 15 at most, are within 2^-17 of themselves (1e-4) of the step's."""
+    cfg, lay, th, batch, params, st, M = setup(kw, 2, dtype, seed=13)
+    tok, tgt, pos = batch
+    D, Vp, V = kw["n_embed"], lay.lm_head.size // kw["n_embed"], kw["vocab_size"]
+    head = slice(lay.lm_head.offset, lay.lm_head.offset + lay.lm_head.size)
+    t = th.clone()
+    t[head] = torch.eye(D, Vp).flatten()
+    x = 15 * torch.atanh(fb.GPT(fb.Params(t.cuda()), cfg, lay, compute_type=dtype).logits(tok, pos)[..., :D].double().flatten(0, 1) / 15)
+    n = 32
+    W = D ** -0.5 * torch.randn(D, V, generator=torch.Generator().manual_seed(1)) * 0.5
+    rows = torch.randperm(x.shape[0], generator=torch.Generator().manual_seed(2))[:n].tolist()
+    W[:, :n] = (torch.linspace(10, 40, n)[:, None] * torch.nn.functional.normalize(x[rows].float().cpu(), dim=1)).T * D ** -0.5
+    full = torch.zeros(D, Vp)
+    full[:, :V] = W
+    th[head] = full.flatten()
+    params = fb.Params(th.cuda())
+    st = fb.gradient_state(params, cfg, lay, tok, tgt, pos, compute_type=dtype)
+    targets = torch.full((tok.numel(),), -1, dtype=torch.int32)
+    targets[rows] = torch.arange(1, n + 1, dtype=torch.int32)
+    targets = targets.view(tok.shape).cuda()
+    if dtype == "bfloat16":
+        x = rows_of_the_head(params, st, lay, cfg, batch, targets, rows)
+        W = W.cuda().bfloat16().double()
+        z = 15 * torch.tanh(x @ W / 15)
+        dz = float((x.abs() @ W.abs()).max()) * D / 8 * 2.0 ** -23 + 8e-6
+    else:
+        z, dz = fb.GPT(params, cfg, lay).logits(tok, pos).double().flatten(0, 1)[rows], 1e-4
+    ls = torch.log_softmax(z, 1)
+    own = torch.arange(n, device="cuda")
+    want = ls[own, own]
+    ls[own, own] = -math.inf
+    left = ls.exp().sum(1)
+    got = fb.forward_token_logprobs(params, st, lay, tok, targets, pos)
+    lp = got.flatten()[rows].double()
+    sure = (left > 1e-8) & (left < 1e-2)
+    assert int(sure.sum()) >= 5
+    # every logit dz off: 1 - p by 2 dz of itself; and the roundings of a sum of V exponentials
+    rel = 2 * dz * 1.01 + 2.0 ** -20 + V * 2.0 ** -24
+    assert not bool(((lp - want).abs() > rel * want.abs())[sure].any()), float(((lp - want) / want)[sure].abs().max())
+    step = fb.policy_loss_and_gradient_(params, st, lay, tok, targets, got, torch.ones_like(got), positions=pos)
+    assert torch.equal(step.logp, got)
+
+
 def test_a_policy_step_trains_a_model():
     """Log-probabilities, steps and updates in turn, as a training loop calls them, on another stream than the default."""
     cfg, lay, th, batch, params, st, M = setup(TC, 4, "bfloat16", seed=7)
