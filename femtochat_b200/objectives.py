@@ -167,6 +167,8 @@ def policy_loss(logits, targets0, old_logp, advantages, ref_logp=None, weights=N
     weight (-min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (e^g - g - 1)) per token, r = exp(logp - old_logp) and
     g = ref_logp - logp.  clip_high=None bounds the ratio below only.  `out` may be the logits themselves."""
     import torch
+    if out is not None and not gradient:
+        raise ValueError("out takes the gradient, which gradient=False leaves out")
     n, V, pitch, code = _rows("logits", logits)
     shape, f32, device = logits.shape[:-1], torch.float32, logits.device
     targets0 = _on_device("targets0", targets0, torch.int32, shape, device)

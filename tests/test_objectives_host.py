@@ -98,6 +98,12 @@ def test_python_refuses_what_is_not_on_the_device():
         fb.preference_loss(torch.zeros(3), torch.tensor([0, 1, 3], dtype=torch.int32))
 
 
+def test_policy_loss_refuses_a_place_for_a_gradient_that_it_does_not_compute():
+    z, t, f = torch.zeros(2, 5), torch.zeros(2, dtype=torch.int32), torch.zeros(2)
+    with pytest.raises(ValueError, match="gradient=False"):
+        fb.policy_loss(z, t, f, f, gradient=False, out=z)
+
+
 def test_python_refuses_options():
     from femtochat_b200 import objectives
     with pytest.raises(ValueError, match="reduction"):
