@@ -302,15 +302,20 @@ int check_rows(int dtype, const void* logits, long long ldl, const int* tgt0, in
   if (reinterpret_cast<uintptr_t>(logits) % size) return femto_fail(FEMTO_ERR_ALIGN, "logits are not aligned to their type");
   return 0;
 }
-// The gradient lies apart from the logits, or in their place.
+// The gradient lies apart from the logits, or in their place.  With one pitch the rows of both may also lie in turn, in one wide buffer: the distance of
+// their first rows, modulo the pitch, leaves room for a row on either side.
 int check_gradient(int dtype, const void* dlogits, long long ldd, const void* logits, long long ldl, int N, int V) {
   if (ldd < V) return femto_fail(FEMTO_ERR_SHAPE, "ldd = %lld is less than V = %d", ldd, V);
   const uintptr_t size = dtype == FEMTO_BF16 ? 2 : 4, a = reinterpret_cast<uintptr_t>(dlogits), b = reinterpret_cast<uintptr_t>(logits);
   if (a % size) return femto_fail(FEMTO_ERR_ALIGN, "dlogits are not aligned to their type");
   if (N == 0 || (a == b && ldd == ldl)) return 0;
-  const uintptr_t a_end = a + size * ((uintptr_t)(N - 1) * ldd + V), b_end = b + size * ((uintptr_t)(N - 1) * ldl + V);
-  if (a < b_end && b < a_end) return femto_fail(FEMTO_ERR_ARG, "dlogits overlap the logits: give the same rows and pitch, or memory of their own");
-  return 0;
+  const uintptr_t row = size * V, pitch = size * ldl, a_end = a + size * ((uintptr_t)(N - 1) * ldd + V), b_end = b + size * ((uintptr_t)(N - 1) * ldl + V);
+  if (a >= b_end || b >= a_end) return 0;
+  if (ldd == ldl) {
+    const uintptr_t apart = (a > b ? a - b : b - a) % pitch;
+    if (apart >= row && pitch - apart >= row) return 0;
+  }
+  return femto_fail(FEMTO_ERR_ARG, "dlogits overlap the logits: give the same rows and pitch, or memory of their own");
 }
 float log2e_over(float temperature) { return (float)(1.4426950408889634074 / (double)temperature); }
 

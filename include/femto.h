@@ -496,7 +496,7 @@ int32_t femto_muon_direction(int32_t dtype, float* X_out, const float* G, float*
 int32_t femto_token_logprobs(int32_t dtype, const void* logits, int64_t ldl, const int32_t* targets0, int32_t N, int32_t V,
                              float temperature, float* logp, float* entropy, void* stream);
 /* The way back: dlogits [N][V] = dlogp d logp / d logits + dentropy d entropy / d logits (dentropy may be NULL), the rows ldd elements apart.
- * Overwrites; dlogits may be the logits themselves (same pitch), and may not overlap them otherwise. */
+ * Overwrites; dlogits may be the logits themselves (same pitch), and their rows may not overlap them otherwise. */
 int32_t femto_token_logprobs_gradient(int32_t dtype, void* dlogits, int64_t ldd, const void* logits, int64_t ldl,
                                       const int32_t* targets0, int32_t N, int32_t V, float temperature, const float* dlogp,
                                       const float* dentropy, void* stream);
@@ -506,7 +506,7 @@ int32_t femto_token_logprobs_gradient(int32_t dtype, void* dlogits, int64_t ldd,
  * advantages A [N]; ref_logp [N] (may be NULL when beta is 0); weights [N] (NULL = 1; where a weight is 0 loss and gradient are 0).
  * Outputs: token_losses [N], logp [N], the reduced loss, n_valid = rows with a target, n_clipped (may be NULL) = those whose minimum is
  * the bounded product, which has no gradient.  dlogits (NULL: loss only) is overwritten with the gradient of the reduced loss, its rows ldd
- * elements apart; it may be the logits themselves (same pitch), and may not overlap them otherwise. */
+ * elements apart; it may be the logits themselves (same pitch), and its rows may not overlap them otherwise. */
 int32_t femto_policy_loss(int32_t dtype, const void* logits, int64_t ldl, const int32_t* targets0, int32_t N, int32_t V,
                           const float* old_logp, const float* advantages, const float* ref_logp, const float* weights,
                           const femto_policy_config* h_cfg, void* dlogits, int64_t ldd, float* token_losses, float* logp,

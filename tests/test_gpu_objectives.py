@@ -702,3 +702,24 @@ def test_kl_term_of_tokens_that_the_model_rules_out(dtype, V, copies, offset):
     near(losses[:, keep], alone.token_losses.expand(copies, 2).double(), 2 * term, "other rows")
     assert bool(alone.dlogits.isfinite().all()) and bool(d[:, keep].isfinite().all())
     assert status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,V", [(5, 300), (300, 300), (300, 9001), (320, 40001), (300, 150001)])
+@pytest.mark.parametrize("logits_first", [True, False])
+def test_gradient_beside_the_logits_in_one_buffer(dtype, N, V, logits_first):
+    """Rows of both in turn, nothing shared, a gap of one element before the next pair."""
+    small, t = make(N, V, dtype, seed=24, masked=0.3)
+    buf = torch.full((N, 2 * V + 1), 7.0, device="cuda", dtype=dtype)
+    z, d = (buf[:, :V], buf[:, V:2 * V]) if logits_first else (buf[:, V:2 * V], buf[:, :V])
+    z.copy_(small)
+    old, A = torch.full((N,), -4.0, device="cuda"), torch.linspace(-1, 1, N, device="cuda")
+    r, want = fb.policy_loss(z, t, old, A, reduction="mean", out=d), fb.policy_loss(small, t, old, A, reduction="mean")
+    near(d, want.dlogits.double(), 2 * slack(V) * want.dlogits.double().abs() + 2 * half_step(dtype) * want.dlogits.double().abs(), "policy")
+    assert torch.equal(r.n_valid, want.n_valid) and torch.equal(z, small) and bool((buf[:, 2 * V] == 7.0).all())
+    fb.token_logprobs_gradient(z, t, A, dentropy=old, out=d)
+    g = fb.token_logprobs_gradient(small, t, A, dentropy=old)
+    _, h, ls = reference(small, t)
+    size = A.double().abs()[:, None] * (torch.nn.functional.one_hot(t.clamp(min=0).long(), V) + ls.exp()) + 4 * ls.exp() * (ls.abs() + h[:, None] + 2)
+    near(d, g.double(), 2 * half_step(dtype) * 1.01 * g.double().abs() + 2 * size * (4 * slack(V) + 2.0 ** -20) + 1e-38, "gradient")
+    assert torch.equal(z, small) and bool((buf[:, 2 * V] == 7.0).all()) and status() == 0

@@ -71,6 +71,17 @@ def test_a_gradient_in_place_has_the_same_rows():
         assert call(dlogits=C.c_void_p(BASE - 2 * 399)) == ARG              # its last element is the first logit
 
 
+def test_rows_of_the_gradient_and_the_logits_in_turn_do_not_overlap():
+    """In one buffer with one pitch, 250 elements of 2 bytes: a row of 100 logits, and one of the gradient in what is left."""
+    for call in (gradient, policy):
+        for d in (0, 2, 198, 302, 498):           # bytes behind the logits' first row: 0 and 498 within a pitch of the row's own place
+            for turns in (0, 1, 2):               # the gradient's first row may be that many pitches on
+                if d or turns:
+                    assert call(ldl=250, ldd=250, dlogits=C.c_void_p(BASE + d + 500 * turns)) == ARG, (d, turns)
+        assert call(ldl=250, ldd=251, dlogits=C.c_void_p(BASE + 200)) == ARG      # of two pitches some rows meet, or may
+        assert call(ldl=199, ldd=199, dlogits=C.c_void_p(BASE + 200)) == ARG      # one element short
+
+
 def test_policy_refuses():
     for name in ("old", "adv", "token_losses", "logp", "loss", "n_valid", "cfg"):
         assert policy(**{name: None}) == ARG, name
