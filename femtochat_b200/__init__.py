@@ -10,5 +10,6 @@ from .generation import KVCache, prefill, decode_step, extend, generate, sample_
 from .decoder import Decoder, DecoderConfig, DecoderState, LayerConfig, decoder_layout
 from .models import MODELS, load_model, register
 from .weights import SafeTensors, save_safetensors
+from .handle import status_word
 from .objectives import (TokenLogprobs, PolicyLoss, PreferenceLoss, token_logprobs, token_logprobs_gradient, policy_loss, preference_loss,
                          PolicyStep, PreferenceStep, forward_token_logprobs, policy_loss_and_gradient_, preference_loss_and_gradient_)

@@ -6,6 +6,17 @@ import ctypes as C
 from . import _lib
 
 
+def status_word(device=None) -> int:
+    """Reads and clears what calls without a handle (`token_logprobs`, `policy_loss`, ...) found on a device, the current one by default; waits for it.
+    0: nothing; bit 1: a token or target outside its vocabulary (its row counted as one without); bit 2: a bounded wait ran out (results are
+    incomplete); bit 8: offsets of answers that leave the rows or descend (the answer counted as empty)."""
+    import torch
+    out = C.c_int32(0)
+    with torch.cuda.device(device):
+        _lib.check(_lib.lib().femto_status_word(None, C.byref(out)))
+    return out.value
+
+
 class Handle:
     def __init__(self):
         self.h = None

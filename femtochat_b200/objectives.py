@@ -1,6 +1,7 @@
 """Objectives on a model's own answers (femto_token_logprobs*, femto_policy_loss, femto_preference_loss): what a host calls after
 pretraining, when answers have rewards or come in pairs.  No counterpart in the reference.  Every call is asynchronous on the current
-stream and returns device tensors; nothing is read back, so a call may be captured into a graph.
+stream and returns device tensors; nothing is read back, so a call may be captured into a graph.  What only the device can see, targets
+outside the vocabulary or offsets that descend, is taken as nothing and reported by `status_word()`.
 
 Logits are [..., V] with unit stride along V and one pitch between rows, as `GPT.logits` and `decode_step` give them, or cut from a wider
 buffer; float32 or bfloat16.  Targets are 0-based here (`targets0`; the model's own ids may start at 1), negative where a row counts for

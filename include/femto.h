@@ -487,8 +487,8 @@ int32_t femto_muon_direction(int32_t dtype, float* X_out, const float* G, float*
 /* ---- objectives on a model's own answers ------------------------------------------------------ */
 /* What comes after pretraining; no counterpart in the reference.  These calls are asynchronous on `stream`, allocate nothing and keep
  * nothing: they may be captured, and calls on different streams do not meet.  Logits are [N][V] rows of `dtype`, ldl >= V elements apart and
- * aligned to their type only.  targets0: 0-based, or negative where a row counts for nothing: neither its logits nor its entries in other
- * arrays are then read, and its results are 0.  A target of V or more counts as none and raises bit 1 of the word that
+ * aligned to their type only.  targets0: 0-based, or negative where a row counts for nothing: its logits are not read then, its entries in
+ * other arrays may hold anything, and its results are 0.  A target of V or more counts as none and raises bit 1 of the word that
  * femto_status_word(NULL, ..) reads (and no other call reports).  Logits of -inf are tokens that cannot be chosen; a row with nothing else has no distribution: its
  * log-probability is -inf, its entropy and its gradient are 0.  NaN or +inf in a counted row give NaN there.  N = 0 is allowed.
  * temperature: 1e-6 .. 1e6.  Outputs lie apart from inputs and from one another, but for dlogits where it says so. */
@@ -527,7 +527,8 @@ int32_t femto_preference_loss(const float* logp, const float* ref_logp, const in
 /* Device status word (0 = ok): bounded waits that ran out (bit 2), out-of-range token ids (bit 1), runs of rows that leave their array (bit 8), ...
  * h == NULL reads AND CLEARS the word of the stand-alone kernel-level entry points on the current device (after a
  * cudaDeviceSynchronize); a bit raised by an asynchronous entry point that nobody read is reported by the next
- * synchronising one as FEMTO_ERR_DEVICE_STATUS + word. */
+ * synchronising one as FEMTO_ERR_DEVICE_STATUS + word, but for those of femto_attention_bwd_static and of the objectives on a model's own answers,
+ * which this call alone reports. */
 int32_t femto_status_word(femto_handle* h, int32_t* h_out);
 int32_t femto_sync(femto_handle* h, void* stream);
 /* Number of kernels launched by this handle since creation (host counter). */

@@ -723,3 +723,15 @@ def test_gradient_beside_the_logits_in_one_buffer(dtype, N, V, logits_first):
     size = A.double().abs()[:, None] * (torch.nn.functional.one_hot(t.clamp(min=0).long(), V) + ls.exp()) + 4 * ls.exp() * (ls.abs() + h[:, None] + 2)
     near(d, g.double(), 2 * half_step(dtype) * 1.01 * g.double().abs() + 2 * size * (4 * slack(V) + 2.0 ** -20) + 1e-38, "gradient")
     assert torch.equal(z, small) and bool((buf[:, 2 * V] == 7.0).all()) and status() == 0
+
+
+def test_python_reads_what_the_device_found():
+    z, t = make(4, 100, torch.float32)
+    logp = fb.token_logprobs(z, t).logp
+    assert fb.status_word() == 0
+    t[1] = 100
+    fb.token_logprobs(z, t)
+    assert fb.status_word(z.device) == 1 and fb.status_word() == 0
+    fb.preference_loss(logp, torch.tensor([0, 3, 2], device="cuda", dtype=torch.int32))
+    fb.token_logprobs(z, t)
+    assert fb.status_word() == 9 and fb.status_word() == 0
