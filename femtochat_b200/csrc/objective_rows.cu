@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(32 * NEAR_WARPS, 3) k_rows_near(const RowsArgs
   const long long step = (long long)gridDim.x * groups;
   long long row = (long long)blockIdx.x * groups + group;
   Targets targets(p, row, step);
-  int t_next = targets(0), k = 0;      // k: rows with a target so far
+  int t_next = targets(0), k = 0, n_asked = 0;      // k: rows with a target so far
   bool alive = true, asked = false;
   float scale = 0.f;
   for (int nth = 1; row < p.N; row += step, nth++) {
@@ -515,7 +515,7 @@ __global__ void __launch_bounds__(32 * NEAR_WARPS, 3) k_rows_near(const RowsArgs
     const int which = k & 1;
     const uint32_t parity = (uint32_t)(k >> 1) & 1u;
     k++;
-    if (!asked && tid == 0 && alive) ask(row, which);      // the row before the last but one, which this buffer held, is done: a barrier lies between
+    if (!asked && tid == 0 && alive) { ask(row, which); n_asked = k; }      // the row before the last but one, which this buffer held, is done: a barrier lies between
     LaneNumbers numbers;
     if (warp == first_warp) numbers = lane_numbers<T, MODE, ENTROPY>(p, row, z, t);
     const bool there = at >= 0 && at != t;
@@ -524,7 +524,7 @@ __global__ void __launch_bounds__(32 * NEAR_WARPS, 3) k_rows_near(const RowsArgs
     const int vt = word_of_target<T>(r, t);
     const bool own = vt >= 0 && (vt & (threads - 1)) == tid;      // the target's word is this thread's (W is a power of two)
     uint4* words = buffer + (size_t)which * pitch;
-    alive = alive && mbar_wait(&full[group][which], parity, &abort_flag, &g_rows_status);
+    alive = alive && mbar_wait_limit(&full[group][which], parity, &abort_flag, &g_rows_status, p.wait_limit);
     if (own) take_out<T>(words + vt, (t - r.head) % VecN<T>::n);
     int v0 = 0;
     for (; v0 + NEAR_WORDS * threads <= r.nvec; v0 += NEAR_WORDS * threads) {
@@ -543,7 +543,7 @@ __global__ void __launch_bounds__(32 * NEAR_WARPS, 3) k_rows_near(const RowsArgs
     } else __syncwarp();
     // all of the group are done with the row before this one: its buffer is free
     asked = t_next >= 0 && t_next < p.V;
-    if (asked && tid == 0 && alive) ask(row + step, which ^ 1);
+    if (asked && tid == 0 && alive) { ask(row + step, which ^ 1); n_asked = k + 1; }
     RowSlope given;
     if (warp == first_warp) given = row_result<MODE, ENTROPY>(p, row, s, numbers.all(), scale, lane == 0);
     if (!STORE) continue;
@@ -575,9 +575,9 @@ __global__ void __launch_bounds__(32 * NEAR_WARPS, 3) k_rows_near(const RowsArgs
     if (at >= 0) slope.store_edge(d, at, edge);
   }
   end_behind_the_count<MODE>(p);
-  if (!alive && tid == 0)      // nothing may still be on its way to this block's memory when it ends
+  if (!alive && tid == 0)      // nothing may still be on its way to this block's memory when it ends: the last row asked for in either buffer
     for (int b = 0; b < 2; b++)
-      for (uint32_t polls = 0; k > b && polls < WAIT_LIMIT && !mbar_try_wait(&full[group][b], (uint32_t)((k - b - 1) >> 1) & 1u); polls++) {}
+      for (uint32_t polls = 0; n_asked > b && polls < WAIT_LIMIT && !mbar_try_wait(&full[group][b], (uint32_t)((n_asked - b - 1) >> 1) & 1u); polls++) {}
 }
 
 // ---- rows through a ring in shared memory -----------------------------------------------------------------------------------------------------
@@ -600,13 +600,16 @@ __device__ __forceinline__ void send_remote(const float4* local, const uint64_t*
   asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];"
                ::"r"(remote_address(local, rank)), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(remote_address(barrier, rank)) : "memory");
 }
-// As mbar_wait, for what another block of the cluster sends.
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  for (uint32_t polls = 0; polls < WAIT_LIMIT; polls++) {
-    uint32_t ok;
-    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
-                 : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-    if (ok) return true;
+// As mbar_wait_limit, for what another block of the cluster sends.
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+               : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint32_t limit) {
+  for (uint32_t polls = 0; polls < limit; polls++) {
+    if (mbar_try_wait_cluster(bar, parity)) return true;
     if ((polls & 255u) == 255u && *abort_flag) return false;
   }
   *abort_flag = 1;
@@ -627,6 +630,7 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
   __shared__ RowSlope slope_s[GROUPS];
   __shared__ uint64_t met[GROUPS][2];      // a group's statistics of a row from the other block of the cluster, two rows in turn
   __shared__ __align__(16) float4 theirs[GROUPS][2];
+  __shared__ int their_sent[GROUPS];      // how many rows' statistics the other block has sent in all
   __shared__ int abort_flag;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = C > 1 ? (int)cluster_rank() : 0;
   const long long first_row = blockIdx.x / C, step = gridDim.x / C;
@@ -658,7 +662,7 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
     bool alive = true;
     auto bring = [&](const uint4* words, int nvec, int n_chunks, int group) {      // by one lane
       for (int c = 0; c < n_chunks; c++) {
-        if (round > 0) alive = mbar_wait(&empty[slot], (round - 1) & 1u, &abort_flag, &g_rows_status);
+        if (round > 0) alive = mbar_wait_limit(&empty[slot], (round - 1) & 1u, &abort_flag, &g_rows_status, p.wait_limit);
         if (!alive) return;
         const int n = min(CHUNK, nvec - c * CHUNK);
         if (n > 0) {
@@ -715,7 +719,8 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
     }
     while (clear_next(INT_MAX)) {}
     if (STORE && lane == 0) bulk_wait_all();
-    if (lane == 0 && !alive)      // nothing may still be on its way to this block's memory when it ends
+    group_barrier(0, R::BLOCK);                                 // every group has dealt with its rows, or given up,
+    if (lane == 0 && *(const volatile int*)&abort_flag)      // and nothing may still be on its way to this block's memory when it ends
       for (int i = 0; i < GROUPS * SLOTS; i++)
         if (used[i / SLOTS] >> (i % SLOTS) & 1u)
           for (uint32_t polls = 0; polls < WAIT_LIMIT && !mbar_try_wait(&full[i / SLOTS][i % SLOTS], (parity[i / SLOTS] >> (i % SLOTS) & 1u) ^ 1u); polls++) {}
@@ -725,16 +730,18 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
   }
 
   const int group = warp / GROUP_WARPS, tid = threadIdx.x - group * GROUP_THREADS, gwarp = warp - group * GROUP_WARPS;
-  bool alive = true;      // after a wait that ran out nothing is waited for any more; barriers of the group are
+  // After a wait that ran out nothing is waited for any more (barriers of the group are), and no slot is handed back: the copy into it may not have come,
+  // and a barrier is not armed for another one before.  (The bringing warp asking for the flag ahead of each copy: 8000 x 16000 in bf16, numbers only, 71 us for 53.)
+  bool alive = true;
   // How often the group has waited for each slot, modulo 2.  A group's barriers are its own: of a barrier for both, a group that waits while the
   // other's row passes through the slot could not tell the phase it waits for from the one before the other's.
   uint32_t parity = 0;
   auto wait_full = [&](int slot) {
-    alive = alive && mbar_wait(&full[group][slot], parity >> slot & 1u, &abort_flag, &g_rows_status);
+    alive = alive && mbar_wait_limit(&full[group][slot], parity >> slot & 1u, &abort_flag, &g_rows_status, p.wait_limit);
     parity ^= 1u << slot;
   };
   int k = 0, nth = 0;
-  uint32_t rows = 0;      // that the group has worked on
+  uint32_t rows = 0, sent = 0;      // that the group has worked on; whose statistics have gone to the other block
   float scale = 0.f;
   Targets targets(p, first_row, step);
   for (long long row = first_row; row < p.N; row += step) {
@@ -766,7 +773,7 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
       auto done = [&]() {
         if (STORE && c >= again) return;
         __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[slot]);
+        if (lane == 0 && alive) mbar_arrive(&empty[slot]);
       };
       if ((c + 1) * CHUNK <= nvec) {
         uint4 q[PER_CHUNK];
@@ -787,12 +794,13 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
       if (C > 1) {
         // Two rows in turn: the other block sends a row's statistics when it has this block's of the row before, and those go out ahead of the wait.
         const int turn = rows & 1u;
-        if (lane == 0) {
+        if (lane == 0 && alive) {
+          sent++;
           mbar_expect_tx(&met[group][turn], 16);
           // the target's logit goes along: it has been read then, and the other block may write over it
           send_remote(&theirs[group][turn], &met[group][turn], rank ^ 1, make_float4(s.m, s.l, s.a, numbers.z));
         }
-        alive = alive && mbar_wait_cluster(&met[group][turn], rows >> 1 & 1u, &abort_flag);
+        alive = alive && mbar_wait_cluster(&met[group][turn], rows >> 1 & 1u, &abort_flag, p.wait_limit);
         __syncwarp();
         const float4 o = theirs[group][turn];
         RowStats other;
@@ -823,13 +831,28 @@ __global__ void __launch_bounds__(R::BLOCK) k_rows_ring(const RowsArgs p, const 
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[slot]);
+      if (lane == 0 && alive) mbar_arrive(&empty[slot]);
     }
     if (own) slope.store_target(d);
     if (at >= 0) slope.store_edge(d, at, edge);
   }
   end_behind_the_count<MODE>(p);
-  if (C > 1) asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");      // nothing is on its way to a block that has ended
+  const bool leader = gwarp == 0 && lane == 0;
+  if (C > 1 && leader) store_remote(&their_sent[group], rank ^ 1, (int)sent);
+  group_barrier(0, R::BLOCK);
+  if (C > 1) {
+    asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");      // the other block sends nothing more
+    // Where every wait came to its end, all that was sent has come.  Behind one that ran out the last of either turn may be on its way to this block's
+    // memory: waited for as well, after arming the barrier for one that this block did not wait for.  (The other block sends a row's when it
+    // has this block's of the row before: one more at the most.)
+    if (leader && *(const volatile int*)&abort_flag)
+      for (int turn = 0; turn < 2; turn++) {
+        const int here = ((int)sent + 1 - turn) / 2, came = (*(const volatile int*)&their_sent[group] + 1 - turn) / 2;
+        auto settle = [&](int n) { for (uint32_t polls = 0; n > 0 && polls < WAIT_LIMIT && !mbar_try_wait_cluster(&met[group][turn], (uint32_t)(n - 1) & 1u); polls++) {} };
+        settle(min(here, came));
+        if (came > here) { mbar_expect_tx(&met[group][turn], 16); settle(came); }
+      }
+  }
 }
 
 // ---- launch -----------------------------------------------------------------------------------------------------------------------------------
@@ -924,4 +947,22 @@ unsigned int objective_rows_status_word() {
   if (cudaMemcpyFromSymbol(&w, g_rows_status, sizeof(w)) != cudaSuccess) return 0;
   if (w) cudaMemcpyToSymbol(g_rows_status, &zero, sizeof(zero));
   return w;
+}
+
+// The gradient, or with dlogits = NULL the log-probabilities, by kernels whose waits give up after `polls` polls: right away with 0, while the
+// copies that they wait for are on their way.
+extern "C" int32_t femto_selftest_rows_wait(int32_t dtype, void* dlogits, const void* logits, int64_t ldl, const int32_t* targets0, int32_t N, int32_t V,
+                                            const float* dlogp, float* logp, int32_t polls, int32_t* h_status, void* stream) {
+  if (!logits || !targets0 || (dlogits ? !dlogp : !logp) || !h_status || (dtype != FEMTO_F32 && dtype != FEMTO_BF16)) return femto_fail(FEMTO_ERR_ARG, "bad argument");
+  if (N <= 0 || V <= 0 || ldl < V || polls < 0) return femto_fail(FEMTO_ERR_SHAPE, "bad shape");
+  cudaStream_t s = (cudaStream_t)stream;
+  RowsArgs p = {};
+  p.logits = logits; p.ldl = p.ldd = ldl; p.dlogits = dlogits; p.tgt0 = targets0; p.N = N; p.V = V;
+  p.c = LOG2E; p.inv_t = 1.f; p.inv_t64 = 1.0; p.dlogp = dlogp; p.logp = logp;
+  p.wait_limit = (uint32_t)polls;
+  objective_rows_status_word();
+  FEMTO_TRY(objective_rows(dtype, dlogits ? GRADIENT : LOGPROBS, p, s));
+  CUDA_TRY(cudaStreamSynchronize(s));
+  *h_status = (int32_t)objective_rows_status_word();
+  return 0;
 }

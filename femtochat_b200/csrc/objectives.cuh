@@ -147,6 +147,7 @@ struct RowsArgs {
   float* token_losses;
   const int* n_valid;            // POLICY, mean: the slopes are divided by it
   PolicyTerm term;
+  uint32_t wait_limit = 1u << 22;      // polls of a wait, as sm100::WAIT_LIMIT
 };
 int objective_rows(int dtype, RowsMode mode, const RowsArgs& p, cudaStream_t s);
 unsigned int objective_rows_status_word();

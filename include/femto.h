@@ -544,6 +544,11 @@ int32_t femto_selftest_bounded_wait(int32_t polls, int32_t* h_status, int32_t* h
  * stays as it was) and return by themselves; the cache goes on where it was. */
 int32_t femto_selftest_decode_wait(femto_handle* h, femto_kv_cache* c, const float* theta, const int32_t* tokens, int32_t B,
                                    float* logits_out, void* stream, int32_t* h_status);
+/* The same of the passes over rows of logits: femto_token_logprobs_gradient (dlogits with the logits' pitch), or with dlogits NULL femto_token_logprobs,
+ * by kernels whose waits give up after `polls` polls (0: at once, while the copies that they wait for are on their way).  They raise bit 2 (*h_status),
+ * wait with the ordinary limit for what is still coming, and return by themselves; outputs are incomplete.  Waits. */
+int32_t femto_selftest_rows_wait(int32_t dtype, void* dlogits, const void* logits, int64_t ldl, const int32_t* targets0, int32_t N, int32_t V,
+                                 const float* dlogp, float* logp, int32_t polls, int32_t* h_status, void* stream);
 /* The product of few rows that prompts and evaluations take where it is the faster one (tiles of 128 rows and `tile_columns` = 64 or 128
  * columns, K shared by a cluster of `splits` = 1, 2, 4 or 8 blocks), with every choice open: C = epilogue(A[M][K] * B) in bf16 with fp32
  * accumulation, epilogue 0 store (+ bias), 1 + aux, 2 relu^2, 5 fp32, 7 silu(gate) * up of B's groups of 32 rows.  Waits.

@@ -735,3 +735,38 @@ def test_python_reads_what_the_device_found():
     fb.preference_loss(logp, torch.tensor([0, 3, 2], device="cuda", dtype=torch.int32))
     fb.token_logprobs(z, t)
     assert fb.status_word() == 9 and fb.status_word() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,V", [(400, 37), (400, 701), (1500, 4003), (400, 20011), (500, 60007), (300, 150001)])      # every kernel that waits, rows that its ring holds or not
+@pytest.mark.parametrize("polls", [0, 1, 50])
+def test_waits_that_run_out(dtype, N, V, polls):
+    """Waits that give up, at once or early, while copies are on their way: the kernels raise bit 2, wait for these and return.  Nothing but the rows of the
+    gradient is written, and the calls that follow are right."""
+    z, t = make(N, V, dtype, 3, 1, seed=25, masked=0.2)
+    dlogp = torch.randn(N, device="cuda", generator=torch.Generator(device="cuda").manual_seed(V))
+    code = _lib.F32 if dtype is torch.float32 else _lib.BF16
+    pitch = z.stride(0)
+    buf = torch.full((N * pitch + 64,), 5.0, device="cuda", dtype=dtype)
+    d = buf[1:1 + N * pitch].view(N, pitch)[:, :V]
+    logp = torch.full((N + 2,), 5.0, device="cuda")
+    word = C.c_int32(-1)
+
+    def run(limit, gradient):
+        _lib.check(_lib.lib().femto_selftest_rows_wait(code, d.data_ptr() if gradient else None, z.data_ptr(), pitch, t.data_ptr(), N, V, dlogp.data_ptr(),
+                                                       logp[1:].data_ptr(), limit, C.byref(word), _lib.stream_ptr()))
+        return word.value
+
+    for gradient in (True, False):
+        for _ in range(3):
+            found = run(polls, gradient)
+            assert found == 2 or (polls > 0 and found == 0)
+        assert status() == 0
+        # with the ordinary limit the same entry gives what the calls give
+        assert run(1 << 22, gradient) == 0
+    assert torch.equal(d, fb.token_logprobs_gradient(z, t, dlogp)) and torch.equal(logp[1:-1], fb.token_logprobs(z, t).logp)
+    d.fill_(5.0)
+    assert bool((buf == 5.0).all()) and float(logp[0]) == float(logp[-1]) == 5.0
+    lp, h, _ = reference(z, t)
+    near(logp[1:-1], lp, slack(V) + 2.0 ** -23 * (lp.abs() + h + 1), "logp")
+    assert status() == 0

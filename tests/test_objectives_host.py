@@ -185,3 +185,15 @@ def test_steps_refuse_no_targets():
     for step in steps_of(ids(2, T), None):
         with pytest.raises(ValueError, match="targets is None"):
             step()
+
+
+def test_self_test_of_the_waits_refuses():
+    word = C.c_int32(0)
+
+    def call(dtype=0, d=at(0), z=at(1), ldl=9, t=at(2), N=3, V=9, dlogp=at(3), logp=at(4), polls=0, out=C.byref(word)):
+        return _lib.lib().femto_selftest_rows_wait(dtype, d, z, ldl, t, N, V, dlogp, logp, polls, out, None)
+
+    for change in (dict(dtype=2), dict(z=None), dict(t=None), dict(dlogp=None), dict(d=None, logp=None), dict(out=None)):
+        assert call(**change) == ARG, change
+    for change in (dict(N=0), dict(V=0), dict(ldl=8), dict(polls=-1)):
+        assert call(**change) == SHAPE, change
