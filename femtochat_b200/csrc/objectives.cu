@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(1024) k_preference_pairs(const Preference p) {
     if (p.kind == FEMTO_PREFERENCE_SIGMOID) {
       // -(1 - e) log sigma(h) - e log sigma(-h), with log(1 + e^-|h|) once
       const double h = beta * delta - (double)p.margin, e = p.smoothing, q = exp(-fabs(h)), s = log1p(q);
-      loss = s + (1.0 - e) * fmax(-h, 0.0) + e * fmax(h, 0.0);
+      loss = s + (e < 1.0 ? (1.0 - e) * fmax(-h, 0.0) : 0.0) + (e > 0.0 ? e * fmax(h, 0.0) : 0.0);      // h may be infinite
       slope = beta * ((h >= 0.0 ? 1.0 / (1.0 + q) : q / (1.0 + q)) - (1.0 - e));
     } else {
       const double u = delta - 0.5 / beta;

@@ -516,6 +516,8 @@ int32_t femto_policy_loss(int32_t dtype, const void* logits, int64_t ldl, const 
  * the chosen and 2 p + 1 the rejected one of pair p; rho_k = sum over its rows of logp - ref_logp (ref_logp may be NULL = 0), without the
  * rows whose target is negative (targets0 may be NULL: all count).  With D = rho_2p - rho_2p+1 and h = beta D - margin:
  *   sigmoid: -(1 - label_smoothing) log sigma(h) - label_smoothing log sigma(-h)        squared: (D - 1 / (2 beta))^2
+ * A factor of 0 counts nothing: with label_smoothing 0, an answer that the model rules out (rho = -inf) costs nothing as the rejected one of its pair, and
+ * +inf as the chosen one.
  * Outputs: the reduced loss, pair_losses [P], ratios [2 P] = rho, dlogp [N] (may be NULL) = the gradient of the reduced loss, 0 in rows that
  * count for nothing or belong to no answer.  Offsets that leave 0 .. N or descend make an answer empty and raise bit 8 of the word that
  * femto_status_word(NULL, ..) reads; where answers then lie over one another, a row's dlogp is that of one of them, or 0. */

@@ -770,3 +770,18 @@ def test_waits_that_run_out(dtype, N, V, polls):
     lp, h, _ = reference(z, t)
     near(logp[1:-1], lp, slack(V) + 2.0 ** -23 * (lp.abs() + h + 1), "logp")
     assert status() == 0
+
+
+@pytest.mark.parametrize("smoothing", [0.0, 0.25, 1.0])
+def test_pairs_with_an_answer_that_the_model_rules_out(smoothing):
+    """log p = -inf in the rejected answer: D = h = +inf and -(1 - e) log sigma(h) = 0; in the chosen one h = -inf and the loss is +inf; with e the other way
+    round.  A factor of 0 counts nothing.  The slopes by D are the limits, beta (sigma(h) - (1 - e))."""
+    logp = torch.tensor([-1.0, -2.0, -1.5, -math.inf, -0.5, -math.inf, -1.0, -1.0], device="cuda")
+    offsets = torch.tensor([0, 2, 4, 6, 8], device="cuda", dtype=torch.int32)
+    r = fb.preference_loss(logp, offsets, beta=0.5, label_smoothing=smoothing, reduction="sum")
+    inf = math.inf
+    assert r.ratios.tolist() == [-3.0, -inf, -inf, -2.0]
+    assert r.pair_losses.tolist() == [0.0 if smoothing == 0 else inf, 0.0 if smoothing == 1 else inf] and float(r.loss) == inf
+    a, b = 0.5 * smoothing, 0.5 * (smoothing - 1)
+    assert r.dlogp.tolist() == [a, a, -a, -a, b, b, -b, -b]
+    assert status() == 0
