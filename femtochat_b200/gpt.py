@@ -104,6 +104,8 @@ def _check_batch(config, device, tokens, targets, positions) -> None:
     """The library is told B alone and walks B x sequence_len entries of every array: a batch of any other shape is refused, before anything
     is copied or launched."""
     T = config.sequence_len
+    if T is None:
+        raise ValueError("a decoder that lists its layers has no such call")
     if tokens.dim() != 2 or tokens.shape[1] != T:
         raise ValueError(f"tokens must be [B][{T}], as long as the model's sequence_len, not {tuple(tokens.shape)}")
     for name, x in (("tokens", tokens), ("targets", targets), ("positions", positions)):

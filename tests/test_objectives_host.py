@@ -197,3 +197,11 @@ def test_self_test_of_the_waits_refuses():
         assert call(**change) == ARG, change
     for change in (dict(N=0), dict(V=0), dict(ldl=8), dict(polls=-1)):
         assert call(**change) == SHAPE, change
+
+
+def test_steps_refuse_a_decoder_by_name():
+    """A decoder that lists its layers has no sequence_len, so that there is no shape to hold its batch to."""
+    from types import SimpleNamespace
+    params, state = SimpleNamespace(theta=torch.zeros(16), delta=None), SimpleNamespace(h=None, config=SimpleNamespace(sequence_len=None))
+    with pytest.raises(ValueError, match="decoder"):
+        fb.forward_token_logprobs(params, state, None, ids(2, T), ids(2, T))
