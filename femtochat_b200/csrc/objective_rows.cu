@@ -4,22 +4,23 @@
 // Three kernels that differ in where a row lies between its reading and the writing of its gradient: in the registers of a cluster (k_rows_few),
 // in a buffer of the group of warps that works on it (k_rows_near), in a ring that a block's groups share (k_rows_ring); launch() says
 // which takes what.  A thread's exponentials are relative to a maximum of its own, the (m, l, a) of threads and warps are added in a fixed order.
+// They are those of the tokens other than the row's own, which is added at the end (with_token).
 //
-// The floor is HBM: every logit is read once and its gradient written once.  Beside it stand two exponentials an element (16 a cycle and
-// multiprocessor: half of the time that bf16 takes to come and go) and some 17 instructions; one block's chain of load, statistics, exchange,
-// slopes and stores is ten times as long as a row's share of the bandwidth, so rows have to overlap.  Measured (time, share of the measured
-// copy rate; bytes of the floor):
+// The floor is HBM: every logit is read once and its gradient written once.  Beside it stand an exponential an element for the numbers, another one for the
+// gradient (16 a cycle and multiprocessor: both together half of the time that bf16 takes to come and go), and with the gradient some 17 instructions;
+// one block's chain of load, statistics, exchange, slopes and stores is ten times as long as a row's share of the bandwidth, so rows have to
+// overlap.  Measured (time, share of the measured copy rate; bytes of the floor):
 //   log-probabilities    gradient          policy loss and gradient
-//     67 us  0.92         170 us  0.84      176 us  0.82    4096 x 65536 bf16, a quarter of the rows without target   ring, a row to two blocks (*)
-//     86     0.96         181     0.91      176     0.93    2048 x 65536 fp32                                         ring, the same
-//     49     0.81         100     0.80      108     0.74    1000 x 131000 bf16                                        ring, the same
-//     30     0.61          48     0.77       52     0.70    2000 x 30000 bf16                                         ring
-//     30     0.69          45     0.91       50     0.81    8192 x 4096 fp32                                          near
-//     21     0.49          32     0.64       39     0.53    8192 x 4096 bf16                                          near
-//     28     0.52          45     0.65       54     0.54    20000 x 2400 bf16                                         near
-//      4.0   0.16           5.1   0.25        7.6   0.17    16 x 65536 fp32                                           few
+//     70 us  0.88         171 us  0.84      175 us  0.82    4096 x 65536 bf16, a quarter of the rows without target   ring, a row to two blocks (*)
+//     89     0.93         170     0.96      178     0.92    2048 x 65536 fp32                                         ring, the same
+//     51     0.79         103     0.77      112     0.71    1000 x 131000 bf16                                        ring, the same
+//     31     0.60          48     0.76       55     0.67    2000 x 30000 bf16                                         ring
+//     30     0.68          44     0.93       49     0.83    8192 x 4096 fp32                                          near
+//     22     0.47          32     0.64       40     0.52    8192 x 4096 bf16                                          near
+//     29     0.51          45     0.66       54     0.54    20000 x 2400 bf16                                         near
+//      3.8   0.17           5.2   0.25        7.6   0.17    16 x 65536 fp32                                           few
 // (* log-probabilities: to one.)
-// The exponential pipe is busy 68 % with 65536 logits in bf16.  Arithmetic in f32x2 pairs or in single floats takes the same time.
+// The exponential pipe is busy 64 % (gradient) to 68 % with 65536 logits in bf16.  Arithmetic in f32x2 pairs or in single floats takes the same time.
 #include <limits.h>
 
 #include <algorithm>

@@ -232,8 +232,8 @@ PreferenceArgs preference_args(const femto_preference_config& c, int N, int P) {
 int preference(const PreferenceArgs& p, float* loss_out, cudaStream_t s) {
   if (p.P > 0) {
     // A thread has some eight rows of an answer of average length; where pairs are few and long, a cluster shares one (one pair of 70000 rows
-    // each: 87 -> 12 us), and where they are many, small blocks let one's reduction pass behind others' loads (1024 pairs of 1536 rows each:
-    // 14.6 us with 128 threads, 15.9 with 256, 21.2 with 512).
+    // each: 87 -> 10 us), and where they are many, small blocks let one's reduction pass behind others' loads (1024 pairs of 1536 rows each, 24 rows a
+    // thread: 13.4 us with 128 threads, half on each answer, 15.9 with 256, 21.2 with 512).
     int threads = 64, C = 1;
     while (threads < (p.P < 4 * device_sm_count() ? 1024 : 128) && (long long)threads * p.P * 8 < p.N) threads *= 2;
     while (C < MOST_CLUSTER && (long long)C * p.P < device_sm_count() && (long long)C * 1024 * p.P * 8 < p.N) C *= 2;

@@ -133,7 +133,8 @@ int32_t femto_loss_and_gradient_host(femto_handle* h, const float* theta, float*
 /* ---- training on a model's own answers ------------------------------------------------------- */
 /* What follows pretraining: answers with rewards, or in pairs.  No counterpart in the reference.  The objectives are those of
  * femto_policy_loss and femto_preference_loss below, of the log-probabilities that the model gives the targets; the step is that of
- * femto_loss_and_gradient (weights, positions, accumulation, data parallelism) with them in the cross-entropy's place. */
+ * femto_loss_and_gradient (weights, positions, accumulation) with them in the cross-entropy's place.  With several ranks delta is summed as that
+ * step's is, and a mean is one over a rank's own rows or pairs (this has not been run on several GPUs). */
 typedef struct femto_policy_config {
   float temperature; /* at which the answers were sampled, 1e-6 .. 1e6 */
   float clip_low, clip_high; /* the ratio r counts up to the range 1 - clip_low .. 1 + clip_high (infinity: no bound above) */
