@@ -310,11 +310,11 @@ __device__ __forceinline__ RowSlope row_result(const RowsArgs& p, long long row,
   float loss, slope;
   policy_token(p.term, lp, k.x[0], k.x[1], k.x[2], k.x[3], &loss, &slope);
   if (write) { p.token_losses[row] = loss; p.logp[row] = (float)lp; }
-  if (k.x[3] == 0.f) return RowSlope();      // whatever the logits are
   if (p.n_valid && scale == 0.f) {      // a kernel of the same call counts the targets beside the first rows
     pdl_wait();
     scale = 1.f / (float)*reinterpret_cast<const volatile int*>(p.n_valid);
   }
+  if (k.x[3] == 0.f) return RowSlope();      // whatever the logits are.  Behind the wait: a kernel of few rows ends behind the count by it
   return row_slope<false>(s, (p.n_valid ? slope * scale : slope) * p.inv_t, 0.f, p.c);
 }
 template <RowsMode MODE, bool ENTROPY> __device__ __forceinline__ void row_without_target(const RowsArgs& p, long long row) {

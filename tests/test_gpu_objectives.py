@@ -785,3 +785,18 @@ def test_pairs_with_an_answer_that_the_model_rules_out(smoothing):
     a, b = 0.5 * smoothing, 0.5 * (smoothing - 1)
     assert r.dlogp.tolist() == [a, a, -a, -a, b, b, -b, -b]
     assert status() == 0
+
+
+@pytest.mark.parametrize("N,V", [(3, 50), (5, 66001), (330, 50), (330, 9001), (330, 70001)])
+def test_rows_of_weight_0_alone_end_behind_the_count(N, V):
+    """A mean whose rows all have weight 0 asks for no count of the targets; the call still ends behind the kernel that counts them, so that what follows in
+    the stream may write over the targets."""
+    z, t = make(N, V, torch.float32, seed=26, masked=0.3)
+    old, zero = torch.full((N,), -4.0, device="cuda"), torch.zeros(N, device="cuda")
+    n = int((t >= 0).sum())
+    for _ in range(20):
+        u = t.clone()
+        r = fb.policy_loss(z, u, old, zero + 1, weights=zero, reduction="mean")
+        u.fill_(-1)
+        assert int(r.n_valid) == n and float(r.loss) == 0 and bool((r.dlogits == 0).all())
+    assert status() == 0
