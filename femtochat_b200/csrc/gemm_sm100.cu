@@ -197,8 +197,10 @@ __device__ __forceinline__ void bf16_chunk(const GemmArgs& g, float (&v)[32], in
   }
 }
 
-// ACT: the instantiation for EPI_SWIGLU, kept apart so that the other epilogues keep their registers.
-template <bool A_K, bool B_K, bool PAIR, bool ACT = false>
+// ACT: the instantiation for EPI_SWIGLU, kept apart so that the other epilogues keep their registers.  LOGPROBS: that for EPI_XENT_STATS with
+// GemmArgs::logprobs, for the same reason (as a branch of the epilogue it cost every product four registers, and d20's step 209.4 -> 211.6 ms).
+enum Variant { PLAIN, SWIGLU, LOGPROBS };
+template <bool A_K, bool B_K, bool PAIR, Variant VARIANT = PLAIN>
 __global__ void __launch_bounds__(NTHREADS, 1)
 gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                const __grid_constant__ CUtensorMap tmC, const TcParams p) {
@@ -419,7 +421,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         }
         tmem_ld_wait();
         const int nc = n0 + c * 32;
-        if constexpr (ACT) {
+        if constexpr (VARIANT == SWIGLU) {
           // chunks come in pairs of 32 gate and 32 up columns; both are taken at the first
           if (nc >= g.N || (ci & 1)) continue;
           uint32_t up[32];
@@ -456,7 +458,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
           for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(dst + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
           continue;
         }
-        switch (g.epi) {
+        switch (VARIANT == LOGPROBS ? (int)EPI_XENT_STATS : (int)g.epi) {
           case EPI_F32: {
             float* dst = reinterpret_cast<float*>(g.C) + (long long)bz * g.strideC + (long long)m * g.ldc + nc;
             if (g.nseg == 0 && full_chunk && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
@@ -500,7 +502,7 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
           case EPI_XENT_STATS: {
             // with a destination the raw logits are kept in bf16 (as the reference materialises them) and
             // the statistics are taken from the rounded values, so a later pass over the stored chunk agrees
-            if (g.logprobs) {
+            if constexpr (VARIANT == LOGPROBS) {
               if (tma_out) stage_store_bf16<true>(v, sbuf, &tmC, sub, flush, nc_pair, m_tile0 + quad * 32, bz, lane);
               // the maximum may be the target's: of others that far below it, what underflows does not count
               float cm = -INFINITY;
@@ -742,6 +744,7 @@ bool gemm_tc_supported(const GemmArgs& g) {
     if (!g.ws) return false;
   } else if (g.epi == EPI_XENT_STATS) {
     if (!g.stats || !g.tz || !g.targets0) return false;
+    if (g.logprobs && (!g.a_kmajor || g.b_kmajor)) return false;
     if (g.C && ((g.ldc & 7) || (g.strideC & 7) || !aligned16(g.C))) return false;  // kept logits leave by TMA only
   } else {
     if (!g.C && g.epi != EPI_XENT_STATS) return false;
@@ -863,7 +866,8 @@ static int launch_tc(const GemmArgs& g, const CUtensorMap& tmA, const CUtensorMa
   const int dev = PerDevice::current();
   if (dev < 0 || !attr.done[dev]) {
     CUDA_TRY(cudaFuncSetAttribute(gemm_tc_kernel<true, true, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM_BYTES));
-    CUDA_TRY(cudaFuncSetAttribute(gemm_tc_kernel<true, true, PAIR, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM_BYTES));
+    CUDA_TRY(cudaFuncSetAttribute(gemm_tc_kernel<true, true, PAIR, SWIGLU>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM_BYTES));
+    CUDA_TRY(cudaFuncSetAttribute(gemm_tc_kernel<true, false, PAIR, LOGPROBS>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM_BYTES));
     CUDA_TRY(cudaFuncSetAttribute(gemm_tc_kernel<true, false, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM_BYTES));
     CUDA_TRY(cudaFuncSetAttribute(gemm_tc_kernel<false, true, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM_BYTES));
     CUDA_TRY(cudaFuncSetAttribute(gemm_tc_kernel<false, false, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM_BYTES));
@@ -872,7 +876,8 @@ static int launch_tc(const GemmArgs& g, const CUtensorMap& tmA, const CUtensorMa
   const size_t smem = G::SMEM_BYTES - (G::STAGES - p.stages) * G::STAGE_BYTES;
   auto launch = [&](auto kernel) { return launch_dependent_clusters(kernel, PAIR ? 2 : 1, grid, NTHREADS, smem, s, tmA, tmB, tmC, p); };
   cudaError_t e;
-  if (g.epi == EPI_SWIGLU) e = launch(gemm_tc_kernel<true, true, PAIR, true>);
+  if (g.epi == EPI_SWIGLU) e = launch(gemm_tc_kernel<true, true, PAIR, SWIGLU>);
+  else if (g.epi == EPI_XENT_STATS && g.logprobs) e = launch(gemm_tc_kernel<true, false, PAIR, LOGPROBS>);
   else if (g.a_kmajor && g.b_kmajor) e = launch(gemm_tc_kernel<true, true, PAIR>);
   else if (g.a_kmajor) e = launch(gemm_tc_kernel<true, false, PAIR>);
   else if (g.b_kmajor) e = launch(gemm_tc_kernel<false, true, PAIR>);
