@@ -378,6 +378,36 @@ def test_the_step_and_the_call_on_the_model_s_logits_agree():
     assert float((fb.token_logprobs(one, t0[:, 9].contiguous()).logp - b.logp[:, 9]).abs().max()) < 1e-3
 
 
+@pytest.mark.parametrize("kw,dtype", [(MID, "float32"), (TC, "bfloat16")])
+def test_captured_steps(kw, dtype):
+    """A step in a graph, replayed on other tokens while eager steps run in between, gives what the eager step gives."""
+    cfg, lay, th, batch, params, st, M = setup(kw, 2, dtype, seed=14)
+    tok, tgt, pos = (x.cuda() for x in batch)
+    other, theirs, _ = (x.cuda() for x in inputs(kw, 2, 15))
+    T = kw["sequence_len"]
+    old = fb.forward_token_logprobs(params, st, lay, tok, tgt, pos) + 0.1
+    A, offsets = torch.randn(old.shape, device="cuda"), torch.tensor([0, T, 2 * T], dtype=torch.int32, device="cuda")
+    calls = [lambda: fb.policy_loss_and_gradient_(params, st, lay, tok, tgt, old, A, positions=pos, reduction="mean"),
+             lambda: fb.preference_loss_and_gradient_(params, st, lay, tok, tgt, offsets, positions=pos, ref_logp=old),
+             lambda: (fb.forward_token_logprobs(params, st, lay, tok, tgt, pos),)]
+    graphs = []
+    for call in calls:
+        call()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = call()
+        graphs.append((g, out))
+    tok.copy_(other), tgt.copy_(theirs)
+    for _ in range(2):
+        for call, (g, out) in zip(calls, graphs):
+            params.delta.zero_()
+            g.replay()
+            got, delta = [x.clone() for x in out], params.delta.clone()
+            params.delta.zero_()
+            assert all(torch.equal(a, b) for a, b in zip(got, call())) and torch.equal(delta, params.delta)
+    assert st.status_word() == 0
+
+
 def test_steps_refuse_a_decoder():
     layers = [fb.LayerConfig(mixer="lightning", heads=2, dim=16, vdim=16, decay=(0.9, 0.8), ff=64)]
     cfg = fb.DecoderConfig(vocab_size=50, width=32, norm_eps=1e-5, layers=layers)
