@@ -506,7 +506,8 @@ int32_t femto_token_logprobs_gradient(int32_t dtype, void* dlogits, int64_t ldd,
  *   token_loss = weight (-min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A) + beta (e^(ref_logp - lp) - (ref_logp - lp) - 1))
  * advantages A [N]; ref_logp [N] (may be NULL when beta is 0); weights [N] (NULL = 1; where a weight is 0 loss and gradient are 0).
  * Outputs: token_losses [N], logp [N], the reduced loss, n_valid = rows with a target, n_clipped (may be NULL) = those whose minimum is
- * the bounded product, which has no gradient.  dlogits (NULL: loss only) is overwritten with the gradient of the reduced loss, its rows ldd
+ * the bounded product, which has no gradient.  A token that the model rules out (lp = -inf) has a KL term of +inf; its row's gradient is -inf there,
+ * +inf at tokens of p > 0 and 0 at others.  A difference of two infinite log-probabilities is NaN, as in the formula.  dlogits (NULL: loss only) is overwritten with the gradient of the reduced loss, its rows ldd
  * elements apart; it may be the logits themselves (same pitch), and its rows may not overlap them otherwise. */
 int32_t femto_policy_loss(int32_t dtype, const void* logits, int64_t ldl, const int32_t* targets0, int32_t N, int32_t V,
                           const float* old_logp, const float* advantages, const float* ref_logp, const float* weights,
